@@ -29,6 +29,18 @@ class Tensor5(ctypes.Structure):
     _fields_ = [("base", ctypes.c_void_p), ("dims", ctypes.c_int32 * 5), ("strides", ctypes.c_int64 * 5)]
 
 
+class AdamwTensor(ctypes.Structure):
+    """``gelib_adamw_tensor``"""
+    _fields_ = [(name, ctypes.c_void_p) for name in ("p", "master", "g", "m", "v", "m_scale", "v_scale")]
+    _fields_ += [("n", ctypes.c_int64), ("type", ctypes.c_int)]
+
+
+class AdamwOptions(ctypes.Structure):
+    """``gelib_adamw_options``"""
+    _fields_ = [(name, ctypes.c_double) for name in ("lr", "beta1", "beta2", "eps", "weight_decay")]
+    _fields_ += [("step", ctypes.c_int64), ("seed", ctypes.c_uint64), ("grad_scale", ctypes.c_void_p), ("state_bits", ctypes.c_int)]
+
+
 _P5 = ctypes.POINTER(Tensor5)
 _lib = None
 
@@ -79,6 +91,8 @@ SYMBOLS = {
                                                 ctypes.c_int, ctypes.c_int, ctypes.c_void_p]),
     "gelib_SO3irrep_matrix": (ctypes.c_int, [ctypes.c_int, ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_void_p]),
     "gelib_SO3part_apply": (ctypes.c_int, [_P5, _P5, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]),
+    "gelib_adamw_step": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(AdamwTensor), ctypes.POINTER(AdamwOptions), ctypes.c_void_p]),
+    "gelib_block8_values": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_longlong, ctypes.c_void_p]),
     "gelib_kernel_launch_count": (ctypes.c_longlong, []),
     "gelib_set_option": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_char_p]),
     "gelib_async_status": (ctypes.c_int, []),

@@ -229,6 +229,66 @@ std::optional<at::Tensor> gather(const at::Tensor& x0, const at::Tensor& row_ptr
   return r;
 }
 
+using OptTensors = std::vector<std::optional<at::Tensor>>;
+
+std::optional<int> type_code(at::ScalarType t) {
+  if (t == at::kFloat || t == at::kComplexFloat) return GELIB_F32;
+  if (t == at::kBFloat16) return GELIB_BF16;
+  if (t == at::kHalf) return GELIB_F16;
+  return std::nullopt;
+}
+
+bool plain_dense(const at::Tensor& t, c10::Device device) {
+  return t.defined() && t.device() == device && t.layout() == at::kStrided && t.is_contiguous() && !t.is_conj() && !t.is_neg();
+}
+
+int64_t reals(const at::Tensor& t) { return t.numel() * (t.is_complex() ? 2 : 1); }
+
+// One step over lists of tensors; None when one of them is not plain, or does not go with the others.
+std::optional<bool> adamw_step(const Tensors& params, const Tensors& grads, const Tensors& m, const Tensors& v, const std::optional<Tensors>& ms,
+                               const std::optional<Tensors>& vs, const std::optional<OptTensors>& master, int64_t step, double lr, double beta1, double beta2, double eps,
+                               double weight_decay, uint64_t seed, const std::optional<at::Tensor>& grad_scale) {
+  const size_t k = params.size();
+  if (k == 0 || grads.size() != k || m.size() != k || v.size() != k || ms.has_value() != vs.has_value()) return std::nullopt;
+  if ((ms && (ms->size() != k || vs->size() != k)) || (master && master->size() != k) || !params[0].defined() || !params[0].is_cuda()) return std::nullopt;
+  const auto device = params[0].device();
+  gelib_adamw_options o = {lr, beta1, beta2, eps, weight_decay, step, seed, nullptr, ms ? 8 : 32};
+  if (grad_scale) {
+    if (!plain_dense(*grad_scale, device) || grad_scale->scalar_type() != at::kFloat || grad_scale->numel() != 1) return std::nullopt;
+    o.grad_scale = grad_scale->data_ptr<float>();
+  }
+  std::vector<gelib_adamw_tensor> t(k);
+  for (size_t i = 0; i < k; i++) {
+    const at::Tensor &p = params[i], &g = grads[i];
+    if (!plain_dense(p, device) || !plain_dense(g, device) || g.scalar_type() != p.scalar_type() || g.sizes() != p.sizes()) return std::nullopt;
+    const auto type = type_code(p.scalar_type());
+    if (!type) return std::nullopt;
+    const int64_t n = reals(p);
+    const auto state = [&](const at::Tensor& s) {
+      return plain_dense(s, device) && reals(s) == n && (ms ? s.scalar_type() == at::kFloat8_e4m3fn : s.scalar_type() == at::kFloat || s.scalar_type() == at::kComplexFloat);
+    };
+    if (!state(m[i]) || !state(v[i])) return std::nullopt;
+    t[i] = {p.data_ptr(), nullptr, g.data_ptr(), m[i].data_ptr(), v[i].data_ptr(), nullptr, nullptr, n, *type};
+    if (ms) {
+      for (const auto* s : {&(*ms)[i], &(*vs)[i]})
+        if (!plain_dense(*s, device) || s->scalar_type() != at::kFloat || s->numel() != (n + 255) / 256) return std::nullopt;
+      t[i].m_scale = (*ms)[i].data_ptr<float>();
+      t[i].v_scale = (*vs)[i].data_ptr<float>();
+    }
+    const bool has = master && (*master)[i].has_value();
+    if (has != (*type != GELIB_F32)) return std::nullopt;
+    if (has) {
+      const at::Tensor& w = *(*master)[i];
+      if (!plain_dense(w, device) || w.scalar_type() != at::kFloat || w.numel() != n) return std::nullopt;
+      t[i].master = w.data_ptr<float>();
+    }
+  }
+  c10::cuda::CUDAGuard guard(device);
+  void* s = stream_of(device);
+  call([&] { return gelib_adamw_step(static_cast<int>(k), t.data(), &o, s); });
+  return true;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_native, m) {
@@ -237,5 +297,6 @@ PYBIND11_MODULE(_native, m) {
   m.def("vec_backward", torch::wrap_pybind_function(&vec_backward));
   m.def("part_forward", torch::wrap_pybind_function(&part_forward));
   m.def("part_backward", torch::wrap_pybind_function(&part_backward));
+  m.def("adamw_step", torch::wrap_pybind_function(&adamw_step));
   m.def("gather", torch::wrap_pybind_function(&gather));
 }

@@ -1,0 +1,107 @@
+// What the readout's kernels (group norm, dense layers) and the optimizer step share: element types, wide accesses, activations.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <type_traits>
+
+#include "common.h"
+
+namespace gelib_b200 {
+
+inline bool known_type(int type) { return type == GELIB_F32 || type == GELIB_BF16 || type == GELIB_F16; }
+inline bool known_activation(int act) { return act >= GELIB_ACT_NONE && act <= GELIB_ACT_GELU_TANH; }
+inline int type_bytes(int type) { return type == GELIB_F32 ? 4 : 2; }
+inline bool is_aligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+// What a launch just made comes to.
+inline int launched(const char* fn) {
+  count_launch();
+  GELIB_CUDA_TRY(fn, cudaGetLastError());
+  return GELIB_OK;
+}
+
+// gw[c] and gb[c] from `parts` rows of partial sums each, (2, parts, n) floats; either may be null.
+int launch_sum_parts(void* gw, void* gb, const float* sums, int parts, int n, int type, cudaStream_t stream);
+
+#ifdef __CUDACC__
+
+template <class T>
+__device__ __forceinline__ float to_float(T v) {
+  if constexpr (std::is_same_v<T, float>) return v;
+  else if constexpr (std::is_same_v<T, __nv_bfloat16>) return __bfloat162float(v);
+  else return __half2float(v);
+}
+template <class T>
+__device__ __forceinline__ T from_float(float v) {
+  if constexpr (std::is_same_v<T, float>) return v;
+  else if constexpr (std::is_same_v<T, __nv_bfloat16>) return __float2bfloat16_rn(v);
+  else return __float2half_rn(v);
+}
+
+template <int kBytes>
+struct Raw;
+template <>
+struct Raw<16> { using type = uint4; };
+template <>
+struct Raw<8> { using type = uint2; };
+template <>
+struct Raw<4> { using type = uint32_t; };
+template <>
+struct Raw<2> { using type = uint16_t; };
+
+// V consecutive elements as one access of V * sizeof(T) bytes.
+template <class T, int V>
+__device__ __forceinline__ void load_vec(const T* src, float (&x)[V]) {
+  union { typename Raw<V * sizeof(T)>::type raw; T t[V]; } w;
+  w.raw = *reinterpret_cast<const typename Raw<V * sizeof(T)>::type*>(src);
+#pragma unroll
+  for (int k = 0; k < V; k++) x[k] = to_float(w.t[k]);
+}
+template <class T, int V>
+__device__ __forceinline__ void store_vec(T* dst, const float (&x)[V]) {
+  union { typename Raw<V * sizeof(T)>::type raw; T t[V]; } w;
+#pragma unroll
+  for (int k = 0; k < V; k++) w.t[k] = from_float<T>(x[k]);
+  *reinterpret_cast<typename Raw<V * sizeof(T)>::type*>(dst) = w.raw;
+}
+
+__device__ __forceinline__ float logistic(float z) { return __fdividef(1.f, 1.f + __expf(-z)); }
+
+constexpr float kGelu0 = 1.5957691216057308f;             // 2 sqrt(2 / pi): 0.5 (1 + tanh u) is the logistic function of 2u
+constexpr float kGelu1 = kGelu0 * 0.044715f;
+
+// x = act(x)
+template <int V>
+__device__ __forceinline__ void activate(float (&x)[V], int act) {
+  if (act == GELIB_ACT_NONE) return;
+#pragma unroll
+  for (int k = 0; k < V; k++) {
+    const float z = x[k];
+    if (act == GELIB_ACT_RELU) x[k] = z < 0.f ? 0.f : z;     // NaN stays NaN
+    else if (act == GELIB_ACT_SILU) x[k] = z * logistic(z);
+    else x[k] = z * logistic(z * (kGelu0 + kGelu1 * z * z));
+  }
+}
+
+// g = g act'(z)
+template <int V>
+__device__ __forceinline__ void activate_back(float (&g)[V], const float (&x)[V], int act) {
+  if (act == GELIB_ACT_NONE) return;
+#pragma unroll
+  for (int k = 0; k < V; k++) {
+    const float z = x[k];
+    if (act == GELIB_ACT_RELU) g[k] = z > 0.f ? g[k] : 0.f;
+    else if (act == GELIB_ACT_SILU) {
+      const float q = logistic(z);
+      g[k] *= q * (1.f + z * (1.f - q));
+    } else {
+      const float z2 = z * z, q = logistic(z * (kGelu0 + kGelu1 * z2));
+      g[k] *= q + z * q * (1.f - q) * (kGelu0 + 3.f * kGelu1 * z2);
+    }
+  }
+}
+
+#endif
+
+}  // namespace gelib_b200

@@ -215,6 +215,45 @@ int gelib_SO3irrep_matrix(int l, double alpha, double beta, double gamma, float*
  * which multiplies by the host-built matrix with torch.matmul).  D: (2l+1)^2 complex64 in DEVICE memory, row-major. */
 int gelib_SO3part_apply(const gelib_tensor5* r, const gelib_tensor5* x, const float* D, int flags, void* stream);
 
+/* ---- readout and training step -------------------------------------------------------------------------------
+ * What follows the last product of a network: the invariants (its l=0 parts) are normalised and go through dense layers, and
+ * the weights take an optimizer step.  GElib leaves these to torch.nn and torch.optim; its tensors are as here, channels last.
+ * All arrays are device memory on the current device.  A workspace is the caller's, 256-byte aligned, of at least the bytes
+ * that the ..._workspace function gives for the same arguments; it may be used for other calls on the same stream right after. */
+enum { GELIB_F32 = 0, GELIB_BF16 = 1, GELIB_F16 = 2 };                                               /* element types */
+enum { GELIB_ACT_NONE = 0, GELIB_ACT_RELU = 1, GELIB_ACT_SILU = 2, GELIB_ACT_GELU_TANH = 3 };        /* activations   */
+
+/* One tensor of an AdamW step.  p: n parameters of `type` (a complex one counts as two); g: their gradients, same type.  A 16-bit
+ * parameter has a float `master` copy that takes the step (NULL for GELIB_F32).  m, v: the moments, n floats each; with states in
+ * 8 bits n codes each (e4m3), block i of 256 elements standing for code * m_scale[i], and v's for (code * v_scale[i])^2. */
+typedef struct gelib_adamw_tensor {
+  void* p;
+  float* master;
+  const void* g;
+  void* m;
+  void* v;
+  float* m_scale;
+  float* v_scale;
+  int64_t n;
+  int type;
+} gelib_adamw_tensor;
+
+typedef struct gelib_adamw_options {
+  double lr, beta1, beta2, eps, weight_decay;
+  int64_t step;            /* the step's number, from 1 */
+  uint64_t seed;           /* of the rounding to 8 bits: another one each step */
+  const float* grad_scale; /* device memory, gradients are multiplied by it; NULL: 1 */
+  int state_bits;          /* 32 or 8 */
+} gelib_adamw_options;
+
+/* m = b1 m + (1-b1) g, v = b2 v + (1-b2) g^2, p = p (1 - lr wd) - lr/(1-b1^t) m / (sqrt(v/(1-b2^t)) + eps) for every tensor, in one
+ * launch per 350 tensors.  Rounding to 8 bits is stochastic; it depends on the seed and on an element's place in the call alone.
+ * A value that is no finite number becomes a NaN of its own element in an 8-bit state. */
+int gelib_adamw_step(int count, const gelib_adamw_tensor* tensors, const gelib_adamw_options* options, void* stream);
+
+/* out[i] = codes[i] * scale[i / 256], bfloat16 (exact): what an 8-bit state stands for (of v: its root). */
+int gelib_block8_values(void* out, const void* codes, const float* scale, long long n, void* stream);
+
 /* ---- introspection ------------------------------------------------------------------------------- */
 
 /* Number of kernels this library has launched in the calling process (all threads, all devices). */
