@@ -93,6 +93,10 @@ SYMBOLS = {
     "gelib_SO3part_apply": (ctypes.c_int, [_P5, _P5, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]),
     "gelib_adamw_step": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(AdamwTensor), ctypes.POINTER(AdamwOptions), ctypes.c_void_p]),
     "gelib_block8_values": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_longlong, ctypes.c_void_p]),
+    "gelib_group_norm_workspace": (ctypes.c_longlong, [ctypes.c_longlong] * 2 + [ctypes.c_int] * 4),
+    "gelib_group_norm": (ctypes.c_int, [ctypes.c_void_p] * 6 + [ctypes.c_longlong] * 2 + [ctypes.c_int] * 2 + [ctypes.c_double]
+                         + [ctypes.c_int] * 2 + [ctypes.c_void_p] * 2),
+    "gelib_group_norm_back": (ctypes.c_int, [ctypes.c_void_p] * 9 + [ctypes.c_longlong] * 2 + [ctypes.c_int] * 4 + [ctypes.c_void_p] * 2),
     "gelib_kernel_launch_count": (ctypes.c_longlong, []),
     "gelib_set_option": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_char_p]),
     "gelib_async_status": (ctypes.c_int, []),

@@ -1,0 +1,850 @@
+// Group norm with an activation, channels last, and its gradients:
+//
+//   x (b, s, n), channel c of group c / (n / groups); mean and variance over the s positions and the group's channels
+//   xh = (x - mean) rstd,  z = xh w + bias,  y = act(z)
+//   gz = gy act'(z),  gw = sum gz xh,  gb = sum gz,  gx = rstd (gz w - mean(gz w) - xh mean(gz w xh))
+//
+// Statistics and sums are float32; the variance is a mean of squares of differences from the mean, not a difference of means, so a
+// large mean costs no digits.  Memory bounds it: a read and a write forward, two reads and a write backward, if the elements that
+// share a statistic stay on the SM between its sum and its use.  Three ways of keeping them, by size:
+//
+//   row    s = 1 and a group of at most 1024 channels (512 in float32): a few lanes of a warp own a (row, group) in registers
+//   tile   a sample's rows of some groups fit a block's shared memory
+//   two    larger samples: sums over pieces of a sample, then a second pass over x (and gy) that applies them
+//
+// Parameter gradients are partial sums per block, added up in a fixed order by a second kernel: results repeat bit for bit.
+#include <algorithm>
+
+#include "readout.h"
+#include "norm.h"
+
+namespace gelib_b200 {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+
+struct Norm {
+  const void *x, *w, *bias, *gy;
+  void *y;               // y, or gx
+  float *mean, *rstd;    // (b, groups)
+  float* part;           // partial sums
+  long long b, s;
+  int n, groups, cg;     // cg: channels of a group
+  float eps;
+  int act;
+};
+
+__device__ __forceinline__ float lanes_sum(float v, int lanes) {
+  for (int d = lanes >> 1; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+  return v;
+}
+
+template <class T, int V>
+__device__ __forceinline__ void load_or(const void* p, long long at, float other, float (&x)[V]) {
+  if (p) load_vec<T, V>(static_cast<const T*>(p) + at, x);
+  else
+#pragma unroll
+    for (int k = 0; k < V; k++) x[k] = other;
+}
+
+// ---- row: s = 1 ----------------------------------------------------------------------------------------------------------------
+// `lanes` lanes (a power of two) own a (row, group): K accesses of V elements each.
+
+template <class T, int V, int K>
+__global__ void __launch_bounds__(kThreads) row_fwd_kernel(Norm a, int lanes) {
+  const int per = 32 / lanes, lane = threadIdx.x % lanes;
+  const long long item = ((long long)blockIdx.x * kWarps + threadIdx.x / 32) * per + (threadIdx.x & 31) / lanes;
+  const bool live = item < a.b * a.groups;
+  const long long row = live ? item / a.groups : 0;
+  const int g = live ? (int)(item - row * a.groups) : 0, c0 = g * a.cg;
+  const T* x = static_cast<const T*>(a.x) + row * a.n + c0;
+  float v[K][V], sum = 0;
+#pragma unroll
+  for (int k = 0; k < K; k++) {
+    const int c = (k * lanes + lane) * V;
+    if (live && c < a.cg) load_vec<T, V>(x + c, v[k]);
+    else
+#pragma unroll
+      for (int j = 0; j < V; j++) v[k][j] = 0;
+#pragma unroll
+    for (int j = 0; j < V; j++) sum += v[k][j];
+  }
+  const float mean = lanes_sum(sum, lanes) / a.cg;
+  float sq = 0;
+#pragma unroll
+  for (int k = 0; k < K; k++)
+    if ((k * lanes + lane) * V < a.cg)
+#pragma unroll
+      for (int j = 0; j < V; j++) sq += (v[k][j] - mean) * (v[k][j] - mean);
+  const float rstd = rsqrtf(lanes_sum(sq, lanes) / a.cg + a.eps);
+  if (!live) return;
+  if (a.mean && lane == 0) {
+    a.mean[item] = mean;
+    a.rstd[item] = rstd;
+  }
+#pragma unroll
+  for (int k = 0; k < K; k++) {
+    const int c = (k * lanes + lane) * V;
+    if (c < a.cg) {
+      float w[V], bias[V];
+      load_or<T, V>(a.w, c0 + c, 1.f, w);
+      load_or<T, V>(a.bias, c0 + c, 0.f, bias);
+#pragma unroll
+      for (int j = 0; j < V; j++) v[k][j] = (v[k][j] - mean) * rstd * w[j] + bias[j];
+      activate(v[k], a.act);
+      store_vec<T, V>(static_cast<T*>(a.y) + row * a.n + c0 + c, v[k]);
+    }
+  }
+}
+
+// A warp keeps its groups and walks rows, so that the sums over rows stay in registers; the block's warps have the same groups.
+template <class T, int V, int K>
+__global__ void __launch_bounds__(kThreads) row_bwd_kernel(Norm a, int lanes, int parts) {
+  __shared__ float sums[kWarps][2][32 * V];
+  const int per = 32 / lanes, lane = threadIdx.x % lanes, warp = threadIdx.x / 32;
+  const int g = blockIdx.x * per + (threadIdx.x & 31) / lanes, c0 = g * a.cg;
+  const bool live = g < a.groups;
+  float w[K][V], bias[K][V], gw[K][V], gb[K][V];
+#pragma unroll
+  for (int k = 0; k < K; k++) {
+    const int c = (k * lanes + lane) * V;
+#pragma unroll
+    for (int j = 0; j < V; j++) w[k][j] = bias[k][j] = gw[k][j] = gb[k][j] = 0;
+    if (live && c < a.cg) {
+      load_or<T, V>(a.w, c0 + c, 1.f, w[k]);
+      load_or<T, V>(a.bias, c0 + c, 0.f, bias[k]);
+    }
+  }
+  for (long long row = (long long)blockIdx.y * kWarps + warp; row < a.b; row += (long long)gridDim.y * kWarps) {
+    const float mean = live ? a.mean[row * a.groups + g] : 0, rstd = live ? a.rstd[row * a.groups + g] : 0;
+    const long long at = row * a.n + c0;
+    float h[K][V], gz[K][V], s1 = 0, s2 = 0;
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+      const int c = (k * lanes + lane) * V;
+      if (live && c < a.cg) {
+        load_vec<T, V>(static_cast<const T*>(a.x) + at + c, h[k]);
+        load_vec<T, V>(static_cast<const T*>(a.gy) + at + c, gz[k]);
+        float z[V];
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+          h[k][j] = (h[k][j] - mean) * rstd;
+          z[j] = h[k][j] * w[k][j] + bias[k][j];
+        }
+        activate_back(gz[k], z, a.act);
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+          gb[k][j] += gz[k][j];
+          gw[k][j] += gz[k][j] * h[k][j];
+          gz[k][j] *= w[k][j];
+          s1 += gz[k][j];
+          s2 += gz[k][j] * h[k][j];
+        }
+      }
+    }
+    if (a.y) {
+      s1 = lanes_sum(s1, lanes) / a.cg;
+      s2 = lanes_sum(s2, lanes) / a.cg;
+#pragma unroll
+      for (int k = 0; k < K; k++) {
+        const int c = (k * lanes + lane) * V;
+        if (live && c < a.cg) {
+#pragma unroll
+          for (int j = 0; j < V; j++) gz[k][j] = rstd * (gz[k][j] - s1 - h[k][j] * s2);
+          store_vec<T, V>(static_cast<T*>(a.y) + at + c, gz[k]);
+        }
+      }
+    }
+  }
+  if (!a.part) return;
+#pragma unroll
+  for (int k = 0; k < K; k++) {
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < V; j++) {
+      sums[warp][0][(threadIdx.x & 31) * V + j] = gw[k][j];
+      sums[warp][1][(threadIdx.x & 31) * V + j] = gb[k][j];
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < 2 * 32 * V; e += kThreads) {
+      const int which = e / (32 * V), q = e % (32 * V), l = q / V;
+      const int group = blockIdx.x * per + l / lanes, c = (k * lanes + l % lanes) * V + q % V;
+      if (group < a.groups && c < a.cg) {
+        float t = 0;
+#pragma unroll
+        for (int i = 0; i < kWarps; i++) t += sums[i][which][q];
+        a.part[((long long)which * parts + blockIdx.y) * a.n + group * a.cg + c] = t;
+      }
+    }
+  }
+}
+
+// ---- tile: a sample's rows of `gpc` groups in shared memory ----------------------------------------------------------------------
+// The channels of the tile are columns of V elements; a thread owns columns and every ty-th row.
+
+struct Columns {
+  int cols;      // of the tile, V channels each
+  int wide;      // threads side by side: min(cols, kThreads)
+  int high;      // rows worked on together
+};
+__device__ __forceinline__ Columns columns_of(int channels, int V) {
+  Columns c;
+  c.cols = channels / V;
+  c.wide = min(c.cols, kThreads);
+  c.high = kThreads / c.wide;
+  return c;
+}
+
+// The sums of f over a column's rows, one per channel and row of threads, then per group: group[g] = sum.  chan has high * channels floats.
+template <int V, class F>
+__device__ __forceinline__ void channel_sums(const Columns& c, int rows, int channels, float* chan, F f) {
+  const int tx = threadIdx.x % c.wide, ty = threadIdx.x / c.wide;
+  if (ty < c.high)
+    for (int col = tx; col < c.cols; col += c.wide) {
+      float sum[V];
+#pragma unroll
+      for (int j = 0; j < V; j++) sum[j] = 0;
+      for (int r = ty; r < rows; r += c.high) f(r, col, sum);
+#pragma unroll
+      for (int j = 0; j < V; j++) chan[ty * channels + col * V + j] = sum[j];
+    }
+}
+
+__device__ __forceinline__ float warp_total(float v) { return lanes_sum(v, 32); }
+
+template <class T, int V>
+__global__ void __launch_bounds__(kThreads) tile_fwd_kernel(Norm a, int gpc, int chunks) {
+  extern __shared__ __align__(16) unsigned char memory[];
+  const int chunk = blockIdx.x % chunks;
+  const long long sample = blockIdx.x / chunks;
+  const int g0 = chunk * gpc, ng = min(gpc, a.groups - g0), channels = ng * a.cg, c0 = g0 * a.cg, rows = (int)a.s;
+  const Columns cl = columns_of(channels, V);
+  T* tile = reinterpret_cast<T*>(memory);
+  float* chan = reinterpret_cast<float*>(memory + ((size_t)rows * channels * sizeof(T) + 15) / 16 * 16);
+  float* group = chan + max(cl.high * channels, 1);
+  const T* x = static_cast<const T*>(a.x) + sample * a.s * a.n + c0;
+  const float count = (float)rows * a.cg;
+  channel_sums<V>(cl, rows, channels, chan, [&](int r, int col, float (&sum)[V]) {
+    using R = typename Raw<V * sizeof(T)>::type;
+    *reinterpret_cast<R*>(tile + r * channels + col * V) = *reinterpret_cast<const R*>(x + (long long)r * a.n + col * V);
+    float v[V];
+    load_vec<T, V>(tile + r * channels + col * V, v);
+#pragma unroll
+    for (int j = 0; j < V; j++) sum[j] += v[j];
+  });
+  __syncthreads();
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  for (int g = warp; g < ng; g += kWarps) {
+    float t = 0;
+    for (int e = lane; e < cl.high * a.cg; e += 32) t += chan[e / a.cg * channels + g * a.cg + e % a.cg];
+    t = warp_total(t);
+    if (lane == 0) group[g] = t / count;
+  }
+  __syncthreads();
+  channel_sums<V>(cl, rows, channels, chan, [&](int r, int col, float (&sum)[V]) {
+    float v[V];
+    load_vec<T, V>(tile + r * channels + col * V, v);
+#pragma unroll
+    for (int j = 0; j < V; j++) {
+      const float d = v[j] - group[(col * V + j) / a.cg];
+      sum[j] += d * d;
+    }
+  });
+  __syncthreads();
+  for (int g = warp; g < ng; g += kWarps) {
+    float t = 0;
+    for (int e = lane; e < cl.high * a.cg; e += 32) t += chan[e / a.cg * channels + g * a.cg + e % a.cg];
+    t = warp_total(t);
+    if (lane == 0) {
+      const float rstd = rsqrtf(t / count + a.eps);
+      group[ng + g] = rstd;
+      if (a.mean) {
+        a.mean[sample * a.groups + g0 + g] = group[g];
+        a.rstd[sample * a.groups + g0 + g] = rstd;
+      }
+    }
+  }
+  __syncthreads();
+  const int tx = threadIdx.x % cl.wide, ty = threadIdx.x / cl.wide;
+  if (ty >= cl.high) return;
+  for (int col = tx; col < cl.cols; col += cl.wide) {
+    float w[V], bias[V], mean[V];
+    load_or<T, V>(a.w, c0 + col * V, 1.f, w);
+    load_or<T, V>(a.bias, c0 + col * V, 0.f, bias);
+#pragma unroll
+    for (int j = 0; j < V; j++) {
+      const int g = (col * V + j) / a.cg;
+      mean[j] = group[g];
+      w[j] *= group[ng + g];
+    }
+    for (int r = ty; r < rows; r += cl.high) {
+      float v[V];
+      load_vec<T, V>(tile + r * channels + col * V, v);
+#pragma unroll
+      for (int j = 0; j < V; j++) v[j] = (v[j] - mean[j]) * w[j] + bias[j];
+      activate(v, a.act);
+      store_vec<T, V>(static_cast<T*>(a.y) + (sample * a.s + r) * a.n + c0 + col * V, v);
+    }
+  }
+}
+
+// Blocks of one chunk walk the samples; the chunk's parameter sums stay in shared memory.
+template <class T, int V>
+__global__ void __launch_bounds__(kThreads) tile_bwd_kernel(Norm a, int gpc, int parts) {
+  extern __shared__ __align__(16) unsigned char memory[];
+  const int chunk = blockIdx.x;
+  const int g0 = chunk * gpc, ng = min(gpc, a.groups - g0), channels = ng * a.cg, c0 = g0 * a.cg, rows = (int)a.s;
+  const Columns cl = columns_of(channels, V);
+  const size_t bytes = ((size_t)rows * channels * sizeof(T) + 15) / 16 * 16;
+  T* tx_ = reinterpret_cast<T*>(memory);
+  T* tg_ = reinterpret_cast<T*>(memory + bytes);
+  float* chan = reinterpret_cast<float*>(memory + 2 * bytes);    // [2][high][channels]
+  float* total = chan + 2 * cl.high * channels;                  // [2][channels]
+  float* group = total + 2 * channels;                           // [4][ng]: mean, rstd, two means of gradients
+  const int tx = threadIdx.x % cl.wide, ty = threadIdx.x / cl.wide, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const float count = (float)rows * a.cg;
+  for (int c = threadIdx.x; c < 2 * channels; c += kThreads) total[c] = 0;
+  for (long long sample = blockIdx.y; sample < a.b; sample += gridDim.y) {
+    const long long base = sample * a.s * a.n + c0;
+    __syncthreads();
+    for (int g = threadIdx.x; g < ng; g += kThreads) {
+      group[g] = a.mean[sample * a.groups + g0 + g];
+      group[ng + g] = a.rstd[sample * a.groups + g0 + g];
+    }
+    __syncthreads();
+    if (ty < cl.high)
+      for (int col = tx; col < cl.cols; col += cl.wide) {
+        float w[V], bias[V], mean[V], rstd[V], sb[V], sw[V];
+        load_or<T, V>(a.w, c0 + col * V, 1.f, w);
+        load_or<T, V>(a.bias, c0 + col * V, 0.f, bias);
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+          const int g = (col * V + j) / a.cg;
+          mean[j] = group[g], rstd[j] = group[ng + g], sb[j] = sw[j] = 0;
+        }
+        for (int r = ty; r < rows; r += cl.high) {
+          using R = typename Raw<V * sizeof(T)>::type;
+          const int at = r * channels + col * V;
+          const long long from = base + (long long)r * a.n + col * V;
+          const R rx = *reinterpret_cast<const R*>(static_cast<const T*>(a.x) + from), rg = *reinterpret_cast<const R*>(static_cast<const T*>(a.gy) + from);
+          *reinterpret_cast<R*>(tx_ + at) = rx;
+          *reinterpret_cast<R*>(tg_ + at) = rg;
+          float h[V], g[V], z[V];
+          load_vec<T, V>(tx_ + at, h);
+          load_vec<T, V>(tg_ + at, g);
+#pragma unroll
+          for (int j = 0; j < V; j++) {
+            h[j] = (h[j] - mean[j]) * rstd[j];
+            z[j] = h[j] * w[j] + bias[j];
+          }
+          activate_back(g, z, a.act);
+#pragma unroll
+          for (int j = 0; j < V; j++) sb[j] += g[j], sw[j] += g[j] * h[j];
+        }
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+          chan[ty * channels + col * V + j] = sw[j];
+          chan[(cl.high + ty) * channels + col * V + j] = sb[j];
+        }
+      }
+    __syncthreads();
+    for (int c = threadIdx.x; c < channels; c += kThreads) {
+      float sw = 0, sb = 0;
+      for (int i = 0; i < cl.high; i++) sw += chan[i * channels + c], sb += chan[(cl.high + i) * channels + c];
+      total[c] += sw;
+      total[channels + c] += sb;
+      const float w = a.w ? to_float(static_cast<const T*>(a.w)[c0 + c]) : 1.f;
+      chan[c] = sw * w;                         // row 0 of its part: read by this thread alone so far
+      chan[cl.high * channels + c] = sb * w;
+    }
+    __syncthreads();
+    for (int g = warp; g < ng; g += kWarps) {
+      float s1 = 0, s2 = 0;
+      for (int c = lane; c < a.cg; c += 32) s2 += chan[g * a.cg + c], s1 += chan[cl.high * channels + g * a.cg + c];
+      s1 = warp_total(s1), s2 = warp_total(s2);
+      if (lane == 0) group[2 * ng + g] = s1 / count, group[3 * ng + g] = s2 / count;
+    }
+    __syncthreads();
+    if (a.y && ty < cl.high)
+      for (int col = tx; col < cl.cols; col += cl.wide) {
+        float w[V], bias[V], mean[V], rstd[V], s1[V], s2[V];
+        load_or<T, V>(a.w, c0 + col * V, 1.f, w);
+        load_or<T, V>(a.bias, c0 + col * V, 0.f, bias);
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+          const int g = (col * V + j) / a.cg;
+          mean[j] = group[g], rstd[j] = group[ng + g], s1[j] = group[2 * ng + g], s2[j] = group[3 * ng + g];
+        }
+        for (int r = ty; r < rows; r += cl.high) {
+          float h[V], g[V], z[V];
+          load_vec<T, V>(tx_ + r * channels + col * V, h);
+          load_vec<T, V>(tg_ + r * channels + col * V, g);
+#pragma unroll
+          for (int j = 0; j < V; j++) {
+            h[j] = (h[j] - mean[j]) * rstd[j];
+            z[j] = h[j] * w[j] + bias[j];
+          }
+          activate_back(g, z, a.act);
+#pragma unroll
+          for (int j = 0; j < V; j++) g[j] = rstd[j] * (g[j] * w[j] - s1[j] - h[j] * s2[j]);
+          store_vec<T, V>(static_cast<T*>(a.y) + base + (long long)r * a.n + col * V, g);
+        }
+      }
+  }
+  __syncthreads();
+  if (a.part)
+    for (int c = threadIdx.x; c < 2 * channels; c += kThreads)
+      a.part[((long long)(c / channels) * parts + blockIdx.y) * a.n + c0 + c % channels] = total[c];
+}
+
+// ---- two: pieces of a sample ---------------------------------------------------------------------------------------------------
+// A block takes `rows` rows of a sample, all channels.
+
+// Sum, and sum of squares of differences from the piece's own mean, of every group of a piece: part (b, pieces, groups, 2).
+template <class T, int V>
+__global__ void __launch_bounds__(kThreads) piece_stats_kernel(Norm a, int pieces, int per) {
+  extern __shared__ __align__(16) unsigned char memory[];
+  const long long sample = blockIdx.x / pieces;
+  const int piece = blockIdx.x % pieces;
+  const long long r0 = (long long)piece * per;
+  const int rows = (int)min((long long)per, a.s - r0);
+  const Columns cl = columns_of(a.n, V);
+  float* chan = reinterpret_cast<float*>(memory);               // [2][high][n]
+  const T* x = static_cast<const T*>(a.x) + (sample * a.s + r0) * a.n;
+  const int tx = threadIdx.x % cl.wide, ty = threadIdx.x / cl.wide, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  if (ty < cl.high)
+    for (int col = tx; col < cl.cols; col += cl.wide) {
+      // sums of differences from the thread's first row: what they lose to cancellation is of the size of the spread, not of the mean
+      float first[V], sum[V], sq[V];
+#pragma unroll
+      for (int j = 0; j < V; j++) first[j] = sum[j] = sq[j] = 0;
+      if (ty < rows) load_vec<T, V>(x + (long long)ty * a.n + col * V, first);
+      for (int r = ty + cl.high; r < rows; r += cl.high) {
+        float v[V];
+        load_vec<T, V>(x + (long long)r * a.n + col * V, v);
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+          const float d = v[j] - first[j];
+          sum[j] += d;
+          sq[j] += d * d;
+        }
+      }
+      const int mine = ty < rows ? (rows - ty + cl.high - 1) / cl.high : 0;
+#pragma unroll
+      for (int j = 0; j < V; j++) {
+        const float m = mine ? sum[j] / mine : 0;
+        chan[ty * a.n + col * V + j] = first[j] + m;                                   // mean of the thread's rows
+        chan[(cl.high + ty) * a.n + col * V + j] = mine ? fmaxf(sq[j] - sum[j] * m, 0.f) : 0;   // their squared differences
+      }
+    }
+  __syncthreads();
+  for (int g = warp; g < a.groups; g += kWarps) {
+    const int e1 = cl.high * a.cg;
+    float t = 0;
+    for (int e = lane; e < e1; e += 32) {
+      const int i = e / a.cg, mine = i < rows ? (rows - i + cl.high - 1) / cl.high : 0;
+      t += mine * chan[i * a.n + g * a.cg + e % a.cg];
+    }
+    const float mean = warp_total(t) / ((float)rows * a.cg);
+    t = 0;
+    for (int e = lane; e < e1; e += 32) {
+      const int i = e / a.cg, mine = i < rows ? (rows - i + cl.high - 1) / cl.high : 0;
+      const float d = chan[i * a.n + g * a.cg + e % a.cg] - mean;
+      t += chan[(cl.high + i) * a.n + g * a.cg + e % a.cg] + mine * d * d;
+    }
+    t = warp_total(t);
+    if (lane == 0) {
+      float* out = a.part + ((sample * pieces + piece) * a.groups + g) * 2;
+      out[0] = mean, out[1] = t;
+    }
+  }
+}
+
+// The pieces' statistics of one (sample, group) as one, by a warp.
+__device__ __forceinline__ void join_pieces(const Norm& a, long long sample, int g, int pieces, int per, float* mean_out, float* rstd_out) {
+  const int lane = threadIdx.x % 32;
+  const float* p = a.part + (sample * pieces * a.groups + g) * 2;
+  const long long step = 2LL * a.groups;
+  float t = 0;
+  for (int i = lane; i < pieces; i += 32) t += p[i * step] * (float)min((long long)per, a.s - (long long)i * per);
+  const float mean = warp_total(t) / (float)a.s;
+  t = 0;
+  for (int i = lane; i < pieces; i += 32) {
+    const float d = p[i * step] - mean;
+    t += p[i * step + 1] + d * d * ((float)min((long long)per, a.s - (long long)i * per) * a.cg);
+  }
+  *mean_out = mean;
+  *rstd_out = rsqrtf(warp_total(t) / ((float)a.s * a.cg) + a.eps);
+}
+
+template <class T, int V>
+__global__ void __launch_bounds__(kThreads) piece_apply_kernel(Norm a, int pieces, int per) {
+  extern __shared__ __align__(16) unsigned char memory[];
+  // the pieces that were read last may still be in L2: they are taken first
+  const long long block = (long long)gridDim.x - 1 - blockIdx.x;
+  const long long sample = block / pieces;
+  const int piece = (int)(block % pieces);
+  const long long r0 = (long long)piece * per;
+  const int rows = (int)min((long long)per, a.s - r0);
+  const Columns cl = columns_of(a.n, V);
+  float* group = reinterpret_cast<float*>(memory);   // [2][groups]
+  const int tx = threadIdx.x % cl.wide, ty = threadIdx.x / cl.wide, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  for (int g = warp; g < a.groups; g += kWarps) {
+    float mean, rstd;
+    join_pieces(a, sample, g, pieces, per, &mean, &rstd);
+    if (lane == 0) {
+      group[g] = mean, group[a.groups + g] = rstd;
+      if (a.mean && piece == 0) a.mean[sample * a.groups + g] = mean, a.rstd[sample * a.groups + g] = rstd;
+    }
+  }
+  __syncthreads();
+  if (ty >= cl.high) return;
+  const long long base = (sample * a.s + r0) * a.n;
+  for (int col = tx; col < cl.cols; col += cl.wide) {
+    float w[V], bias[V], mean[V];
+    load_or<T, V>(a.w, col * V, 1.f, w);
+    load_or<T, V>(a.bias, col * V, 0.f, bias);
+#pragma unroll
+    for (int j = 0; j < V; j++) {
+      const int g = (col * V + j) / a.cg;
+      mean[j] = group[g];
+      w[j] *= group[a.groups + g];
+    }
+    for (int r = ty; r < rows; r += cl.high) {
+      float v[V];
+      load_vec<T, V>(static_cast<const T*>(a.x) + base + (long long)r * a.n + col * V, v);
+#pragma unroll
+      for (int j = 0; j < V; j++) v[j] = (v[j] - mean[j]) * w[j] + bias[j];
+      activate(v, a.act);
+      store_vec<T, V>(static_cast<T*>(a.y) + base + (long long)r * a.n + col * V, v);
+    }
+  }
+}
+
+// gz xh and gz summed over a piece's rows, per channel: part (2, b * pieces, n).
+template <class T, int V>
+__global__ void __launch_bounds__(kThreads) piece_back_sums_kernel(Norm a, int pieces, int per) {
+  extern __shared__ __align__(16) unsigned char memory[];
+  const long long sample = blockIdx.x / pieces;
+  const int piece = blockIdx.x % pieces;
+  const long long r0 = (long long)piece * per;
+  const int rows = (int)min((long long)per, a.s - r0);
+  const Columns cl = columns_of(a.n, V);
+  float* chan = reinterpret_cast<float*>(memory);   // [2][high][n]
+  const int tx = threadIdx.x % cl.wide, ty = threadIdx.x / cl.wide;
+  const long long base = (sample * a.s + r0) * a.n;
+  if (ty < cl.high)
+    for (int col = tx; col < cl.cols; col += cl.wide) {
+      float w[V], bias[V], mean[V], rstd[V], sw[V], sb[V];
+      load_or<T, V>(a.w, col * V, 1.f, w);
+      load_or<T, V>(a.bias, col * V, 0.f, bias);
+#pragma unroll
+      for (int j = 0; j < V; j++) {
+        const long long g = sample * a.groups + (col * V + j) / a.cg;
+        mean[j] = a.mean[g], rstd[j] = a.rstd[g], sw[j] = sb[j] = 0;
+      }
+      for (int r = ty; r < rows; r += cl.high) {
+        float h[V], g[V], z[V];
+        load_vec<T, V>(static_cast<const T*>(a.x) + base + (long long)r * a.n + col * V, h);
+        load_vec<T, V>(static_cast<const T*>(a.gy) + base + (long long)r * a.n + col * V, g);
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+          h[j] = (h[j] - mean[j]) * rstd[j];
+          z[j] = h[j] * w[j] + bias[j];
+        }
+        activate_back(g, z, a.act);
+#pragma unroll
+        for (int j = 0; j < V; j++) sb[j] += g[j], sw[j] += g[j] * h[j];
+      }
+#pragma unroll
+      for (int j = 0; j < V; j++) {
+        chan[ty * a.n + col * V + j] = sw[j];
+        chan[(cl.high + ty) * a.n + col * V + j] = sb[j];
+      }
+    }
+  __syncthreads();
+  for (int c = threadIdx.x; c < 2 * a.n; c += kThreads) {
+    const int which = c / a.n, q = c % a.n;
+    float t = 0;
+    for (int i = 0; i < cl.high; i++) t += chan[(which * cl.high + i) * a.n + q];
+    a.part[((long long)which * (a.b * pieces) + blockIdx.x) * a.n + q] = t;
+  }
+}
+
+// The two means of a (sample, group), from its channels' sums: back (b, groups, 2).
+template <class T>
+__global__ void __launch_bounds__(kThreads) piece_back_groups_kernel(Norm a, int pieces, float* back) {
+  const long long sample = blockIdx.x / a.groups;
+  const int g = blockIdx.x % a.groups;
+  __shared__ float sums[2][kWarps];
+  float s1 = 0, s2 = 0;
+  for (long long e = threadIdx.x; e < (long long)pieces * a.cg; e += kThreads) {
+    const int c = g * a.cg + (int)(e % a.cg);
+    const long long row = sample * pieces + e / a.cg;
+    const float w = a.w ? to_float(static_cast<const T*>(a.w)[c]) : 1.f;
+    s2 += w * a.part[row * a.n + c];
+    s1 += w * a.part[(a.b * pieces + row) * a.n + c];
+  }
+  s1 = warp_total(s1), s2 = warp_total(s2);
+  if (threadIdx.x % 32 == 0) sums[0][threadIdx.x / 32] = s1, sums[1][threadIdx.x / 32] = s2;
+  __syncthreads();
+  if (threadIdx.x < 2) {
+    float t = 0;
+    for (int i = 0; i < kWarps; i++) t += sums[threadIdx.x][i];
+    back[(sample * a.groups + g) * 2 + threadIdx.x] = t / ((float)a.s * a.cg);
+  }
+}
+
+template <class T, int V>
+__global__ void __launch_bounds__(kThreads) piece_back_apply_kernel(Norm a, int pieces, int per, const float* back) {
+  const long long block = (long long)gridDim.x - 1 - blockIdx.x;
+  const long long sample = block / pieces;
+  const long long r0 = (block % pieces) * (long long)per;
+  const int rows = (int)min((long long)per, a.s - r0);
+  const Columns cl = columns_of(a.n, V);
+  const int tx = threadIdx.x % cl.wide, ty = threadIdx.x / cl.wide;
+  const long long base = (sample * a.s + r0) * a.n;
+  if (ty >= cl.high) return;
+  for (int col = tx; col < cl.cols; col += cl.wide) {
+    float w[V], bias[V], mean[V], rstd[V], s1[V], s2[V];
+    load_or<T, V>(a.w, col * V, 1.f, w);
+    load_or<T, V>(a.bias, col * V, 0.f, bias);
+#pragma unroll
+    for (int j = 0; j < V; j++) {
+      const long long g = sample * a.groups + (col * V + j) / a.cg;
+      mean[j] = a.mean[g], rstd[j] = a.rstd[g], s1[j] = back[2 * g], s2[j] = back[2 * g + 1];
+    }
+    for (int r = ty; r < rows; r += cl.high) {
+      float h[V], g[V], z[V];
+      load_vec<T, V>(static_cast<const T*>(a.x) + base + (long long)r * a.n + col * V, h);
+      load_vec<T, V>(static_cast<const T*>(a.gy) + base + (long long)r * a.n + col * V, g);
+#pragma unroll
+      for (int j = 0; j < V; j++) {
+        h[j] = (h[j] - mean[j]) * rstd[j];
+        z[j] = h[j] * w[j] + bias[j];
+      }
+      activate_back(g, z, a.act);
+#pragma unroll
+      for (int j = 0; j < V; j++) g[j] = rstd[j] * (g[j] * w[j] - s1[j] - h[j] * s2[j]);
+      store_vec<T, V>(static_cast<T*>(a.y) + base + (long long)r * a.n + col * V, g);
+    }
+  }
+}
+
+// ---- sums over parts -------------------------------------------------------------------------------------------------------------
+
+template <class T>
+__global__ void __launch_bounds__(1024) sum_parts_kernel(T* gw, T* gb, const float* sums, int parts, int n) {
+  __shared__ float t[32][33];
+  const int c = blockIdx.x * 32 + threadIdx.x;
+  T* out = blockIdx.y ? gb : gw;
+  if (!out) return;
+  const float* p = sums + (long long)blockIdx.y * parts * n;
+  float s = 0;
+  if (c < n)
+    for (int i = threadIdx.y; i < parts; i += 32) s += p[(long long)i * n + c];
+  t[threadIdx.y][threadIdx.x] = s;
+  __syncthreads();
+  if (threadIdx.y == 0 && c < n) {
+    s = 0;
+#pragma unroll
+    for (int i = 0; i < 32; i++) s += t[i][threadIdx.x];
+    out[c] = from_float<T>(s);
+  }
+}
+
+// ---- which way, and with which sizes ---------------------------------------------------------------------------------------------
+
+constexpr int kSms = 148;
+constexpr int kSharedLimit = 200 * 1024;
+
+struct Way {
+  enum { kRow, kTile, kTwo } way;
+  int V;             // elements of an access
+  int lanes, K;      // row
+  int gpc, chunks;   // tile: groups of a chunk
+  size_t shared;     // tile, two
+  int parts;         // backward: rows of partial sums
+  int pieces, per;   // two
+};
+
+int high_of(int channels, int V) { return kThreads / std::min(channels / V, kThreads); }
+
+Way choose(long long b, long long s, int n, int groups, int type, bool wide16, bool wide8, bool backward) {
+  Way w = {};
+  const int cg = n / groups, size = type_bytes(type);
+  auto fits = [&](int bytes) { return bytes >= size && cg * size % bytes == 0 && (bytes <= size || (bytes == 16 ? wide16 : wide8)); };
+  if (s == 1) {
+    const int V = (fits(16) ? 16 : fits(8) ? 8 : size) / size;
+    const int need = (cg + V - 1) / V;
+    if (need <= 128) {
+      w.way = Way::kRow, w.V = V;
+      w.lanes = 1;
+      while (w.lanes < need && w.lanes < 32) w.lanes *= 2;
+      w.K = need <= 32 ? 1 : 4;
+      const int across = (groups + 32 / w.lanes - 1) / (32 / w.lanes);
+      w.parts = (int)std::max(1LL, std::min((b + kWarps - 1) / kWarps, (long long)(kSms * 4 + across - 1) / across));
+      return w;
+    }
+  }
+  // an access may hold channels of two groups, but not of two rows or chunks
+  auto fits_row = [&](int channels, int bytes) {
+    return bytes >= size && n * size % bytes == 0 && channels * size % bytes == 0 && (bytes <= size || (bytes == 16 ? wide16 : wide8));
+  };
+  auto vector = [&](int channels) { return (fits_row(channels, 16) ? 16 : fits_row(channels, 8) ? 8 : size) / size; };
+  auto shared_of = [&](int gpc) {
+    const long long channels = (long long)gpc * cg;
+    const int V = vector((int)channels), high = high_of((int)channels, V);
+    const long long tile = (s * channels * size + 15) / 16 * 16;
+    return backward ? 2 * tile + (2LL * high * channels + 2 * channels + 4 * gpc) * 4 : tile + (high * channels + 2LL * gpc) * 4;
+  };
+  if (s <= 1 << 20) {
+    // whole samples where they leave room for several blocks on an SM and there are enough of them, else fewer groups
+    int gpc = groups;
+    while (gpc > 1 && (shared_of(gpc) > kSharedLimit / 4 || b * ((groups + gpc - 1) / gpc) < kSms) &&
+           (long long)((gpc + 1) / 2) * cg * size >= 64)
+      gpc = (gpc + 1) / 2;
+    // chunks have to begin on an access's boundary, and the last one may be smaller
+    if (shared_of(gpc) <= kSharedLimit) {
+      w.way = Way::kTile, w.gpc = gpc, w.chunks = (groups + gpc - 1) / gpc;
+      const int last = (groups - (w.chunks - 1) * gpc) * cg;
+      w.V = std::min(vector(gpc * cg), vector(last));
+      const int high = std::max(high_of(gpc * cg, w.V), high_of(last, w.V));
+      const long long channels = (long long)gpc * cg, tile = (s * channels * size + 15) / 16 * 16;
+      w.shared = backward ? 2 * tile + (2LL * high * channels + 2 * channels + 4 * gpc) * 4 : tile + (high * channels + 2LL * gpc) * 4;
+      if (w.shared <= (size_t)kSharedLimit) {
+        const long long resident = std::max(1LL, std::min(8LL, (long long)(220 * 1024) / (long long)(w.shared + 1024)));
+        w.parts = (int)std::max(1LL, std::min(b, (kSms * resident + w.chunks - 1) / w.chunks));
+        return w;
+      }
+    }
+  }
+  w.way = Way::kTwo, w.V = vector(n);
+  const int high = high_of(n, w.V);
+  w.shared = std::max(2LL * high * n, 2LL * groups) * 4;
+  // about eight blocks for each SM, and rows enough in a piece that its sums are few beside it
+  const long long wanted = std::max(1LL, (kSms * 8 + b - 1) / b);
+  w.per = (int)std::min((long long)1 << 24, std::max({(s + wanted - 1) / wanted, (long long)4 * high, std::min(s, (long long)16)}));
+  w.pieces = (int)((s + w.per - 1) / w.per);
+  w.parts = (int)std::min(b * w.pieces, 0x7fffffffLL);
+  return w;
+}
+
+bool wide_at(std::initializer_list<const void*> p, int bytes) {
+  for (const void* q : p)
+    if (!is_aligned(q, bytes)) return false;
+  return true;
+}
+
+template <class T, class F>
+int with_vector(int V, F f) {
+  if constexpr (sizeof(T) == 4) {
+    if (V == 4) return f(std::integral_constant<int, 4>{});
+    if (V == 2) return f(std::integral_constant<int, 2>{});
+  } else {
+    if (V == 8) return f(std::integral_constant<int, 8>{});
+    if (V == 4) return f(std::integral_constant<int, 4>{});
+  }
+  return f(std::integral_constant<int, 1>{});
+}
+
+template <class F>
+int with_type(int type, F f) {
+  if (type == GELIB_F32) return f((float*)nullptr);
+  if (type == GELIB_BF16) return f((__nv_bfloat16*)nullptr);
+  return f((__half*)nullptr);
+}
+
+template <class K>
+int room(const char* fn, K kernel, size_t bytes) {
+  if (bytes > 48 * 1024) GELIB_CUDA_TRY(fn, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  return GELIB_OK;
+}
+
+}  // namespace
+
+int launch_sum_parts(void* gw, void* gb, const float* sums, int parts, int n, int type, cudaStream_t stream) {
+  if (!gw && !gb) return GELIB_OK;
+  return with_type(type, [&](auto* t) -> int {
+    using T = std::remove_pointer_t<decltype(t)>;
+    sum_parts_kernel<T><<<dim3((n + 31) / 32, 2), dim3(32, 32), 0, stream>>>((T*)gw, (T*)gb, sums, parts, n);
+    return launched("sum_parts");
+  });
+}
+
+long long group_norm_workspace(long long b, long long s, int n, int groups, int type, bool backward) {
+  // alignment may only make accesses narrower; what depends on them is bounded by the narrowest
+  long long most = 0;
+  for (int k = 0; k < 3; k++) {
+    const Way w = choose(b, s, n, groups, type, k == 2, k >= 1, backward);
+    long long floats = 0;
+    if (w.way == Way::kTwo) floats = backward ? 2LL * w.parts * n + 2 * b * groups : 2LL * b * w.pieces * groups;
+    else if (backward) floats = 2LL * w.parts * n;
+    most = std::max(most, floats);
+  }
+  return most * 4;
+}
+
+int launch_group_norm(const GroupNormCall& c, cudaStream_t stream) {
+  const char* fn = c.gy ? "group_norm_back" : "group_norm";
+  const bool back = c.gy != nullptr;
+  const Way w = choose(c.b, c.s, c.n, c.groups, c.type, wide_at({c.x, c.w, c.bias, c.gy, c.y}, 16), wide_at({c.x, c.w, c.bias, c.gy, c.y}, 8), back);
+  Norm a = {c.x, c.w, c.bias, c.gy, c.y, c.mean, c.rstd, c.workspace, c.b, c.s, c.n, c.groups, c.n / c.groups, c.eps, c.act};
+  const bool sums = c.gw || c.gb;
+  if (w.way != Way::kTwo && !sums) a.part = nullptr;
+  const long long samples = w.way == Way::kTwo ? c.b * w.pieces : w.way == Way::kTile ? c.b * w.chunks : (c.b * c.groups + kWarps * (32 / w.lanes) - 1) / (kWarps * (32 / w.lanes));
+  if (samples > 0x7fffffffLL || (back && c.b * c.groups > 0x7fffffffLL)) return fail(GELIB_INVALID, fn, "too many samples");
+  const int st = with_type(c.type, [&](auto* t) -> int {
+    using T = std::remove_pointer_t<decltype(t)>;
+    return with_vector<T>(w.V, [&](auto v) -> int {
+      constexpr int V = decltype(v)::value;
+      int st;
+      if (w.way == Way::kRow) {
+        if (!back) {
+          auto kernel = w.K == 1 ? row_fwd_kernel<T, V, 1> : row_fwd_kernel<T, V, 4>;
+          kernel<<<(unsigned)samples, kThreads, 0, stream>>>(a, w.lanes);
+        } else {
+          auto kernel = w.K == 1 ? row_bwd_kernel<T, V, 1> : row_bwd_kernel<T, V, 4>;
+          const int per = 32 / w.lanes;
+          kernel<<<dim3((c.groups + per - 1) / per, w.parts), kThreads, 0, stream>>>(a, w.lanes, w.parts);
+        }
+        return launched(fn);
+      }
+      if (w.way == Way::kTile) {
+        if (!back) {
+          if ((st = room(fn, tile_fwd_kernel<T, V>, w.shared)) != GELIB_OK) return st;
+          tile_fwd_kernel<T, V><<<(unsigned)samples, kThreads, w.shared, stream>>>(a, w.gpc, w.chunks);
+        } else {
+          if ((st = room(fn, tile_bwd_kernel<T, V>, w.shared)) != GELIB_OK) return st;
+          tile_bwd_kernel<T, V><<<dim3(w.chunks, w.parts), kThreads, w.shared, stream>>>(a, w.gpc, w.parts);
+        }
+        return launched(fn);
+      }
+      if (w.shared > (size_t)kSharedLimit) return fail(GELIB_INVALID, fn, "too many channels");  // not up to GELIB_NORM_MAX_CHANNELS
+      if (!back) {
+        if ((st = room(fn, piece_stats_kernel<T, V>, w.shared)) != GELIB_OK) return st;
+        piece_stats_kernel<T, V><<<(unsigned)samples, kThreads, w.shared, stream>>>(a, w.pieces, w.per);
+        if ((st = launched(fn)) != GELIB_OK) return st;
+        const size_t shared = 2ULL * c.groups * 4;
+        if ((st = room(fn, piece_apply_kernel<T, V>, shared)) != GELIB_OK) return st;
+        piece_apply_kernel<T, V><<<(unsigned)samples, kThreads, shared, stream>>>(a, w.pieces, w.per);
+        return launched(fn);
+      }
+      if ((st = room(fn, piece_back_sums_kernel<T, V>, w.shared)) != GELIB_OK) return st;
+      piece_back_sums_kernel<T, V><<<(unsigned)samples, kThreads, w.shared, stream>>>(a, w.pieces, w.per);
+      if ((st = launched(fn)) != GELIB_OK) return st;
+      if (!a.y) return GELIB_OK;
+      float* means = c.workspace + 2LL * w.parts * c.n;
+      piece_back_groups_kernel<T><<<(unsigned)(c.b * c.groups), kThreads, 0, stream>>>(a, w.pieces, means);
+      if ((st = launched(fn)) != GELIB_OK) return st;
+      piece_back_apply_kernel<T, V><<<(unsigned)samples, kThreads, 0, stream>>>(a, w.pieces, w.per, means);
+      return launched(fn);
+    });
+  });
+  if (st != GELIB_OK || !back) return st;
+  return launch_sum_parts(c.gw, c.gb, c.workspace, w.parts, c.n, c.type, stream);
+}
+
+}  // namespace gelib_b200

@@ -1,7 +1,9 @@
 // extern "C" entry points of the readout and the training step: argument checks, then the kernels.  No exception passes them.
+#include <algorithm>
 #include <cmath>
 #include <exception>
 
+#include "norm.h"
 #include "plan.h"
 #include "readout.h"
 
@@ -18,6 +20,21 @@ int guarded(const char* fn, F f) {
   } catch (...) {
     return fail(GELIB_INVALID, fn, "unknown error");
   }
+}
+
+int check_norm(const char* fn, long long b, long long s, int n, int groups, double eps, int act, int type) {
+  if (b < 0 || s < 0 || n < 0 || groups < 1 || n % groups) return fail(GELIB_INVALID, fn, "negative size, or channels that do not divide into the groups");
+  if (!known_activation(act) || !known_type(type)) return fail(GELIB_INVALID, fn, "unknown activation or type");
+  if (!(eps >= 0)) return fail(GELIB_INVALID, fn, "eps is negative");
+  if (n > GELIB_NORM_MAX_CHANNELS) return fail(GELIB_INVALID, fn, "more than GELIB_NORM_MAX_CHANNELS channels");
+  if (n && (b > (1LL << 40) / n || s > (1LL << 50) / n / std::max(b, 1LL))) return fail(GELIB_INVALID, fn, "too many elements");
+  return GELIB_OK;
+}
+
+bool all_aligned(int bytes, std::initializer_list<const void*> p) {
+  for (const void* q : p)
+    if (!is_aligned(q, bytes)) return false;
+  return true;
 }
 
 }  // namespace
@@ -54,6 +71,48 @@ int gelib_block8_values(void* out, const void* codes, const float* scale, long l
     if (n < 0 || (n && (!out || !codes || !scale))) return fail(GELIB_INVALID, fn, "negative size or null pointer");
     if (!is_aligned(out, 2) || !is_aligned(scale, 4)) return fail(GELIB_INVALID, fn, "data pointer not aligned to its type");
     return launch_block8_values(out, codes, scale, n, (cudaStream_t)stream);
+  });
+}
+
+long long gelib_group_norm_workspace(long long b, long long s, int n, int groups, int type, int backward) {
+  if (b <= 0 || s <= 0 || n <= 0 || groups < 1 || n % groups || !known_type(type) || n > GELIB_NORM_MAX_CHANNELS) return 0;
+  return group_norm_workspace(b, s, n, groups, type, backward != 0);
+}
+
+int gelib_group_norm(void* y, float* mean, float* rstd, const void* x, const void* weight, const void* bias, long long b, long long s, int n,
+                     int groups, double eps, int act, int type, void* workspace, void* stream) {
+  static const char* fn = "group_norm";
+  return guarded(fn, [&]() -> int {
+    int st = check_norm(fn, b, s, n, groups, eps, act, type);
+    if (st != GELIB_OK) return st;
+    if (b == 0 || s == 0 || n == 0) return GELIB_OK;
+    if (!x || !y || !mean != !rstd) return fail(GELIB_INVALID, fn, "null pointer");
+    if (!workspace && group_norm_workspace(b, s, n, groups, type, false) > 0) return fail(GELIB_INVALID, fn, "no workspace");
+    if (!all_aligned(type_bytes(type), {x, y, weight, bias}) || !all_aligned(4, {mean, rstd, workspace}))
+      return fail(GELIB_INVALID, fn, "data pointer not aligned to its type");
+    return launch_group_norm({y, mean, rstd, x, weight, bias, nullptr, nullptr, nullptr, b, s, n, groups, (float)eps, act, type, (float*)workspace},
+                             (cudaStream_t)stream);
+  });
+}
+
+int gelib_group_norm_back(void* gx, void* gw, void* gb, const void* gy, const void* x, const void* weight, const void* bias, const float* mean,
+                          const float* rstd, long long b, long long s, int n, int groups, int act, int type, void* workspace, void* stream) {
+  static const char* fn = "group_norm_back";
+  return guarded(fn, [&]() -> int {
+    int st = check_norm(fn, b, s, n, groups, 0, act, type);
+    if (st != GELIB_OK) return st;
+    if (n == 0 || (!gx && !gw && !gb)) return GELIB_OK;
+    if (b == 0 || s == 0) {  // sums of nothing
+      for (void* g : {gw, gb})
+        if (g) GELIB_CUDA_TRY(fn, cudaMemsetAsync(g, 0, (size_t)n * type_bytes(type), (cudaStream_t)stream));
+      return GELIB_OK;
+    }
+    if (!x || !gy || !mean || !rstd) return fail(GELIB_INVALID, fn, "null pointer");
+    if (!workspace && group_norm_workspace(b, s, n, groups, type, true) > 0) return fail(GELIB_INVALID, fn, "no workspace");
+    if (!all_aligned(type_bytes(type), {x, gy, gx, gw, gb, weight, bias}) || !all_aligned(4, {mean, rstd, workspace}))
+      return fail(GELIB_INVALID, fn, "data pointer not aligned to its type");
+    return launch_group_norm({gx, (float*)mean, (float*)rstd, x, weight, bias, gy, gw, gb, b, s, n, groups, 0.f, act, type, (float*)workspace},
+                             (cudaStream_t)stream);
   });
 }
 

@@ -254,6 +254,16 @@ int gelib_adamw_step(int count, const gelib_adamw_tensor* tensors, const gelib_a
 /* out[i] = codes[i] * scale[i / 256], bfloat16 (exact): what an 8-bit state stands for (of v: its root). */
 int gelib_block8_values(void* out, const void* codes, const float* scale, long long n, void* stream);
 
+/* y = act(xh w + bias) with xh = (x - mean) / sqrt(var + eps): x and y dense (b, s, n) of `type`, weight and bias (n) of it or NULL (1 and
+ * 0); mean and variance of every b over the s positions and the n / groups channels of a group, in float.  mean, rstd: (b, groups)
+ * floats for the backward call, or NULL.  The backward call gives gx, gw and gb (overwritten; any may be NULL). */
+#define GELIB_NORM_MAX_CHANNELS 16384
+long long gelib_group_norm_workspace(long long b, long long s, int n, int groups, int type, int backward);
+int gelib_group_norm(void* y, float* mean, float* rstd, const void* x, const void* weight, const void* bias, long long b, long long s, int n,
+                     int groups, double eps, int act, int type, void* workspace, void* stream);
+int gelib_group_norm_back(void* gx, void* gw, void* gb, const void* gy, const void* x, const void* weight, const void* bias, const float* mean,
+                          const float* rstd, long long b, long long s, int n, int groups, int act, int type, void* workspace, void* stream);
+
 /* ---- introspection ------------------------------------------------------------------------------- */
 
 /* Number of kernels this library has launched in the calling process (all threads, all devices). */
