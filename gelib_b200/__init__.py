@@ -16,7 +16,7 @@ from .SO3part import (SO3part, SO3partArr, SO3part_CGproductFn, SO3part_DiagCGpr
 from .SO3vec import (SO3vec, SO3vecArr, SO3vec_SpharmCGproductFn, SO3vec_CGproductFn, SO3vec_DiagCGproductFn, SO3vecArr_CGproductFn,
                      SO3vecArr_DiagCGproductFn, MakeZeroSO3parts, MakeZeroSO3partArrs)
 from .SO3weights import SO3weights, SO3linear
-from .readout import GroupNorm, GroupNormFn, group_norm
+from .readout import GroupNorm, GroupNormFn, Linear, LinearFn, group_norm, linear
 from .adamw import AdamW, adamw_step, block8_values
 from .O3 import (O3element, O3irrep, O3type, O3part, O3vec, O3part_CGproductFn, O3part_DiagCGproductFn, O3vec_CGproductFn,
                  O3vec_DiagCGproductFn)

@@ -41,6 +41,13 @@ class AdamwOptions(ctypes.Structure):
     _fields_ += [("step", ctypes.c_int64), ("seed", ctypes.c_uint64), ("grad_scale", ctypes.c_void_p), ("state_bits", ctypes.c_int)]
 
 
+class LinearArgs(ctypes.Structure):
+    """``gelib_linear_args``"""
+    _fields_ = [(name, ctypes.c_void_p) for name in ("x", "w", "bias", "residual", "gy", "y", "z", "gx", "gw", "gb")]
+    _fields_ += [("m", ctypes.c_int64), ("k", ctypes.c_int), ("n", ctypes.c_int), ("ldx", ctypes.c_int64), ("ldw", ctypes.c_int64)]
+    _fields_ += [(name, ctypes.c_int) for name in ("w_transposed", "act", "type")]
+
+
 _P5 = ctypes.POINTER(Tensor5)
 _lib = None
 
@@ -97,6 +104,9 @@ SYMBOLS = {
     "gelib_group_norm": (ctypes.c_int, [ctypes.c_void_p] * 6 + [ctypes.c_longlong] * 2 + [ctypes.c_int] * 2 + [ctypes.c_double]
                          + [ctypes.c_int] * 2 + [ctypes.c_void_p] * 2),
     "gelib_group_norm_back": (ctypes.c_int, [ctypes.c_void_p] * 9 + [ctypes.c_longlong] * 2 + [ctypes.c_int] * 4 + [ctypes.c_void_p] * 2),
+    "gelib_linear_workspace": (ctypes.c_longlong, [ctypes.POINTER(LinearArgs), ctypes.c_int]),
+    "gelib_linear": (ctypes.c_int, [ctypes.POINTER(LinearArgs), ctypes.c_void_p, ctypes.c_void_p]),
+    "gelib_linear_back": (ctypes.c_int, [ctypes.POINTER(LinearArgs), ctypes.c_void_p, ctypes.c_void_p]),
     "gelib_kernel_launch_count": (ctypes.c_longlong, []),
     "gelib_set_option": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_char_p]),
     "gelib_async_status": (ctypes.c_int, []),

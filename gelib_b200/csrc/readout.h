@@ -90,8 +90,9 @@ __device__ __forceinline__ void activate_back(float (&g)[V], const float (&x)[V]
   if (act == GELIB_ACT_NONE) return;
 #pragma unroll
   for (int k = 0; k < V; k++) {
-    const float z = x[k];
-    if (act == GELIB_ACT_RELU) g[k] = z > 0.f ? g[k] : 0.f;
+    // beyond +-128 the derivatives are 1 and 0 to the last bit, and their terms are no longer products of 0 and infinity
+    const float z = x[k] < -128.f ? -128.f : x[k] > 128.f ? 128.f : x[k];
+    if (act == GELIB_ACT_RELU) g[k] = z > 0.f ? g[k] : z != z ? z : 0.f;
     else if (act == GELIB_ACT_SILU) {
       const float q = logistic(z);
       g[k] *= q * (1.f + z * (1.f - q));

@@ -3,6 +3,7 @@
 #include <cmath>
 #include <exception>
 
+#include "linear.h"
 #include "norm.h"
 #include "plan.h"
 #include "readout.h"
@@ -28,6 +29,22 @@ int check_norm(const char* fn, long long b, long long s, int n, int groups, doub
   if (!(eps >= 0)) return fail(GELIB_INVALID, fn, "eps is negative");
   if (n > GELIB_NORM_MAX_CHANNELS) return fail(GELIB_INVALID, fn, "more than GELIB_NORM_MAX_CHANNELS channels");
   if (n && (b > (1LL << 40) / n || s > (1LL << 50) / n / std::max(b, 1LL))) return fail(GELIB_INVALID, fn, "too many elements");
+  return GELIB_OK;
+}
+
+int check_linear(const char* fn, const gelib_linear_args* p, bool back) {
+  if (!p) return fail(GELIB_INVALID, fn, "null pointer");
+  if (p->m < 0 || p->k < 0 || p->n < 0) return fail(GELIB_INVALID, fn, "negative size");
+  if (!known_activation(p->act) || !known_type(p->type)) return fail(GELIB_INVALID, fn, "unknown activation or type");
+  if (p->ldx < p->k || p->ldw < (p->w_transposed ? p->k : p->n)) return fail(GELIB_INVALID, fn, "rows overlap");
+  if (p->m > 0x7fffffffLL) return fail(GELIB_INVALID, fn, "too many rows");
+  const int width = type_bytes(p->type);
+  for (const void* q : {p->x, p->w, p->bias, p->residual, p->gy, (const void*)p->y, (const void*)p->z, (const void*)p->gx, (const void*)p->gw, (const void*)p->gb})
+    if (!is_aligned(q, width)) return fail(GELIB_INVALID, fn, "data pointer not aligned to its type");
+  if (p->m && p->n) {
+    if (p->k && (!p->x || !p->w)) return fail(GELIB_INVALID, fn, "null pointer");
+    if (back ? !p->gy || (p->act != GELIB_ACT_NONE && !p->z) : !p->y) return fail(GELIB_INVALID, fn, "null pointer");
+  }
   return GELIB_OK;
 }
 
@@ -113,6 +130,38 @@ int gelib_group_norm_back(void* gx, void* gw, void* gb, const void* gy, const vo
       return fail(GELIB_INVALID, fn, "data pointer not aligned to its type");
     return launch_group_norm({gx, (float*)mean, (float*)rstd, x, weight, bias, gy, gw, gb, b, s, n, groups, 0.f, act, type, (float*)workspace},
                              (cudaStream_t)stream);
+  });
+}
+
+long long gelib_linear_workspace(const gelib_linear_args* p, int backward) {
+  long long bytes = 0;
+  guarded("linear_workspace", [&]() -> int {
+    const int st = check_linear("linear_workspace", p, backward != 0);
+    if (st == GELIB_OK) bytes = linear_workspace(*p, backward != 0);
+    return st;
+  });
+  return bytes;
+}
+
+int gelib_linear(const gelib_linear_args* p, void* workspace, void* stream) {
+  static const char* fn = "linear";
+  return guarded(fn, [&]() -> int {
+    int st = check_linear(fn, p, false);
+    if (st != GELIB_OK || p->m == 0 || p->n == 0) return st;
+    if (!workspace && linear_workspace(*p, false) > 0) return fail(GELIB_INVALID, fn, "no workspace");
+    if (!is_aligned(workspace, 256)) return fail(GELIB_INVALID, fn, "the workspace is not 256-byte aligned");
+    return launch_linear(*p, workspace, (cudaStream_t)stream);
+  });
+}
+
+int gelib_linear_back(const gelib_linear_args* p, void* workspace, void* stream) {
+  static const char* fn = "linear_back";
+  return guarded(fn, [&]() -> int {
+    int st = check_linear(fn, p, true);
+    if (st != GELIB_OK) return st;
+    if (!workspace && linear_workspace(*p, true) > 0) return fail(GELIB_INVALID, fn, "no workspace");
+    if (!is_aligned(workspace, 256)) return fail(GELIB_INVALID, fn, "the workspace is not 256-byte aligned");
+    return launch_linear_back(*p, workspace, (cudaStream_t)stream);
   });
 }
 

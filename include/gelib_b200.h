@@ -264,6 +264,24 @@ int gelib_group_norm(void* y, float* mean, float* rstd, const void* x, const voi
 int gelib_group_norm_back(void* gx, void* gw, void* gb, const void* gy, const void* x, const void* weight, const void* bias, const float* mean,
                           const float* rstd, long long b, long long s, int n, int groups, int act, int type, void* workspace, void* stream);
 
+/* A dense layer, z = x w + bias, y = act(z) + residual, and its gradients.  x (m, k) with rows of ldx elements; w (k, n) with rows of
+ * ldw elements, or with w_transposed (n, k); bias (n); residual, y, z, gy dense (m, n); all of `type`.
+ * Forward: y, and z where it is not NULL (a backward call with an activation needs it; in float16 it is held within that type's range).
+ * Backward: of gy the gradients gx dense (m, k), gw dense and in w's own layout (k, n) or (n, k), gb (n); each may be NULL.
+ * bias, residual may be NULL.  Sums are float; float operands are multiplied as three bfloat16 parts each, which keeps float's precision
+ * (an infinity among them gives infinity or NaN). */
+typedef struct gelib_linear_args {
+  const void *x, *w, *bias, *residual, *gy;
+  void *y, *z, *gx, *gw, *gb;
+  int64_t m;
+  int k, n;
+  int64_t ldx, ldw;
+  int w_transposed, act, type;
+} gelib_linear_args;
+long long gelib_linear_workspace(const gelib_linear_args* args, int backward);
+int gelib_linear(const gelib_linear_args* args, void* workspace, void* stream);
+int gelib_linear_back(const gelib_linear_args* args, void* workspace, void* stream);
+
 /* ---- introspection ------------------------------------------------------------------------------- */
 
 /* Number of kernels this library has launched in the calling process (all threads, all devices). */
