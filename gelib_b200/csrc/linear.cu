@@ -8,8 +8,9 @@
 // in a fixed order.
 #include <algorithm>
 
-#include "linear.h"
 #include "readout.h"
+#include "linear.h"
+#include "plan.h"
 
 namespace gelib_b200 {
 
@@ -17,6 +18,13 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kSms = 148;
+
+// Element (i, k) of an operand at base[i * si + k * sk], i the row of A or the column of B.
+struct Strided {
+  const void* base;
+  long long si, sk;
+};
+Strided strided(const Operand& o) { return {o.s.base, o.by_sum ? 1 : o.s.ld, o.by_sum ? o.s.ld : 1}; }
 
 // ---- simple product: 64 x 64 tiles, 4 x 4 sums per thread, any strides -------------------------------------------------------
 
@@ -26,11 +34,7 @@ template <class T>
 __device__ __forceinline__ void finish(const Epilogue& e, long long at, int col, float d) {
   float z[1] = {d};
   if (e.bias) z[0] += to_float(static_cast<const T*>(e.bias)[col]);
-  if (e.z) {
-    float q = z[0];
-    if constexpr (std::is_same_v<T, __half>) q = q < -65504.f ? -65504.f : q > 65504.f ? 65504.f : q;   // an infinity would have no derivative
-    static_cast<T*>(e.z)[at] = from_float<T>(q);
-  }
+  if (e.z) static_cast<T*>(e.z)[at] = held<T>(z[0]);
   activate(z, e.act);
   if (e.residual) z[0] += to_float(static_cast<const T*>(e.residual)[at]);
   static_cast<T*>(e.y)[at] = from_float<T>(z[0]);
@@ -38,31 +42,31 @@ __device__ __forceinline__ void finish(const Epilogue& e, long long at, int col,
 
 // Block (x, y): tile, columns fastest, and part y of the sum.  part: partial sums (parts, M, N), or null.
 template <class T>
-__global__ void __launch_bounds__(kThreads) simple_gemm_kernel(Gemm g, float* part, long long depth) {
+__global__ void __launch_bounds__(kThreads) simple_gemm_kernel(Strided a, Strided b, Gemm g, float* part, long long depth) {
   __shared__ float sa[kDepth][kTile + 4], sb[kDepth][kTile + 4];
   const long long across = (g.N + kTile - 1) / kTile, m0 = blockIdx.x / across * kTile, n0 = blockIdx.x % across * kTile;
   const long long k0 = (long long)blockIdx.y * depth, k1 = min(g.K, k0 + depth);
   const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
   float d[4][4] = {};
-  const T *A = static_cast<const T*>(g.a.base), *B = static_cast<const T*>(g.b.base);
+  const T *A = static_cast<const T*>(a.base), *B = static_cast<const T*>(b.base);
   for (long long k = k0; k < k1; k += kDepth) {
     for (int e = threadIdx.x; e < kTile * kDepth; e += kThreads) {
       // the index that is dense in memory runs fastest over the threads
-      const int ia = g.a.sk == 1 ? e / kDepth : e % kTile, ka = g.a.sk == 1 ? e % kDepth : e / kTile;
-      const int ib = g.b.sk == 1 ? e / kDepth : e % kTile, kb = g.b.sk == 1 ? e % kDepth : e / kTile;
-      sa[ka][ia] = m0 + ia < g.M && k + ka < k1 ? to_float(A[(m0 + ia) * g.a.si + (k + ka) * g.a.sk]) : 0.f;
-      sb[kb][ib] = n0 + ib < g.N && k + kb < k1 ? to_float(B[(n0 + ib) * g.b.si + (k + kb) * g.b.sk]) : 0.f;
+      const int ia = a.sk == 1 ? e / kDepth : e % kTile, ka = a.sk == 1 ? e % kDepth : e / kTile;
+      const int ib = b.sk == 1 ? e / kDepth : e % kTile, kb = b.sk == 1 ? e % kDepth : e / kTile;
+      sa[ka][ia] = m0 + ia < g.M && k + ka < k1 ? to_float(A[(m0 + ia) * a.si + (k + ka) * a.sk]) : 0.f;
+      sb[kb][ib] = n0 + ib < g.N && k + kb < k1 ? to_float(B[(n0 + ib) * b.si + (k + kb) * b.sk]) : 0.f;
     }
     __syncthreads();
 #pragma unroll
     for (int q = 0; q < kDepth; q++) {
-      float a[4], b[4];
+      float u[4], v[4];
 #pragma unroll
-      for (int i = 0; i < 4; i++) a[i] = sa[q][ty * 4 + i], b[i] = sb[q][tx * 4 + i];
+      for (int i = 0; i < 4; i++) u[i] = sa[q][ty * 4 + i], v[i] = sb[q][tx * 4 + i];
 #pragma unroll
       for (int i = 0; i < 4; i++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) d[i][j] += a[i] * b[j];
+        for (int j = 0; j < 4; j++) d[i][j] += u[i] * v[j];
     }
     __syncthreads();
   }
@@ -100,35 +104,33 @@ Split split_of(long long M, long long N, long long K) {
   parts = std::max(1LL, depth ? (K + depth - 1) / depth : 1);
   return {(int)parts, depth};
 }
-long long gemm_workspace(long long M, long long N, long long K) {
+long long simple_workspace(long long M, long long N, long long K) {
   const Split s = split_of(M, N, K);
   return s.parts > 1 ? s.parts * M * N * 4 : 0;
 }
 
 template <class T>
-int launch_simple(const Gemm& g, float* part, const Split& s, dim3 grid, cudaStream_t stream) {
-  simple_gemm_kernel<T><<<grid, kThreads, 0, stream>>>(g, part, s.depth);
+int launch_simple_as(const Gemm& g, float* part, const Split& s, unsigned tiles, cudaStream_t stream) {
+  simple_gemm_kernel<T><<<dim3(tiles, s.parts), kThreads, 0, stream>>>(strided(g.a), strided(g.b), g, part, s.depth);
   const int st = launched("linear");
-  if (st != GELIB_OK || !part) return st;
-  join_kernel<T><<<(unsigned)std::min((g.M * g.N + kThreads - 1) / kThreads, 1LL << 20), kThreads, 0, stream>>>(g.e, part, s.parts, g.M, (int)g.N);
-  return launched("linear");
+  return st != GELIB_OK || !part ? st : launch_join(g, part, s.parts, stream);
 }
 
-int launch_gemm(const Gemm& g, void* workspace, cudaStream_t stream) {
+int launch_simple(const Gemm& g, void* workspace, cudaStream_t stream) {
   const Split s = split_of(g.M, g.N, g.K);
   float* part = s.parts > 1 ? (float*)workspace : nullptr;
   const long long tiles = ((g.N + kTile - 1) / kTile) * ((g.M + kTile - 1) / kTile);
   if (tiles > 0x7fffffffLL) return fail(GELIB_INVALID, "linear", "too many elements");
-  const dim3 grid((unsigned)tiles, s.parts);
-  return g.type == GELIB_F32 ? launch_simple<float>(g, part, s, grid, stream)
-         : g.type == GELIB_BF16 ? launch_simple<__nv_bfloat16>(g, part, s, grid, stream) : launch_simple<__half>(g, part, s, grid, stream);
+  return g.type == GELIB_F32 ? launch_simple_as<float>(g, part, s, (unsigned)tiles, stream)
+         : g.type == GELIB_BF16 ? launch_simple_as<__nv_bfloat16>(g, part, s, (unsigned)tiles, stream)
+                                : launch_simple_as<__half>(g, part, s, (unsigned)tiles, stream);
 }
 
 // ---- gz = gy act'(z) and its column sums ------------------------------------------------------------------------------------------
 
-// Block (x, y): `wide` accesses of V columns, piece y of the rows.  gz may be null (no activation: gy itself), sums too.
+// Block (x, y): `wide` accesses of V columns, piece y of the rows.  gz.base may be null (not wanted), sums too.
 template <class T, int V>
-__global__ void __launch_bounds__(kThreads) act_back_kernel(T* gz, float* sums, const T* gy, const T* z, long long M, int N, int act, int wide, long long per) {
+__global__ void __launch_bounds__(kThreads) act_back_kernel(Stored gz, float* sums, const T* gy, const T* z, long long M, int N, int act, int wide, long long per) {
   __shared__ float chan[kThreads * V];
   const int tx = threadIdx.x % wide, ty = threadIdx.x / wide, high = kThreads / wide;
   const int c = ((int)blockIdx.x * wide + tx) * V;
@@ -144,7 +146,22 @@ __global__ void __launch_bounds__(kThreads) act_back_kernel(T* gz, float* sums, 
         float q[V];
         load_vec<T, V>(z + r * N + c, q);
         activate_back(g, q, act);
-        if (gz) store_vec<T, V>(gz + r * N + c, g);
+      }
+      if (gz.base) {
+        if (sizeof(T) == 4 && gz.planes == 3) {
+          union { __nv_bfloat16 t[V]; typename Raw<V * 2>::type raw; } w[3];
+#pragma unroll
+          for (int j = 0; j < V; j++) {
+            __nv_bfloat16 p[3];
+            split3(g[j], p);
+            w[0].t[j] = p[0], w[1].t[j] = p[1], w[2].t[j] = p[2];
+          }
+#pragma unroll
+          for (int i = 0; i < 3; i++)
+            *reinterpret_cast<typename Raw<V * 2>::type*>((__nv_bfloat16*)gz.base + i * gz.plane + r * gz.ld + c) = w[i].raw;
+        } else {
+          store_vec<T, V>((T*)gz.base + r * gz.ld + c, g);
+        }
       }
 #pragma unroll
       for (int j = 0; j < V; j++) s[j] += g[j];
@@ -179,33 +196,79 @@ Pieces pieces_of(long long M, int N, int type, bool aligned) {
 }
 
 template <class T>
-int launch_act_back(void* gz, float* sums, const gelib_linear_args& p, const Pieces& q, cudaStream_t stream) {
+int launch_act_back(const Stored& gz, float* sums, const gelib_linear_args& p, const Pieces& q, cudaStream_t stream) {
   constexpr int kWide = 16 / sizeof(T);
   const auto kernel = q.V > 1 ? act_back_kernel<T, kWide> : act_back_kernel<T, 1>;
-  kernel<<<dim3(q.chunks, q.parts), kThreads, 0, stream>>>((T*)gz, sums, (const T*)p.gy, (const T*)p.z, p.m, p.n, p.act, q.wide, q.per);
+  kernel<<<dim3(q.chunks, q.parts), kThreads, 0, stream>>>(gz, sums, (const T*)p.gy, (const T*)p.z, p.m, p.n, p.act, q.wide, q.per);
   return launched("linear_back");
 }
 
 long long up(long long bytes) { return (bytes + 255) / 256 * 256; }
 
+// Which product a layer's call takes: the tensor cores from `kTcWork` multiplications on, which is where their operands' copies (float, or
+// rows off their 16-byte boundaries) and a longer start are made up for.
+constexpr double kTcWork = 4e6;
+bool takes_tc(long long m, long long k, long long n) { return k > 0 && m > 16 && (double)m * k * n >= kTcWork && device_has_tcgen05(); }
+
+Stored x_of(const gelib_linear_args& p) { return {p.x, p.m, p.k, p.ldx, 0, 1}; }
+Stored w_of(const gelib_linear_args& p) { return {p.w, p.w_transposed ? p.n : p.k, p.w_transposed ? p.k : p.n, p.ldw, 0, 1}; }
+
+// Bytes that an operand's copy takes, 0 where it is used as it lies.
+long long copy_bytes(const Stored& s, int type) { return tc_ready(s, type) ? 0 : up(planes_bytes(s.rows, s.cols, type)); }
+
+long long sums_bytes(const gelib_linear_args& p) {
+  return up(4LL * p.n * std::max(pieces_of(p.m, p.n, p.type, false).parts, pieces_of(p.m, p.n, p.type, true).parts));
+}
+
+// Puts copies of those that need one behind each other at `at`, by one launch.
+int ready(Stored** of, int count, int type, char*& at, cudaStream_t stream) {
+  Stored from[3], to[3];
+  int n = 0;
+  for (int i = 0; i < count; i++) {
+    if (tc_ready(*of[i], type)) continue;
+    from[n] = *of[i];
+    to[n] = planes_of(*of[i], type, at);
+    at += up(planes_bytes(of[i]->rows, of[i]->cols, type));
+    *of[i] = to[n++];
+  }
+  return launch_planes(from, to, n, type, stream);
+}
+
 }  // namespace
+
+int launch_join(const Gemm& g, const float* part, int parts, cudaStream_t stream) {
+  const unsigned blocks = (unsigned)std::min((g.M * g.N + kThreads - 1) / kThreads, 1LL << 20);
+  if (g.type == GELIB_F32) join_kernel<float><<<blocks, kThreads, 0, stream>>>(g.e, part, parts, g.M, (int)g.N);
+  else if (g.type == GELIB_BF16) join_kernel<__nv_bfloat16><<<blocks, kThreads, 0, stream>>>(g.e, part, parts, g.M, (int)g.N);
+  else join_kernel<__half><<<blocks, kThreads, 0, stream>>>(g.e, part, parts, g.M, (int)g.N);
+  return launched("linear");
+}
 
 long long linear_workspace(const gelib_linear_args& p, bool backward) {
   if (p.m == 0 || p.n == 0) return 0;
-  if (!backward) return gemm_workspace(p.m, p.n, p.k);
-  long long bytes = 0;
-  if (p.act != GELIB_ACT_NONE) bytes += up(p.m * p.n * type_bytes(p.type));
-  bytes += up(4LL * p.n * std::max(pieces_of(p.m, p.n, p.type, false).parts, pieces_of(p.m, p.n, p.type, true).parts));
-  return bytes + std::max(gemm_workspace(p.m, p.k, p.n), std::max(gemm_workspace(p.k, p.n, p.m), gemm_workspace(p.n, p.k, p.m)));
+  const bool tc = takes_tc(p.m, p.k, p.n);
+  const auto gemm = [&](long long M, long long N, long long K) { return tc ? tc_gemm_workspace(M, N, K, p.type) : simple_workspace(M, N, K); };
+  const long long copies = tc ? copy_bytes(x_of(p), p.type) + copy_bytes(w_of(p), p.type) : 0;
+  if (!backward) return copies + gemm(p.m, p.n, p.k);
+  const long long gz = up(planes_bytes(p.m, p.n, p.type));
+  return gz + copies + sums_bytes(p) + std::max(gemm(p.m, p.k, p.n), p.w_transposed ? gemm(p.n, p.k, p.m) : gemm(p.k, p.n, p.m));
 }
 
 int launch_linear(const gelib_linear_args& p, void* workspace, cudaStream_t stream) {
   Gemm g;
-  g.a = {p.x, p.ldx, 1};
-  g.b = {p.w, p.w_transposed ? p.ldw : 1, p.w_transposed ? 1 : p.ldw};
+  Stored x = x_of(p), w = w_of(p);
+  const bool tc = takes_tc(p.m, p.k, p.n);
+  char* at = (char*)workspace;
+  if (tc) {
+    Stored* both[2] = {&x, &w};
+    const int st = ready(both, 2, p.type, at, stream);
+    if (st != GELIB_OK) return st;
+  }
+  g.a = {x, false};
+  g.b = {w, !p.w_transposed};
   g.e = {p.y, p.z, p.bias, p.residual, p.act};
   g.M = p.m, g.N = p.n, g.K = p.k, g.type = p.type;
-  return launch_gemm(g, workspace, stream);
+  return tc ? launch_tc_gemm(g, at, stream) : launch_simple(g, at, stream);
 }
 
 int launch_linear_back(const gelib_linear_args& p, void* workspace, cudaStream_t stream) {
@@ -217,49 +280,52 @@ int launch_linear_back(const gelib_linear_args& p, void* workspace, cudaStream_t
     if (p.gb && p.n) GELIB_CUDA_TRY(fn, cudaMemsetAsync(p.gb, 0, (size_t)p.n * width, stream));
     return GELIB_OK;
   }
+  const bool tc = takes_tc(p.m, p.k, p.n), products = (p.gx || p.gw) && p.k;
   char* at = (char*)workspace;
-  const void* gz = p.gy;
-  const bool act = p.act != GELIB_ACT_NONE;
-  if (act) {
-    gz = at;
-    at += up(p.m * p.n * width);
-  }
   float* sums = (float*)at;
-  const Pieces q = pieces_of(p.m, p.n, p.type, is_aligned(p.gy, 16) && is_aligned(p.z, 16));
-  at += up(4LL * p.n * std::max(pieces_of(p.m, p.n, p.type, false).parts, pieces_of(p.m, p.n, p.type, true).parts));
-  if (act || p.gb) {
-    void* out = act ? workspace : nullptr;
+  at += sums_bytes(p);
+  // gz: gy as it lies, or written (as the tensor cores want it) by the pass that also sums its columns
+  Stored gz = {p.gy, p.m, p.n, p.n, 0, 1}, out = {nullptr, 0, 0, 0, 0, 0};
+  if (products && (p.act != GELIB_ACT_NONE || (tc && !tc_ready(gz, p.type)))) {
+    out = tc ? planes_of(gz, p.type, at) : Stored{at, p.m, p.n, p.n, 0, 1};
+    gz = out;
+    at += up(planes_bytes(p.m, p.n, p.type));
+  }
+  int st;
+  if (out.base || p.gb) {
+    const Pieces q = pieces_of(p.m, p.n, p.type, is_aligned(p.gy, 16) && is_aligned(p.z, 16));
     float* s = p.gb ? sums : nullptr;
-    const int st = p.type == GELIB_F32 ? launch_act_back<float>(out, s, p, q, stream)
-                   : p.type == GELIB_BF16 ? launch_act_back<__nv_bfloat16>(out, s, p, q, stream) : launch_act_back<__half>(out, s, p, q, stream);
+    st = p.type == GELIB_F32 ? launch_act_back<float>(out, s, p, q, stream)
+         : p.type == GELIB_BF16 ? launch_act_back<__nv_bfloat16>(out, s, p, q, stream) : launch_act_back<__half>(out, s, p, q, stream);
     if (st != GELIB_OK) return st;
-    if (p.gb) {
-      const int s2 = launch_sum_parts(p.gb, nullptr, sums, q.parts, p.n, p.type, stream);
-      if (s2 != GELIB_OK) return s2;
-    }
+    if (p.gb && (st = launch_sum_parts(p.gb, nullptr, sums, q.parts, p.n, p.type, stream)) != GELIB_OK) return st;
+  }
+  if (!products) return GELIB_OK;
+  Stored x = x_of(p), w = w_of(p);
+  if (tc) {
+    Stored* of[2];
+    int n = 0;
+    if (p.gw) of[n++] = &x;
+    if (p.gx) of[n++] = &w;
+    if ((st = ready(of, n, p.type, at, stream)) != GELIB_OK) return st;
   }
   Gemm g;
   g.e = {nullptr, nullptr, nullptr, nullptr, GELIB_ACT_NONE};
   g.type = p.type;
-  if (p.gx && p.k) {
-    g.a = {gz, p.n, 1};
-    g.b = {p.w, p.w_transposed ? 1 : p.ldw, p.w_transposed ? p.ldw : 1};
+  if (p.gx) {
+    g.a = {gz, false};
+    g.b = {w, p.w_transposed != 0};
     g.e.y = p.gx;
     g.M = p.m, g.N = p.k, g.K = p.n;
-    const int st = launch_gemm(g, at, stream);
-    if (st != GELIB_OK) return st;
+    if ((st = tc ? launch_tc_gemm(g, at, stream) : launch_simple(g, at, stream)) != GELIB_OK) return st;
   }
-  if (p.gw && p.k) {
+  if (p.gw) {
     // in w's own layout: x^T gz, or its transpose gz^T x
-    g.a = {p.x, 1, p.ldx};
-    g.b = {gz, 1, p.n};
+    g.a = {p.w_transposed ? gz : x, true};
+    g.b = {p.w_transposed ? x : gz, true};
     g.e.y = p.gw;
-    g.M = p.k, g.N = p.n, g.K = p.m;
-    if (p.w_transposed) {
-      std::swap(g.a, g.b);
-      std::swap(g.M, g.N);
-    }
-    return launch_gemm(g, at, stream);
+    g.M = p.w_transposed ? p.n : p.k, g.N = p.w_transposed ? p.k : p.n, g.K = p.m;
+    if ((st = tc ? launch_tc_gemm(g, at, stream) : launch_simple(g, at, stream)) != GELIB_OK) return st;
   }
   return GELIB_OK;
 }

@@ -1,32 +1,72 @@
-// Dense layers: what the C ABI hands to the kernels, and the matrix product that they are made of.
+// Dense layers: what the C ABI hands to the kernels, and the matrix products that they are made of.
 #pragma once
 #include "common.h"
 
 namespace gelib_b200 {
 
-// One operand of D = A B: element (i, k) at base[i * si + k * sk]; one of the strides is 1 (i: the row of A, the column of B).
-struct Operand {
-  const void* base;
-  long long si, sk;
-};
-
-// What happens to a sum d before it is stored: z = d + bias, y = act(z) + residual; z is stored too where it is asked for.
+// What happens to a sum d before it is stored: z = d + bias, y = act(z) + residual; z is stored too where it is asked for.  y, z, residual are dense.
 struct Epilogue {
   void* y;
-  void* z;                 // or null
+  void* z;                       // or null
   const void *bias, *residual;   // or null
   int act;
+};
+
+// A matrix as it lies in memory: rows of dense columns, `ld` elements apart.  planes 3: a float matrix as the sum of three bfloat16
+// ones, `plane` elements apart (each holds the next eight bits of the significand).
+struct Stored {
+  const void* base;
+  long long rows, cols, ld, plane;
+  int planes;
+};
+
+// One operand of D = A B, M x K or K x N: its rows are the sum's index, or (by_sum false) M's or N's.
+struct Operand {
+  Stored s;
+  bool by_sum;
 };
 
 struct Gemm {
   Operand a, b;
   Epilogue e;
   long long M, N, K;
-  int type;
+  int type;      // of the result, and of the operands that have one plane
 };
+
+// Tensor-core products (gemm_tc.cu).  Operands must be `tc_ready`: three planes of a float matrix, or 16-bit, on 16-byte
+// boundaries; launch_planes makes such copies.
+bool tc_ready(const Stored& s, int type);
+Stored planes_of(const Stored& s, int type, void* memory);                // where launch_planes will put it
+long long planes_bytes(long long rows, long long cols, int type);
+int launch_planes(const Stored* from, const Stored* to, int count, int type, cudaStream_t stream);
+long long tc_gemm_workspace(long long M, long long N, long long K, int type);
+int launch_tc_gemm(const Gemm& g, void* workspace, cudaStream_t stream);
+int launch_join(const Gemm& g, const float* part, int parts, cudaStream_t stream);   // partial sums (parts, M, N) and the epilogue
 
 long long linear_workspace(const gelib_linear_args& p, bool backward);
 int launch_linear(const gelib_linear_args& p, void* workspace, cudaStream_t stream);
 int launch_linear_back(const gelib_linear_args& p, void* workspace, cudaStream_t stream);
+
+#ifdef __CUDACC__
+template <class T>
+__device__ __forceinline__ T held(float z) {   // z as it is kept for the backward pass: an infinity would have no derivative
+  if constexpr (std::is_same_v<T, __half>) z = z < -65504.f ? -65504.f : z > 65504.f ? 65504.f : z;
+  return from_float<T>(z);
+}
+
+// x as the sum of three bfloat16 numbers, each the next eight bits, cut and not rounded: the sum is x to the last bit, and none of them is an infinity
+// that x is not.  An infinity or NaN is its first part, and the others are zero.
+__device__ __forceinline__ void split3(float x, __nv_bfloat16 (&p)[3]) {
+  float r = x;
+  const bool finite = fabsf(x) <= 3.402823466e38f;
+#pragma unroll
+  for (int i = 0; i < 3; i++) {
+    unsigned bits = __float_as_uint(r) & 0xffff0000u;
+    if (i == 0 && x != x) bits = 0x7fc00000u;
+    p[i] = __ushort_as_bfloat16((unsigned short)(bits >> 16));
+    r = finite ? r - __uint_as_float(bits) : 0.f;
+  }
+}
+#endif
 
 }  // namespace gelib_b200

@@ -166,7 +166,8 @@ int poll_async_status(const char* fn) {
   volatile int* w = status_words();
   static const char* what[kStatusCount] = {"the tensor-core forward kernel (cg_fwd_tc_kernel); its output is incomplete",
                                            "the tensor-core backward kernel (cg_bwd_tc_kernel); its gradients are incomplete",
-                                           "the backward kernel (cg_bwd_pair_kernel); its gradients are incomplete"};
+                                           "the backward kernel (cg_bwd_pair_kernel); its gradients are incomplete",
+                                           "the dense layers' product (gemm_tc_kernel); its output is incomplete"};
   std::string msg;
   for (int i = 0; i < kStatusCount; i++)
     if (w[i] != 0) {

@@ -99,7 +99,7 @@ int set_option(const char* name, const char* value);  // GELIB_OK or GELIB_INVAL
 
 // Host-mapped status words that kernels with bounded waits set when a wait ran out.  One word per kernel family;
 // every C-ABI product call and gelib_async_status() poll and clear them.
-enum { kStatusFwdTc = 0, kStatusBwdTc = 1, kStatusBwdPair = 2, kStatusCount = 3 };
+enum { kStatusFwdTc = 0, kStatusBwdTc = 1, kStatusBwdPair = 2, kStatusGemmTc = 3, kStatusCount = 4 };
 int* async_status_word(int which);        // nullptr when the mapped allocation failed
 int poll_async_status(const char* fn);    // GELIB_OK, or GELIB_CUDA_ERROR with the message set (words cleared)
 

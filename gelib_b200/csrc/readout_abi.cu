@@ -3,10 +3,10 @@
 #include <cmath>
 #include <exception>
 
+#include "readout.h"
 #include "linear.h"
 #include "norm.h"
 #include "plan.h"
-#include "readout.h"
 
 using namespace gelib_b200;
 
@@ -146,7 +146,8 @@ long long gelib_linear_workspace(const gelib_linear_args* p, int backward) {
 int gelib_linear(const gelib_linear_args* p, void* workspace, void* stream) {
   static const char* fn = "linear";
   return guarded(fn, [&]() -> int {
-    int st = check_linear(fn, p, false);
+    int st = poll_async_status(fn);
+    if (st == GELIB_OK) st = check_linear(fn, p, false);
     if (st != GELIB_OK || p->m == 0 || p->n == 0) return st;
     if (!workspace && linear_workspace(*p, false) > 0) return fail(GELIB_INVALID, fn, "no workspace");
     if (!is_aligned(workspace, 256)) return fail(GELIB_INVALID, fn, "the workspace is not 256-byte aligned");
@@ -157,7 +158,8 @@ int gelib_linear(const gelib_linear_args* p, void* workspace, void* stream) {
 int gelib_linear_back(const gelib_linear_args* p, void* workspace, void* stream) {
   static const char* fn = "linear_back";
   return guarded(fn, [&]() -> int {
-    int st = check_linear(fn, p, true);
+    int st = poll_async_status(fn);
+    if (st == GELIB_OK) st = check_linear(fn, p, true);
     if (st != GELIB_OK) return st;
     if (!workspace && linear_workspace(*p, true) > 0) return fail(GELIB_INVALID, fn, "no workspace");
     if (!is_aligned(workspace, 256)) return fail(GELIB_INVALID, fn, "the workspace is not 256-byte aligned");

@@ -311,3 +311,34 @@ def test_a_device_is_asked_of_all(cabi):
     import gelib_b200 as G
     with pytest.raises(RuntimeError, match="bias must be of x's type on x's device"):
         G.linear(torch.zeros(2, 8, device="cuda"), torch.zeros(8, 4, device="cuda"), torch.zeros(4))
+
+
+@pytest.mark.gpu
+def test_a_wait_that_runs_out_is_reported():
+    """The tensor-core product gives up when a test makes its first waits run out (no fault is involved), and the next call says so."""
+    import gelib_b200 as G
+    x, w, _, _, _ = make(512, 512, 512, torch.bfloat16)
+    good = G.linear(x, w)
+    G._lib.set_option("inject_timeout", "1")
+    try:
+        G.linear(x, w)
+        torch.cuda.synchronize()
+    finally:
+        G._lib.set_option("inject_timeout", "0")
+    with pytest.raises(RuntimeError, match="gemm_tc_kernel"):
+        G.linear(x, w)
+    assert torch.equal(G.linear(x, w), good)
+    torch.cuda.synchronize()
+    G._lib.async_status()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_long_sums_and_many_tiles(dtype):
+    """Sums of 20000 products, split and whole; more tiles than SMs; one tile of one column."""
+    import gelib_b200 as G
+    for m, k, n in ((300, 20000, 40), (5000, 64, 1100), (129, 20000, 1), (40000, 20, 9)):
+        x, w, bias, residual, gy = make(m, k, n, dtype)
+        got = run(G, x, w, bias, residual, "silu", gy)
+        for t, want, what in zip(got, reference(x, w, bias, residual, "silu", gy), ("y", "gx", "gw", "gb")):
+            near(t, want, (what, m, k, n))
