@@ -6,7 +6,10 @@
 // with its rows along the sum or across it: the 128-byte swizzle serves both, and the instruction is told which.
 //
 // float matrices come as three bfloat16 planes a = a0 + a1 + a2; the six products a_i b_j with i + j <= 2 are summed, the rest is below 2^-22 of a product.
-// A plane's slabs of A and B share a stage, so that a group of three stages carries the six.
+// A plane's slabs of A and B share a stage, so that a group of three stages carries the six.  The tensor cores cut every sum
+// off at float's last bit instead of rounding it: over 1280 products in one accumulator the results were 9e-6 off, all to the same side.  So the
+// five small products of a slab come first and a0 b0 last, and after every slab the sums leave tensor memory for registers, where
+// they are added with rounding: four cuts at full size and no more (7e-7).
 //
 // Every wait has a limit; a kernel that gives up says so in a status word, and ends.
 #include <cuda.h>
@@ -27,9 +30,6 @@ namespace {
 using tc::smem_u32;
 
 constexpr int kDepth = 64;            // of a slab: 128 bytes of 16-bit numbers
-constexpr int kThreads = 192;         // a warp for copies, one for multiplications, four for the results
-constexpr int kPitch = 36;            // floats of a row of a warp's staging block: 16-byte accesses by rows and by columns without conflicts
-constexpr int kStaging = 4 * 32 * kPitch * 4;
 constexpr int kSms = 148;
 
 struct TcArgs {
@@ -47,10 +47,16 @@ struct TcArgs {
 
 template <int CG, int BN, int P>
 struct Shape {
+  static constexpr int kWarps = P == 3 ? 8 : 4;                        // that take the results
+  static constexpr int kThreads = 64 + 32 * kWarps;                    // beside a warp for copies and one for multiplications
+  static constexpr int kCols = BN / (kWarps / 4);                      // columns of a tile that such a warp has
+  static constexpr int kChunk = P == 3 ? 16 : 32;                      // columns that it stages at a time
+  static constexpr int kPitch = kChunk + 4;                            // floats of a staged row: 16-byte accesses by rows and by columns, no conflicts
+  static constexpr int kStaging = kWarps * 32 * kPitch * 4;
   static constexpr int kBn = BN / CG;                                  // columns of B that a block holds
   static constexpr int kA = 128 * 128, kB = kBn * 128;                 // bytes of a slab
   static constexpr int kStage = kA + kB;
-  static constexpr int kFit = (220 * 1024 - kStaging) / kStage;
+  static constexpr int kFit = (222 * 1024 - kStaging) / kStage;
   static constexpr int kStages = P == 3 ? kFit / 3 * 3 : kFit < 8 ? kFit : 8;
   static constexpr int kShared = kStages * kStage + kStaging + 1024 + 256;
 };
@@ -160,8 +166,50 @@ __device__ __forceinline__ void finish_vec(const Epilogue& e, long long at, cons
   store_vec<T, V>(static_cast<T*>(e.y) + at, d);
 }
 
+// A warp's 32 rows from m0 on of W columns, a row per lane in r, through shared memory, so that lanes store along rows.
+template <class T, int W>
+__device__ __forceinline__ void store_chunk(const TcArgs& g, int split, const uint32_t (&r)[W], float* block, long long m0, int n0, int lane) {
+  constexpr int kPitch = W + 4, kAcross = W / 4, kRows = 32 / kAcross;
+  const uint32_t at_block = smem_u32(block);
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < kAcross; j++) tc::sts128(at_block + (lane * kPitch + 4 * j) * 4, r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+  __syncwarp();
+  const int col = lane % kAcross * 4, n = n0 + col, live = min(4, g.N - n);
+  float bias[4] = {0, 0, 0, 0};
+  if (g.e.bias && !g.part)
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      if (j < live) bias[j] = to_float(static_cast<const T*>(g.e.bias)[n + j]);
+#pragma unroll
+  for (int pass = 0; pass < 32 / kRows; pass++) {
+    const int row = pass * kRows + lane / kAcross;
+    const float4 v = tc::lds128(at_block + (row * kPitch + col) * 4);
+    if (m0 + row >= g.M || live <= 0) continue;
+    float d[4] = {v.x, v.y, v.z, v.w};
+    const long long at = (m0 + row) * g.N + n;
+    if (g.part) {
+      float* p = g.part + (long long)split * g.M * g.N + at;
+      if (g.vec) *reinterpret_cast<float4*>(p) = v;
+      else
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+          if (j < live) p[j] = d[j];
+    } else if (g.vec) {
+      finish_vec<T, 4>(g.e, at, bias, d, g.e.act);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        if (j < live) {
+          float one[1] = {d[j]}, add[1] = {bias[j]};
+          finish_vec<T, 1>(g.e, at + j, add, one, g.e.act);
+        }
+    }
+  }
+}
+
 template <class T, int CG, int BN, int P>
-__global__ void __launch_bounds__(kThreads, 1) gemm_tc_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mb, TcArgs g) {
+__global__ void __launch_bounds__(Shape<CG, BN, P>::kThreads, 1) gemm_tc_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mb, TcArgs g) {
   using S = Shape<CG, BN, P>;
   extern __shared__ unsigned char raw[];
   unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
@@ -175,7 +223,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_tc_kernel(const __grid_const
 
   if (warp == 0 && lane == 0) {
     for (int i = 0; i < S::kStages; i++) tc::mbar_init(&bars.full[i], 1), tc::mbar_init(&bars.empty[i], 1);
-    for (int i = 0; i < 2; i++) tc::mbar_init(&bars.sums_full[i], 1), tc::mbar_init(&bars.sums_empty[i], 4 * CG);
+    for (int i = 0; i < 2; i++) tc::mbar_init(&bars.sums_full[i], 1), tc::mbar_init(&bars.sums_empty[i], S::kWarps * CG);
     tc::mbar_init(&bars.done, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -242,111 +290,118 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_tc_kernel(const __grid_const
     for (int i = first; ok && i < items; i += stride) {
       const Item it = item_of(g, i);
       const int k0 = it.split * g.per, k1 = min(g.slabs, k0 + g.per);
-      if (!(ok = wait(&bars.sums_empty[buf], buf_phase ^ 1, g.limit))) break;
-      tc::tc_fence_after();
-      const uint32_t d = tmem + buf * BN;
       bool more = false;
       auto slab = [&](int sa, int sb) {
         const uint64_t a = slab_desc(ring_at + sa * S::kStage, g.a_across), b = slab_desc(ring_at + sb * S::kStage + S::kA, g.b_across);
 #pragma unroll
         for (int q = 0; q < kDepth / 16; q++) {
-          mma<CG>(d, a + q * step_a, b + q * step_b, idesc, more);
+          mma<CG>(tmem + buf * BN, a + q * step_a, b + q * step_b, idesc, more);
           more = true;
         }
       };
-      for (int k = k0; ok && k < k1; k++) {
-        if constexpr (P == 1) {
-          if (!(ok = wait(&bars.full[stage], phase))) break;
-          tc::tc_fence_after();
+      auto begin = [&] {
+        if (!(ok = wait(&bars.sums_empty[buf], buf_phase ^ 1, g.limit))) return false;
+        tc::tc_fence_after();
+        more = false;
+        return true;
+      };
+      auto end = [&] {
+        commit<CG>(&bars.sums_full[buf]);
+        buf ^= 1;
+        if (buf == 0) buf_phase ^= 1;
+      };
+      auto arrived = [&](int s) {
+        ok = wait(&bars.full[s], phase);
+        tc::tc_fence_after();
+        return ok;
+      };
+      if constexpr (P == 1) {
+        if (!begin()) break;
+        for (int k = k0; k < k1; k++) {
+          if (!arrived(stage)) break;
           slab(stage, stage);
           commit<CG>(&bars.empty[stage]);
           if (++stage == S::kStages) stage = 0, phase ^= 1;
-        } else {
-          const int s = stage;   // three stages of a turn: the ring has a multiple of three
-          for (int p = 0; p < 3; p++) {
-            if (!(ok = wait(&bars.full[s + p], phase))) break;
-            tc::tc_fence_after();
-            if (p == 0) slab(s, s);
-            if (p == 1) {
-              slab(s + 1, s);
-              slab(s, s + 1);
-              slab(s + 1, s + 1);
-              commit<CG>(&bars.empty[s + 1]);
-            }
-            if (p == 2) {
-              slab(s + 2, s);
-              slab(s, s + 2);
-              commit<CG>(&bars.empty[s]);
-              commit<CG>(&bars.empty[s + 2]);
-            }
-          }
+        }
+        end();
+      } else {
+        for (int k = k0; k < k1; k++) {   // three stages of a turn: the ring has a multiple of three
+          const int s = stage;
+          if (!begin() || !arrived(s) || !arrived(s + 1)) break;
+          slab(s + 1, s + 1);
+          slab(s + 1, s);
+          slab(s, s + 1);
+          commit<CG>(&bars.empty[s + 1]);
+          if (!arrived(s + 2)) break;
+          slab(s + 2, s);
+          slab(s, s + 2);
+          commit<CG>(&bars.empty[s + 2]);
+          slab(s, s);
+          commit<CG>(&bars.empty[s]);
+          end();
           stage += 3;
           if (stage == S::kStages) stage = 0, phase ^= 1;
         }
       }
-      commit<CG>(&bars.sums_full[buf]);
-      buf ^= 1;
-      if (buf == 0) buf_phase ^= 1;
     }
     if (!ok) {   // what was issued ends before tensor memory is given back
       commit<CG>(&bars.done);
       wait(&bars.done, 0);
     }
   } else if (warp >= 2) {
-    const int q = warp & 3;   // the quarter of tensor memory that the warp may read
-    float* block = staging + (warp - 2) * 32 * kPitch;
-    const uint32_t block_at = smem_u32(block);
+    const int q = warp & 3;                          // the quarter of tensor memory that the warp may read
+    const int half = (warp - 2) / 4 * S::kCols;      // its first column
+    float* block = staging + (warp - 2) * 32 * S::kPitch;
     int buf = 0;
     uint32_t buf_phase = 0;
-    for (int i = first; ok && i < items; i += stride) {
-      const Item it = item_of(g, i);
-      if (!(ok = __all_sync(0xffffffffu, wait(&bars.sums_full[buf], buf_phase, g.limit)))) break;
-      tc::tc_fence_after();
-      const long long m0 = ((long long)it.m * CG + rank) * 128 + q * 32;
-      const int n0 = it.n * BN;
-      const int col = lane % 8 * 4;
-      for (int c = 0; c < BN && n0 + c < g.N; c += 32) {
-        uint32_t r[32];
-        tc::tmem_ld32(tmem + ((uint32_t)q << 21) + buf * BN + c, r);
-        __syncwarp();
-#pragma unroll
-        for (int j = 0; j < 8; j++) tc::sts128(block_at + (lane * kPitch + 4 * j) * 4, r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
-        __syncwarp();
-        const int n = n0 + c + col, live = min(4, g.N - n);
-        float bias[4] = {0, 0, 0, 0};
-        if (g.e.bias && !g.part)
-#pragma unroll
-          for (int j = 0; j < 4; j++)
-            if (j < live) bias[j] = to_float(static_cast<const T*>(g.e.bias)[n + j]);
-#pragma unroll
-        for (int pass = 0; pass < 8; pass++) {
-          const int row = pass * 4 + lane / 8;
-          const float4 v = tc::lds128(block_at + (row * kPitch + col) * 4);
-          if (m0 + row >= g.M || live <= 0) continue;
-          float d[4] = {v.x, v.y, v.z, v.w};
-          const long long at = (m0 + row) * g.N + n;
-          if (g.part) {
-            float* p = g.part + (long long)it.split * g.M * g.N + at;
-            if (g.vec) *reinterpret_cast<float4*>(p) = v;
-            else
-              for (int j = 0; j < live; j++) p[j] = d[j];
-          } else if (g.vec) {
-            finish_vec<T, 4>(g.e, at, bias, d, g.e.act);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-              if (j < live) {
-                float one[1] = {d[j]}, add[1] = {bias[j]};
-                finish_vec<T, 1>(g.e, at + j, add, one, g.e.act);
-              }
-          }
-        }
-      }
+    auto taken = [&] {   // tensor memory has been read
       tc::tc_fence_before();
       __syncwarp();
       if (lane == 0) arrive_at(at_rank(smem_u32(&bars.sums_empty[buf]), 0));
       buf ^= 1;
       if (buf == 0) buf_phase ^= 1;
+    };
+    for (int i = first; ok && i < items; i += stride) {
+      const Item it = item_of(g, i);
+      const long long m0 = ((long long)it.m * CG + rank) * 128 + q * 32;
+      const int n0 = it.n * BN + half;
+      const uint32_t from = tmem + ((uint32_t)q << 21) + half;
+      if constexpr (P == 1) {
+        if (!(ok = __all_sync(0xffffffffu, wait(&bars.sums_full[buf], buf_phase, g.limit)))) break;
+        tc::tc_fence_after();
+        for (int c = 0; c < S::kCols && n0 + c < g.N; c += 32) {
+          uint32_t r[32];
+          tc::tmem_ld32(from + buf * BN + c, r);
+          store_chunk<T, S::kChunk>(g, it.split, r, block, m0, n0 + c, lane);
+        }
+        taken();
+      } else {
+        float sum[S::kCols];
+#pragma unroll
+        for (int j = 0; j < S::kCols; j++) sum[j] = 0;
+        const int k0 = it.split * g.per, k1 = min(g.slabs, k0 + g.per);
+        for (int k = k0; k < k1; k++) {
+          if (!(ok = __all_sync(0xffffffffu, wait(&bars.sums_full[buf], buf_phase, g.limit)))) break;
+          tc::tc_fence_after();
+#pragma unroll
+          for (int c = 0; c < S::kCols; c += 32) {
+            uint32_t r[32];
+            tc::tmem_ld32(from + buf * BN + c, r);
+#pragma unroll
+            for (int j = 0; j < 32; j++) sum[c + j] += __uint_as_float(r[j]);
+          }
+          taken();
+        }
+        if (!ok) break;
+#pragma unroll
+        for (int c = 0; c < S::kCols; c += S::kChunk)
+          if (n0 + c < g.N) {
+            uint32_t r[S::kChunk];
+#pragma unroll
+            for (int j = 0; j < S::kChunk; j++) r[j] = __float_as_uint(sum[c + j]);
+            store_chunk<T, S::kChunk>(g, it.split, r, block, m0, n0 + c, lane);
+          }
+      }
     }
   }
   if (!ok && g.status) *reinterpret_cast<volatile int*>(g.status) = 1;
@@ -460,7 +515,7 @@ int launch_as(const CUtensorMap& ma, const CUtensorMap& mb, const TcArgs& a, cud
   const long long items = (long long)a.tiles_m * a.tiles_n * a.splits;
   cudaLaunchConfig_t c = {};
   c.gridDim = dim3((unsigned)std::min<long long>(items, kSms / CG) * CG);
-  c.blockDim = dim3(kThreads);
+  c.blockDim = dim3(Shape<CG, BN, P>::kThreads);
   c.dynamicSmemBytes = shared;
   c.stream = stream;
   cudaLaunchAttribute at[1];
