@@ -57,19 +57,15 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, *, step, lr, betas=(0.9, 0.99
     step, seed = int(step), int(seed) % (1 << 64)
     if len(params) == 0 and not (len(grads) or len(exp_avg) or len(exp_avg_sq)):
         return
-    if params[0].is_cuda and torch.cuda.is_current_stream_capturing():
-        raise RuntimeError("adamw_step: the step's number and its rate are host values, which a captured graph would repeat")
+    if native().adamw_step(params, grads, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, master, step, lr, beta1, beta2, eps, weight_decay,
+                           seed, grad_scale) is not None:
+        return
     with torch.no_grad(), plain():
-        if native().adamw_step(params, grads, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, master, step, lr, beta1, beta2, eps,
-                               weight_decay, seed, grad_scale) is None:
-            _adamw_step(list(params), list(grads), list(exp_avg), list(exp_avg_sq), exp_avg_scale, exp_avg_sq_scale, master, step, lr, beta1,
-                        beta2, eps, weight_decay, seed, grad_scale)
+        _adamw_step(list(params), list(grads), list(exp_avg), list(exp_avg_sq), exp_avg_scale, exp_avg_sq_scale, master, step, lr, beta1, beta2, eps,
+                    weight_decay, seed, grad_scale)
         # what autograd has saved of these tensors is no longer what they hold
-        for written in (params, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale):
-            if written is not None:
-                torch.autograd.graph.increment_version(written)
-        if master is not None:
-            torch.autograd.graph.increment_version([t for t in master if t is not None])
+        for written in (params, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, master):
+            torch.autograd.graph.increment_version([t for t in written or () if t is not None])
 
 
 def _adamw_step(params, grads, m, v, ms, vs, master, step, lr, beta1, beta2, eps, weight_decay, seed, grad_scale):
@@ -82,6 +78,8 @@ def _adamw_step(params, grads, m, v, ms, vs, master, step, lr, beta1, beta2, eps
     device = params[0].device
     if device.type != "cuda":
         raise RuntimeError("gelib_b200 computes on CUDA tensors only (this build has no CPU path); got a %s tensor" % device.type)
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("adamw_step: the step's number and its rate are host values, which a captured graph would repeat")
     options = AdamwOptions(lr, beta1, beta2, eps, weight_decay, step, seed, None, 32 if ms is None else 8)
     if grad_scale is not None:
         options.grad_scale = _dense("grad_scale", grad_scale, device, (torch.float32,), 1)

@@ -384,11 +384,11 @@ __global__ void __launch_bounds__(Shape<CG, BN, P>::kThreads, 1) gemm_tc_kernel(
           if (!(ok = __all_sync(0xffffffffu, wait(&bars.sums_full[buf], buf_phase, g.limit)))) break;
           tc::tc_fence_after();
 #pragma unroll
-          for (int c = 0; c < S::kCols; c += 32) {
-            uint32_t r[32];
-            tc::tmem_ld32(from + buf * BN + c, r);
+          for (int c = 0; c < S::kCols; c += 16) {
+            uint32_t r[16];
+            tc::tmem_ld16(from + buf * BN + c, r);
 #pragma unroll
-            for (int j = 0; j < 32; j++) sum[c + j] += __uint_as_float(r[j]);
+            for (int j = 0; j < 16; j++) sum[c + j] += __uint_as_float(r[j]);
           }
           taken();
         }

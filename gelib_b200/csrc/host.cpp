@@ -1,13 +1,16 @@
-// The host side of the Python products, in native code: what SO3part.py and SO3vec.py do around one C-ABI call -- output
-// type, output tensors, zero-filled gradients, descriptors, device, stream -- for operands that need nothing special.  Each
+// The host side of the Python products, in native code: what SO3part.py, SO3vec.py, readout.py and adamw.py do around one C-ABI call --
+// output type, output tensors, zero-filled gradients, descriptors, device, stream -- for operands that need nothing special.  Each
 // function returns None, having done nothing, when an operand is not plain (not on a CUDA device, not complex64, lazily
 // conjugated, more than two grid dimensions, two parts of one l, ...), when sizes do not fit together, and when the library
 // skips the call: the Python code then takes it from the start and says what there is to say.
 #include <ATen/ATen.h>
 #include <ATen/ops/_foreach_zero.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <algorithm>
@@ -76,14 +79,15 @@ bool describe_all(const Tensors& parts, c10::Device device, Vec* v) {
   return true;
 }
 
-// Makes the call without the interpreter lock (a first call of a signature builds its plan).  True: done; false: the library
+// Makes the call without the interpreter lock (a first call of a signature builds its plan; autograd's threads do not hold it).  True: done; false: the library
 // skipped it.  Errors raise, as in _lib.check.
 template <class F>
 bool call(F f) {
   int status;
   std::string message;
   {
-    pybind11::gil_scoped_release release;
+    std::optional<pybind11::gil_scoped_release> release;
+    if (PyGILState_Check()) release.emplace();
     status = f();
     if (status != GELIB_OK && status != GELIB_SKIPPED) message = gelib_last_error();
   }
@@ -284,9 +288,221 @@ std::optional<bool> adamw_step(const Tensors& params, const Tensors& grads, cons
     }
   }
   c10::cuda::CUDAGuard guard(device);
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) return std::nullopt;
   void* s = stream_of(device);
   call([&] { return gelib_adamw_step(static_cast<int>(k), t.data(), &o, s); });
+  // what autograd has saved of these tensors is no longer what they hold
+  const auto written = [](const at::Tensor& w) {
+    if (!w.is_inference()) w.unsafeGetTensorImpl()->bump_version();
+  };
+  for (const Tensors* list : {&params, &m, &v, ms ? &*ms : nullptr, vs ? &*vs : nullptr})
+    if (list)
+      for (const auto& w : *list) written(w);
+  if (master)
+    for (const auto& w : *master)
+      if (w) written(*w);
   return true;
+}
+
+// ---- readout ---------------------------------------------------------------------------------------------------------------------
+
+using OptTensor = std::optional<at::Tensor>;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+void* ptr(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+at::Tensor or_none(const OptTensor& t) { return t ? *t : at::Tensor(); }
+
+// Real, of x's type and device, of the given shape.
+bool goes_with(const at::Tensor& x, const OptTensor& t, at::IntArrayRef shape) {
+  return !t || (t->defined() && t->device() == x.device() && t->scalar_type() == x.scalar_type() && t->layout() == at::kStrided && t->sizes() == shape && !t->is_neg());
+}
+bool is_plain(const at::Tensor& x) {
+  return x.defined() && x.is_cuda() && x.layout() == at::kStrided && !x.is_neg() && !x.is_complex() && type_code(x.scalar_type()).has_value();
+}
+
+at::Tensor workspace(int64_t bytes, const at::Tensor& like) {
+  return bytes > 0 ? at::empty({bytes}, like.options().dtype(at::kByte)) : at::Tensor();
+}
+
+// Gradients of a call whose own gradient is asked for: an error when that is wanted, not zeros.
+variable_list differentiable_once(variable_list grads, const char* name) {
+  if (!at::GradMode::is_enabled()) return grads;
+  variable_list some;
+  for (auto& g : grads)
+    if (g.defined()) some.push_back(g.detach().requires_grad_());
+  auto error = std::make_shared<torch::autograd::DelayedError>(std::string(name) + " can be differentiated once", static_cast<int>(some.size()));
+  some = (*error)(std::move(some));
+  size_t i = 0;
+  for (auto& g : grads)
+    if (g.defined()) g = some[i++];
+  return grads;
+}
+
+// x as rows of n elements `ld` apart, over all its leading dimensions; copied where it does not lie like that.
+at::Tensor as_rows(const at::Tensor& x, int64_t n, int64_t* ld) {
+  *ld = n;
+  if (x.is_contiguous()) return x;
+  if (x.dim() == 2 && (x.stride(1) == 1 || n == 1) && x.stride(0) >= n) {
+    *ld = x.stride(0);
+    return x;
+  }
+  return x.contiguous();
+}
+
+struct Layer {
+  gelib_linear_args a = {};
+  at::Tensor x, w, z;
+};
+void describe_layer(Layer* l, const at::Tensor& x, const at::Tensor& w, int act) {
+  l->a.k = static_cast<int>(w.size(0));
+  l->a.n = static_cast<int>(w.size(1));
+  int64_t m = 1;
+  for (int64_t d = 0; d + 1 < x.dim(); d++) m *= x.size(d);
+  l->a.m = m;
+  l->x = as_rows(x, l->a.k, &l->a.ldx);
+  // the view v.t() of a matrix (n_out, n_in) is used as it lies
+  l->a.w_transposed = w.stride(0) == 1 && w.stride(1) != 1 && w.stride(1) >= l->a.k;
+  if (l->a.w_transposed) l->w = w, l->a.ldw = w.stride(1);
+  else l->w = as_rows(w, l->a.n, &l->a.ldw);
+  l->a.x = l->x.data_ptr(), l->a.w = l->w.data_ptr();
+  l->a.act = act, l->a.type = *type_code(x.scalar_type());
+}
+
+at::Tensor linear_call(Layer* l, const at::Tensor& x, const at::Tensor& w, const at::Tensor& bias, const at::Tensor& residual, int act, bool keep) {
+  c10::cuda::CUDAGuard guard(x.device());
+  describe_layer(l, x, w, act);
+  std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
+  shape.back() = l->a.n;
+  const at::Tensor y = at::empty(shape, x.options()), b = bias.defined() ? bias.contiguous() : bias, r = residual.defined() ? residual.contiguous() : residual;
+  if (keep && act != GELIB_ACT_NONE) l->z = at::empty({l->a.m, l->a.n}, x.options());
+  l->a.bias = ptr(b), l->a.residual = ptr(r), l->a.y = ptr(y), l->a.z = ptr(l->z);
+  const at::Tensor space = workspace(gelib_linear_workspace(&l->a, 0), x);
+  void* s = stream_of(x.device());
+  call([&] { return gelib_linear(&l->a, ptr(space), s); });
+  return y;
+}
+
+struct LinearFunction : torch::autograd::Function<LinearFunction> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, const OptTensor& bias, const OptTensor& residual, int64_t act) {
+    Layer l;
+    const bool keep = x.requires_grad() || w.requires_grad() || (bias && bias->requires_grad());
+    at::Tensor y = linear_call(&l, x, w, or_none(bias), or_none(residual), static_cast<int>(act), keep);
+    if (keep) ctx->save_for_backward({x, w, l.z});
+    ctx->saved_data["act"] = act;
+    ctx->saved_data["bias"] = bias.has_value();
+    ctx->saved_data["residual"] = residual.has_value();
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list out(5);
+    // edges are counted over the tensors that were given
+    const bool has_bias = ctx->saved_data["bias"].toBool();
+    const bool need[3] = {ctx->needs_input_grad(0), ctx->needs_input_grad(1), has_bias && ctx->needs_input_grad(2)};
+    if (ctx->saved_data["residual"].toBool()) out[3] = grads[0];
+    if (!grads[0].defined() || !(need[0] || need[1] || need[2])) return out;
+    {
+      const at::NoGradGuard off;
+      const auto saved = ctx->get_saved_variables();
+      const at::Tensor &x = saved[0], &w = saved[1], gy = grads[0].resolve_neg().contiguous();
+      c10::cuda::CUDAGuard guard(x.device());
+      Layer l;
+      describe_layer(&l, x, w, static_cast<int>(ctx->saved_data["act"].toInt()));
+      if (need[0]) out[0] = at::empty(x.sizes(), x.options());
+      if (need[1]) out[1] = at::empty(l.a.w_transposed ? std::vector<int64_t>{l.a.n, l.a.k} : std::vector<int64_t>{l.a.k, l.a.n}, x.options());
+      if (need[2]) out[2] = at::empty({l.a.n}, x.options());
+      l.a.gy = ptr(gy), l.a.z = ptr(saved[2]), l.a.gx = ptr(out[0]), l.a.gw = ptr(out[1]), l.a.gb = ptr(out[2]);
+      const at::Tensor space = workspace(gelib_linear_workspace(&l.a, 1), x);
+      void* s = stream_of(x.device());
+      call([&] { return gelib_linear_back(&l.a, ptr(space), s); });
+      if (need[1] && l.a.w_transposed) out[1] = out[1].t();
+    }
+    const at::Tensor residual = out[3];
+    out[3] = at::Tensor();
+    out = differentiable_once(std::move(out), "linear");
+    out[3] = residual;
+    return out;
+  }
+};
+
+std::optional<at::Tensor> linear(const at::Tensor& x, const at::Tensor& w, const OptTensor& bias, const OptTensor& residual, int act) {
+  if (!is_plain(x) || x.dim() < 1 || !w.defined() || w.dim() != 2 || x.size(-1) != w.size(0) || !goes_with(x, w, w.sizes())) return std::nullopt;
+  if (w.size(0) > INT_MAX || w.size(1) > INT_MAX) return std::nullopt;
+  c10::SmallVector<int64_t, 6> shape(x.sizes().begin(), x.sizes().end());
+  shape.back() = w.size(1);
+  if (!goes_with(x, bias, {w.size(1)}) || !goes_with(x, residual, shape)) return std::nullopt;
+  const at::Tensor b = or_none(bias), r = or_none(residual);
+  const auto wants = [](const at::Tensor& t) { return t.defined() && t.requires_grad(); };
+  if (at::GradMode::is_enabled() && (wants(x) || wants(w) || wants(b) || wants(r))) return LinearFunction::apply(x, w, bias, residual, static_cast<int64_t>(act));
+  Layer l;
+  return linear_call(&l, x, w, b, r, act, false);
+}
+
+struct NormSizes {
+  int64_t b, s;
+  int n, type;
+};
+NormSizes norm_sizes(const at::Tensor& x) {
+  NormSizes z = {x.size(0), 1, static_cast<int>(x.size(-1)), *type_code(x.scalar_type())};
+  for (int64_t d = 1; d + 1 < x.dim(); d++) z.s *= x.size(d);
+  return z;
+}
+
+// stats: (2, b, groups) for the means and the inverse deviations, or undefined.
+at::Tensor norm_call(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& bias, int groups, double eps, int act, const at::Tensor& stats) {
+  c10::cuda::CUDAGuard guard(x.device());
+  const NormSizes z = norm_sizes(x);
+  const at::Tensor y = at::empty(x.sizes(), x.options()), space = workspace(gelib_group_norm_workspace(z.b, z.s, z.n, groups, z.type, 0), x);
+  float* mean = stats.defined() ? stats.data_ptr<float>() : nullptr;
+  void* s = stream_of(x.device());
+  call([&] {
+    return gelib_group_norm(ptr(y), mean, mean ? mean + z.b * groups : nullptr, ptr(x), ptr(weight), ptr(bias), z.b, z.s, z.n, groups, eps, act, z.type, ptr(space), s);
+  });
+  return y;
+}
+
+struct GroupNormFunction : torch::autograd::Function<GroupNormFunction> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const OptTensor& weight, const OptTensor& bias, int64_t groups, double eps, int64_t act) {
+    const at::Tensor stats = at::empty({2, x.size(0), groups}, x.options().dtype(at::kFloat));
+    at::Tensor y = norm_call(x, or_none(weight), or_none(bias), static_cast<int>(groups), eps, static_cast<int>(act), stats);
+    ctx->save_for_backward({x, or_none(weight), or_none(bias), stats});
+    ctx->saved_data["groups"] = groups;
+    ctx->saved_data["act"] = act;
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list out(6);
+    if (!grads[0].defined()) return out;
+    {
+      const at::NoGradGuard off;
+      const auto saved = ctx->get_saved_variables();
+      const at::Tensor &x = saved[0], &stats = saved[3], gy = grads[0].resolve_neg().contiguous();
+      c10::cuda::CUDAGuard guard(x.device());
+      const NormSizes z = norm_sizes(x);
+      const int groups = static_cast<int>(ctx->saved_data["groups"].toInt()), act = static_cast<int>(ctx->saved_data["act"].toInt());
+      for (int i = 0, edge = 0; i < 3; i++)   // edges are counted over the tensors that were given
+        if (saved[i].defined() && ctx->needs_input_grad(edge++)) out[i] = at::empty(saved[i].sizes(), x.options());
+      const at::Tensor space = workspace(gelib_group_norm_workspace(z.b, z.s, z.n, groups, z.type, 1), x);
+      const float* mean = stats.data_ptr<float>();
+      void* s = stream_of(x.device());
+      call([&] {
+        return gelib_group_norm_back(ptr(out[0]), ptr(out[1]), ptr(out[2]), ptr(gy), ptr(x), ptr(saved[1]), ptr(saved[2]), mean, mean + z.b * groups, z.b, z.s, z.n, groups,
+                                     act, z.type, ptr(space), s);
+      });
+    }
+    return differentiable_once(std::move(out), "group_norm");
+  }
+};
+
+std::optional<at::Tensor> group_norm(const at::Tensor& x, int groups, const OptTensor& weight, const OptTensor& bias, double eps, int act) {
+  if (!is_plain(x) || x.dim() < 2 || !x.is_contiguous() || x.size(-1) > INT_MAX || groups < 1 || x.size(-1) % groups) return std::nullopt;
+  for (const OptTensor* t : {&weight, &bias})
+    if (!goes_with(x, *t, {x.size(-1)}) || (*t && !(*t)->is_contiguous())) return std::nullopt;
+  const at::Tensor w = or_none(weight), b = or_none(bias);
+  const auto wants = [](const at::Tensor& t) { return t.defined() && t.requires_grad(); };
+  if (at::GradMode::is_enabled() && (wants(x) || wants(w) || wants(b)))
+    return GroupNormFunction::apply(x, weight, bias, static_cast<int64_t>(groups), eps, static_cast<int64_t>(act));
+  return norm_call(x, w, b, groups, eps, act, at::Tensor());
 }
 
 }  // namespace
@@ -297,6 +513,8 @@ PYBIND11_MODULE(_native, m) {
   m.def("vec_backward", torch::wrap_pybind_function(&vec_backward));
   m.def("part_forward", torch::wrap_pybind_function(&part_forward));
   m.def("part_backward", torch::wrap_pybind_function(&part_backward));
+  m.def("linear", torch::wrap_pybind_function(&linear));
+  m.def("group_norm", torch::wrap_pybind_function(&group_norm));
   m.def("adamw_step", torch::wrap_pybind_function(&adamw_step));
   m.def("gather", torch::wrap_pybind_function(&gather));
 }

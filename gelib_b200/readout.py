@@ -2,13 +2,13 @@
 
 What the reference leaves to torch.nn (its Python layer ends with the products, python/src/gelib): the invariants of a network -- the l=0
 parts of its last product, (b, [grid...], channels) with the channels last as in every part -- are normalised and go through dense layers.
-Both operators compute on CUDA tensors in float32, bfloat16 or float16 with float32 sums, and have gradients.
+Both operators compute on CUDA tensors in float32, bfloat16 or float16 with float32 sums, and have gradients; they can be differentiated once.  Calls whose operands need nothing special are made by the native host side.
 """
 import ctypes
 
 import torch
 
-from ._lib import LinearArgs, check, device_guard, lib, stream_of
+from ._lib import LinearArgs, check, device_guard, lib, native, stream_of
 from .gelib_common import plain
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
@@ -88,6 +88,10 @@ def group_norm(x, groups, weight=None, bias=None, eps=1e-5, activation=None):
     x with other strides than a dense tensor's is copied first.  n is at most 16384.
     """
     act, groups, eps = _activation(activation), int(groups), float(eps)
+    if isinstance(x, torch.Tensor):
+        y = native().group_norm(x, groups, weight, bias, eps, act)
+        if y is not None:
+            return y
     with plain():
         if not isinstance(x, torch.Tensor) or x.dim() < 2:
             raise RuntimeError("group_norm: x must have at least 2 dimensions (batch, channels)")
@@ -169,6 +173,10 @@ def linear(x, w, bias=None, residual=None, activation=None):
     gradient.  x may have strided rows; other strides are copied.  With an activation and gradients, x w + bias is kept in x's type.
     """
     act = _activation(activation)
+    if isinstance(x, torch.Tensor) and isinstance(w, torch.Tensor):
+        y = native().linear(x, w, bias, residual, act)
+        if y is not None:
+            return y
     with plain():
         if not isinstance(x, torch.Tensor) or x.dim() < 1 or not isinstance(w, torch.Tensor) or w.dim() != 2 or x.size(-1) != w.size(0):
             raise RuntimeError("linear: x must be (..., n_in) and w (n_in, n_out)")

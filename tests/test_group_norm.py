@@ -259,3 +259,27 @@ def test_refusals(what):
     a = {k: v.cuda() if isinstance(v, torch.Tensor) else v for k, v in {**dict(x=torch.zeros(2, 8), groups=2), **change}.items()}
     with pytest.raises((RuntimeError, ValueError), match=match):
         G.group_norm(a.pop("x"), a.pop("groups"), **a)
+
+
+@pytest.mark.gpu
+def test_without_the_native_host_side(monkeypatch):
+    import gelib_b200 as G
+    for b, s, n, groups in ((5, 1, 24, 3), (5, 7, 24, 3), (2, 9000, 24, 3)):
+        x, w, bias, gy = make(b, s, n, torch.bfloat16)
+        want = run(G, x, groups, w, bias, "silu", gy)
+        with monkeypatch.context() as patch:
+            patch.setattr(G._lib, "_native", G._lib._Declines())
+            got = run(G, x, groups, w, bias, "silu", gy)
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("native", [True, False])
+def test_a_second_derivative_is_refused(native, monkeypatch):
+    import gelib_b200 as G
+    if not native:
+        monkeypatch.setattr(G._lib, "_native", G._lib._Declines())
+    x = torch.randn(3, 8, device="cuda", requires_grad=True)
+    g, = torch.autograd.grad(G.group_norm(x, 2, activation="silu").square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once"):
+        g.sum().backward()

@@ -342,3 +342,28 @@ def test_long_sums_and_many_tiles(dtype):
         got = run(G, x, w, bias, residual, "silu", gy)
         for t, want, what in zip(got, reference(x, w, bias, residual, "silu", gy), ("y", "gx", "gw", "gb")):
             near(t, want, (what, m, k, n))
+
+
+@pytest.mark.gpu
+def test_without_the_native_host_side(monkeypatch):
+    import gelib_b200 as G
+    for m, k, n, dtype, wt in ((5, 12, 9, torch.float32, False), (5, 12, 9, torch.float32, True), (300, 200, 100, torch.bfloat16, True), (300, 200, 100, torch.float32, False)):
+        x, w, bias, residual, gy = make(m, k, n, dtype, wt)
+        want = run(G, x, w, bias, residual, "silu", gy)
+        with monkeypatch.context() as patch:
+            patch.setattr(G._lib, "_native", G._lib._Declines())
+            got = run(G, x, w, bias, residual, "silu", gy)
+            plain = G.linear(x.view(1, m, k), w, bias, residual.view(1, m, n), "silu")
+        assert all(torch.equal(p, q) for p, q in zip(got, want)) and torch.equal(plain[0], want[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("native", [True, False])
+def test_a_second_derivative_is_refused(native, monkeypatch):
+    import gelib_b200 as G
+    if not native:
+        monkeypatch.setattr(G._lib, "_native", G._lib._Declines())
+    x = torch.randn(3, 8, device="cuda", requires_grad=True)
+    g, = torch.autograd.grad(G.linear(x, torch.randn(8, 4, device="cuda"), activation="silu").square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once"):
+        g.sum().backward()
