@@ -75,13 +75,13 @@ __device__ __forceinline__ uint32_t at_rank(uint32_t local, uint32_t rank) {
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// At most `limit` naps of a tenth of a millisecond.
+// At most `limit` naps of a tenth of a millisecond; all lanes of a warp wait.
 constexpr int kWaitLimit = 20000;
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, int limit = kWaitLimit) {
   const uint32_t a = smem_u32(bar);
   for (int i = 0; i < limit; i++) {
     uint32_t ok;
-    asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3; selp.u32 %0, 1, 0, p; }"
+    asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3; selp.u32 %0, 1, 0, p; }"
                  : "=r"(ok)
                  : "r"(a), "r"(parity), "r"(100000u)
                  : "memory");
@@ -89,8 +89,14 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, int limit =
   }
   return false;
 }
+__device__ __forceinline__ bool all_wait(uint64_t* bar, uint32_t parity, int limit = kWaitLimit) {
+  return __all_sync(0xffffffffu, wait(bar, parity, limit));
+}
+// The copies, multiplications and their barriers below are issued by one elected lane of a converged warp: with a branch for lane 0 around the loop the
+// compiler kept descriptors and addresses out of the uniform registers that these instructions take, and a slab's four multiplications
+// took 240 cycles to issue, its two copies 210.
 __device__ __forceinline__ void expect_bytes(uint64_t* bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+  asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; @p mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1; }" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void arrive_at(uint32_t cluster_bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
@@ -99,11 +105,13 @@ __device__ __forceinline__ void arrive_at(uint32_t cluster_bar) {
 template <int CG>
 __device__ __forceinline__ void copy_box(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
   if constexpr (CG == 2)
-    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+    asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff;\n"
+                 "@p cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4}], [%5]; }" ::"r"(dst),
                  "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
                  : "memory");
   else
-    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map),
+    asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff;\n"
+                 "@p cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5]; }" ::"r"(dst), "l"(map),
                  "r"(x), "r"(y), "r"(z), "r"(bar)
                  : "memory");
 }
@@ -111,11 +119,11 @@ __device__ __forceinline__ void copy_box(uint32_t dst, const CUtensorMap* map, i
 template <int CG>
 __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
   if constexpr (CG == 2)
-    asm volatile("{ .reg .pred q; setp.ne.b32 q, %4, 0; tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, q; }" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
+    asm volatile("{ .reg .pred p, q; elect.sync _|p, 0xffffffff; setp.ne.b32 q, %4, 0; @p tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, q; }" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
                  "r"((uint32_t)accumulate)
                  : "memory");
   else
-    asm volatile("{ .reg .pred q; setp.ne.b32 q, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, q; }" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
+    asm volatile("{ .reg .pred p, q; elect.sync _|p, 0xffffffff; setp.ne.b32 q, %4, 0; @p tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, q; }" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
                  "r"((uint32_t)accumulate)
                  : "memory");
 }
@@ -123,10 +131,10 @@ __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t
 template <int CG>
 __device__ __forceinline__ void commit(uint64_t* bar) {
   if constexpr (CG == 2)
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "h"((uint16_t)3)
+    asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; @p tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1; }" ::"r"(smem_u32(bar)), "h"((uint16_t)3)
                  : "memory");
   else
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+    asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; @p tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0]; }" ::"r"(smem_u32(bar)) : "memory");
 }
 
 // Shared-memory descriptor of a slab, 128-byte swizzle.  Rows across the sum: 64 deep, eight rows of 128 bytes to a swizzle atom, atoms
@@ -215,7 +223,7 @@ __global__ void __launch_bounds__(Shape<CG, BN, P>::kThreads, 1) gemm_tc_kernel(
   unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
   float* staging = reinterpret_cast<float*>(ring + S::kStages * S::kStage);
   __shared__ Bars bars;
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;   // the compiler sees that a warp's lanes agree
   const uint32_t rank = CG == 2 ? blockIdx.x & 1 : 0;
   const int first = CG == 2 ? blockIdx.x >> 1 : blockIdx.x, stride = CG == 2 ? gridDim.x >> 1 : gridDim.x;
   const int items = g.tiles_m * g.tiles_n * g.splits;
@@ -242,7 +250,7 @@ __global__ void __launch_bounds__(Shape<CG, BN, P>::kThreads, 1) gemm_tc_kernel(
   const uint32_t tmem = bars.tmem, ring_at = smem_u32(ring);
   bool ok = true;
 
-  if (warp == 0 && lane == 0) {
+  if (warp == 0) {
     int stage = 0;
     uint32_t phase = 0;
     long long issued = 0;
@@ -252,7 +260,7 @@ __global__ void __launch_bounds__(Shape<CG, BN, P>::kThreads, 1) gemm_tc_kernel(
       const int k0 = it.split * g.per, k1 = min(g.slabs, k0 + g.per);
       for (int k = k0; ok && k < k1; k++)
         for (int p = 0; p < P; p++) {
-          if (!wait(&bars.empty[stage], phase ^ 1, g.limit)) {
+          if (!all_wait(&bars.empty[stage], phase ^ 1, g.limit)) {
             ok = false;
             break;
           }
@@ -280,7 +288,7 @@ __global__ void __launch_bounds__(Shape<CG, BN, P>::kThreads, 1) gemm_tc_kernel(
         const long long n = (issued - 1 - i) / S::kStages;   // how often stage i was filled before its last time
         wait(&bars.full[i], (uint32_t)(n & 1));
       }
-  } else if (warp == 1 && lane == 0 && rank == 0) {
+  } else if (warp == 1 && rank == 0) {
     const uint32_t type = g.bf16 ? 1u : 0u;
     const uint32_t idesc = 1u << 4 | type << 7 | type << 10 | (uint32_t)g.a_across << 15 | (uint32_t)g.b_across << 16 | (BN >> 3) << 17 | ((128u * CG) >> 4) << 24;
     // 16 deep further: 32 bytes along a row, or two atoms of eight rows
@@ -300,7 +308,7 @@ __global__ void __launch_bounds__(Shape<CG, BN, P>::kThreads, 1) gemm_tc_kernel(
         }
       };
       auto begin = [&] {
-        if (!(ok = wait(&bars.sums_empty[buf], buf_phase ^ 1, g.limit))) return false;
+        if (!(ok = all_wait(&bars.sums_empty[buf], buf_phase ^ 1, g.limit))) return false;
         tc::tc_fence_after();
         more = false;
         return true;
@@ -311,7 +319,7 @@ __global__ void __launch_bounds__(Shape<CG, BN, P>::kThreads, 1) gemm_tc_kernel(
         if (buf == 0) buf_phase ^= 1;
       };
       auto arrived = [&](int s) {
-        ok = wait(&bars.full[s], phase);
+        ok = all_wait(&bars.full[s], phase);
         tc::tc_fence_after();
         return ok;
       };
@@ -367,7 +375,7 @@ __global__ void __launch_bounds__(Shape<CG, BN, P>::kThreads, 1) gemm_tc_kernel(
       const int n0 = it.n * BN + half;
       const uint32_t from = tmem + ((uint32_t)q << 21) + half;
       if constexpr (P == 1) {
-        if (!(ok = __all_sync(0xffffffffu, wait(&bars.sums_full[buf], buf_phase, g.limit)))) break;
+        if (!(ok = all_wait(&bars.sums_full[buf], buf_phase, g.limit))) break;
         tc::tc_fence_after();
         for (int c = 0; c < S::kCols && n0 + c < g.N; c += 32) {
           uint32_t r[32];
@@ -381,7 +389,7 @@ __global__ void __launch_bounds__(Shape<CG, BN, P>::kThreads, 1) gemm_tc_kernel(
         for (int j = 0; j < S::kCols; j++) sum[j] = 0;
         const int k0 = it.split * g.per, k1 = min(g.slabs, k0 + g.per);
         for (int k = k0; k < k1; k++) {
-          if (!(ok = __all_sync(0xffffffffu, wait(&bars.sums_full[buf], buf_phase, g.limit)))) break;
+          if (!(ok = all_wait(&bars.sums_full[buf], buf_phase, g.limit))) break;
           tc::tc_fence_after();
 #pragma unroll
           for (int c = 0; c < S::kCols; c += 16) {
