@@ -1,8 +1,8 @@
 // D = A B on the 5th-generation tensor cores, with the epilogue of a dense layer.
 //
-// A persistent block (or a pair of blocks on neighbouring SMs, which then share a tile of 256 rows and each hold half of B's columns) has a warp
-// that brings 64-deep slabs of A and B into a ring in shared memory by tensor copies, a thread that issues the multiplications, and four
-// warps that take finished sums out of tensor memory while the next tile is summed in its other half.  Either operand may lie
+// A persistent block (or a pair of blocks on neighbouring SMs, which then share a tile of 256 rows and each hold half of B's columns) has two
+// warps that bring 64-deep slabs of A and of B into a ring in shared memory by tensor copies, one that issues the multiplications, and eight
+// that take finished sums out of tensor memory while the next tile is summed in its other half.  Either operand may lie
 // with its rows along the sum or across it: the 128-byte swizzle serves both, and the instruction is told which.
 //
 // float matrices come as three bfloat16 planes a = a0 + a1 + a2; the six products a_i b_j with i + j <= 2 are summed, the rest is below 2^-22 of a product.
@@ -31,6 +31,11 @@ using tc::smem_u32;
 
 constexpr int kDepth = 64;            // of a slab: 128 bytes of 16-bit numbers
 constexpr int kSms = 148;
+constexpr int kWarps = 8;              // that take the results: two for each quarter of tensor memory, which share a tile's columns
+constexpr int kThreads = 96 + 32 * kWarps;   // beside two warps for copies and one for multiplications
+constexpr int kChunk = 16;             // columns that such a warp takes at a time, every other chunk of the tile
+constexpr int kPitch = kChunk + 4;     // floats of a staged row: 16-byte accesses by rows and by columns without conflicts
+constexpr int kStaging = kWarps * 32 * kPitch * 4;
 
 struct TcArgs {
   Epilogue e;
@@ -41,24 +46,19 @@ struct TcArgs {
   int N;
   int slabs, per;                     // slabs of the sum, and of one split
   int splits, tiles_m, tiles_n;
+  int bn;                             // columns of a tile
   int a_across, b_across;             // the operand's rows are the sum's index
   int bf16, vec;                      // operand type; columns may be taken four at a time
 };
 
-template <int CG, int BN, int P>
+// A tile has 128 CG rows and up to kBnMost columns, a multiple of 16 (32 in a pair).
+template <int CG, int P>
 struct Shape {
-  static constexpr int kWarps = P == 3 ? 8 : 4;                        // that take the results
-  static constexpr int kThreads = 64 + 32 * kWarps;                    // beside a warp for copies and one for multiplications
-  static constexpr int kCols = BN / (kWarps / 4);                      // columns of a tile that such a warp has
-  static constexpr int kChunk = P == 3 ? 16 : 32;                      // columns that it stages at a time
-  static constexpr int kPitch = kChunk + 4;                            // floats of a staged row: 16-byte accesses by rows and by columns, no conflicts
-  static constexpr int kStaging = kWarps * 32 * kPitch * 4;
-  static constexpr int kBn = BN / CG;                                  // columns of B that a block holds
-  static constexpr int kA = 128 * 128, kB = kBn * 128;                 // bytes of a slab
+  static constexpr int kBnMost = 128 * CG;
+  static constexpr int kA = 128 * 128, kB = kBnMost / CG * 128;        // bytes of a slab in a block
   static constexpr int kStage = kA + kB;
-  static constexpr int kFit = (222 * 1024 - kStaging) / kStage;
-  static constexpr int kStages = P == 3 ? kFit / 3 * 3 : kFit < 8 ? kFit : 8;
-  static constexpr int kShared = kStages * kStage + kStaging + 1024 + 256;
+  static constexpr int kStages = 6;                                    // a multiple of three
+  static constexpr int kShared = kStages * kStage + kStaging + 1024;
 };
 
 struct Bars {
@@ -88,6 +88,12 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, int limit =
     if (ok) return true;
   }
   return false;
+}
+// Whether a phase is over now; asked ahead of other work, so that the answer is there when that is done.
+__device__ __forceinline__ uint32_t over(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{ .reg .pred p; mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }" : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+  return ok;
 }
 __device__ __forceinline__ bool all_wait(uint64_t* bar, uint32_t parity, int limit = kWaitLimit) {
   return __all_sync(0xffffffffu, wait(bar, parity, limit));
@@ -154,48 +160,37 @@ __device__ __forceinline__ Item item_of(const TcArgs& g, int i) {
   return {first + t % width % high, t % width / high, i / tiles};
 }
 
-template <class T, int V>
-__device__ __forceinline__ void finish_vec(const Epilogue& e, long long at, const float (&bias)[V], float (&d)[V], int act) {
-#pragma unroll
-  for (int j = 0; j < V; j++) d[j] += bias[j];
-  if (e.z) {
-    T q[V];
-#pragma unroll
-    for (int j = 0; j < V; j++) q[j] = held<T>(d[j]);
-    *reinterpret_cast<typename Raw<V * sizeof(T)>::type*>(static_cast<T*>(e.z) + at) = *reinterpret_cast<typename Raw<V * sizeof(T)>::type*>(q);
-  }
-  activate(d, act);
-  if (e.residual) {
-    float r[V];
-    load_vec<T, V>(static_cast<const T*>(e.residual) + at, r);
-#pragma unroll
-    for (int j = 0; j < V; j++) d[j] += r[j];
-  }
-  store_vec<T, V>(static_cast<T*>(e.y) + at, d);
-}
-
-// A warp's 32 rows from m0 on of W columns, a row per lane in r, through shared memory, so that lanes store along rows.
-template <class T, int W>
-__device__ __forceinline__ void store_chunk(const TcArgs& g, int split, const uint32_t (&r)[W], float* block, long long m0, int n0, int lane) {
-  constexpr int kPitch = W + 4, kAcross = W / 4, kRows = 32 / kAcross;
-  const uint32_t at_block = smem_u32(block);
-  __syncwarp();
-#pragma unroll
-  for (int j = 0; j < kAcross; j++) tc::sts128(at_block + (lane * kPitch + 4 * j) * 4, r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
-  __syncwarp();
+// A warp's 32 rows from m0 on of 16 columns from n0 on, a row per lane in r, through shared memory, so that lanes store along rows.
+template <class T>
+__device__ __forceinline__ void store_chunk(const TcArgs& g, int split, const uint32_t (&r)[kChunk], uint32_t block, long long m0, int n0, int lane, const float (&bias)[4]) {
+  constexpr int kAcross = kChunk / 4, kRows = 32 / kAcross, kPasses = 32 / kRows;
   const int col = lane % kAcross * 4, n = n0 + col, live = min(4, g.N - n);
-  float bias[4] = {0, 0, 0, 0};
-  if (g.e.bias && !g.part)
+  const long long m = m0 + lane / kAcross;
+  const T* residual = g.part ? nullptr : static_cast<const T*>(g.e.residual);
+  __syncwarp();
 #pragma unroll
-    for (int j = 0; j < 4; j++)
-      if (j < live) bias[j] = to_float(static_cast<const T*>(g.e.bias)[n + j]);
+  for (int j = 0; j < kAcross; j++) tc::sts128(block + (lane * kPitch + 4 * j) * 4, r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+  float add[kPasses][4];
 #pragma unroll
-  for (int pass = 0; pass < 32 / kRows; pass++) {
-    const int row = pass * kRows + lane / kAcross;
-    const float4 v = tc::lds128(at_block + (row * kPitch + col) * 4);
-    if (m0 + row >= g.M || live <= 0) continue;
+  for (int pass = 0; pass < kPasses; pass++) {   // all of them asked for before the first is needed
+    const long long at = (m + pass * kRows) * g.N + n;
+#pragma unroll
+    for (int j = 0; j < 4; j++) add[pass][j] = 0;
+    if (residual && live > 0 && m + pass * kRows < g.M) {
+      if (g.vec) load_vec<T, 4>(residual + at, add[pass]);
+      else
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+          if (j < live) add[pass][j] = to_float(residual[at + j]);
+    }
+  }
+  __syncwarp();
+#pragma unroll
+  for (int pass = 0; pass < kPasses; pass++) {
+    const float4 v = tc::lds128(block + ((pass * kRows + lane / kAcross) * kPitch + col) * 4);
+    if (m + pass * kRows >= g.M || live <= 0) continue;
     float d[4] = {v.x, v.y, v.z, v.w};
-    const long long at = (m0 + row) * g.N + n;
+    const long long at = (m + pass * kRows) * g.N + n;
     if (g.part) {
       float* p = g.part + (long long)split * g.M * g.N + at;
       if (g.vec) *reinterpret_cast<float4*>(p) = v;
@@ -203,35 +198,61 @@ __device__ __forceinline__ void store_chunk(const TcArgs& g, int split, const ui
 #pragma unroll
         for (int j = 0; j < 4; j++)
           if (j < live) p[j] = d[j];
-    } else if (g.vec) {
-      finish_vec<T, 4>(g.e, at, bias, d, g.e.act);
-    } else {
+      continue;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++) d[j] += bias[j];
+    if (g.e.z) {
+      T q[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++) q[j] = held<T>(d[j]);
+      T* z = static_cast<T*>(g.e.z) + at;
+      if (g.vec) {
+        union { typename Raw<4 * sizeof(T)>::type raw; T t[4]; } w;
+#pragma unroll
+        for (int j = 0; j < 4; j++) w.t[j] = q[j];
+        *reinterpret_cast<typename Raw<4 * sizeof(T)>::type*>(z) = w.raw;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+          if (j < live) z[j] = q[j];
+      }
+    }
+    activate(d, g.e.act);
+#pragma unroll
+    for (int j = 0; j < 4; j++) d[j] += add[pass][j];
+    T* y = static_cast<T*>(g.e.y) + at;
+    if (g.vec) store_vec<T, 4>(y, d);
+    else
 #pragma unroll
       for (int j = 0; j < 4; j++)
-        if (j < live) {
-          float one[1] = {d[j]}, add[1] = {bias[j]};
-          finish_vec<T, 1>(g.e, at + j, add, one, g.e.act);
-        }
-    }
+        if (j < live) y[j] = from_float<T>(d[j]);
   }
 }
 
-template <class T, int CG, int BN, int P>
-__global__ void __launch_bounds__(Shape<CG, BN, P>::kThreads, 1) gemm_tc_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mb, TcArgs g) {
-  using S = Shape<CG, BN, P>;
+// A lane's part of the bias in the chunk of columns from n0 on.
+template <class T>
+__device__ __forceinline__ void load_bias(const TcArgs& g, int n0, int lane, float (&bias)[4]) {
+  const int n = n0 + lane % (kChunk / 4) * 4;
+#pragma unroll
+  for (int j = 0; j < 4; j++) bias[j] = g.e.bias && n + j < g.N ? to_float(static_cast<const T*>(g.e.bias)[n + j]) : 0.f;
+}
+
+template <class T, int CG, int P>
+__global__ void __launch_bounds__(kThreads, 1) gemm_tc_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mb, TcArgs g) {
+  using S = Shape<CG, P>;
   extern __shared__ unsigned char raw[];
   unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
-  float* staging = reinterpret_cast<float*>(ring + S::kStages * S::kStage);
   __shared__ Bars bars;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;   // the compiler sees that a warp's lanes agree
   const uint32_t rank = CG == 2 ? blockIdx.x & 1 : 0;
   const int first = CG == 2 ? blockIdx.x >> 1 : blockIdx.x, stride = CG == 2 ? gridDim.x >> 1 : gridDim.x;
   const int items = g.tiles_m * g.tiles_n * g.splits;
-  constexpr int kColumns = 2 * BN;
+  constexpr int kColumns = 2 * S::kBnMost;
 
   if (warp == 0 && lane == 0) {
-    for (int i = 0; i < S::kStages; i++) tc::mbar_init(&bars.full[i], 1), tc::mbar_init(&bars.empty[i], 1);
-    for (int i = 0; i < 2; i++) tc::mbar_init(&bars.sums_full[i], 1), tc::mbar_init(&bars.sums_empty[i], S::kWarps * CG);
+    for (int i = 0; i < S::kStages; i++) tc::mbar_init(&bars.full[i], 2), tc::mbar_init(&bars.empty[i], 1);
+    for (int i = 0; i < 2; i++) tc::mbar_init(&bars.sums_full[i], 1), tc::mbar_init(&bars.sums_empty[i], kWarps * CG);
     tc::mbar_init(&bars.done, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -250,37 +271,33 @@ __global__ void __launch_bounds__(Shape<CG, BN, P>::kThreads, 1) gemm_tc_kernel(
   const uint32_t tmem = bars.tmem, ring_at = smem_u32(ring);
   bool ok = true;
 
-  if (warp == 0) {
+  if (warp == 0 || warp == 2) {   // copies of A, of B
+    const bool of_b = warp == 2, across = of_b ? g.b_across : g.a_across;
+    const CUtensorMap* map = of_b ? &mb : &ma;
+    const int mine = of_b ? g.bn / CG : 128, boxes = across ? (mine + 63) / 64 : 1;   // rows or columns in this block
+    const uint32_t bytes = CG * (across ? boxes * 8192 : mine * 128), ring_mine = ring_at + (of_b ? S::kA : 0);
     int stage = 0;
-    uint32_t phase = 0;
+    uint32_t phase = 0, ready = g.limit > 0 && over(&bars.empty[0], 1);
     long long issued = 0;
     for (int i = first; ok && i < items; i += stride) {
       const Item it = item_of(g, i);
-      const int m0 = (it.m * CG + (int)rank) * 128, n0 = it.n * BN + (int)rank * S::kBn;
+      const int at = of_b ? it.n * g.bn + (int)rank * mine : (it.m * CG + (int)rank) * 128;
       const int k0 = it.split * g.per, k1 = min(g.slabs, k0 + g.per);
       for (int k = k0; ok && k < k1; k++)
         for (int p = 0; p < P; p++) {
-          if (!all_wait(&bars.empty[stage], phase ^ 1, g.limit)) {
+          if (!__all_sync(0xffffffffu, ready) && !all_wait(&bars.empty[stage], phase ^ 1, g.limit)) {
             ok = false;
             break;
           }
-          if (rank == 0) expect_bytes(&bars.full[stage], CG * S::kStage);
-          const uint32_t bar = CG == 2 ? at_rank(smem_u32(&bars.full[stage]), 0) : smem_u32(&bars.full[stage]);
-          const uint32_t a = ring_at + stage * S::kStage, b = a + S::kA;
-          if (g.a_across) {
-#pragma unroll
-            for (int j = 0; j < 2; j++) copy_box<CG>(a + j * 8192, &ma, m0 + j * 64, k * kDepth, p, bar);
-          } else {
-            copy_box<CG>(a, &ma, k * kDepth, m0, p, bar);
-          }
-          if (g.b_across) {
-#pragma unroll
-            for (int j = 0; j < S::kBn / 64; j++) copy_box<CG>(b + j * 8192, &mb, n0 + j * 64, k * kDepth, p, bar);
-          } else {
-            copy_box<CG>(b, &mb, k * kDepth, n0, p, bar);
-          }
-          issued++;
+          const uint32_t to = ring_mine + stage * S::kStage, full = smem_u32(&bars.full[stage]), bar = CG == 2 ? at_rank(full, 0) : full;
+          if (rank == 0) expect_bytes(&bars.full[stage], bytes);
           if (++stage == S::kStages) stage = 0, phase ^= 1;
+          ready = over(&bars.empty[stage], phase ^ 1);
+          if (across)
+            for (int j = 0; j < boxes; j++) copy_box<CG>(to + j * 8192, map, at + j * 64, k * kDepth, p, bar);
+          else
+            copy_box<CG>(to, map, k * kDepth, at, p, bar);
+          issued++;
         }
     }
     if (!ok && rank == 0)   // copies in flight land before the block ends
@@ -290,11 +307,11 @@ __global__ void __launch_bounds__(Shape<CG, BN, P>::kThreads, 1) gemm_tc_kernel(
       }
   } else if (warp == 1 && rank == 0) {
     const uint32_t type = g.bf16 ? 1u : 0u;
-    const uint32_t idesc = 1u << 4 | type << 7 | type << 10 | (uint32_t)g.a_across << 15 | (uint32_t)g.b_across << 16 | (BN >> 3) << 17 | ((128u * CG) >> 4) << 24;
+    const uint32_t idesc = 1u << 4 | type << 7 | type << 10 | (uint32_t)g.a_across << 15 | (uint32_t)g.b_across << 16 | (uint32_t)(g.bn >> 3) << 17 | ((128u * CG) >> 4) << 24;
     // 16 deep further: 32 bytes along a row, or two atoms of eight rows
     const uint32_t step_a = (g.a_across ? 2048 : 32) >> 4, step_b = (g.b_across ? 2048 : 32) >> 4;
     int stage = 0, buf = 0;
-    uint32_t phase = 0, buf_phase = 0;
+    uint32_t phase = 0, buf_phase = 0, ready = 0;
     for (int i = first; ok && i < items; i += stride) {
       const Item it = item_of(g, i);
       const int k0 = it.split * g.per, k1 = min(g.slabs, k0 + g.per);
@@ -303,7 +320,7 @@ __global__ void __launch_bounds__(Shape<CG, BN, P>::kThreads, 1) gemm_tc_kernel(
         const uint64_t a = slab_desc(ring_at + sa * S::kStage, g.a_across), b = slab_desc(ring_at + sb * S::kStage + S::kA, g.b_across);
 #pragma unroll
         for (int q = 0; q < kDepth / 16; q++) {
-          mma<CG>(tmem + buf * BN, a + q * step_a, b + q * step_b, idesc, more);
+          mma<CG>(tmem + buf * S::kBnMost, a + q * step_a, b + q * step_b, idesc, more);
           more = true;
         }
       };
@@ -319,7 +336,8 @@ __global__ void __launch_bounds__(Shape<CG, BN, P>::kThreads, 1) gemm_tc_kernel(
         if (buf == 0) buf_phase ^= 1;
       };
       auto arrived = [&](int s) {
-        ok = all_wait(&bars.full[s], phase);
+        ok = __all_sync(0xffffffffu, ready) || all_wait(&bars.full[s], phase);
+        ready = 0;
         tc::tc_fence_after();
         return ok;
       };
@@ -327,9 +345,11 @@ __global__ void __launch_bounds__(Shape<CG, BN, P>::kThreads, 1) gemm_tc_kernel(
         if (!begin()) break;
         for (int k = k0; k < k1; k++) {
           if (!arrived(stage)) break;
-          slab(stage, stage);
-          commit<CG>(&bars.empty[stage]);
+          const int now = stage;
           if (++stage == S::kStages) stage = 0, phase ^= 1;
+          ready = over(&bars.full[stage], phase);
+          slab(now, now);
+          commit<CG>(&bars.empty[now]);
         }
         end();
       } else {
@@ -356,10 +376,11 @@ __global__ void __launch_bounds__(Shape<CG, BN, P>::kThreads, 1) gemm_tc_kernel(
       commit<CG>(&bars.done);
       wait(&bars.done, 0);
     }
-  } else if (warp >= 2) {
+  } else if (warp >= 3) {
     const int q = warp & 3;                          // the quarter of tensor memory that the warp may read
-    const int half = (warp - 2) / 4 * S::kCols;      // its first column
-    float* block = staging + (warp - 2) * 32 * S::kPitch;
+    const int mine = (warp - 3) / 4 * kChunk;        // its first chunk
+    const uint32_t block = ring_at + S::kStages * S::kStage + (warp - 3) * 32 * kPitch * 4;
+    constexpr int kChunks = S::kBnMost / (2 * kChunk);   // at most
     int buf = 0;
     uint32_t buf_phase = 0;
     auto taken = [&] {   // tensor memory has been read
@@ -372,42 +393,52 @@ __global__ void __launch_bounds__(Shape<CG, BN, P>::kThreads, 1) gemm_tc_kernel(
     for (int i = first; ok && i < items; i += stride) {
       const Item it = item_of(g, i);
       const long long m0 = ((long long)it.m * CG + rank) * 128 + q * 32;
-      const int n0 = it.n * BN + half;
-      const uint32_t from = tmem + ((uint32_t)q << 21) + half;
+      const int n0 = it.n * g.bn + mine;
+      const uint32_t from = tmem + ((uint32_t)q << 21) + mine;
+      auto has = [&](int c) { return mine + c * 2 * kChunk < g.bn && n0 + c * 2 * kChunk < g.N; };
+      float bias[P == 1 ? kChunks : 1][4];
       if constexpr (P == 1) {
+#pragma unroll
+        for (int c = 0; c < kChunks; c++) load_bias<T>(g, n0 + c * 2 * kChunk, lane, bias[c]);
         if (!(ok = all_wait(&bars.sums_full[buf], buf_phase, g.limit))) break;
         tc::tc_fence_after();
-        for (int c = 0; c < S::kCols && n0 + c < g.N; c += 32) {
-          uint32_t r[32];
-          tc::tmem_ld32(from + buf * BN + c, r);
-          store_chunk<T, S::kChunk>(g, it.split, r, block, m0, n0 + c, lane);
-        }
+#pragma unroll
+        for (int c = 0; c < kChunks; c++)
+          if (has(c)) {
+            uint32_t r[kChunk];
+            tc::tmem_ld16(from + buf * S::kBnMost + c * 2 * kChunk, r);
+            store_chunk<T>(g, it.split, r, block, m0, n0 + c * 2 * kChunk, lane, bias[c]);
+          }
         taken();
       } else {
-        float sum[S::kCols];
+        float sum[kChunks][kChunk];
 #pragma unroll
-        for (int j = 0; j < S::kCols; j++) sum[j] = 0;
+        for (int c = 0; c < kChunks; c++)
+#pragma unroll
+          for (int j = 0; j < kChunk; j++) sum[c][j] = 0;
         const int k0 = it.split * g.per, k1 = min(g.slabs, k0 + g.per);
         for (int k = k0; k < k1; k++) {
           if (!(ok = all_wait(&bars.sums_full[buf], buf_phase, g.limit))) break;
           tc::tc_fence_after();
 #pragma unroll
-          for (int c = 0; c < S::kCols; c += 16) {
-            uint32_t r[16];
-            tc::tmem_ld16(from + buf * BN + c, r);
+          for (int c = 0; c < kChunks; c++)
+            if (has(c)) {
+              uint32_t r[kChunk];
+              tc::tmem_ld16(from + buf * S::kBnMost + c * 2 * kChunk, r);
 #pragma unroll
-            for (int j = 0; j < 16; j++) sum[c + j] += __uint_as_float(r[j]);
-          }
+              for (int j = 0; j < kChunk; j++) sum[c][j] += __uint_as_float(r[j]);
+            }
           taken();
         }
         if (!ok) break;
 #pragma unroll
-        for (int c = 0; c < S::kCols; c += S::kChunk)
-          if (n0 + c < g.N) {
-            uint32_t r[S::kChunk];
+        for (int c = 0; c < kChunks; c++)
+          if (has(c)) {
+            load_bias<T>(g, n0 + c * 2 * kChunk, lane, bias[0]);
+            uint32_t r[kChunk];
 #pragma unroll
-            for (int j = 0; j < S::kChunk; j++) r[j] = __float_as_uint(sum[c + j]);
-            store_chunk<T, S::kChunk>(g, it.split, r, block, m0, n0 + c, lane);
+            for (int j = 0; j < kChunk; j++) r[j] = __float_as_uint(sum[c][j]);
+            store_chunk<T>(g, it.split, r, block, m0, n0 + c * 2 * kChunk, lane, bias[0]);
           }
       }
     }
@@ -477,28 +508,29 @@ struct Config {
   int cg, bn, splits;
 };
 
-// The tile and the number of splits with the least estimated time, in microseconds at 1.9 GHz: slabs of 64 at the tensor cores' rate,
-// a fixed time per tile, the partial sums' way through memory.
+// The tile and the number of splits with the least estimated time, in microseconds.  Measured, of a slab 64 deep with every SM at work: a
+// pair's tile of 256 columns 0.38, narrower ones in proportion but not below 0.2; a block's of 128 columns 0.3, of 64 0.25.
+// float: six products and three pairs of copies.
 Config choose_config(long long M, long long N, long long K, int type) {
-  const int products = type == GELIB_F32 ? 6 : 1;
   const long long slabs = (K + kDepth - 1) / kDepth;
-  const int shapes[3][2] = {{2, 256}, {1, 128}, {1, 64}};
-  const double cycles[3] = {540, 290, 200};   // of a slab on an SM
   Config best = {1, 128, 1};
   double best_time = 1e30;
-  for (int s = 0; s < 3; s++) {
-    const int cg = shapes[s][0], bn = shapes[s][1];
-    const long long tiles = ((M + 128 * cg - 1) / (128 * cg)) * ((N + bn - 1) / bn);
-    const int slots = kSms / cg;
-    for (int splits = 1; splits <= 64 && splits <= slabs; splits++) {
-      if (splits > 1 && (tiles * splits > 4 * slots || slabs / splits < 4)) break;
-      const long long per = (slabs + splits - 1) / splits;
-      const double waves = std::ceil((double)tiles * splits / slots);
-      double time = waves * (per * products * cycles[s] + 900 + 4.0 * bn) / 1900;
-      if (splits > 1) time += 2.5 + (double)(splits + 1) * M * N * 4 / 4e6;
-      if (time < best_time) best_time = time, best = {cg, bn, (int)((slabs + per - 1) / per)};
+  for (int cg = 1; cg <= 2; cg++)
+    for (int bn = 128 * cg; bn >= 32 * cg; bn -= 16 * cg) {
+      if (bn > 32 * cg && (N + bn - 1) / bn == (N + bn - 16 * cg - 1) / (bn - 16 * cg)) continue;   // a narrower tile covers N as often
+      const long long tiles = ((M + 128 * cg - 1) / (128 * cg)) * ((N + bn - 1) / bn);
+      const int slots = kSms / cg;
+      const double slab = type == GELIB_F32 ? std::max(0.75, bn * (cg == 2 ? 0.0068 : 0.0075)) : cg == 2 ? std::max(0.2, bn * 0.00148) : 0.2 + bn * 0.0008;
+      for (int splits = 1; splits <= 64 && splits <= slabs; splits++) {
+        if (splits > 1 && (tiles * splits > 4 * slots || slabs / splits < 4)) break;
+        const long long per = (slabs + splits - 1) / splits;
+        const double waves = std::ceil((double)tiles * splits / slots), results = 0.6 + bn * (cg == 2 ? 0.012 : 0.01);
+        // a tile's results leave while the next is summed; the last one's do not
+        double time = 2 + waves * std::max(per * slab, results) + results;
+        if (splits > 1) time += 2.5 + (double)(splits + 1) * M * N * 4 / 4e6;
+        if (time < best_time) best_time = time, best = {cg, bn, (int)((slabs + per - 1) / per)};
+      }
     }
-  }
   return best;
 }
 
@@ -514,16 +546,16 @@ bool encode(CUtensorMap* map, const Stored& s, int type, int box_x, int box_y) {
              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <class T, int CG, int BN, int P>
+template <class T, int CG, int P>
 int launch_as(const CUtensorMap& ma, const CUtensorMap& mb, const TcArgs& a, cudaStream_t stream) {
   static const char* fn = "linear";
-  auto kernel = gemm_tc_kernel<T, CG, BN, P>;
-  constexpr int shared = Shape<CG, BN, P>::kShared;
+  auto kernel = gemm_tc_kernel<T, CG, P>;
+  constexpr int shared = Shape<CG, P>::kShared;
   GELIB_CUDA_TRY(fn, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared));
   const long long items = (long long)a.tiles_m * a.tiles_n * a.splits;
   cudaLaunchConfig_t c = {};
   c.gridDim = dim3((unsigned)std::min<long long>(items, kSms / CG) * CG);
-  c.blockDim = dim3(Shape<CG, BN, P>::kThreads);
+  c.blockDim = dim3(kThreads);
   c.dynamicSmemBytes = shared;
   c.stream = stream;
   cudaLaunchAttribute at[1];
@@ -537,9 +569,7 @@ int launch_as(const CUtensorMap& ma, const CUtensorMap& mb, const TcArgs& a, cud
 
 template <class T, int P>
 int launch_config(const Config& c, const CUtensorMap& ma, const CUtensorMap& mb, const TcArgs& a, cudaStream_t stream) {
-  if (c.cg == 2) return launch_as<T, 2, 256, P>(ma, mb, a, stream);
-  if (c.bn == 128) return launch_as<T, 1, 128, P>(ma, mb, a, stream);
-  return launch_as<T, 1, 64, P>(ma, mb, a, stream);
+  return c.cg == 2 ? launch_as<T, 2, P>(ma, mb, a, stream) : launch_as<T, 1, P>(ma, mb, a, stream);
 }
 
 }  // namespace
@@ -600,6 +630,7 @@ int launch_tc_gemm(const Gemm& g, void* workspace, cudaStream_t stream) {
   const long long tm = (g.M + 128 * c.cg - 1) / (128 * c.cg), tn = (g.N + c.bn - 1) / c.bn;
   if (tm * tn * c.splits > 0x3fffffffLL) return fail(GELIB_INVALID, fn, "too many elements");
   a.tiles_m = (int)tm, a.tiles_n = (int)tn;
+  a.bn = c.bn;
   a.a_across = g.a.by_sum, a.b_across = g.b.by_sum;
   a.bf16 = g.type != GELIB_F16;
   const int four = 4 * type_bytes(g.type);
