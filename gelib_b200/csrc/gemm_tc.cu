@@ -508,9 +508,9 @@ struct Config {
   int cg, bn, splits;
 };
 
-// The tile and the number of splits with the least estimated time, in microseconds.  Measured, of a slab 64 deep with every SM at work: a
-// pair's tile of 256 columns 0.38, narrower ones in proportion but not below 0.2; a block's of 128 columns 0.3, of 64 0.25.
-// float: six products and three pairs of copies.
+// The tile and the number of splits with the least estimated time, in microseconds.  Measured of a slab 64 deep, with every SM at work
+// (4096 x 7168 x 2048): a pair's tile of 64, 128, 160, 192, 224, 256 columns 0.20, 0.24, 0.28, 0.29, 0.31, 0.40, a block's of 64, 128 0.20, 0.24;
+// in float (4096 x 4096 x 4096) a pair's of 64, 128, 256 1.4, 1.7, 2.3, a block's of 32, 64, 128 1.2, 1.3, 1.5.
 Config choose_config(long long M, long long N, long long K, int type) {
   const long long slabs = (K + kDepth - 1) / kDepth;
   Config best = {1, 128, 1};
@@ -520,7 +520,7 @@ Config choose_config(long long M, long long N, long long K, int type) {
       if (bn > 32 * cg && (N + bn - 1) / bn == (N + bn - 16 * cg - 1) / (bn - 16 * cg)) continue;   // a narrower tile covers N as often
       const long long tiles = ((M + 128 * cg - 1) / (128 * cg)) * ((N + bn - 1) / bn);
       const int slots = kSms / cg;
-      const double slab = type == GELIB_F32 ? std::max(0.75, bn * (cg == 2 ? 0.0068 : 0.0075)) : cg == 2 ? std::max(0.2, bn * 0.00148) : 0.2 + bn * 0.0008;
+      const double slab = type == GELIB_F32 ? 1.15 + bn * (cg == 2 ? 0.0044 : 0.0031) : cg == 2 ? 0.13 + bn * 0.00101 : 0.16 + bn * 0.00064;
       for (int splits = 1; splits <= 64 && splits <= slabs; splits++) {
         if (splits > 1 && (tiles * splits > 4 * slots || slabs / splits < 4)) break;
         const long long per = (slabs + splits - 1) / splits;

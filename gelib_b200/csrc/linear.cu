@@ -117,6 +117,7 @@ int launch_simple_as(const Gemm& g, float* part, const Split& s, unsigned tiles,
 }
 
 int launch_simple(const Gemm& g, void* workspace, cudaStream_t stream) {
+  if (takes_rows(g)) return launch_rows(g, stream);
   const Split s = split_of(g.M, g.N, g.K);
   float* part = s.parts > 1 ? (float*)workspace : nullptr;
   const long long tiles = ((g.N + kTile - 1) / kTile) * ((g.M + kTile - 1) / kTile);

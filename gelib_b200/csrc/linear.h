@@ -43,6 +43,10 @@ long long tc_gemm_workspace(long long M, long long N, long long K, int type);
 int launch_tc_gemm(const Gemm& g, void* workspace, cudaStream_t stream);
 int launch_join(const Gemm& g, const float* part, int parts, cudaStream_t stream);   // partial sums (parts, M, N) and the epilogue
 
+// Products of at most eight rows (linear_rows.cu).
+bool takes_rows(const Gemm& g);
+int launch_rows(const Gemm& g, cudaStream_t stream);
+
 long long linear_workspace(const gelib_linear_args& p, bool backward);
 int launch_linear(const gelib_linear_args& p, void* workspace, cudaStream_t stream);
 int launch_linear_back(const gelib_linear_args& p, void* workspace, cudaStream_t stream);
