@@ -15,7 +15,11 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
+#include <map>
+#include <mutex>
+#include <vector>
 
 #include "readout.h"
 #include "linear.h"
@@ -37,18 +41,29 @@ constexpr int kChunk = 16;             // columns that such a warp takes at a ti
 constexpr int kPitch = kChunk + 4;     // floats of a staged row: 16-byte accesses by rows and by columns without conflicts
 constexpr int kStaging = kWarps * 32 * kPitch * 4;
 
-struct TcArgs {
+// One product of a launch.
+struct TcProblem {
   Epilogue e;
   float* part;                        // partial sums (splits, M, N), or null
-  int* status;
-  int limit;                          // of the first waits: kWaitLimit, or 0 where a test makes them run out
   long long M;
   int N;
   int slabs, per;                     // slabs of the sum, and of one split
-  int splits, tiles_m, tiles_n;
+  int splits, tiles_m, tiles_n, items;
   int bn;                             // columns of a tile
   int a_across, b_across;             // the operand's rows are the sum's index
-  int bf16, vec;                      // operand type; columns may be taken four at a time
+  int vec;                            // columns may be taken four at a time
+};
+constexpr int kProblems = 2;
+struct TcArgs {
+  TcProblem p[kProblems];             // those with longer items first
+  int items;                          // of all
+  int flip;                           // every other round of items is handed out from the last block on
+  int* status;
+  int limit;                          // of the first waits: kWaitLimit, or 0 where a test makes them run out
+  int bf16;
+};
+struct TcMaps {
+  CUtensorMap a[kProblems], b[kProblems];
 };
 
 // A tile has 128 CG rows and up to kBnMost columns, a multiple of 16 (32 in a pair).
@@ -151,40 +166,108 @@ __device__ __forceinline__ uint64_t slab_desc(uint32_t addr, bool across) {
 }
 
 struct Item {
-  int m, n, split;
+  int m, n, split, k0, k1;
 };
-__device__ __forceinline__ Item item_of(const TcArgs& g, int i) {
-  const int tiles = g.tiles_m * g.tiles_n, t = i % tiles;
+__device__ __forceinline__ Item item_of(const TcProblem& g, int i) {
+  const int tiles = g.tiles_m * g.tiles_n, t = i % tiles, split = i / tiles;
   // groups of eight tiles of rows, so that the tiles at work at a time share operands in L2
   const int width = 8 * g.tiles_n, first = t / width * 8, high = min(8, g.tiles_m - first);
-  return {first + t % width % high, t % width / high, i / tiles};
+  return {first + t % width % high, t % width / high, split, split * g.per, min(g.slabs, (split + 1) * g.per)};
 }
 
-// A warp's 32 rows from m0 on of 16 columns from n0 on, a row per lane in r, through shared memory, so that lanes store along rows.
+// The items of a block (or pair) in their order: item `at` of problem `which`, until there are no more.
+struct Walk {
+  int round, at, which;
+  __device__ __forceinline__ bool next(const TcArgs& a, int mine, int blocks) {
+    at = round * blocks + (a.flip && (round & 1) ? blocks - 1 - mine : mine);
+    round++;
+    if (at >= a.items) return false;
+    which = at >= a.p[0].items;
+    if (which) at -= a.p[0].items;
+    return true;
+  }
+};
+
+constexpr int kAcross = kChunk / 4, kRows = 32 / kAcross, kPasses = 32 / kRows;
+
+// A lane's part of the residual in the warp's 32 rows from m0 on of 16 columns from n0 on, as it lies.
 template <class T>
-__device__ __forceinline__ void store_chunk(const TcArgs& g, int split, const uint32_t (&r)[kChunk], uint32_t block, long long m0, int n0, int lane, const float (&bias)[4]) {
-  constexpr int kAcross = kChunk / 4, kRows = 32 / kAcross, kPasses = 32 / kRows;
+struct Rest {
+  typename Raw<4 * sizeof(T)>::type raw[kPasses];
+};
+template <class T>
+__device__ __forceinline__ void load_rest(const TcProblem& g, long long m0, int n0, int lane, Rest<T>& rest) {
+  const T* residual = static_cast<const T*>(g.e.residual);
+  if (!residual || g.part) return;
+  const int n = n0 + lane % kAcross * 4;
+#pragma unroll
+  for (int pass = 0; pass < kPasses; pass++) {
+    const long long m = m0 + pass * kRows + lane / kAcross, at = m * g.N + n;
+    if (m < g.M && n < g.N) {
+      if (g.vec) rest.raw[pass] = *reinterpret_cast<const typename Raw<4 * sizeof(T)>::type*>(residual + at);
+      else {
+        union { typename Raw<4 * sizeof(T)>::type raw; T t[4]; } w;
+#pragma unroll
+        for (int j = 0; j < 4; j++) w.t[j] = n + j < g.N ? residual[at + j] : from_float<T>(0.f);
+        rest.raw[pass] = w.raw;
+      }
+    }
+  }
+}
+
+// Those rows and columns, a row per lane in r, through shared memory, so that lanes store along rows.
+template <class T>
+__device__ __forceinline__ void store_chunk(const TcProblem& g, int split, const uint32_t (&r)[kChunk], uint32_t block, long long m0, int n0, int lane, const float (&bias)[4],
+                                            const Rest<T>& rest) {
   const int col = lane % kAcross * 4, n = n0 + col, live = min(4, g.N - n);
   const long long m = m0 + lane / kAcross;
-  const T* residual = g.part ? nullptr : static_cast<const T*>(g.e.residual);
   __syncwarp();
 #pragma unroll
   for (int j = 0; j < kAcross; j++) tc::sts128(block + (lane * kPitch + 4 * j) * 4, r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
-  float add[kPasses][4];
-#pragma unroll
-  for (int pass = 0; pass < kPasses; pass++) {   // all of them asked for before the first is needed
-    const long long at = (m + pass * kRows) * g.N + n;
-#pragma unroll
-    for (int j = 0; j < 4; j++) add[pass][j] = 0;
-    if (residual && live > 0 && m + pass * kRows < g.M) {
-      if (g.vec) load_vec<T, 4>(residual + at, add[pass]);
-      else
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-          if (j < live) add[pass][j] = to_float(residual[at + j]);
-    }
-  }
   __syncwarp();
+  if (g.vec && m0 + 32 <= g.M && n0 + kChunk <= g.N) {
+    // nothing to be left out: all sixteen sums of the lane go through each step together
+    float d[kPasses][4];
+#pragma unroll
+    for (int pass = 0; pass < kPasses; pass++) {
+      const float4 v = tc::lds128(block + ((pass * kRows + lane / kAcross) * kPitch + col) * 4);
+      d[pass][0] = v.x, d[pass][1] = v.y, d[pass][2] = v.z, d[pass][3] = v.w;
+    }
+    const long long at = m * g.N + n, step = (long long)kRows * g.N;
+    if (g.part) {
+      float* p = g.part + (long long)split * g.M * g.N + at;
+#pragma unroll
+      for (int pass = 0; pass < kPasses; pass++) store_vec<float, 4>(p + pass * step, d[pass]);
+      return;
+    }
+#pragma unroll
+    for (int pass = 0; pass < kPasses; pass++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) d[pass][j] += bias[j];
+    if (g.e.z) {
+      T* z = static_cast<T*>(g.e.z) + at;
+#pragma unroll
+      for (int pass = 0; pass < kPasses; pass++) {
+        union { typename Raw<4 * sizeof(T)>::type raw; T t[4]; } w;
+#pragma unroll
+        for (int j = 0; j < 4; j++) w.t[j] = held<T>(d[pass][j]);
+        *reinterpret_cast<typename Raw<4 * sizeof(T)>::type*>(z + pass * step) = w.raw;
+      }
+    }
+    activate(reinterpret_cast<float(&)[4 * kPasses]>(d), g.e.act);
+    if (g.e.residual)
+#pragma unroll
+      for (int pass = 0; pass < kPasses; pass++) {
+        union { typename Raw<4 * sizeof(T)>::type raw; T t[4]; } w;
+        w.raw = rest.raw[pass];
+#pragma unroll
+        for (int j = 0; j < 4; j++) d[pass][j] += to_float(w.t[j]);
+      }
+    T* y = static_cast<T*>(g.e.y) + at;
+#pragma unroll
+    for (int pass = 0; pass < kPasses; pass++) store_vec<T, 4>(y + pass * step, d[pass]);
+    return;
+  }
 #pragma unroll
   for (int pass = 0; pass < kPasses; pass++) {
     const float4 v = tc::lds128(block + ((pass * kRows + lane / kAcross) * kPitch + col) * 4);
@@ -202,25 +285,23 @@ __device__ __forceinline__ void store_chunk(const TcArgs& g, int split, const ui
     }
 #pragma unroll
     for (int j = 0; j < 4; j++) d[j] += bias[j];
+    union { typename Raw<4 * sizeof(T)>::type raw; T t[4]; } w;
     if (g.e.z) {
-      T q[4];
 #pragma unroll
-      for (int j = 0; j < 4; j++) q[j] = held<T>(d[j]);
+      for (int j = 0; j < 4; j++) w.t[j] = held<T>(d[j]);
       T* z = static_cast<T*>(g.e.z) + at;
-      if (g.vec) {
-        union { typename Raw<4 * sizeof(T)>::type raw; T t[4]; } w;
-#pragma unroll
-        for (int j = 0; j < 4; j++) w.t[j] = q[j];
-        *reinterpret_cast<typename Raw<4 * sizeof(T)>::type*>(z) = w.raw;
-      } else {
+      if (g.vec) *reinterpret_cast<typename Raw<4 * sizeof(T)>::type*>(z) = w.raw;
+      else
 #pragma unroll
         for (int j = 0; j < 4; j++)
-          if (j < live) z[j] = q[j];
-      }
+          if (j < live) z[j] = w.t[j];
     }
     activate(d, g.e.act);
+    if (g.e.residual) {
+      w.raw = rest.raw[pass];
 #pragma unroll
-    for (int j = 0; j < 4; j++) d[j] += add[pass][j];
+      for (int j = 0; j < 4; j++) d[j] += to_float(w.t[j]);
+    }
     T* y = static_cast<T*>(g.e.y) + at;
     if (g.vec) store_vec<T, 4>(y, d);
     else
@@ -232,22 +313,22 @@ __device__ __forceinline__ void store_chunk(const TcArgs& g, int split, const ui
 
 // A lane's part of the bias in the chunk of columns from n0 on.
 template <class T>
-__device__ __forceinline__ void load_bias(const TcArgs& g, int n0, int lane, float (&bias)[4]) {
-  const int n = n0 + lane % (kChunk / 4) * 4;
+__device__ __forceinline__ void load_bias(const TcProblem& g, int n0, int lane, float (&bias)[4]) {
+  const int n = n0 + lane % kAcross * 4;
 #pragma unroll
   for (int j = 0; j < 4; j++) bias[j] = g.e.bias && n + j < g.N ? to_float(static_cast<const T*>(g.e.bias)[n + j]) : 0.f;
 }
 
 template <class T, int CG, int P>
-__global__ void __launch_bounds__(kThreads, 1) gemm_tc_kernel(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mb, TcArgs g) {
+__global__ void __launch_bounds__(kThreads, 1) gemm_tc_kernel(const __grid_constant__ TcMaps maps, const __grid_constant__ TcArgs args) {
   using S = Shape<CG, P>;
   extern __shared__ unsigned char raw[];
   unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
   __shared__ Bars bars;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;   // the compiler sees that a warp's lanes agree
   const uint32_t rank = CG == 2 ? blockIdx.x & 1 : 0;
-  const int first = CG == 2 ? blockIdx.x >> 1 : blockIdx.x, stride = CG == 2 ? gridDim.x >> 1 : gridDim.x;
-  const int items = g.tiles_m * g.tiles_n * g.splits;
+  const int mine_of = CG == 2 ? blockIdx.x >> 1 : blockIdx.x, blocks = CG == 2 ? gridDim.x >> 1 : gridDim.x;
+  Walk walk = {0, 0, 0};
   constexpr int kColumns = 2 * S::kBnMost;
 
   if (warp == 0 && lane == 0) {
@@ -272,20 +353,23 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_tc_kernel(const __grid_const
   bool ok = true;
 
   if (warp == 0 || warp == 2) {   // copies of A, of B
-    const bool of_b = warp == 2, across = of_b ? g.b_across : g.a_across;
-    const CUtensorMap* map = of_b ? &mb : &ma;
-    const int mine = of_b ? g.bn / CG : 128, boxes = across ? (mine + 63) / 64 : 1;   // rows or columns in this block
-    const uint32_t bytes = CG * (across ? boxes * 8192 : mine * 128), ring_mine = ring_at + (of_b ? S::kA : 0);
+    const bool of_b = warp == 2;
+    const uint32_t ring_mine = ring_at + (of_b ? S::kA : 0);
     int stage = 0;
-    uint32_t phase = 0, ready = g.limit > 0 && over(&bars.empty[0], 1);
+    uint32_t phase = 0, ready = args.limit > 0 && over(&bars.empty[0], 1);
     long long issued = 0;
-    for (int i = first; ok && i < items; i += stride) {
-      const Item it = item_of(g, i);
+    while (ok && walk.next(args, mine_of, blocks)) {
+      const TcProblem& g = args.p[walk.which];
+      const Item it = item_of(g, walk.at);
+      const bool across = of_b ? g.b_across : g.a_across;
+      const CUtensorMap* map = of_b ? &maps.b[walk.which] : &maps.a[walk.which];
+      const int mine = of_b ? g.bn / CG : 128, boxes = across ? (mine + 63) / 64 : 1;   // rows or columns in this block
+      const uint32_t bytes = CG * (across ? boxes * 8192 : mine * 128);
       const int at = of_b ? it.n * g.bn + (int)rank * mine : (it.m * CG + (int)rank) * 128;
-      const int k0 = it.split * g.per, k1 = min(g.slabs, k0 + g.per);
+      const int k0 = it.k0, k1 = it.k1;
       for (int k = k0; ok && k < k1; k++)
         for (int p = 0; p < P; p++) {
-          if (!__all_sync(0xffffffffu, ready) && !all_wait(&bars.empty[stage], phase ^ 1, g.limit)) {
+          if (!__all_sync(0xffffffffu, ready) && !all_wait(&bars.empty[stage], phase ^ 1, args.limit)) {
             ok = false;
             break;
           }
@@ -306,18 +390,20 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_tc_kernel(const __grid_const
         wait(&bars.full[i], (uint32_t)(n & 1));
       }
   } else if (warp == 1 && rank == 0) {
-    const uint32_t type = g.bf16 ? 1u : 0u;
-    const uint32_t idesc = 1u << 4 | type << 7 | type << 10 | (uint32_t)g.a_across << 15 | (uint32_t)g.b_across << 16 | (uint32_t)(g.bn >> 3) << 17 | ((128u * CG) >> 4) << 24;
-    // 16 deep further: 32 bytes along a row, or two atoms of eight rows
-    const uint32_t step_a = (g.a_across ? 2048 : 32) >> 4, step_b = (g.b_across ? 2048 : 32) >> 4;
+    const uint32_t type = args.bf16 ? 1u : 0u;
     int stage = 0, buf = 0;
     uint32_t phase = 0, buf_phase = 0, ready = 0;
-    for (int i = first; ok && i < items; i += stride) {
-      const Item it = item_of(g, i);
-      const int k0 = it.split * g.per, k1 = min(g.slabs, k0 + g.per);
+    while (ok && walk.next(args, mine_of, blocks)) {
+      const TcProblem& g = args.p[walk.which];
+      const Item it = item_of(g, walk.at);
+      const int k0 = it.k0, k1 = it.k1;
+      const uint32_t a_across = g.a_across, b_across = g.b_across;
+      const uint32_t idesc = 1u << 4 | type << 7 | type << 10 | a_across << 15 | b_across << 16 | (uint32_t)(g.bn >> 3) << 17 | ((128u * CG) >> 4) << 24;
+      // 16 deep further: 32 bytes along a row, or two atoms of eight rows
+      const uint32_t step_a = (a_across ? 2048 : 32) >> 4, step_b = (b_across ? 2048 : 32) >> 4;
       bool more = false;
       auto slab = [&](int sa, int sb) {
-        const uint64_t a = slab_desc(ring_at + sa * S::kStage, g.a_across), b = slab_desc(ring_at + sb * S::kStage + S::kA, g.b_across);
+        const uint64_t a = slab_desc(ring_at + sa * S::kStage, a_across), b = slab_desc(ring_at + sb * S::kStage + S::kA, b_across);
 #pragma unroll
         for (int q = 0; q < kDepth / 16; q++) {
           mma<CG>(tmem + buf * S::kBnMost, a + q * step_a, b + q * step_b, idesc, more);
@@ -325,7 +411,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_tc_kernel(const __grid_const
         }
       };
       auto begin = [&] {
-        if (!(ok = all_wait(&bars.sums_empty[buf], buf_phase ^ 1, g.limit))) return false;
+        if (!(ok = all_wait(&bars.sums_empty[buf], buf_phase ^ 1, args.limit))) return false;
         tc::tc_fence_after();
         more = false;
         return true;
@@ -390,24 +476,31 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_tc_kernel(const __grid_const
       buf ^= 1;
       if (buf == 0) buf_phase ^= 1;
     };
-    for (int i = first; ok && i < items; i += stride) {
-      const Item it = item_of(g, i);
+    while (ok && walk.next(args, mine_of, blocks)) {
+      const TcProblem g = walk.which ? args.p[1] : args.p[0];   // in registers: the choice costs a load at every use otherwise
+      const Item it = item_of(g, walk.at);
       const long long m0 = ((long long)it.m * CG + rank) * 128 + q * 32;
       const int n0 = it.n * g.bn + mine;
       const uint32_t from = tmem + ((uint32_t)q << 21) + mine;
       auto has = [&](int c) { return mine + c * 2 * kChunk < g.bn && n0 + c * 2 * kChunk < g.N; };
-      float bias[P == 1 ? kChunks : 1][4];
+      Rest<T> rest[2];   // of a chunk, and of the next, asked for before the first is stored
+      auto store = [&](int c, const uint32_t (&r)[kChunk], const float (&bias)[4]) {
+        if (c + 1 < kChunks && has(c + 1)) load_rest<T>(g, m0, n0 + (c + 1) * 2 * kChunk, lane, rest[(c + 1) & 1]);
+        store_chunk<T>(g, it.split, r, block, m0, n0 + c * 2 * kChunk, lane, bias, rest[c & 1]);
+      };
       if constexpr (P == 1) {
+        float bias[kChunks][4];
 #pragma unroll
         for (int c = 0; c < kChunks; c++) load_bias<T>(g, n0 + c * 2 * kChunk, lane, bias[c]);
-        if (!(ok = all_wait(&bars.sums_full[buf], buf_phase, g.limit))) break;
+        load_rest<T>(g, m0, n0, lane, rest[0]);
+        if (!(ok = all_wait(&bars.sums_full[buf], buf_phase, args.limit))) break;
         tc::tc_fence_after();
 #pragma unroll
         for (int c = 0; c < kChunks; c++)
           if (has(c)) {
             uint32_t r[kChunk];
             tc::tmem_ld16(from + buf * S::kBnMost + c * 2 * kChunk, r);
-            store_chunk<T>(g, it.split, r, block, m0, n0 + c * 2 * kChunk, lane, bias[c]);
+            store(c, r, bias[c]);
           }
         taken();
       } else {
@@ -416,9 +509,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_tc_kernel(const __grid_const
         for (int c = 0; c < kChunks; c++)
 #pragma unroll
           for (int j = 0; j < kChunk; j++) sum[c][j] = 0;
-        const int k0 = it.split * g.per, k1 = min(g.slabs, k0 + g.per);
-        for (int k = k0; k < k1; k++) {
-          if (!(ok = all_wait(&bars.sums_full[buf], buf_phase, g.limit))) break;
+        for (int k = it.k0; k < it.k1; k++) {
+          if (!(ok = all_wait(&bars.sums_full[buf], buf_phase, args.limit))) break;
           tc::tc_fence_after();
 #pragma unroll
           for (int c = 0; c < kChunks; c++)
@@ -431,19 +523,21 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_tc_kernel(const __grid_const
           taken();
         }
         if (!ok) break;
+        load_rest<T>(g, m0, n0, lane, rest[0]);
 #pragma unroll
         for (int c = 0; c < kChunks; c++)
           if (has(c)) {
-            load_bias<T>(g, n0 + c * 2 * kChunk, lane, bias[0]);
+            float bias[4];
+            load_bias<T>(g, n0 + c * 2 * kChunk, lane, bias);
             uint32_t r[kChunk];
 #pragma unroll
             for (int j = 0; j < kChunk; j++) r[j] = __float_as_uint(sum[c][j]);
-            store_chunk<T>(g, it.split, r, block, m0, n0 + c * 2 * kChunk, lane, bias[0]);
+            store(c, r, bias);
           }
       }
     }
   }
-  if (!ok && g.status) *reinterpret_cast<volatile int*>(g.status) = 1;
+  if (!ok && args.status) *reinterpret_cast<volatile int*>(args.status) = 1;
   __syncwarp();
   tc::tc_fence_before();
   if constexpr (CG == 2) cluster_sync(); else __syncthreads();
@@ -454,84 +548,128 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_tc_kernel(const __grid_const
   }
 }
 
-// ---- operands as the kernel wants them ----------------------------------------------------------------------------------------------
-
-struct PlaneJobs {
-  Stored from[3];
-  void* to[3];
-  long long first[4];   // number of a job's first chunk of eight columns; the last entry is the end
-  int wide[3];          // rows begin on 16-byte boundaries
-  int count;
-};
-
-template <class T>
-__global__ void __launch_bounds__(256) planes_kernel(const __grid_constant__ PlaneJobs jobs) {
-  for (long long c = (long long)blockIdx.x * 256 + threadIdx.x; c < jobs.first[jobs.count]; c += (long long)gridDim.x * 256) {
-    int job = 0;
-    while (job + 1 < jobs.count && c >= jobs.first[job + 1]) job++;
-    const Stored& f = jobs.from[job];
-    const long long chunks = (f.cols + 7) / 8, at = c - jobs.first[job], row = at / chunks, col = (at - row * chunks) * 8;
-    const T* src = static_cast<const T*>(f.base) + row * f.ld + col;
-    const int live = (int)min(8LL, f.cols - col);
-    const long long ld = chunks * 8;
-    if constexpr (sizeof(T) == 4) {
-      float x[8];
-      if (jobs.wide[job] && live == 8) {
-        const float4 u = *reinterpret_cast<const float4*>(src), v = *reinterpret_cast<const float4*>(src + 4);
-        x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w, x[4] = v.x, x[5] = v.y, x[6] = v.z, x[7] = v.w;
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; j++) x[j] = j < live ? src[j] : 0.f;
-      }
-      union { uint4 u; __nv_bfloat16 t[8]; } w[3];
-#pragma unroll
-      for (int j = 0; j < 8; j++) {
-        __nv_bfloat16 p[3];
-        split3(x[j], p);
-#pragma unroll
-        for (int i = 0; i < 3; i++) w[i].t[j] = p[i];
-      }
-#pragma unroll
-      for (int i = 0; i < 3; i++) *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(jobs.to[job]) + i * f.rows * ld + row * ld + col) = w[i].u;
-    } else {
-      union { uint4 u; T t[8]; } w;
-#pragma unroll
-      for (int j = 0; j < 8; j++) w.t[j] = j < live ? src[j] : from_float<T>(0.f);
-      *reinterpret_cast<uint4*>(static_cast<T*>(jobs.to[job]) + row * ld + col) = w.u;
-    }
-  }
-}
-
 // ---- host -----------------------------------------------------------------------------------------------------------------------------
 
 struct Config {
-  int cg, bn, splits;
+  int bn, splits;
+};
+struct Plan {
+  int cg, flip;
+  Config c[kProblems];
+};
+struct Sizes {
+  long long M, N, K;
 };
 
-// The tile and the number of splits with the least estimated time, in microseconds.  Measured of a slab 64 deep, with every SM at work
-// (4096 x 7168 x 2048): a pair's tile of 64, 128, 160, 192, 224, 256 columns 0.20, 0.24, 0.28, 0.29, 0.31, 0.40, a block's of 64, 128 0.20, 0.24;
-// in float (4096 x 4096 x 4096) a pair's of 64, 128, 256 1.4, 1.7, 2.3, a block's of 32, 64, 128 1.2, 1.3, 1.5.
-Config choose_config(long long M, long long N, long long K, int type) {
-  const long long slabs = (K + kDepth - 1) / kDepth;
-  Config best = {1, 128, 1};
+// Estimates in microseconds.  Measured of a slab 64 deep, with every SM at work (4096 x 7168 x 2048): a pair's tile of 64, 128, 160, 192, 224, 256
+// columns 0.20, 0.24, 0.28, 0.29, 0.31, 0.40, a block's of 64, 128 0.20, 0.24; in float (4096 x 4096 x 4096) a pair's of 64, 128, 256 1.4,
+// 1.7, 2.3, a block's of 32, 64, 128 1.2, 1.3, 1.5.
+double slab_time(int cg, int bn, int type) {
+  if (type == GELIB_F32) return 1.15 + bn * (cg == 2 ? 0.0044 : 0.0031);
+  return cg == 2 ? 0.13 + bn * 0.00101 : 0.16 + bn * 0.00064;
+}
+
+struct Work {
+  double items, each;   // how many, and the time of one
+  double join;          // of the partial sums
+};
+Work work_of(const Sizes& z, int cg, const Config& c, int type) {
+  const long long slabs = (z.K + kDepth - 1) / kDepth, per = (slabs + c.splits - 1) / c.splits;
+  const double items = (double)((z.M + 128 * cg - 1) / (128 * cg)) * ((z.N + c.bn - 1) / c.bn) * c.splits;
+  // a tile's results leave while the next is summed, if that takes as long
+  const double results = 0.6 + c.bn * (cg == 2 ? 0.012 : 0.01);
+  return {items, std::max(per * slab_time(cg, c.bn, type), results), c.splits > 1 ? (double)(c.splits + 1) * z.M * z.N * 4 / 4e6 : 0};
+}
+
+// The time of a launch of one or two products, whose items are handed out round by round, longer ones first.
+double launch_time(const Work* w, int count, int slots) {
+  double join = 0, all = 0, most = 0, items = 0, least = 1e30;
+  for (int i = 0; i < count; i++) {
+    join += w[i].join, all += w[i].items * w[i].each, items += w[i].items;
+    most = std::max(most, w[i].each), least = std::min(least, w[i].each);
+  }
+  const double rounds = std::ceil(items / slots);
+  // with one kind of item whole rounds; with two the shorter ones fill in
+  const double time = items <= slots ? most : count == 1 ? rounds * most : std::max(most, all / slots + 0.6 * least);
+  return 3 + time + (join > 0 ? 2.5 + join : 0);
+}
+
+// The tiles and splits of a launch's products with the least estimated time.
+Plan choose_plan(const Sizes* z, int count, int type) {
+  Plan best = {1, 0, {{128, 1}, {128, 1}}};
   double best_time = 1e30;
-  for (int cg = 1; cg <= 2; cg++)
-    for (int bn = 128 * cg; bn >= 32 * cg; bn -= 16 * cg) {
-      if (bn > 32 * cg && (N + bn - 1) / bn == (N + bn - 16 * cg - 1) / (bn - 16 * cg)) continue;   // a narrower tile covers N as often
-      const long long tiles = ((M + 128 * cg - 1) / (128 * cg)) * ((N + bn - 1) / bn);
-      const int slots = kSms / cg;
-      const double slab = type == GELIB_F32 ? 1.15 + bn * (cg == 2 ? 0.0044 : 0.0031) : cg == 2 ? 0.13 + bn * 0.00101 : 0.16 + bn * 0.00064;
-      for (int splits = 1; splits <= 64 && splits <= slabs; splits++) {
-        if (splits > 1 && (tiles * splits > 4 * slots || slabs / splits < 4)) break;
-        const long long per = (slabs + splits - 1) / splits;
-        const double waves = std::ceil((double)tiles * splits / slots), results = 0.6 + bn * (cg == 2 ? 0.012 : 0.01);
-        // a tile's results leave while the next is summed; the last one's do not
-        double time = 2 + waves * std::max(per * slab, results) + results;
-        if (splits > 1) time += 2.5 + (double)(splits + 1) * M * N * 4 / 4e6;
-        if (time < best_time) best_time = time, best = {cg, bn, (int)((slabs + per - 1) / per)};
+  for (int cg = 1; cg <= 2; cg++) {
+    const int slots = kSms / cg;
+    std::vector<Config> may[kProblems];
+    for (int i = 0; i < count; i++) {
+      const long long N = z[i].N, slabs = (z[i].K + kDepth - 1) / kDepth;
+      for (int bn = 128 * cg; bn >= 32 * cg; bn -= 16 * cg) {
+        const int next = bn - 16 * cg;
+        if (bn > 32 * cg && (N + bn - 1) / bn == (N + next - 1) / next) continue;   // a narrower tile covers N as often
+        const double tiles = (double)((z[i].M + 128 * cg - 1) / (128 * cg)) * ((N + bn - 1) / bn);
+        static const int kSplits[] = {1, 2, 3, 4, 5, 6, 8, 12, 16, 24, 32, 48, 64};
+        for (int splits : kSplits) {
+          if (splits > 1 && (splits > slabs || tiles * splits > 2 * slots || slabs / splits < (type == GELIB_F32 ? 2 : 4))) break;
+          const long long per = (slabs + splits - 1) / splits;
+          may[i].push_back({bn, (int)((slabs + per - 1) / per)});
+        }
       }
     }
+    for (const Config& c0 : may[0]) {
+      Work w[kProblems] = {work_of(z[0], cg, c0, type), {}};
+      if (count == 1) {
+        const double t = launch_time(w, 1, slots);
+        if (t < best_time) best_time = t, best = {cg, 0, {c0, c0}};
+        continue;
+      }
+      for (const Config& c1 : may[1]) {
+        w[1] = work_of(z[1], cg, c1, type);
+        const double t = launch_time(w, 2, slots);
+        if (t < best_time) best_time = t, best = {cg, 0, {c0, c1}};
+      }
+    }
+  }
+  if (count == 2) {   // whether handing every other round out backwards evens the blocks' times out
+    Work w[kProblems] = {work_of(z[0], best.cg, best.c[0], type), work_of(z[1], best.cg, best.c[1], type)};
+    if (w[1].each > w[0].each) std::swap(w[0], w[1]);
+    const int slots = kSms / best.cg;
+    const double items = w[0].items + w[1].items;
+    if (items <= 16.0 * slots) {
+      double most[2] = {0, 0};
+      for (int flip = 0; flip < 2; flip++) {
+        std::vector<double> load(slots, 0.0);
+        for (int i = 0; i < (int)items; i++) {
+          const int round = i / slots, at = i % slots;
+          double& l = load[flip && (round & 1) ? slots - 1 - at : at];
+          l += i < w[0].items ? w[0].each : w[1].each;
+          most[flip] = std::max(most[flip], l);
+        }
+      }
+      best.flip = most[1] < most[0];
+    }
+  }
   return best;
+}
+
+// Plans are kept by sizes and type: finding one takes some ten microseconds.
+Plan plan_of(const Gemm* g, int count) {
+  Sizes z[kProblems];
+  std::vector<long long> key = {g[0].type};
+  for (int i = 0; i < count; i++) {
+    z[i] = {g[i].M, g[i].N, g[i].K};
+    key.insert(key.end(), {g[i].M, g[i].N, g[i].K});
+  }
+  static std::mutex mu;
+  static std::map<std::vector<long long>, Plan> known;
+  {
+    std::lock_guard<std::mutex> lock(mu);
+    auto it = known.find(key);
+    if (it != known.end()) return it->second;
+  }
+  const Plan plan = choose_plan(z, count, g[0].type);
+  std::lock_guard<std::mutex> lock(mu);
+  if (known.size() > 4096) known.clear();
+  return known[key] = plan;
 }
 
 bool encode(CUtensorMap* map, const Stored& s, int type, int box_x, int box_y) {
@@ -547,14 +685,20 @@ bool encode(CUtensorMap* map, const Stored& s, int type, int box_x, int box_y) {
 }
 
 template <class T, int CG, int P>
-int launch_as(const CUtensorMap& ma, const CUtensorMap& mb, const TcArgs& a, cudaStream_t stream) {
+int launch_as(const TcMaps& maps, const TcArgs& a, cudaStream_t stream) {
   static const char* fn = "linear";
   auto kernel = gemm_tc_kernel<T, CG, P>;
   constexpr int shared = Shape<CG, P>::kShared;
-  GELIB_CUDA_TRY(fn, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared));
-  const long long items = (long long)a.tiles_m * a.tiles_n * a.splits;
+  static std::atomic<uint64_t> allowed{0};   // devices on which the kernel may have this much shared memory
+  int device = 0;
+  GELIB_CUDA_TRY(fn, cudaGetDevice(&device));
+  const uint64_t bit = device < 64 ? 1ull << device : 0;
+  if (!(allowed.load(std::memory_order_relaxed) & bit)) {
+    GELIB_CUDA_TRY(fn, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared));
+    allowed.fetch_or(bit, std::memory_order_relaxed);
+  }
   cudaLaunchConfig_t c = {};
-  c.gridDim = dim3((unsigned)std::min<long long>(items, kSms / CG) * CG);
+  c.gridDim = dim3((unsigned)std::min(a.items, kSms / CG) * CG);
   c.blockDim = dim3(kThreads);
   c.dynamicSmemBytes = shared;
   c.stream = stream;
@@ -563,13 +707,13 @@ int launch_as(const CUtensorMap& ma, const CUtensorMap& mb, const TcArgs& a, cud
   at[0].val.clusterDim.x = CG, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
   c.attrs = at;
   c.numAttrs = CG > 1 ? 1 : 0;
-  GELIB_CUDA_TRY(fn, cudaLaunchKernelEx(&c, kernel, ma, mb, a));
+  GELIB_CUDA_TRY(fn, cudaLaunchKernelEx(&c, kernel, maps, a));
   return launched(fn);
 }
 
 template <class T, int P>
-int launch_config(const Config& c, const CUtensorMap& ma, const CUtensorMap& mb, const TcArgs& a, cudaStream_t stream) {
-  return c.cg == 2 ? launch_as<T, 2, P>(ma, mb, a, stream) : launch_as<T, 1, P>(ma, mb, a, stream);
+int launch_config(int cg, const TcMaps& maps, const TcArgs& a, cudaStream_t stream) {
+  return cg == 2 ? launch_as<T, 2, P>(maps, a, stream) : launch_as<T, 1, P>(maps, a, stream);
 }
 
 }  // namespace
@@ -579,68 +723,57 @@ bool tc_ready(const Stored& s, int type) {
   return is_aligned(s.base, 16) && (s.rows <= 1 || s.ld % 8 == 0);
 }
 
-long long planes_bytes(long long rows, long long cols, int type) { return (cols + 7) / 8 * 8 * rows * (type == GELIB_F32 ? 6 : 2); }
-
-Stored planes_of(const Stored& s, int type, void* memory) {
-  const long long ld = (s.cols + 7) / 8 * 8;
-  return {memory, s.rows, s.cols, ld, s.rows * ld, type == GELIB_F32 ? 3 : 1};
+long long tc_gemm_workspace(const Gemm* g, int count) {
+  const Plan p = plan_of(g, count);
+  long long bytes = 0;
+  for (int i = 0; i < count; i++)
+    if (p.c[i].splits > 1) bytes += (p.c[i].splits * g[i].M * g[i].N * 4 + 255) / 256 * 256;
+  return bytes;
 }
 
-int launch_planes(const Stored* from, const Stored* to, int count, int type, cudaStream_t stream) {
-  PlaneJobs jobs = {};
-  long long chunks = 0;
-  for (int i = 0; i < count; i++) {
-    jobs.from[i] = from[i];
-    jobs.to[i] = const_cast<void*>(to[i].base);
-    jobs.wide[i] = is_aligned(from[i].base, 16) && from[i].ld * type_bytes(type) % 16 == 0;
-    jobs.first[i] = chunks;
-    chunks += (from[i].cols + 7) / 8 * from[i].rows;
-  }
-  jobs.first[count] = chunks;
-  jobs.count = count;
-  if (chunks == 0) return GELIB_OK;
-  const unsigned blocks = (unsigned)std::min((chunks + 255) / 256, (long long)kSms * 16);
-  if (type == GELIB_F32) planes_kernel<float><<<blocks, 256, 0, stream>>>(jobs);
-  else if (type == GELIB_BF16) planes_kernel<__nv_bfloat16><<<blocks, 256, 0, stream>>>(jobs);
-  else planes_kernel<__half><<<blocks, 256, 0, stream>>>(jobs);
-  return launched("linear");
-}
-
-long long tc_gemm_workspace(long long M, long long N, long long K, int type) {
-  const Config c = choose_config(M, N, K, type);
-  return c.splits > 1 ? (long long)c.splits * M * N * 4 : 0;
-}
-
-int launch_tc_gemm(const Gemm& g, void* workspace, cudaStream_t stream) {
+int launch_tc_gemm(const Gemm* g, int count, void* workspace, Joins* joins, cudaStream_t stream) {
   static const char* fn = "linear";
-  const Config c = choose_config(g.M, g.N, g.K, g.type);
-  CUtensorMap ma, mb;
-  // rows across the sum: 64 deep and a tile's rows; rows along it: 64 columns and 64 deep
-  if (!encode(&ma, g.a.s, g.type, 64, g.a.by_sum ? 64 : 128) || !encode(&mb, g.b.s, g.type, 64, g.b.by_sum ? 64 : c.bn / c.cg))
-    return fail(GELIB_CUDA_ERROR, fn, "a tensor map could not be made");
+  const Plan plan = plan_of(g, count);
+  TcMaps maps;
   TcArgs a = {};
-  a.e = g.e;
-  a.part = c.splits > 1 ? (float*)workspace : nullptr;
+  char* at = (char*)workspace;
+  const Work w0 = work_of({g[0].M, g[0].N, g[0].K}, plan.cg, plan.c[0], g[0].type);
+  const bool swapped = count == 2 && work_of({g[1].M, g[1].N, g[1].K}, plan.cg, plan.c[1], g[1].type).each > w0.each;   // longer items first
+  for (int i = 0; i < count; i++) {
+    const Gemm& q = g[i];
+    const Config& c = plan.c[i];
+    const int k = swapped ? 1 - i : i;
+    // rows across the sum: 64 deep and a tile's rows; rows along it: 64 columns and 64 deep
+    if (!encode(&maps.a[k], q.a.s, q.type, 64, q.a.by_sum ? 64 : 128) || !encode(&maps.b[k], q.b.s, q.type, 64, q.b.by_sum ? 64 : c.bn / plan.cg))
+      return fail(GELIB_CUDA_ERROR, fn, "a tensor map could not be made");
+    TcProblem& p = a.p[k];
+    p.e = q.e;
+    if (c.splits > 1) {
+      p.part = (float*)at;
+      at += (c.splits * q.M * q.N * 4 + 255) / 256 * 256;
+      joins->add(q, p.part, c.splits);
+    }
+    p.M = q.M, p.N = (int)q.N;
+    p.slabs = (int)((q.K + kDepth - 1) / kDepth);
+    p.per = (p.slabs + c.splits - 1) / c.splits;
+    p.splits = c.splits;
+    const long long tm = (q.M + 128 * plan.cg - 1) / (128 * plan.cg), tn = (q.N + c.bn - 1) / c.bn;
+    if (tm * tn * c.splits > 0x1fffffffLL) return fail(GELIB_INVALID, fn, "too many elements");
+    p.tiles_m = (int)tm, p.tiles_n = (int)tn, p.items = (int)(tm * tn * c.splits);
+    p.bn = c.bn;
+    p.a_across = q.a.by_sum, p.b_across = q.b.by_sum;
+    const int four = 4 * type_bytes(q.type);
+    p.vec = q.N % 4 == 0 && is_aligned(q.e.y, four) && is_aligned(q.e.z, four) && is_aligned(q.e.residual, four);
+    a.items += p.items;
+  }
+  if (count == 1) maps.a[1] = maps.a[0], maps.b[1] = maps.b[0];
+  a.flip = plan.flip;
   a.status = async_status_word(kStatusGemmTc);
   a.limit = inject_timeout() ? 0 : kWaitLimit;
-  a.M = g.M, a.N = (int)g.N;
-  a.slabs = (int)((g.K + kDepth - 1) / kDepth);
-  a.per = (a.slabs + c.splits - 1) / c.splits;
-  a.splits = c.splits;
-  const long long tm = (g.M + 128 * c.cg - 1) / (128 * c.cg), tn = (g.N + c.bn - 1) / c.bn;
-  if (tm * tn * c.splits > 0x3fffffffLL) return fail(GELIB_INVALID, fn, "too many elements");
-  a.tiles_m = (int)tm, a.tiles_n = (int)tn;
-  a.bn = c.bn;
-  a.a_across = g.a.by_sum, a.b_across = g.b.by_sum;
-  a.bf16 = g.type != GELIB_F16;
-  const int four = 4 * type_bytes(g.type);
-  a.vec = g.N % 4 == 0 && is_aligned(g.e.y, four) && is_aligned(g.e.z, four) && is_aligned(g.e.residual, four);
-  int st;
-  if (g.type == GELIB_F32) st = launch_config<float, 3>(c, ma, mb, a, stream);
-  else if (g.type == GELIB_BF16) st = launch_config<__nv_bfloat16, 1>(c, ma, mb, a, stream);
-  else st = launch_config<__half, 1>(c, ma, mb, a, stream);
-  if (st != GELIB_OK || !a.part) return st;
-  return launch_join(g, a.part, c.splits, stream);
+  a.bf16 = g[0].type != GELIB_F16;
+  if (g[0].type == GELIB_F32) return launch_config<float, 3>(plan.cg, maps, a, stream);
+  if (g[0].type == GELIB_BF16) return launch_config<__nv_bfloat16, 1>(plan.cg, maps, a, stream);
+  return launch_config<__half, 1>(plan.cg, maps, a, stream);
 }
 
 }  // namespace gelib_b200

@@ -81,14 +81,74 @@ __global__ void __launch_bounds__(kThreads) simple_gemm_kernel(Strided a, Stride
     }
 }
 
-// The partial sums added up in their order, and the epilogue.
+// The partial sums added up in their order, and the epilogue; columns' sums in the last blocks.  A block has 32 accesses side by side and eight
+// threads for each, which share the parts where there are many; their sums are added in a fixed order.
+struct JoinArgs {
+  Joins joins;
+  long long blocks[3];   // of the two joins and of the sums
+};
+
+template <class T, int V>
+__device__ __forceinline__ void join_block(const Joins::Join& a, long long block, float (&t)[8][32][5]) {
+  const int lane = threadIdx.x % 32, group = threadIdx.x / 32;
+  const bool shared = a.parts >= 16;
+  const long long at = shared ? (block * 32 + lane) * V : (block * kThreads + threadIdx.x) * V;
+  float d[V];
+#pragma unroll
+  for (int j = 0; j < V; j++) d[j] = 0;
+  if (at < a.size) {
+    const int step = shared ? 8 : 1;
+#pragma unroll 4
+    for (int i = shared ? group : 0; i < a.parts; i += step) {
+      float v[V];
+      load_vec<float, V>(a.part + i * a.size + at, v);
+#pragma unroll
+      for (int j = 0; j < V; j++) d[j] += v[j];
+    }
+  }
+  if (shared) {
+#pragma unroll
+    for (int j = 0; j < V; j++) t[group][lane][j] = d[j];
+    __syncthreads();
+    if (group > 0) return;
+#pragma unroll
+    for (int j = 0; j < V; j++) {
+      d[j] = 0;
+#pragma unroll
+      for (int i = 0; i < 8; i++) d[j] += t[i][lane][j];
+    }
+  }
+  if (at < a.size)
+#pragma unroll
+    for (int j = 0; j < V; j++) finish<T>(a.e, at + j, (int)((at + j) % a.N), d[j]);
+}
+
 template <class T>
-__global__ void __launch_bounds__(kThreads) join_kernel(Epilogue e, const float* part, int parts, long long M, int N) {
-  const long long size = M * N;
-  for (long long at = (long long)blockIdx.x * kThreads + threadIdx.x; at < size; at += (long long)gridDim.x * kThreads) {
-    float d = 0;
-    for (int i = 0; i < parts; i++) d += part[i * size + at];
-    finish<T>(e, at, (int)(at % N), d);
+__global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ JoinArgs a) {
+  __shared__ float t[8][32][5];
+  long long block = blockIdx.x;
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    if (block < a.blocks[i]) {
+      if (a.joins.j[i].vec) join_block<T, 4>(a.joins.j[i], block, t);
+      else join_block<T, 1>(a.joins.j[i], block, t);
+      return;
+    }
+    block -= a.blocks[i];
+  }
+  const int lane = threadIdx.x % 32, group = threadIdx.x / 32, n = a.joins.sum_n;
+  const long long c = block * 32 + lane;
+  float s = 0;
+  if (c < n)
+#pragma unroll 8
+    for (int i = group; i < a.joins.sum_parts; i += 8) s += a.joins.sums[(long long)i * n + c];
+  t[group][lane][0] = s;
+  __syncthreads();
+  if (group == 0 && c < n) {
+    s = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) s += t[i][lane][0];
+    static_cast<T*>(a.joins.gb)[c] = from_float<T>(s);
   }
 }
 
@@ -104,43 +164,115 @@ Split split_of(long long M, long long N, long long K) {
   parts = std::max(1LL, depth ? (K + depth - 1) / depth : 1);
   return {(int)parts, depth};
 }
-long long simple_workspace(long long M, long long N, long long K) {
-  const Split s = split_of(M, N, K);
-  return s.parts > 1 ? s.parts * M * N * 4 : 0;
+long long simple_workspace(const Gemm& g) {
+  if (takes_rows(g)) return 0;
+  const Split s = split_of(g.M, g.N, g.K);
+  return s.parts > 1 ? (s.parts * g.M * g.N * 4 + 255) / 256 * 256 : 0;
 }
 
-template <class T>
-int launch_simple_as(const Gemm& g, float* part, const Split& s, unsigned tiles, cudaStream_t stream) {
-  simple_gemm_kernel<T><<<dim3(tiles, s.parts), kThreads, 0, stream>>>(strided(g.a), strided(g.b), g, part, s.depth);
-  const int st = launched("linear");
-  return st != GELIB_OK || !part ? st : launch_join(g, part, s.parts, stream);
-}
-
-int launch_simple(const Gemm& g, void* workspace, cudaStream_t stream) {
+int launch_simple(const Gemm& g, void* workspace, Joins* joins, cudaStream_t stream) {
   if (takes_rows(g)) return launch_rows(g, stream);
   const Split s = split_of(g.M, g.N, g.K);
   float* part = s.parts > 1 ? (float*)workspace : nullptr;
+  if (part) joins->add(g, part, s.parts);
   const long long tiles = ((g.N + kTile - 1) / kTile) * ((g.M + kTile - 1) / kTile);
   if (tiles > 0x7fffffffLL) return fail(GELIB_INVALID, "linear", "too many elements");
-  return g.type == GELIB_F32 ? launch_simple_as<float>(g, part, s, (unsigned)tiles, stream)
-         : g.type == GELIB_BF16 ? launch_simple_as<__nv_bfloat16>(g, part, s, (unsigned)tiles, stream)
-                                : launch_simple_as<__half>(g, part, s, (unsigned)tiles, stream);
+  const dim3 grid((unsigned)tiles, s.parts);
+  const Strided a = strided(g.a), b = strided(g.b);
+  if (g.type == GELIB_F32) simple_gemm_kernel<float><<<grid, kThreads, 0, stream>>>(a, b, g, part, s.depth);
+  else if (g.type == GELIB_BF16) simple_gemm_kernel<__nv_bfloat16><<<grid, kThreads, 0, stream>>>(a, b, g, part, s.depth);
+  else simple_gemm_kernel<__half><<<grid, kThreads, 0, stream>>>(a, b, g, part, s.depth);
+  return launched("linear");
 }
 
-// ---- gz = gy act'(z) and its column sums ------------------------------------------------------------------------------------------
+// ---- before the products: gz = gy act'(z) and its column sums, and operands as the tensor cores want them --------------------------
 
-// Block (x, y): `wide` accesses of V columns, piece y of the rows.  gz.base may be null (not wanted), sums too.
+// Operands to be copied: as three planes, or with rows on 16-byte boundaries.
+struct PlaneJobs {
+  Stored from[3];
+  Stored to[3];
+  long long first[4];   // number of a job's first chunk of eight columns; the last entry is the end
+  int wide[3];          // rows begin on 16-byte boundaries
+  int count;
+  void add(const Stored& f, const Stored& t, int type) {
+    from[count] = f, to[count] = t;
+    wide[count] = is_aligned(f.base, 16) && f.ld * type_bytes(type) % 16 == 0;
+    first[count + 1] = first[count] + (f.cols + 7) / 8 * f.rows;
+    count++;
+  }
+};
+
+template <class T>
+__device__ __forceinline__ void copy_planes(const PlaneJobs& jobs, long long block, long long blocks) {
+  for (long long c = block * kThreads + threadIdx.x; c < jobs.first[jobs.count]; c += blocks * kThreads) {
+    int job = 0;
+    while (job + 1 < jobs.count && c >= jobs.first[job + 1]) job++;
+    const Stored& f = jobs.from[job];
+    const Stored& t = jobs.to[job];
+    const long long chunks = (f.cols + 7) / 8, at = c - jobs.first[job], row = at / chunks, col = (at - row * chunks) * 8;
+    const T* src = static_cast<const T*>(f.base) + row * f.ld + col;
+    const int live = (int)min(8LL, f.cols - col);
+    T x[8];
+    if (jobs.wide[job] && live == 8) {
+      constexpr int kLoads = sizeof(T) / 2;   // of 16 bytes
+      union { uint4 u[kLoads]; T t[8]; } w;
+#pragma unroll
+      for (int i = 0; i < kLoads; i++) w.u[i] = reinterpret_cast<const uint4*>(src)[i];
+#pragma unroll
+      for (int j = 0; j < 8; j++) x[j] = w.t[j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; j++) x[j] = j < live ? src[j] : from_float<T>(0.f);
+    }
+    if constexpr (sizeof(T) == 4) {
+      union { uint4 u; __nv_bfloat16 t[8]; } w[3];
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        __nv_bfloat16 p[3];
+        split3(x[j], p);
+#pragma unroll
+        for (int i = 0; i < 3; i++) w[i].t[j] = p[i];
+      }
+#pragma unroll
+      for (int i = 0; i < 3; i++) *reinterpret_cast<uint4*>((__nv_bfloat16*)t.base + i * t.plane + row * t.ld + col) = w[i].u;
+    } else {
+      union { uint4 u; T t[8]; } w;
+#pragma unroll
+      for (int j = 0; j < 8; j++) w.t[j] = x[j];
+      *reinterpret_cast<uint4*>((T*)t.base + row * t.ld + col) = w.u;
+    }
+  }
+}
+
+struct ActBack {
+  Stored gz;              // base null: not wanted
+  float* sums;            // (parts, N), or null
+  const void *gy, *z;
+  long long M, per;       // rows, and of a piece
+  int N, act;
+  int wide, chunks, parts;   // a block has `wide` accesses side by side; chunks * parts blocks, 0 where there is nothing to do
+};
+
 template <class T, int V>
-__global__ void __launch_bounds__(kThreads) act_back_kernel(Stored gz, float* sums, const T* gy, const T* z, long long M, int N, int act, int wide, long long per) {
+__global__ void __launch_bounds__(kThreads) prepare_kernel(const __grid_constant__ ActBack a, const __grid_constant__ PlaneJobs jobs) {
   __shared__ float chan[kThreads * V];
-  const int tx = threadIdx.x % wide, ty = threadIdx.x / wide, high = kThreads / wide;
-  const int c = ((int)blockIdx.x * wide + tx) * V;
-  const long long r1 = min(M, ((long long)blockIdx.y + 1) * per);
+  const int blocks = a.chunks * a.parts;
+  if ((int)blockIdx.x >= blocks) {
+    copy_planes<T>(jobs, blockIdx.x - blocks, gridDim.x - blocks);
+    return;
+  }
+  const Stored& gz = a.gz;
+  float* sums = a.sums;
+  const T *gy = static_cast<const T*>(a.gy), *z = static_cast<const T*>(a.z);
+  const long long M = a.M, piece = blockIdx.x / a.chunks;
+  const int N = a.N, act = a.act, wide = a.wide, tx = threadIdx.x % wide, ty = threadIdx.x / wide, high = kThreads / wide;
+  const int c = ((int)blockIdx.x % a.chunks * wide + tx) * V;
+  const long long r1 = min(M, (piece + 1) * a.per);
   float s[V];
 #pragma unroll
   for (int j = 0; j < V; j++) s[j] = 0;
   if (ty < high && c < N)
-    for (long long r = blockIdx.y * per + ty; r < r1; r += high) {
+    for (long long r = piece * a.per + ty; r < r1; r += high) {
       float g[V];
       load_vec<T, V>(gy + r * N + c, g);
       if (act != GELIB_ACT_NONE) {
@@ -176,7 +308,7 @@ __global__ void __launch_bounds__(kThreads) act_back_kernel(Stored gz, float* su
     for (int j = 0; j < V; j++) {
       float t = 0;
       for (int i = 0; i < high; i++) t += chan[(i * wide + tx) * V + j];
-      sums[(long long)blockIdx.y * N + c + j] = t;
+      sums[piece * N + c + j] = t;
     }
 }
 
@@ -190,18 +322,24 @@ Pieces pieces_of(long long M, int N, int type, bool aligned) {
   p.wide = std::min(N / p.V, kThreads);
   p.chunks = (N / p.V + p.wide - 1) / p.wide;
   const int high = kThreads / p.wide;
-  const long long parts = std::max(1LL, std::min((M + 4 * high - 1) / (4 * high), (long long)(kSms * 8 + p.chunks - 1) / p.chunks));
+  const long long parts = std::max(1LL, std::min((M + 4 * high - 1) / (4 * high), (long long)(kSms * 4 + p.chunks - 1) / p.chunks));
   p.per = (M + parts - 1) / parts;
   p.parts = (int)((M + p.per - 1) / p.per);
   return p;
 }
 
 template <class T>
-int launch_act_back(const Stored& gz, float* sums, const gelib_linear_args& p, const Pieces& q, cudaStream_t stream) {
-  constexpr int kWide = 16 / sizeof(T);
-  const auto kernel = q.V > 1 ? act_back_kernel<T, kWide> : act_back_kernel<T, 1>;
-  kernel<<<dim3(q.chunks, q.parts), kThreads, 0, stream>>>(gz, sums, (const T*)p.gy, (const T*)p.z, p.m, p.n, p.act, q.wide, q.per);
-  return launched("linear_back");
+int launch_prepare_as(const ActBack& a, int V, const PlaneJobs& jobs, cudaStream_t stream) {
+  const long long copies = std::min((jobs.first[jobs.count] + kThreads - 1) / kThreads, (long long)kSms * 8);
+  const unsigned blocks = (unsigned)(a.chunks * a.parts + copies);
+  if (blocks == 0) return GELIB_OK;
+  if (V > 1) prepare_kernel<T, 16 / sizeof(T)><<<blocks, kThreads, 0, stream>>>(a, jobs);
+  else prepare_kernel<T, 1><<<blocks, kThreads, 0, stream>>>(a, jobs);
+  return launched("linear");
+}
+int launch_prepare(const ActBack& a, int V, const PlaneJobs& jobs, int type, cudaStream_t stream) {
+  return type == GELIB_F32 ? launch_prepare_as<float>(a, V, jobs, stream)
+         : type == GELIB_BF16 ? launch_prepare_as<__nv_bfloat16>(a, V, jobs, stream) : launch_prepare_as<__half>(a, V, jobs, stream);
 }
 
 long long up(long long bytes) { return (bytes + 255) / 256 * 256; }
@@ -214,62 +352,129 @@ bool takes_tc(long long m, long long k, long long n) { return k > 0 && m > 16 &&
 Stored x_of(const gelib_linear_args& p) { return {p.x, p.m, p.k, p.ldx, 0, 1}; }
 Stored w_of(const gelib_linear_args& p) { return {p.w, p.w_transposed ? p.n : p.k, p.w_transposed ? p.k : p.n, p.ldw, 0, 1}; }
 
+long long planes_bytes(long long rows, long long cols, int type) { return up((cols + 7) / 8 * 8 * rows * (type == GELIB_F32 ? 6 : 2)); }
+Stored planes_at(const Stored& s, int type, char*& at) {
+  const long long ld = (s.cols + 7) / 8 * 8;
+  const Stored to = {at, s.rows, s.cols, ld, s.rows * ld, type == GELIB_F32 ? 3 : 1};
+  at += planes_bytes(s.rows, s.cols, type);
+  return to;
+}
+
 // Bytes that an operand's copy takes, 0 where it is used as it lies.
-long long copy_bytes(const Stored& s, int type) { return tc_ready(s, type) ? 0 : up(planes_bytes(s.rows, s.cols, type)); }
+long long copy_bytes(const Stored& s, int type) { return tc_ready(s, type) ? 0 : planes_bytes(s.rows, s.cols, type); }
+void copy_if_needed(Stored* s, int type, char*& at, PlaneJobs* jobs) {
+  if (tc_ready(*s, type)) return;
+  const Stored to = planes_at(*s, type, at);
+  jobs->add(*s, to, type);
+  *s = to;
+}
 
 long long sums_bytes(const gelib_linear_args& p) {
   return up(4LL * p.n * std::max(pieces_of(p.m, p.n, p.type, false).parts, pieces_of(p.m, p.n, p.type, true).parts));
 }
 
-// Puts copies of those that need one behind each other at `at`, by one launch.
-int ready(Stored** of, int count, int type, char*& at, cudaStream_t stream) {
-  Stored from[3], to[3];
-  int n = 0;
-  for (int i = 0; i < count; i++) {
-    if (tc_ready(*of[i], type)) continue;
-    from[n] = *of[i];
-    to[n] = planes_of(*of[i], type, at);
-    at += up(planes_bytes(of[i]->rows, of[i]->cols, type));
-    *of[i] = to[n++];
+// The forward's product; the backward's, those of them that are wanted, whose operands x, w, gz may be copies.
+Gemm forward_of(const gelib_linear_args& p, const Stored& x, const Stored& w) {
+  Gemm g = {};
+  g.a = {x, false};
+  g.b = {w, !p.w_transposed};
+  g.e = {p.y, p.z, p.bias, p.residual, p.act};
+  g.M = p.m, g.N = p.n, g.K = p.k, g.type = p.type;
+  return g;
+}
+int backward_of(const gelib_linear_args& p, const Stored& x, const Stored& w, const Stored& gz, Gemm (&g)[2]) {
+  int count = 0;
+  if (p.gx && p.k) {
+    Gemm& q = g[count++];
+    q = {};
+    q.a = {gz, false};
+    q.b = {w, p.w_transposed != 0};
+    q.e.y = p.gx;
+    q.M = p.m, q.N = p.k, q.K = p.n, q.type = p.type;
   }
-  return launch_planes(from, to, n, type, stream);
+  if (p.gw && p.k) {   // in w's own layout: x^T gz, or its transpose gz^T x
+    Gemm& q = g[count++];
+    q = {};
+    q.a = {p.w_transposed ? gz : x, true};
+    q.b = {p.w_transposed ? x : gz, true};
+    q.e.y = p.gw;
+    q.M = p.w_transposed ? p.n : p.k, q.N = p.w_transposed ? p.k : p.n, q.K = p.m, q.type = p.type;
+  }
+  return count;
+}
+
+long long products_workspace(const Gemm* g, int count, bool tc) {
+  if (tc) return count ? tc_gemm_workspace(g, count) : 0;
+  long long bytes = 0;
+  for (int i = 0; i < count; i++) bytes += simple_workspace(g[i]);
+  return bytes;
+}
+int launch_products(const Gemm* g, int count, bool tc, char* at, Joins* joins, cudaStream_t stream) {
+  if (tc) return count ? launch_tc_gemm(g, count, at, joins, stream) : GELIB_OK;
+  for (int i = 0; i < count; i++) {
+    const int st = launch_simple(g[i], at, joins, stream);
+    if (st != GELIB_OK) return st;
+    at += simple_workspace(g[i]);
+  }
+  return GELIB_OK;
 }
 
 }  // namespace
 
-int launch_join(const Gemm& g, const float* part, int parts, cudaStream_t stream) {
-  const unsigned blocks = (unsigned)std::min((g.M * g.N + kThreads - 1) / kThreads, 1LL << 20);
-  if (g.type == GELIB_F32) join_kernel<float><<<blocks, kThreads, 0, stream>>>(g.e, part, parts, g.M, (int)g.N);
-  else if (g.type == GELIB_BF16) join_kernel<__nv_bfloat16><<<blocks, kThreads, 0, stream>>>(g.e, part, parts, g.M, (int)g.N);
-  else join_kernel<__half><<<blocks, kThreads, 0, stream>>>(g.e, part, parts, g.M, (int)g.N);
+void Joins::add(const Gemm& g, const float* part, int parts) {
+  const int four = 4 * type_bytes(g.type);
+  const bool vec = g.N % 4 == 0 && is_aligned(g.e.y, four);
+  j[count++] = {g.e, part, parts, (int)g.N, vec, g.M * g.N};
+}
+
+int launch_joins(const Joins& joins, int type, cudaStream_t stream) {
+  JoinArgs a = {};
+  a.joins = joins;
+  long long blocks = 0;
+  for (int i = 0; i < joins.count; i++) {
+    const Joins::Join& q = joins.j[i];
+    const long long each = (long long)(q.parts >= 16 ? 32 : kThreads) * (q.vec ? 4 : 1);
+    a.blocks[i] = (q.size + each - 1) / each;
+    blocks += a.blocks[i];
+  }
+  if (joins.gb) blocks += a.blocks[2] = (joins.sum_n + 31) / 32;
+  if (blocks == 0) return GELIB_OK;
+  if (blocks > 0x7fffffffLL) return fail(GELIB_INVALID, "linear", "too many elements");
+  if (type == GELIB_F32) join_kernel<float><<<(unsigned)blocks, kThreads, 0, stream>>>(a);
+  else if (type == GELIB_BF16) join_kernel<__nv_bfloat16><<<(unsigned)blocks, kThreads, 0, stream>>>(a);
+  else join_kernel<__half><<<(unsigned)blocks, kThreads, 0, stream>>>(a);
   return launched("linear");
 }
 
 long long linear_workspace(const gelib_linear_args& p, bool backward) {
   if (p.m == 0 || p.n == 0) return 0;
   const bool tc = takes_tc(p.m, p.k, p.n);
-  const auto gemm = [&](long long M, long long N, long long K) { return tc ? tc_gemm_workspace(M, N, K, p.type) : simple_workspace(M, N, K); };
-  const long long copies = tc ? copy_bytes(x_of(p), p.type) + copy_bytes(w_of(p), p.type) : 0;
-  if (!backward) return copies + gemm(p.m, p.n, p.k);
-  const long long gz = up(planes_bytes(p.m, p.n, p.type));
-  return gz + copies + sums_bytes(p) + std::max(gemm(p.m, p.k, p.n), p.w_transposed ? gemm(p.n, p.k, p.m) : gemm(p.k, p.n, p.m));
+  const Stored x = x_of(p), w = w_of(p), gz = {p.gy, p.m, p.n, p.n, 0, 1};
+  const long long copies = tc ? copy_bytes(x, p.type) + copy_bytes(w, p.type) : 0;
+  if (!backward) {
+    const Gemm g = forward_of(p, x, w);
+    return copies + products_workspace(&g, 1, tc);
+  }
+  Gemm g[2];
+  const int count = backward_of(p, x, w, gz, g);
+  return planes_bytes(p.m, p.n, p.type) + copies + sums_bytes(p) + products_workspace(g, count, tc);
 }
 
 int launch_linear(const gelib_linear_args& p, void* workspace, cudaStream_t stream) {
-  Gemm g;
   Stored x = x_of(p), w = w_of(p);
   const bool tc = takes_tc(p.m, p.k, p.n);
   char* at = (char*)workspace;
+  int st;
   if (tc) {
-    Stored* both[2] = {&x, &w};
-    const int st = ready(both, 2, p.type, at, stream);
-    if (st != GELIB_OK) return st;
+    PlaneJobs jobs = {};
+    copy_if_needed(&x, p.type, at, &jobs);
+    copy_if_needed(&w, p.type, at, &jobs);
+    if ((st = launch_prepare({}, 1, jobs, p.type, stream)) != GELIB_OK) return st;
   }
-  g.a = {x, false};
-  g.b = {w, !p.w_transposed};
-  g.e = {p.y, p.z, p.bias, p.residual, p.act};
-  g.M = p.m, g.N = p.n, g.K = p.k, g.type = p.type;
-  return tc ? launch_tc_gemm(g, at, stream) : launch_simple(g, at, stream);
+  const Gemm g = forward_of(p, x, w);
+  Joins joins;
+  if ((st = launch_products(&g, 1, tc, at, &joins, stream)) != GELIB_OK) return st;
+  return launch_joins(joins, p.type, stream);
 }
 
 int launch_linear_back(const gelib_linear_args& p, void* workspace, cudaStream_t stream) {
@@ -283,52 +488,40 @@ int launch_linear_back(const gelib_linear_args& p, void* workspace, cudaStream_t
   }
   const bool tc = takes_tc(p.m, p.k, p.n), products = (p.gx || p.gw) && p.k;
   char* at = (char*)workspace;
-  float* sums = (float*)at;
-  at += sums_bytes(p);
+  Joins joins;
+  if (p.gb) {
+    joins.sums = (float*)at;
+    joins.gb = p.gb;
+    joins.sum_n = p.n;
+    at += sums_bytes(p);
+  }
   // gz: gy as it lies, or written (as the tensor cores want it) by the pass that also sums its columns
-  Stored gz = {p.gy, p.m, p.n, p.n, 0, 1}, out = {nullptr, 0, 0, 0, 0, 0};
+  Stored gz = {p.gy, p.m, p.n, p.n, 0, 1}, x = x_of(p), w = w_of(p);
+  ActBack back = {};
+  PlaneJobs jobs = {};
   if (products && (p.act != GELIB_ACT_NONE || (tc && !tc_ready(gz, p.type)))) {
-    out = tc ? planes_of(gz, p.type, at) : Stored{at, p.m, p.n, p.n, 0, 1};
-    gz = out;
-    at += up(planes_bytes(p.m, p.n, p.type));
+    if (tc) gz = planes_at(gz, p.type, at);
+    else {
+      gz.base = at;
+      at += planes_bytes(p.m, p.n, p.type);
+    }
+    back.gz = gz;
   }
-  int st;
-  if (out.base || p.gb) {
-    const Pieces q = pieces_of(p.m, p.n, p.type, is_aligned(p.gy, 16) && is_aligned(p.z, 16));
-    float* s = p.gb ? sums : nullptr;
-    st = p.type == GELIB_F32 ? launch_act_back<float>(out, s, p, q, stream)
-         : p.type == GELIB_BF16 ? launch_act_back<__nv_bfloat16>(out, s, p, q, stream) : launch_act_back<__half>(out, s, p, q, stream);
-    if (st != GELIB_OK) return st;
-    if (p.gb && (st = launch_sum_parts(p.gb, nullptr, sums, q.parts, p.n, p.type, stream)) != GELIB_OK) return st;
+  if (tc && p.gw) copy_if_needed(&x, p.type, at, &jobs);
+  if (tc && p.gx) copy_if_needed(&w, p.type, at, &jobs);
+  const Pieces q = pieces_of(p.m, p.n, p.type, is_aligned(p.gy, 16) && is_aligned(p.z, 16));
+  if (back.gz.base || p.gb) {
+    back.sums = (float*)joins.sums;
+    back.gy = p.gy, back.z = p.z, back.M = p.m, back.N = p.n, back.act = p.act;
+    back.per = q.per, back.wide = q.wide, back.chunks = q.chunks, back.parts = q.parts;
+    joins.sum_parts = q.parts;
   }
-  if (!products) return GELIB_OK;
-  Stored x = x_of(p), w = w_of(p);
-  if (tc) {
-    Stored* of[2];
-    int n = 0;
-    if (p.gw) of[n++] = &x;
-    if (p.gx) of[n++] = &w;
-    if ((st = ready(of, n, p.type, at, stream)) != GELIB_OK) return st;
-  }
-  Gemm g;
-  g.e = {nullptr, nullptr, nullptr, nullptr, GELIB_ACT_NONE};
-  g.type = p.type;
-  if (p.gx) {
-    g.a = {gz, false};
-    g.b = {w, p.w_transposed != 0};
-    g.e.y = p.gx;
-    g.M = p.m, g.N = p.k, g.K = p.n;
-    if ((st = tc ? launch_tc_gemm(g, at, stream) : launch_simple(g, at, stream)) != GELIB_OK) return st;
-  }
-  if (p.gw) {
-    // in w's own layout: x^T gz, or its transpose gz^T x
-    g.a = {p.w_transposed ? gz : x, true};
-    g.b = {p.w_transposed ? x : gz, true};
-    g.e.y = p.gw;
-    g.M = p.w_transposed ? p.n : p.k, g.N = p.w_transposed ? p.k : p.n, g.K = p.m;
-    if ((st = tc ? launch_tc_gemm(g, at, stream) : launch_simple(g, at, stream)) != GELIB_OK) return st;
-  }
-  return GELIB_OK;
+  int st = launch_prepare(back, q.V, jobs, p.type, stream);
+  if (st != GELIB_OK) return st;
+  Gemm g[2];
+  const int count = backward_of(p, x, w, gz, g);
+  if ((st = launch_products(g, count, tc, at, &joins, stream)) != GELIB_OK) return st;
+  return launch_joins(joins, p.type, stream);
 }
 
 }  // namespace gelib_b200

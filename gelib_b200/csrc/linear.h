@@ -33,15 +33,27 @@ struct Gemm {
   int type;      // of the result, and of the operands that have one plane
 };
 
-// Tensor-core products (gemm_tc.cu).  Operands must be `tc_ready`: three planes of a float matrix, or 16-bit, on 16-byte
-// boundaries; launch_planes makes such copies.
+// What is left to do after the products of a call, by one launch: partial sums to be joined, and the bias's gradient.
+struct Joins {
+  struct Join {
+    Epilogue e;
+    const float* part;     // (parts, M, N)
+    int parts, N, vec;
+    long long size;        // M N
+  } j[2];
+  int count = 0;
+  const float* sums = nullptr;   // (sum_parts, sum_n): added up into gb
+  void* gb = nullptr;
+  int sum_parts = 0, sum_n = 0;
+  void add(const Gemm& g, const float* part, int parts);
+};
+int launch_joins(const Joins& joins, int type, cudaStream_t stream);
+
+// Tensor-core products (gemm_tc.cu), one or two of them by one launch.  Operands must be `tc_ready`: three planes of a float matrix, or 16-bit, on 16-byte
+// boundaries.
 bool tc_ready(const Stored& s, int type);
-Stored planes_of(const Stored& s, int type, void* memory);                // where launch_planes will put it
-long long planes_bytes(long long rows, long long cols, int type);
-int launch_planes(const Stored* from, const Stored* to, int count, int type, cudaStream_t stream);
-long long tc_gemm_workspace(long long M, long long N, long long K, int type);
-int launch_tc_gemm(const Gemm& g, void* workspace, cudaStream_t stream);
-int launch_join(const Gemm& g, const float* part, int parts, cudaStream_t stream);   // partial sums (parts, M, N) and the epilogue
+long long tc_gemm_workspace(const Gemm* g, int count);
+int launch_tc_gemm(const Gemm* g, int count, void* workspace, Joins* joins, cudaStream_t stream);
 
 // Products of at most eight rows (linear_rows.cu).
 bool takes_rows(const Gemm& g);

@@ -41,6 +41,14 @@ __device__ __forceinline__ float lanes_sum(float v, int lanes) {
   return v;
 }
 
+// Each of R sums over the lanes, their exchanges side by side.
+template <int R>
+__device__ __forceinline__ void lanes_sums(float (&v)[R], int lanes) {
+  for (int d = lanes >> 1; d; d >>= 1)
+#pragma unroll
+    for (int r = 0; r < R; r++) v[r] += __shfl_xor_sync(0xffffffffu, v[r], d);
+}
+
 template <class T, int V>
 __device__ __forceinline__ void load_or(const void* p, long long at, float other, float (&x)[V]) {
   if (p) load_vec<T, V>(static_cast<const T*>(p) + at, x);
@@ -50,62 +58,109 @@ __device__ __forceinline__ void load_or(const void* p, long long at, float other
 }
 
 // ---- row: s = 1 ----------------------------------------------------------------------------------------------------------------
-// `lanes` lanes (a power of two) own a (row, group): K accesses of V elements each.
+// `lanes` lanes (a power of two) own a group: K accesses of V elements each.  A warp keeps its groups, whose weights it holds, and walks rows, R
+// at a time: their loads and the exchanges of their sums overlap.  Block (x, y): groups, and every gridDim.y-th set of 8 R rows.
 
-template <class T, int V, int K>
+template <class T, int V>
+struct Piece {   // an access as it lies
+  typename Raw<V * sizeof(T)>::type raw;
+  __device__ __forceinline__ void load(const T* p) { raw = *reinterpret_cast<const typename Raw<V * sizeof(T)>::type*>(p); }
+  __device__ __forceinline__ void get(float (&x)[V]) const {
+    union { typename Raw<V * sizeof(T)>::type raw; T t[V]; } w;
+    w.raw = raw;
+#pragma unroll
+    for (int j = 0; j < V; j++) x[j] = to_float(w.t[j]);
+  }
+};
+
+template <class T, int V, int K, int R>
 __global__ void __launch_bounds__(kThreads) row_fwd_kernel(Norm a, int lanes) {
-  const int per = 32 / lanes, lane = threadIdx.x % lanes;
-  const long long item = ((long long)blockIdx.x * kWarps + threadIdx.x / 32) * per + (threadIdx.x & 31) / lanes;
-  const bool live = item < a.b * a.groups;
-  const long long row = live ? item / a.groups : 0;
-  const int g = live ? (int)(item - row * a.groups) : 0, c0 = g * a.cg;
-  const T* x = static_cast<const T*>(a.x) + row * a.n + c0;
-  float v[K][V], sum = 0;
+  const int per = 32 / lanes, lane = threadIdx.x % lanes, warp = threadIdx.x / 32;
+  const int g = blockIdx.x * per + (threadIdx.x & 31) / lanes, c0 = g * a.cg;
+  const bool live = g < a.groups;
+  const float inv = 1.f / a.cg;
+  float w[K][V], bias[K][V];
 #pragma unroll
   for (int k = 0; k < K; k++) {
     const int c = (k * lanes + lane) * V;
-    if (live && c < a.cg) load_vec<T, V>(x + c, v[k]);
-    else
 #pragma unroll
-      for (int j = 0; j < V; j++) v[k][j] = 0;
-#pragma unroll
-    for (int j = 0; j < V; j++) sum += v[k][j];
+    for (int j = 0; j < V; j++) w[k][j] = bias[k][j] = 0;
+    if (live && c < a.cg) {
+      load_or<T, V>(a.w, c0 + c, 1.f, w[k]);
+      load_or<T, V>(a.bias, c0 + c, 0.f, bias[k]);
+    }
   }
-  const float mean = lanes_sum(sum, lanes) / a.cg;
-  float sq = 0;
+  const long long step = (long long)gridDim.y * kWarps * R;
+  for (long long row = ((long long)blockIdx.y * kWarps + warp) * R; row < a.b; row += step) {
+    const T* x = static_cast<const T*>(a.x) + row * a.n + c0;
+    Piece<T, V> v[R][K];
 #pragma unroll
-  for (int k = 0; k < K; k++)
-    if ((k * lanes + lane) * V < a.cg)
+    for (int r = 0; r < R; r++)
 #pragma unroll
-      for (int j = 0; j < V; j++) sq += (v[k][j] - mean) * (v[k][j] - mean);
-  const float rstd = rsqrtf(lanes_sum(sq, lanes) / a.cg + a.eps);
-  if (!live) return;
-  if (a.mean && lane == 0) {
-    a.mean[item] = mean;
-    a.rstd[item] = rstd;
-  }
+      for (int k = 0; k < K; k++) {
+        const int c = (k * lanes + lane) * V;
+        if (live && c < a.cg && row + r < a.b) v[r][k].load(x + (long long)r * a.n + c);
+        else v[r][k].raw = {};
+      }
+    float mean[R], rstd[R];
 #pragma unroll
-  for (int k = 0; k < K; k++) {
-    const int c = (k * lanes + lane) * V;
-    if (c < a.cg) {
-      float w[V], bias[V];
-      load_or<T, V>(a.w, c0 + c, 1.f, w);
-      load_or<T, V>(a.bias, c0 + c, 0.f, bias);
+    for (int r = 0; r < R; r++) {
+      mean[r] = 0;
 #pragma unroll
-      for (int j = 0; j < V; j++) v[k][j] = (v[k][j] - mean) * rstd * w[j] + bias[j];
-      activate(v[k], a.act);
-      store_vec<T, V>(static_cast<T*>(a.y) + row * a.n + c0 + c, v[k]);
+      for (int k = 0; k < K; k++) {
+        float f[V];
+        v[r][k].get(f);
+#pragma unroll
+        for (int j = 0; j < V; j++) mean[r] += f[j];
+      }
+    }
+    lanes_sums(mean, lanes);
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+      mean[r] *= inv;
+      rstd[r] = 0;
+#pragma unroll
+      for (int k = 0; k < K; k++)
+        if ((k * lanes + lane) * V < a.cg) {
+          float f[V];
+          v[r][k].get(f);
+#pragma unroll
+          for (int j = 0; j < V; j++) rstd[r] += (f[j] - mean[r]) * (f[j] - mean[r]);
+        }
+    }
+    lanes_sums(rstd, lanes);
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+      rstd[r] = rsqrtf(rstd[r] * inv + a.eps);
+      if (!live || row + r >= a.b) continue;
+      if (a.mean && lane == 0) {
+        a.mean[(row + r) * a.groups + g] = mean[r];
+        a.rstd[(row + r) * a.groups + g] = rstd[r];
+      }
+#pragma unroll
+      for (int k = 0; k < K; k++) {
+        const int c = (k * lanes + lane) * V;
+        if (c < a.cg) {
+          float f[V];
+          v[r][k].get(f);
+#pragma unroll
+          for (int j = 0; j < V; j++) f[j] = (f[j] - mean[r]) * rstd[r] * w[k][j] + bias[k][j];
+          activate(f, a.act);
+          store_vec<T, V>(static_cast<T*>(a.y) + (row + r) * a.n + c0 + c, f);
+        }
+      }
     }
   }
 }
 
-// A warp keeps its groups and walks rows, so that the sums over rows stay in registers; the block's warps have the same groups.
-template <class T, int V, int K>
+// The sums over rows stay in registers; a block's warps have the same groups and add theirs up at the end.
+template <class T, int V, int K, int R>
 __global__ void __launch_bounds__(kThreads) row_bwd_kernel(Norm a, int lanes, int parts) {
   __shared__ float sums[kWarps][2][32 * V];
   const int per = 32 / lanes, lane = threadIdx.x % lanes, warp = threadIdx.x / 32;
   const int g = blockIdx.x * per + (threadIdx.x & 31) / lanes, c0 = g * a.cg;
   const bool live = g < a.groups;
+  const float inv = 1.f / a.cg;
   float w[K][V], bias[K][V], gw[K][V], gb[K][V];
 #pragma unroll
   for (int k = 0; k < K; k++) {
@@ -117,43 +172,76 @@ __global__ void __launch_bounds__(kThreads) row_bwd_kernel(Norm a, int lanes, in
       load_or<T, V>(a.bias, c0 + c, 0.f, bias[k]);
     }
   }
-  for (long long row = (long long)blockIdx.y * kWarps + warp; row < a.b; row += (long long)gridDim.y * kWarps) {
-    const float mean = live ? a.mean[row * a.groups + g] : 0, rstd = live ? a.rstd[row * a.groups + g] : 0;
-    const long long at = row * a.n + c0;
-    float h[K][V], gz[K][V], s1 = 0, s2 = 0;
+  const long long step = (long long)gridDim.y * kWarps * R;
+  Piece<T, V> px[R][K], pg[R][K];
+  float pm[R], pr[R];
+  auto fetch = [&](long long row) {
 #pragma unroll
-    for (int k = 0; k < K; k++) {
-      const int c = (k * lanes + lane) * V;
-      if (live && c < a.cg) {
-        load_vec<T, V>(static_cast<const T*>(a.x) + at + c, h[k]);
-        load_vec<T, V>(static_cast<const T*>(a.gy) + at + c, gz[k]);
+    for (int r = 0; r < R; r++) {
+      const bool there = live && row + r < a.b;
+      pm[r] = there ? a.mean[(row + r) * a.groups + g] : 0.f;
+      pr[r] = there ? a.rstd[(row + r) * a.groups + g] : 0.f;
+#pragma unroll
+      for (int k = 0; k < K; k++) {
+        const int c = (k * lanes + lane) * V;
+        const long long at = (row + r) * a.n + c0 + c;
+        if (there && c < a.cg) {
+          px[r][k].load(static_cast<const T*>(a.x) + at);
+          pg[r][k].load(static_cast<const T*>(a.gy) + at);
+        } else {
+          px[r][k].raw = {};
+          pg[r][k].raw = {};
+        }
+      }
+    }
+  };
+  long long row = ((long long)blockIdx.y * kWarps + warp) * R;
+  if (row < a.b) fetch(row);
+  for (; row < a.b; row += step) {
+    float h[R][K][V], gz[R][K][V], mean[R], rstd[R], s1[R], s2[R];
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+      mean[r] = pm[r], rstd[r] = pr[r];
+#pragma unroll
+      for (int k = 0; k < K; k++) px[r][k].get(h[r][k]), pg[r][k].get(gz[r][k]);
+    }
+    if (row + step < a.b) fetch(row + step);   // on their way while these rows are worked on
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+      s1[r] = s2[r] = 0;
+#pragma unroll
+      for (int k = 0; k < K; k++) {
         float z[V];
 #pragma unroll
         for (int j = 0; j < V; j++) {
-          h[k][j] = (h[k][j] - mean) * rstd;
-          z[j] = h[k][j] * w[k][j] + bias[k][j];
+          h[r][k][j] = (h[r][k][j] - mean[r]) * rstd[r];
+          z[j] = h[r][k][j] * w[k][j] + bias[k][j];
         }
-        activate_back(gz[k], z, a.act);
+        activate_back(gz[r][k], z, a.act);
 #pragma unroll
         for (int j = 0; j < V; j++) {
-          gb[k][j] += gz[k][j];
-          gw[k][j] += gz[k][j] * h[k][j];
-          gz[k][j] *= w[k][j];
-          s1 += gz[k][j];
-          s2 += gz[k][j] * h[k][j];
+          gb[k][j] += gz[r][k][j];
+          gw[k][j] += gz[r][k][j] * h[r][k][j];
+          gz[r][k][j] *= w[k][j];
+          s1[r] += gz[r][k][j];
+          s2[r] += gz[r][k][j] * h[r][k][j];
         }
       }
     }
     if (a.y) {
-      s1 = lanes_sum(s1, lanes) / a.cg;
-      s2 = lanes_sum(s2, lanes) / a.cg;
+      lanes_sums(s1, lanes);
+      lanes_sums(s2, lanes);
 #pragma unroll
-      for (int k = 0; k < K; k++) {
-        const int c = (k * lanes + lane) * V;
-        if (live && c < a.cg) {
+      for (int r = 0; r < R; r++) {
+        s1[r] *= inv, s2[r] *= inv;
 #pragma unroll
-          for (int j = 0; j < V; j++) gz[k][j] = rstd * (gz[k][j] - s1 - h[k][j] * s2);
-          store_vec<T, V>(static_cast<T*>(a.y) + at + c, gz[k]);
+        for (int k = 0; k < K; k++) {
+          const int c = (k * lanes + lane) * V;
+          if (live && c < a.cg && row + r < a.b) {
+#pragma unroll
+            for (int j = 0; j < V; j++) gz[r][k][j] = rstd[r] * (gz[r][k][j] - s1[r] - h[r][k][j] * s2[r]);
+            store_vec<T, V>(static_cast<T*>(a.y) + (row + r) * a.n + c0 + c, gz[r][k]);
+          }
         }
       }
     }
@@ -421,15 +509,24 @@ __global__ void __launch_bounds__(kThreads) piece_stats_kernel(Norm a, int piece
 #pragma unroll
       for (int j = 0; j < V; j++) first[j] = sum[j] = sq[j] = 0;
       if (ty < rows) load_vec<T, V>(x + (long long)ty * a.n + col * V, first);
-      for (int r = ty + cl.high; r < rows; r += cl.high) {
-        float v[V];
-        load_vec<T, V>(x + (long long)r * a.n + col * V, v);
+      constexpr int U = 8;   // rows on their way together
+      for (int r = ty + cl.high; r < rows; r += U * cl.high) {
+        Piece<T, V> p[U];
 #pragma unroll
-        for (int j = 0; j < V; j++) {
-          const float d = v[j] - first[j];
-          sum[j] += d;
-          sq[j] += d * d;
-        }
+        for (int u = 0; u < U; u++)
+          if (r + u * cl.high < rows) p[u].load(x + (long long)(r + u * cl.high) * a.n + col * V);
+#pragma unroll
+        for (int u = 0; u < U; u++)
+          if (r + u * cl.high < rows) {
+            float v[V];
+            p[u].get(v);
+#pragma unroll
+            for (int j = 0; j < V; j++) {
+              const float d = v[j] - first[j];
+              sum[j] += d;
+              sq[j] += d * d;
+            }
+          }
       }
       const int mine = ty < rows ? (rows - ty + cl.high - 1) / cl.high : 0;
 #pragma unroll
@@ -512,20 +609,60 @@ __global__ void __launch_bounds__(kThreads) piece_apply_kernel(Norm a, int piece
       mean[j] = group[g];
       w[j] *= group[a.groups + g];
     }
-    for (int r = ty; r < rows; r += cl.high) {
-      float v[V];
-      load_vec<T, V>(static_cast<const T*>(a.x) + base + (long long)r * a.n + col * V, v);
+    constexpr int U = 4;
+    for (int r = ty; r < rows; r += U * cl.high) {
+      Piece<T, V> p[U];
 #pragma unroll
-      for (int j = 0; j < V; j++) v[j] = (v[j] - mean[j]) * w[j] + bias[j];
-      activate(v, a.act);
-      store_vec<T, V>(static_cast<T*>(a.y) + base + (long long)r * a.n + col * V, v);
+      for (int u = 0; u < U; u++)
+        if (r + u * cl.high < rows) p[u].load(static_cast<const T*>(a.x) + base + (long long)(r + u * cl.high) * a.n + col * V);
+#pragma unroll
+      for (int u = 0; u < U; u++)
+        if (r + u * cl.high < rows) {
+          float v[V];
+          p[u].get(v);
+#pragma unroll
+          for (int j = 0; j < V; j++) v[j] = (v[j] - mean[j]) * w[j] + bias[j];
+          activate(v, a.act);
+          store_vec<T, V>(static_cast<T*>(a.y) + base + (long long)(r + u * cl.high) * a.n + col * V, v);
+        }
     }
   }
 }
 
-// gz xh and gz summed over a piece's rows, per channel: part (2, b * pieces, n).
+// Rows r, r + high, .. of x and gy as they lie, U of them on their way together: f(x - mean times rstd, gz, z's row).
+template <class T, int V, class F>
+__device__ __forceinline__ void each_row(const Norm& a, long long base, int rows, int ty, int high, int col, const float (&w)[V], const float (&bias)[V], const float (&mean)[V],
+                                         const float (&rstd)[V], F f) {
+  constexpr int U = 4;
+  const T *x = static_cast<const T*>(a.x) + base + col * V, *gy = static_cast<const T*>(a.gy) + base + col * V;
+  for (int r = ty; r < rows; r += U * high) {
+    Piece<T, V> px[U], pg[U];
+#pragma unroll
+    for (int u = 0; u < U; u++)
+      if (r + u * high < rows) {
+        px[u].load(x + (long long)(r + u * high) * a.n);
+        pg[u].load(gy + (long long)(r + u * high) * a.n);
+      }
+#pragma unroll
+    for (int u = 0; u < U; u++)
+      if (r + u * high < rows) {
+        float h[V], g[V], z[V];
+        px[u].get(h);
+        pg[u].get(g);
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+          h[j] = (h[j] - mean[j]) * rstd[j];
+          z[j] = h[j] * w[j] + bias[j];
+        }
+        activate_back(g, z, a.act);
+        f(r + u * high, h, g);
+      }
+  }
+}
+
+// gz xh and gz summed over a piece's rows, per channel: part (2, b * pieces, n); and times w, per group: back (b, pieces, groups, 2).
 template <class T, int V>
-__global__ void __launch_bounds__(kThreads) piece_back_sums_kernel(Norm a, int pieces, int per) {
+__global__ void __launch_bounds__(kThreads) piece_back_sums_kernel(Norm a, int pieces, int per, float* back) {
   extern __shared__ __align__(16) unsigned char memory[];
   const long long sample = blockIdx.x / pieces;
   const int piece = blockIdx.x % pieces;
@@ -533,7 +670,7 @@ __global__ void __launch_bounds__(kThreads) piece_back_sums_kernel(Norm a, int p
   const int rows = (int)min((long long)per, a.s - r0);
   const Columns cl = columns_of(a.n, V);
   float* chan = reinterpret_cast<float*>(memory);   // [2][high][n]
-  const int tx = threadIdx.x % cl.wide, ty = threadIdx.x / cl.wide;
+  const int tx = threadIdx.x % cl.wide, ty = threadIdx.x / cl.wide, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const long long base = (sample * a.s + r0) * a.n;
   if (ty < cl.high)
     for (int col = tx; col < cl.cols; col += cl.wide) {
@@ -545,19 +682,10 @@ __global__ void __launch_bounds__(kThreads) piece_back_sums_kernel(Norm a, int p
         const long long g = sample * a.groups + (col * V + j) / a.cg;
         mean[j] = a.mean[g], rstd[j] = a.rstd[g], sw[j] = sb[j] = 0;
       }
-      for (int r = ty; r < rows; r += cl.high) {
-        float h[V], g[V], z[V];
-        load_vec<T, V>(static_cast<const T*>(a.x) + base + (long long)r * a.n + col * V, h);
-        load_vec<T, V>(static_cast<const T*>(a.gy) + base + (long long)r * a.n + col * V, g);
-#pragma unroll
-        for (int j = 0; j < V; j++) {
-          h[j] = (h[j] - mean[j]) * rstd[j];
-          z[j] = h[j] * w[j] + bias[j];
-        }
-        activate_back(g, z, a.act);
+      each_row<T, V>(a, base, rows, ty, cl.high, col, w, bias, mean, rstd, [&](int, const float (&h)[V], const float (&g)[V]) {
 #pragma unroll
         for (int j = 0; j < V; j++) sb[j] += g[j], sw[j] += g[j] * h[j];
-      }
+      });
 #pragma unroll
       for (int j = 0; j < V; j++) {
         chan[ty * a.n + col * V + j] = sw[j];
@@ -570,42 +698,42 @@ __global__ void __launch_bounds__(kThreads) piece_back_sums_kernel(Norm a, int p
     float t = 0;
     for (int i = 0; i < cl.high; i++) t += chan[(which * cl.high + i) * a.n + q];
     a.part[((long long)which * (a.b * pieces) + blockIdx.x) * a.n + q] = t;
+    chan[which * cl.high * a.n + q] = t * (a.w ? to_float(static_cast<const T*>(a.w)[q]) : 1.f);   // row 0 of its part: read by this thread alone so far
   }
-}
-
-// The two means of a (sample, group), from its channels' sums: back (b, groups, 2).
-template <class T>
-__global__ void __launch_bounds__(kThreads) piece_back_groups_kernel(Norm a, int pieces, float* back) {
-  const long long sample = blockIdx.x / a.groups;
-  const int g = blockIdx.x % a.groups;
-  __shared__ float sums[2][kWarps];
-  float s1 = 0, s2 = 0;
-  for (long long e = threadIdx.x; e < (long long)pieces * a.cg; e += kThreads) {
-    const int c = g * a.cg + (int)(e % a.cg);
-    const long long row = sample * pieces + e / a.cg;
-    const float w = a.w ? to_float(static_cast<const T*>(a.w)[c]) : 1.f;
-    s2 += w * a.part[row * a.n + c];
-    s1 += w * a.part[(a.b * pieces + row) * a.n + c];
-  }
-  s1 = warp_total(s1), s2 = warp_total(s2);
-  if (threadIdx.x % 32 == 0) sums[0][threadIdx.x / 32] = s1, sums[1][threadIdx.x / 32] = s2;
+  if (!a.y) return;
   __syncthreads();
-  if (threadIdx.x < 2) {
-    float t = 0;
-    for (int i = 0; i < kWarps; i++) t += sums[threadIdx.x][i];
-    back[(sample * a.groups + g) * 2 + threadIdx.x] = t / ((float)a.s * a.cg);
+  for (int g = warp; g < a.groups; g += kWarps) {
+    float s1 = 0, s2 = 0;
+    for (int c = lane; c < a.cg; c += 32) s2 += chan[g * a.cg + c], s1 += chan[cl.high * a.n + g * a.cg + c];
+    s1 = warp_total(s1), s2 = warp_total(s2);
+    if (lane == 0) {
+      float* out = back + ((sample * pieces + piece) * a.groups + g) * 2;
+      out[0] = s1, out[1] = s2;
+    }
   }
 }
 
 template <class T, int V>
 __global__ void __launch_bounds__(kThreads) piece_back_apply_kernel(Norm a, int pieces, int per, const float* back) {
-  const long long block = (long long)gridDim.x - 1 - blockIdx.x;
+  extern __shared__ __align__(16) unsigned char memory[];
+  const long long block = (long long)gridDim.x - 1 - blockIdx.x;   // what was read last first
   const long long sample = block / pieces;
   const long long r0 = (block % pieces) * (long long)per;
   const int rows = (int)min((long long)per, a.s - r0);
   const Columns cl = columns_of(a.n, V);
-  const int tx = threadIdx.x % cl.wide, ty = threadIdx.x / cl.wide;
+  const int tx = threadIdx.x % cl.wide, ty = threadIdx.x / cl.wide, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const long long base = (sample * a.s + r0) * a.n;
+  float* means = reinterpret_cast<float*>(memory);   // [2][groups]
+  for (int g = warp; g < a.groups; g += kWarps) {
+    float s1 = 0, s2 = 0;
+    for (int i = lane; i < pieces; i += 32) {
+      const float2 q = *reinterpret_cast<const float2*>(back + ((sample * pieces + i) * a.groups + g) * 2);
+      s1 += q.x, s2 += q.y;
+    }
+    s1 = warp_total(s1), s2 = warp_total(s2);
+    if (lane == 0) means[g] = s1 / ((float)a.s * a.cg), means[a.groups + g] = s2 / ((float)a.s * a.cg);
+  }
+  __syncthreads();
   if (ty >= cl.high) return;
   for (int col = tx; col < cl.cols; col += cl.wide) {
     float w[V], bias[V], mean[V], rstd[V], s1[V], s2[V];
@@ -613,23 +741,16 @@ __global__ void __launch_bounds__(kThreads) piece_back_apply_kernel(Norm a, int 
     load_or<T, V>(a.bias, col * V, 0.f, bias);
 #pragma unroll
     for (int j = 0; j < V; j++) {
-      const long long g = sample * a.groups + (col * V + j) / a.cg;
-      mean[j] = a.mean[g], rstd[j] = a.rstd[g], s1[j] = back[2 * g], s2[j] = back[2 * g + 1];
+      const int q = (col * V + j) / a.cg;
+      const long long g = sample * a.groups + q;
+      mean[j] = a.mean[g], rstd[j] = a.rstd[g], s1[j] = means[q], s2[j] = means[a.groups + q];
     }
-    for (int r = ty; r < rows; r += cl.high) {
-      float h[V], g[V], z[V];
-      load_vec<T, V>(static_cast<const T*>(a.x) + base + (long long)r * a.n + col * V, h);
-      load_vec<T, V>(static_cast<const T*>(a.gy) + base + (long long)r * a.n + col * V, g);
+    each_row<T, V>(a, base, rows, ty, cl.high, col, w, bias, mean, rstd, [&](int r, const float (&h)[V], const float (&g)[V]) {
+      float out[V];
 #pragma unroll
-      for (int j = 0; j < V; j++) {
-        h[j] = (h[j] - mean[j]) * rstd[j];
-        z[j] = h[j] * w[j] + bias[j];
-      }
-      activate_back(g, z, a.act);
-#pragma unroll
-      for (int j = 0; j < V; j++) g[j] = rstd[j] * (g[j] * w[j] - s1[j] - h[j] * s2[j]);
-      store_vec<T, V>(static_cast<T*>(a.y) + base + (long long)r * a.n + col * V, g);
-    }
+      for (int j = 0; j < V; j++) out[j] = rstd[j] * (g[j] * w[j] - s1[j] - h[j] * s2[j]);
+      store_vec<T, V>(static_cast<T*>(a.y) + base + (long long)r * a.n + col * V, out);
+    });
   }
 }
 
@@ -644,6 +765,7 @@ __global__ void __launch_bounds__(1024) sum_parts_kernel(T* gw, T* gb, const flo
   const float* p = sums + (long long)blockIdx.y * parts * n;
   float s = 0;
   if (c < n)
+#pragma unroll 8
     for (int i = threadIdx.y; i < parts; i += 32) s += p[(long long)i * n + c];
   t[threadIdx.y][threadIdx.x] = s;
   __syncthreads();
@@ -663,7 +785,7 @@ constexpr int kSharedLimit = 200 * 1024;
 struct Way {
   enum { kRow, kTile, kTwo } way;
   int V;             // elements of an access
-  int lanes, K;      // row
+  int lanes, K, R, across;   // row
   int gpc, chunks;   // tile: groups of a chunk
   size_t shared;     // tile, two
   int parts;         // backward: rows of partial sums
@@ -685,7 +807,10 @@ Way choose(long long b, long long s, int n, int groups, int type, bool wide16, b
       while (w.lanes < need && w.lanes < 32) w.lanes *= 2;
       w.K = need <= 32 ? 1 : 4;
       const int across = (groups + 32 / w.lanes - 1) / (32 / w.lanes);
-      w.parts = (int)std::max(1LL, std::min((b + kWarps - 1) / kWarps, (long long)(kSms * 4 + across - 1) / across));
+      w.across = across;
+      w.R = w.K > 1 ? 1 : backward ? 2 : 4;
+      // rows for every warp, on as many blocks as the SMs hold
+      w.parts = (int)std::max(1LL, std::min((b + kWarps * w.R - 1) / (kWarps * w.R), (long long)(kSms * (backward ? 2 : 4) + across - 1) / across));
       return w;
     }
   }
@@ -780,7 +905,7 @@ long long group_norm_workspace(long long b, long long s, int n, int groups, int 
   for (int k = 0; k < 3; k++) {
     const Way w = choose(b, s, n, groups, type, k == 2, k >= 1, backward);
     long long floats = 0;
-    if (w.way == Way::kTwo) floats = backward ? 2LL * w.parts * n + 2 * b * groups : 2LL * b * w.pieces * groups;
+    if (w.way == Way::kTwo) floats = 2LL * b * w.pieces * groups + (backward ? 2LL * w.parts * n : 0);
     else if (backward) floats = 2LL * w.parts * n;
     most = std::max(most, floats);
   }
@@ -794,7 +919,7 @@ int launch_group_norm(const GroupNormCall& c, cudaStream_t stream) {
   Norm a = {c.x, c.w, c.bias, c.gy, c.y, c.mean, c.rstd, c.workspace, c.b, c.s, c.n, c.groups, c.n / c.groups, c.eps, c.act};
   const bool sums = c.gw || c.gb;
   if (w.way != Way::kTwo && !sums) a.part = nullptr;
-  const long long samples = w.way == Way::kTwo ? c.b * w.pieces : w.way == Way::kTile ? c.b * w.chunks : (c.b * c.groups + kWarps * (32 / w.lanes) - 1) / (kWarps * (32 / w.lanes));
+  const long long samples = w.way == Way::kTwo ? c.b * w.pieces : w.way == Way::kTile ? c.b * w.chunks : 1;
   if (samples > 0x7fffffffLL || (back && c.b * c.groups > 0x7fffffffLL)) return fail(GELIB_INVALID, fn, "too many samples");
   const int st = with_type(c.type, [&](auto* t) -> int {
     using T = std::remove_pointer_t<decltype(t)>;
@@ -802,13 +927,13 @@ int launch_group_norm(const GroupNormCall& c, cudaStream_t stream) {
       constexpr int V = decltype(v)::value;
       int st;
       if (w.way == Way::kRow) {
+        const dim3 grid(w.across, w.parts);
         if (!back) {
-          auto kernel = w.K == 1 ? row_fwd_kernel<T, V, 1> : row_fwd_kernel<T, V, 4>;
-          kernel<<<(unsigned)samples, kThreads, 0, stream>>>(a, w.lanes);
+          auto kernel = w.K == 1 ? row_fwd_kernel<T, V, 1, 4> : row_fwd_kernel<T, V, 4, 1>;
+          kernel<<<grid, kThreads, 0, stream>>>(a, w.lanes);
         } else {
-          auto kernel = w.K == 1 ? row_bwd_kernel<T, V, 1> : row_bwd_kernel<T, V, 4>;
-          const int per = 32 / w.lanes;
-          kernel<<<dim3((c.groups + per - 1) / per, w.parts), kThreads, 0, stream>>>(a, w.lanes, w.parts);
+          auto kernel = w.K == 1 ? row_bwd_kernel<T, V, 1, 2> : row_bwd_kernel<T, V, 4, 1>;
+          kernel<<<grid, kThreads, 0, stream>>>(a, w.lanes, w.parts);
         }
         return launched(fn);
       }
@@ -833,13 +958,12 @@ int launch_group_norm(const GroupNormCall& c, cudaStream_t stream) {
         return launched(fn);
       }
       if ((st = room(fn, piece_back_sums_kernel<T, V>, w.shared)) != GELIB_OK) return st;
-      piece_back_sums_kernel<T, V><<<(unsigned)samples, kThreads, w.shared, stream>>>(a, w.pieces, w.per);
-      if ((st = launched(fn)) != GELIB_OK) return st;
-      if (!a.y) return GELIB_OK;
-      float* means = c.workspace + 2LL * w.parts * c.n;
-      piece_back_groups_kernel<T><<<(unsigned)(c.b * c.groups), kThreads, 0, stream>>>(a, w.pieces, means);
-      if ((st = launched(fn)) != GELIB_OK) return st;
-      piece_back_apply_kernel<T, V><<<(unsigned)samples, kThreads, 0, stream>>>(a, w.pieces, w.per, means);
+      float* back = c.workspace + 2LL * w.parts * c.n;
+      piece_back_sums_kernel<T, V><<<(unsigned)samples, kThreads, w.shared, stream>>>(a, w.pieces, w.per, back);
+      if ((st = launched(fn)) != GELIB_OK || !a.y) return st;
+      const size_t shared = 2ULL * c.groups * 4;
+      if ((st = room(fn, piece_back_apply_kernel<T, V>, shared)) != GELIB_OK) return st;
+      piece_back_apply_kernel<T, V><<<(unsigned)samples, kThreads, shared, stream>>>(a, w.pieces, w.per, back);
       return launched(fn);
     });
   });

@@ -75,12 +75,15 @@ constexpr float kGelu1 = kGelu0 * 0.044715f;
 template <int V>
 __device__ __forceinline__ void activate(float (&x)[V], int act) {
   if (act == GELIB_ACT_NONE) return;
+  if (act == GELIB_ACT_RELU) {
 #pragma unroll
-  for (int k = 0; k < V; k++) {
-    const float z = x[k];
-    if (act == GELIB_ACT_RELU) x[k] = z < 0.f ? 0.f : z;     // NaN stays NaN
-    else if (act == GELIB_ACT_SILU) x[k] = z * logistic(z);
-    else x[k] = z * logistic(z * (kGelu0 + kGelu1 * z * z));
+    for (int k = 0; k < V; k++) x[k] = x[k] < 0.f ? 0.f : x[k];     // NaN stays NaN
+  } else if (act == GELIB_ACT_SILU) {
+#pragma unroll
+    for (int k = 0; k < V; k++) x[k] *= logistic(x[k]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; k++) x[k] *= logistic(x[k] * (kGelu0 + kGelu1 * x[k] * x[k]));
   }
 }
 
@@ -88,12 +91,17 @@ __device__ __forceinline__ void activate(float (&x)[V], int act) {
 template <int V>
 __device__ __forceinline__ void activate_back(float (&g)[V], const float (&x)[V], int act) {
   if (act == GELIB_ACT_NONE) return;
+  if (act == GELIB_ACT_RELU) {
+#pragma unroll
+    for (int k = 0; k < V; k++) g[k] = x[k] > 0.f ? g[k] : x[k] != x[k] ? x[k] : 0.f;
+    return;
+  }
+  // beyond +-128 the derivatives are 1 and 0 to the last bit, and their terms are no longer products of 0 and infinity
+  const bool silu = act == GELIB_ACT_SILU;
 #pragma unroll
   for (int k = 0; k < V; k++) {
-    // beyond +-128 the derivatives are 1 and 0 to the last bit, and their terms are no longer products of 0 and infinity
     const float z = x[k] < -128.f ? -128.f : x[k] > 128.f ? 128.f : x[k];
-    if (act == GELIB_ACT_RELU) g[k] = z > 0.f ? g[k] : z != z ? z : 0.f;
-    else if (act == GELIB_ACT_SILU) {
+    if (silu) {
       const float q = logistic(z);
       g[k] *= q * (1.f + z * (1.f - q));
     } else {

@@ -105,7 +105,7 @@ int gelib_group_norm(void* y, float* mean, float* rstd, const void* x, const voi
     if (b == 0 || s == 0 || n == 0) return GELIB_OK;
     if (!x || !y || !mean != !rstd) return fail(GELIB_INVALID, fn, "null pointer");
     if (!workspace && group_norm_workspace(b, s, n, groups, type, false) > 0) return fail(GELIB_INVALID, fn, "no workspace");
-    if (!all_aligned(type_bytes(type), {x, y, weight, bias}) || !all_aligned(4, {mean, rstd, workspace}))
+    if (!all_aligned(type_bytes(type), {x, y, weight, bias}) || !all_aligned(4, {mean, rstd}) || !is_aligned(workspace, 256))
       return fail(GELIB_INVALID, fn, "data pointer not aligned to its type");
     return launch_group_norm({y, mean, rstd, x, weight, bias, nullptr, nullptr, nullptr, b, s, n, groups, (float)eps, act, type, (float*)workspace},
                              (cudaStream_t)stream);
@@ -126,7 +126,7 @@ int gelib_group_norm_back(void* gx, void* gw, void* gb, const void* gy, const vo
     }
     if (!x || !gy || !mean || !rstd) return fail(GELIB_INVALID, fn, "null pointer");
     if (!workspace && group_norm_workspace(b, s, n, groups, type, true) > 0) return fail(GELIB_INVALID, fn, "no workspace");
-    if (!all_aligned(type_bytes(type), {x, gy, gx, gw, gb, weight, bias}) || !all_aligned(4, {mean, rstd, workspace}))
+    if (!all_aligned(type_bytes(type), {x, gy, gx, gw, gb, weight, bias}) || !all_aligned(4, {mean, rstd}) || !is_aligned(workspace, 256))
       return fail(GELIB_INVALID, fn, "data pointer not aligned to its type");
     return launch_group_norm({gx, (float*)mean, (float*)rstd, x, weight, bias, gy, gw, gb, b, s, n, groups, 0.f, act, type, (float*)workspace},
                              (cudaStream_t)stream);
