@@ -24,6 +24,14 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
+#ifndef RF
+#define RF 2
+#define RB 1
+#define BF 4
+#define BB 3
+#endif
+constexpr int kRowsAhead = RF, kRowsBack = RB;        // of a warp at a time, forward and backward
+constexpr int kBlocksAhead = BF, kBlocksBack = BB;    // of an SM
 
 struct Norm {
   const void *x, *w, *bias, *gy;
@@ -65,16 +73,11 @@ template <class T, int V>
 struct Piece {   // an access as it lies
   typename Raw<V * sizeof(T)>::type raw;
   __device__ __forceinline__ void load(const T* p) { raw = *reinterpret_cast<const typename Raw<V * sizeof(T)>::type*>(p); }
-  __device__ __forceinline__ void get(float (&x)[V]) const {
-    union { typename Raw<V * sizeof(T)>::type raw; T t[V]; } w;
-    w.raw = raw;
-#pragma unroll
-    for (int j = 0; j < V; j++) x[j] = to_float(w.t[j]);
-  }
+  __device__ __forceinline__ void get(float (&x)[V]) const { unpack<T, V>(raw, x); }
 };
 
 template <class T, int V, int K, int R>
-__global__ void __launch_bounds__(kThreads) row_fwd_kernel(Norm a, int lanes) {
+__global__ void __launch_bounds__(kThreads, K == 1 ? kBlocksAhead : 1) row_fwd_kernel(Norm a, int lanes) {
   const int per = 32 / lanes, lane = threadIdx.x % lanes, warp = threadIdx.x / 32;
   const int g = blockIdx.x * per + (threadIdx.x & 31) / lanes, c0 = g * a.cg;
   const bool live = g < a.groups;
@@ -91,29 +94,32 @@ __global__ void __launch_bounds__(kThreads) row_fwd_kernel(Norm a, int lanes) {
     }
   }
   const long long step = (long long)gridDim.y * kWarps * R;
-  for (long long row = ((long long)blockIdx.y * kWarps + warp) * R; row < a.b; row += step) {
-    const T* x = static_cast<const T*>(a.x) + row * a.n + c0;
-    Piece<T, V> v[R][K];
+  Piece<T, V> next[R][K];
+  auto fetch = [&](long long row) {
 #pragma unroll
     for (int r = 0; r < R; r++)
 #pragma unroll
       for (int k = 0; k < K; k++) {
         const int c = (k * lanes + lane) * V;
-        if (live && c < a.cg && row + r < a.b) v[r][k].load(x + (long long)r * a.n + c);
-        else v[r][k].raw = {};
+        if (live && c < a.cg && row + r < a.b) next[r][k].load(static_cast<const T*>(a.x) + (row + r) * a.n + c0 + c);
+        else next[r][k].raw = {};
       }
-    float mean[R], rstd[R];
+  };
+  long long row = ((long long)blockIdx.y * kWarps + warp) * R;
+  if (row < a.b) fetch(row);
+  for (; row < a.b; row += step) {
+    float v[R][K][V], mean[R], rstd[R];
 #pragma unroll
     for (int r = 0; r < R; r++) {
       mean[r] = 0;
 #pragma unroll
       for (int k = 0; k < K; k++) {
-        float f[V];
-        v[r][k].get(f);
+        next[r][k].get(v[r][k]);
 #pragma unroll
-        for (int j = 0; j < V; j++) mean[r] += f[j];
+        for (int j = 0; j < V; j++) mean[r] += v[r][k][j];
       }
     }
+    if (row + step < a.b) fetch(row + step);   // on their way while these rows are worked on
     lanes_sums(mean, lanes);
 #pragma unroll
     for (int r = 0; r < R; r++) {
@@ -121,12 +127,12 @@ __global__ void __launch_bounds__(kThreads) row_fwd_kernel(Norm a, int lanes) {
       rstd[r] = 0;
 #pragma unroll
       for (int k = 0; k < K; k++)
-        if ((k * lanes + lane) * V < a.cg) {
-          float f[V];
-          v[r][k].get(f);
+        if ((k * lanes + lane) * V < a.cg)
 #pragma unroll
-          for (int j = 0; j < V; j++) rstd[r] += (f[j] - mean[r]) * (f[j] - mean[r]);
-        }
+          for (int j = 0; j < V; j++) {
+            v[r][k][j] -= mean[r];
+            rstd[r] += v[r][k][j] * v[r][k][j];
+          }
     }
     lanes_sums(rstd, lanes);
 #pragma unroll
@@ -141,12 +147,10 @@ __global__ void __launch_bounds__(kThreads) row_fwd_kernel(Norm a, int lanes) {
       for (int k = 0; k < K; k++) {
         const int c = (k * lanes + lane) * V;
         if (c < a.cg) {
-          float f[V];
-          v[r][k].get(f);
 #pragma unroll
-          for (int j = 0; j < V; j++) f[j] = (f[j] - mean[r]) * rstd[r] * w[k][j] + bias[k][j];
-          activate(f, a.act);
-          store_vec<T, V>(static_cast<T*>(a.y) + (row + r) * a.n + c0 + c, f);
+          for (int j = 0; j < V; j++) v[r][k][j] = v[r][k][j] * rstd[r] * w[k][j] + bias[k][j];
+          activate(v[r][k], a.act);
+          store_vec<T, V>(static_cast<T*>(a.y) + (row + r) * a.n + c0 + c, v[r][k]);
         }
       }
     }
@@ -155,7 +159,7 @@ __global__ void __launch_bounds__(kThreads) row_fwd_kernel(Norm a, int lanes) {
 
 // The sums over rows stay in registers; a block's warps have the same groups and add theirs up at the end.
 template <class T, int V, int K, int R>
-__global__ void __launch_bounds__(kThreads) row_bwd_kernel(Norm a, int lanes, int parts) {
+__global__ void __launch_bounds__(kThreads, K == 1 ? kBlocksBack : 1) row_bwd_kernel(Norm a, int lanes, int parts) {
   __shared__ float sums[kWarps][2][32 * V];
   const int per = 32 / lanes, lane = threadIdx.x % lanes, warp = threadIdx.x / 32;
   const int g = blockIdx.x * per + (threadIdx.x & 31) / lanes, c0 = g * a.cg;
@@ -808,9 +812,9 @@ Way choose(long long b, long long s, int n, int groups, int type, bool wide16, b
       w.K = need <= 32 ? 1 : 4;
       const int across = (groups + 32 / w.lanes - 1) / (32 / w.lanes);
       w.across = across;
-      w.R = w.K > 1 ? 1 : backward ? 2 : 4;
+      w.R = w.K > 1 ? 1 : backward ? kRowsBack : kRowsAhead;
       // rows for every warp, on as many blocks as the SMs hold
-      w.parts = (int)std::max(1LL, std::min((b + kWarps * w.R - 1) / (kWarps * w.R), (long long)(kSms * (backward ? 2 : 4) + across - 1) / across));
+      w.parts = (int)std::max(1LL, std::min((b + kWarps * w.R - 1) / (kWarps * w.R), (long long)(kSms * (backward ? kBlocksBack : kBlocksAhead)) / across));
       return w;
     }
   }
@@ -849,8 +853,8 @@ Way choose(long long b, long long s, int n, int groups, int type, bool wide16, b
   w.way = Way::kTwo, w.V = vector(n);
   const int high = high_of(n, w.V);
   w.shared = std::max(2LL * high * n, 2LL * groups) * 4;
-  // about eight blocks for each SM, and rows enough in a piece that its sums are few beside it
-  const long long wanted = std::max(1LL, (kSms * 8 + b - 1) / b);
+  // as many blocks as the SMs hold at a time, so that all of them end together; rows enough in a piece that its sums are few beside it
+  const long long wanted = std::max(1LL, kSms * (backward ? 3 : 4) / b);
   w.per = (int)std::min((long long)1 << 24, std::max({(s + wanted - 1) / wanted, (long long)4 * high, std::min(s, (long long)16)}));
   w.pieces = (int)((s + w.per - 1) / w.per);
   w.parts = (int)std::min(b * w.pieces, 0x7fffffffLL);
@@ -929,10 +933,10 @@ int launch_group_norm(const GroupNormCall& c, cudaStream_t stream) {
       if (w.way == Way::kRow) {
         const dim3 grid(w.across, w.parts);
         if (!back) {
-          auto kernel = w.K == 1 ? row_fwd_kernel<T, V, 1, 4> : row_fwd_kernel<T, V, 4, 1>;
+          auto kernel = w.K == 1 ? row_fwd_kernel<T, V, 1, kRowsAhead> : row_fwd_kernel<T, V, 4, 1>;
           kernel<<<grid, kThreads, 0, stream>>>(a, w.lanes);
         } else {
-          auto kernel = w.K == 1 ? row_bwd_kernel<T, V, 1, 2> : row_bwd_kernel<T, V, 4, 1>;
+          auto kernel = w.K == 1 ? row_bwd_kernel<T, V, 1, kRowsBack> : row_bwd_kernel<T, V, 4, 1>;
           kernel<<<grid, kThreads, 0, stream>>>(a, w.lanes, w.parts);
         }
         return launched(fn);

@@ -50,23 +50,70 @@ struct Raw<4> { using type = uint32_t; };
 template <>
 struct Raw<2> { using type = uint16_t; };
 
+// Numbers as they lie, and in float; 16-bit ones in pairs, which is half the instructions.
+template <class T, int V>
+__device__ __forceinline__ void unpack(const typename Raw<V * sizeof(T)>::type& raw, float (&x)[V]) {
+  if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+    union { typename Raw<V * sizeof(T)>::type raw; uint32_t u[V / 2]; } w;
+    w.raw = raw;
+#pragma unroll
+    for (int k = 0; k < V / 2; k++) {
+      if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+        x[2 * k] = __uint_as_float(w.u[k] << 16);
+        x[2 * k + 1] = __uint_as_float(w.u[k] & 0xffff0000u);
+      } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w.u[k]));
+        x[2 * k] = f.x, x[2 * k + 1] = f.y;
+      }
+    }
+  } else {
+    union { typename Raw<V * sizeof(T)>::type raw; T t[V]; } w;
+    w.raw = raw;
+#pragma unroll
+    for (int k = 0; k < V; k++) x[k] = to_float(w.t[k]);
+  }
+}
+template <class T, int V>
+__device__ __forceinline__ typename Raw<V * sizeof(T)>::type pack(const float (&x)[V]) {
+  if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+    union { typename Raw<V * sizeof(T)>::type raw; uint32_t u[V / 2]; } w;
+#pragma unroll
+    for (int k = 0; k < V / 2; k++) {
+      if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * k], x[2 * k + 1]);
+        w.u[k] = *reinterpret_cast<const uint32_t*>(&h);
+      } else {
+        const __half2 h = __floats2half2_rn(x[2 * k], x[2 * k + 1]);
+        w.u[k] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
+    return w.raw;
+  } else {
+    union { typename Raw<V * sizeof(T)>::type raw; T t[V]; } w;
+#pragma unroll
+    for (int k = 0; k < V; k++) w.t[k] = from_float<T>(x[k]);
+    return w.raw;
+  }
+}
+
 // V consecutive elements as one access of V * sizeof(T) bytes.
 template <class T, int V>
 __device__ __forceinline__ void load_vec(const T* src, float (&x)[V]) {
-  union { typename Raw<V * sizeof(T)>::type raw; T t[V]; } w;
-  w.raw = *reinterpret_cast<const typename Raw<V * sizeof(T)>::type*>(src);
-#pragma unroll
-  for (int k = 0; k < V; k++) x[k] = to_float(w.t[k]);
+  unpack<T, V>(*reinterpret_cast<const typename Raw<V * sizeof(T)>::type*>(src), x);
 }
 template <class T, int V>
 __device__ __forceinline__ void store_vec(T* dst, const float (&x)[V]) {
-  union { typename Raw<V * sizeof(T)>::type raw; T t[V]; } w;
-#pragma unroll
-  for (int k = 0; k < V; k++) w.t[k] = from_float<T>(x[k]);
-  *reinterpret_cast<typename Raw<V * sizeof(T)>::type*>(dst) = w.raw;
+  *reinterpret_cast<typename Raw<V * sizeof(T)>::type*>(dst) = pack<T, V>(x);
 }
 
-__device__ __forceinline__ float logistic(float z) { return __fdividef(1.f, 1.f + __expf(-z)); }
+// 1 / (1 + exp(-z)) from the approximations of 2^x and 1 / x, without their treatment of subnormal numbers, which took most of the instructions: where
+// exp(-z) is subnormal it is nothing beside 1, and where 1 + exp(-z) is so large that the quotient is subnormal, that is 0 here.
+__device__ __forceinline__ float logistic(float z) {
+  float e, q;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z * -1.4426950408889634f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(1.f + e));
+  return q;
+}
 
 constexpr float kGelu0 = 1.5957691216057308f;             // 2 sqrt(2 / pi): 0.5 (1 + tanh u) is the logistic function of 2u
 constexpr float kGelu1 = kGelu0 * 0.044715f;
@@ -96,16 +143,15 @@ __device__ __forceinline__ void activate_back(float (&g)[V], const float (&x)[V]
     for (int k = 0; k < V; k++) g[k] = x[k] > 0.f ? g[k] : x[k] != x[k] ? x[k] : 0.f;
     return;
   }
-  // beyond +-128 the derivatives are 1 and 0 to the last bit, and their terms are no longer products of 0 and infinity
   const bool silu = act == GELIB_ACT_SILU;
 #pragma unroll
   for (int k = 0; k < V; k++) {
-    const float z = x[k] < -128.f ? -128.f : x[k] > 128.f ? 128.f : x[k];
+    const float z = x[k];
     if (silu) {
       const float q = logistic(z);
       g[k] *= q * (1.f + z * (1.f - q));
     } else {
-      const float z2 = z * z, q = logistic(z * (kGelu0 + kGelu1 * z2));
+      const float z2 = fminf(z * z, 1e30f), q = logistic(z * (kGelu0 + kGelu1 * z2));   // finite: where q (1 - q) is 0 the product is
       g[k] *= q + z * q * (1.f - q) * (kGelu0 + 3.f * kGelu1 * z2);
     }
   }
