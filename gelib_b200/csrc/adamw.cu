@@ -52,35 +52,48 @@ struct Args {
   Entry e[N];
 };
 
-// Two rounds of multiplication and shifts over the element's number and the seed.
-__device__ __forceinline__ unsigned random_bits(unsigned seed_mix, unsigned long long i) {
-  unsigned h = (unsigned)i * 0x9E3779B1u + (unsigned)(i >> 32) * 0x7FEB352Du + seed_mix;
+// Two rounds of multiplication and shifts; h is the element's number and the seed, each times an odd number.
+__device__ __forceinline__ unsigned random_bits(unsigned h) {
   h = (h ^ (h >> 15)) * 0x2C1B3C6Du;
   h = (h ^ (h >> 12)) * 0x297A2D39u;
   return h ^ (h >> 15);
 }
 
-__device__ __forceinline__ void update(const Scalars& s, float g, float& p, float& m, float& v) {
-  m = s.b1 * m + s.one_b1 * g;
-  v = s.b2 * v + s.one_b2 * g * g;
-  p = p * s.keep - s.step * m / (sqrtf(v) * s.root + s.eps);
+// Eight elements; r: the new root of v.  The approximate root and reciprocal are a unit or two in the last place off.
+__device__ __forceinline__ void update(const Scalars& s, float (&g)[8], float (&p)[8], float (&m)[8], float (&v)[8], float (&r)[8]) {
+  float t[8];
+  mul_all(m, m, s.b1);
+  fma_all(m, g, s.one_b1, m);
+  mul_all(t, g, g);
+  mul_all(v, v, s.b2);
+  fma_all(v, t, s.one_b2, v);
+#pragma unroll
+  for (int k = 0; k < 8; k++) asm("sqrt.approx.f32 %0, %1;" : "=f"(r[k]) : "f"(v[k]));
+  fma_all(t, r, s.root, s.eps);
+#pragma unroll
+  for (int k = 0; k < 8; k++) asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t[k]) : "f"(t[k]));
+  mul_all(t, t, m);
+  mul_all(p, p, s.keep);
+  fma_all(p, t, -s.step, p);
 }
 
 // The power of two that brings `top` into [128, 256): codes then reach 256 after rounding up, below e4m3's 448.  No smaller than
 // 2^-100, so that scale times code stays a normal number; a block whose values are all zero has that scale too.
 __device__ __forceinline__ int scale_exponent(float top) { return max((int)(__float_as_uint(top) >> 23) - 127 - 7, -100); }
 
-// |y| < 256 on the grid of e4m3: three bits of mantissa, steps of 2^-9 below 2^-6; u in [0, 2^16) decides between the neighbours.
-__device__ __forceinline__ float on_grid(float y, unsigned u) {
-  const bool small = y < 0.015625f;
-  const float t = small ? y + 0.015625f : y;
-  const float q = __uint_as_float((__float_as_uint(t) + (u * 16 + 8)) & 0xfff00000u);
-  return small ? q - 0.015625f : q;
+// 0 <= y < 256 on the grid of e4m3: three bits of mantissa, steps of 2^-9 below 2^-6; u in [0, 2^16), sixteen times it and 8 more, decides between the
+// neighbours.  What is no finite number becomes NaN.
+__device__ __forceinline__ float on_grid(float y, unsigned u16) {
+  const float more = y < 0.015625f ? 0.015625f : 0.f;
+  const float q = __uint_as_float((__float_as_uint(y + more) + u16) & 0xfff00000u);
+  return fmaf(y, 0.f, q - more);
 }
 
-__device__ __forceinline__ unsigned char code_of(float q) { return (unsigned char)__nv_cvt_float_to_fp8(q, __NV_SATFINITE, __NV_E4M3); }
-__device__ __forceinline__ float value_of(unsigned char c) {
-  return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3)));
+// Pairs of codes and their values, the first in the low byte.
+__device__ __forceinline__ unsigned short codes_of(float q0, float q1) { return __nv_cvt_float2_to_fp8x2(make_float2(q0, q1), __NV_SATFINITE, __NV_E4M3); }
+__device__ __forceinline__ float2 values_of(unsigned short c) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(c, __NV_E4M3);
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
 template <int N>
@@ -101,10 +114,7 @@ __device__ __forceinline__ void load_n(const T* src, long long i, long long n, f
         const float4 a = *reinterpret_cast<const float4*>(src + i), b = *reinterpret_cast<const float4*>(src + i + 4);
         x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
       } else {
-        union { uint4 u; T t[8]; } w;
-        w.u = *reinterpret_cast<const uint4*>(src + i);
-#pragma unroll
-        for (int k = 0; k < 8; k++) x[k] = to_float(w.t[k]);
+        load_vec<T, 8>(src + i, x);
       }
       return;
     }
@@ -121,10 +131,7 @@ __device__ __forceinline__ void store_n(T* dst, long long i, long long n, const 
         *reinterpret_cast<float4*>(dst + i) = make_float4(x[0], x[1], x[2], x[3]);
         *reinterpret_cast<float4*>(dst + i + 4) = make_float4(x[4], x[5], x[6], x[7]);
       } else {
-        union { uint4 u; T t[8]; } w;
-#pragma unroll
-        for (int k = 0; k < 8; k++) w.t[k] = from_float<T>(x[k]);
-        *reinterpret_cast<uint4*>(dst + i) = w.u;
+        store_vec<T, 8>(dst + i, x);
       }
       return;
     }
@@ -135,30 +142,30 @@ __device__ __forceinline__ void store_n(T* dst, long long i, long long n, const 
 }
 
 template <bool kWide>
-__device__ __forceinline__ void load_codes(const unsigned char* src, long long i, long long n, unsigned char (&c)[8]) {
+__device__ __forceinline__ void load_codes(const unsigned char* src, long long i, long long n, unsigned short (&c)[4]) {
+  union { uint2 u; unsigned short p[4]; unsigned char c[8]; } w;
   if (kWide && i + 8 <= n) {
-    union { uint2 u; unsigned char c[8]; } w;
     w.u = *reinterpret_cast<const uint2*>(src + i);
+  } else {
 #pragma unroll
-    for (int k = 0; k < 8; k++) c[k] = w.c[k];
-    return;
+    for (int k = 0; k < 8; k++) w.c[k] = i + k < n ? src[i + k] : 0;
   }
 #pragma unroll
-  for (int k = 0; k < 8; k++) c[k] = i + k < n ? src[i + k] : 0;
+  for (int k = 0; k < 4; k++) c[k] = w.p[k];
 }
 
 template <bool kWide>
-__device__ __forceinline__ void store_codes(unsigned char* dst, long long i, long long n, const unsigned char (&c)[8]) {
-  if (kWide && i + 8 <= n) {
-    union { uint2 u; unsigned char c[8]; } w;
+__device__ __forceinline__ void store_codes(unsigned char* dst, long long i, long long n, const unsigned short (&c)[4]) {
+  union { uint2 u; unsigned short p[4]; unsigned char c[8]; } w;
 #pragma unroll
-    for (int k = 0; k < 8; k++) w.c[k] = c[k];
+  for (int k = 0; k < 4; k++) w.p[k] = c[k];
+  if (kWide && i + 8 <= n) {
     *reinterpret_cast<uint2*>(dst + i) = w.u;
     return;
   }
 #pragma unroll
   for (int k = 0; k < 8; k++)
-    if (i + k < n) dst[i + k] = c[k];
+    if (i + k < n) dst[i + k] = w.c[k];
 }
 
 // A lane's eight consecutive elements; with 8-bit states a warp's 256 are one block.
@@ -173,59 +180,71 @@ __device__ __forceinline__ void step_piece(const Entry& e, const Scalars& s, lon
   unsigned char *mc = static_cast<unsigned char*>(e.m), *vc = static_cast<unsigned char*>(e.v);
   const long long block = i / kBlock;
   if constexpr (k8) {
-    unsigned char a[8], b[8];
+    unsigned short a[4], b[4];
     load_codes<kWide>(mc, i, n, a);
     load_codes<kWide>(vc, i, n, b);
     const float ms = e.ms[block], vs = e.vs[block];
 #pragma unroll
-    for (int k = 0; k < 8; k++) {
-      m[k] = value_of(a[k]) * ms;
-      const float r = value_of(b[k]) * vs;
-      v[k] = r * r;
+    for (int k = 0; k < 4; k++) {
+      const float2 p = values_of(a[k]), r = values_of(b[k]);
+      m[2 * k] = p.x, m[2 * k + 1] = p.y, v[2 * k] = r.x, v[2 * k + 1] = r.y;
     }
+    mul_all(m, m, ms);
+    mul_all(v, v, vs);
+    mul_all(v, v, v);
   } else {
     load_n<float, kWide>(static_cast<const float*>(e.m), i, n, m);
     load_n<float, kWide>(static_cast<const float*>(e.v), i, n, v);
   }
-  const float scale = s.grad_scale ? *s.grad_scale : 1.f;
-#pragma unroll
-  for (int k = 0; k < 8; k++) update(s, s.grad_scale ? g[k] * scale : g[k], p[k], m[k], v[k]);
+  if (s.grad_scale) mul_all(g, g, *s.grad_scale);
+  float r[8];
+  update(s, g, p, m, v, r);
   store_n<float, kWide>(master, i, n, p);
   if constexpr (sizeof(T) == 2) store_n<T, kWide>(static_cast<T*>(e.p), i, n, p);
   if constexpr (!k8) {
     store_n<float, kWide>(static_cast<float*>(e.m), i, n, m);
     store_n<float, kWide>(static_cast<float*>(e.v), i, n, v);
   } else {
-    // a value that is no number spoils its own element and not its block: it takes no part in the scale and has the code of NaN
-    float tm = 0, tv = 0;
+    // a value that is no finite number spoils its own element and not its block: it takes no part in the scale
+    constexpr float kMost = 3.402823466e38f;
+    float tm = 0, tr = 0;
 #pragma unroll
-    for (int k = 0; k < 8; k++) {
-      v[k] = sqrtf(v[k]);
-      if (fabsf(m[k]) <= 3.402823466e38f) tm = fmaxf(tm, fabsf(m[k]));
-      if (v[k] <= 3.402823466e38f) tv = fmaxf(tv, v[k]);
+    for (int k = 0; k < 8; k++) tm = fmaxf(tm, fabsf(m[k])), tr = fmaxf(tr, r[k]);   // NaN drops out
+    if (!(tm <= kMost && tr <= kMost)) {
+      tm = tr = 0;
+#pragma unroll
+      for (int k = 0; k < 8; k++) {
+        if (fabsf(m[k]) <= kMost) tm = fmaxf(tm, fabsf(m[k]));
+        if (r[k] <= kMost) tr = fmaxf(tr, r[k]);
+      }
     }
+    // neither is negative: their order is that of their bits, and a warp has the largest of those in one step
+    tm = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(tm)));
+    tr = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(tr)));
+    const int em = scale_exponent(tm), er = scale_exponent(tr);
+    const float im = __uint_as_float((127 - em) << 23), ir = __uint_as_float((127 - er) << 23);
+    const unsigned long long number = (unsigned long long)e.at * kBlock + (unsigned long long)i;
+    unsigned h = (unsigned)number * 0x9E3779B1u + (unsigned)(number >> 32) * 0x7FEB352Du + s.seed_mix;   // eight elements lie in one multiple of 2^32
+    unsigned short a[4], b[4];
 #pragma unroll
-    for (int d = 16; d; d >>= 1) {
-      tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, d));
-      tv = fmaxf(tv, __shfl_xor_sync(0xffffffffu, tv, d));
-    }
-    const int em = scale_exponent(tm), ev = scale_exponent(tv);
-    const float im = __uint_as_float((127 - em) << 23), iv = __uint_as_float((127 - ev) << 23);
-    unsigned char a[8], b[8];
+    for (int k = 0; k < 8; k += 2) {
+      float qm[2], qr[2];
 #pragma unroll
-    for (int k = 0; k < 8; k++) {
-      const unsigned u = random_bits(s.seed_mix, (unsigned long long)e.at * kBlock + (unsigned long long)(i + k));
-      float q = copysignf(on_grid(fabsf(m[k]) * im, u & 0xffff), m[k]);
-      a[k] = fabsf(m[k]) <= 3.402823466e38f ? code_of(q) : 0x7f;
-      q = on_grid(v[k] * iv, u >> 16);
-      if (v[k] > 0) q = fmaxf(q, 0.001953125f);
-      b[k] = v[k] <= 3.402823466e38f ? code_of(q) : 0x7f;
+      for (int j = 0; j < 2; j++) {
+        const unsigned u = random_bits(h);
+        h += 0x9E3779B1u;
+        qm[j] = copysignf(on_grid(fabsf(m[k + j]) * im, (u & 0xffff) * 16 + 8), m[k + j]);
+        qr[j] = on_grid(r[k + j] * ir, (u >> 12 & 0xffff0) + 8);
+        if (r[k + j] > 0 && qr[j] < 0.001953125f) qr[j] = 0.001953125f;
+      }
+      a[k / 2] = codes_of(qm[0], qm[1]);
+      b[k / 2] = codes_of(qr[0], qr[1]);
     }
     store_codes<kWide>(mc, i, n, a);
     store_codes<kWide>(vc, i, n, b);
     if ((threadIdx.x & 31) == 0) {
       e.ms[block] = __uint_as_float((em + 127) << 23);
-      e.vs[block] = __uint_as_float((ev + 127) << 23);
+      e.vs[block] = __uint_as_float((er + 127) << 23);
     }
   }
 }
@@ -271,12 +290,15 @@ __global__ void __launch_bounds__(kThreads) block8_values_kernel(__nv_bfloat16* 
                                                                 const float* __restrict__ scale, long long n, bool wide) {
   const long long i = ((long long)blockIdx.x * kThreads + threadIdx.x) * 8;
   if (i >= n) return;
-  unsigned char c[8];
+  unsigned short c[4];
   float x[8];
   wide ? load_codes<true>(codes, i, n, c) : load_codes<false>(codes, i, n, c);
   const float s = scale[i / kBlock];
 #pragma unroll
-  for (int k = 0; k < 8; k++) x[k] = value_of(c[k]) * s;
+  for (int k = 0; k < 4; k++) {
+    const float2 f = values_of(c[k]);
+    x[2 * k] = f.x * s, x[2 * k + 1] = f.y * s;
+  }
   wide ? store_n<__nv_bfloat16, true>(out, i, n, x) : store_n<__nv_bfloat16, false>(out, i, n, x);
 }
 

@@ -24,14 +24,9 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-#ifndef RF
-#define RF 2
-#define RB 1
-#define BF 4
-#define BB 3
-#endif
-constexpr int kRowsAhead = RF, kRowsBack = RB;        // of a warp at a time, forward and backward
-constexpr int kBlocksAhead = BF, kBlocksBack = BB;    // of an SM
+constexpr int kRowsAhead = 4, kRowsBack = 2;        // of a warp at a time, forward and backward
+constexpr int kBlocksAhead = 2, kBlocksBack = 2;    // of an SM
+constexpr int kPieceBlocks = 4, kPieceBlocksBack = 2;   // of an SM, where samples are taken in pieces
 
 struct Norm {
   const void *x, *w, *bias, *gy;
@@ -49,12 +44,19 @@ __device__ __forceinline__ float lanes_sum(float v, int lanes) {
   return v;
 }
 
-// Each of R sums over the lanes, their exchanges side by side.
-template <int R>
+// Each of R sums over the lanes, their exchanges side by side.  L: the number of lanes, 0 where it is known at run time only.
+template <int L, int R>
 __device__ __forceinline__ void lanes_sums(float (&v)[R], int lanes) {
-  for (int d = lanes >> 1; d; d >>= 1)
+  if constexpr (L > 0) {
 #pragma unroll
-    for (int r = 0; r < R; r++) v[r] += __shfl_xor_sync(0xffffffffu, v[r], d);
+    for (int d = L >> 1; d; d >>= 1)
+#pragma unroll
+      for (int r = 0; r < R; r++) v[r] += __shfl_xor_sync(0xffffffffu, v[r], d);
+  } else {
+    for (int d = lanes >> 1; d; d >>= 1)
+#pragma unroll
+      for (int r = 0; r < R; r++) v[r] += __shfl_xor_sync(0xffffffffu, v[r], d);
+  }
 }
 
 template <class T, int V>
@@ -76,38 +78,41 @@ struct Piece {   // an access as it lies
   __device__ __forceinline__ void get(float (&x)[V]) const { unpack<T, V>(raw, x); }
 };
 
-template <class T, int V, int K, int R>
+template <class T, int V, int K, int R, int L>
 __global__ void __launch_bounds__(kThreads, K == 1 ? kBlocksAhead : 1) row_fwd_kernel(Norm a, int lanes) {
+  if (L > 0) lanes = L;
   const int per = 32 / lanes, lane = threadIdx.x % lanes, warp = threadIdx.x / 32;
-  const int g = blockIdx.x * per + (threadIdx.x & 31) / lanes, c0 = g * a.cg;
+  const int g = blockIdx.x * per + (threadIdx.x & 31) / lanes, c0 = g * a.cg + lane * V;
   const bool live = g < a.groups;
   const float inv = 1.f / a.cg;
+  bool has[K];
   float w[K][V], bias[K][V];
 #pragma unroll
   for (int k = 0; k < K; k++) {
-    const int c = (k * lanes + lane) * V;
+    has[k] = live && (k * lanes + lane) * V < a.cg;
 #pragma unroll
     for (int j = 0; j < V; j++) w[k][j] = bias[k][j] = 0;
-    if (live && c < a.cg) {
-      load_or<T, V>(a.w, c0 + c, 1.f, w[k]);
-      load_or<T, V>(a.bias, c0 + c, 0.f, bias[k]);
+    if (has[k]) {
+      load_or<T, V>(a.w, c0 + k * lanes * V, 1.f, w[k]);
+      load_or<T, V>(a.bias, c0 + k * lanes * V, 0.f, bias[k]);
     }
   }
   const long long step = (long long)gridDim.y * kWarps * R;
   Piece<T, V> next[R][K];
+  long long row = ((long long)blockIdx.y * kWarps + warp) * R;
+  const T* x = static_cast<const T*>(a.x) + row * a.n + c0;
+  T* y = static_cast<T*>(a.y) + row * a.n + c0;
   auto fetch = [&](long long row) {
 #pragma unroll
     for (int r = 0; r < R; r++)
 #pragma unroll
       for (int k = 0; k < K; k++) {
-        const int c = (k * lanes + lane) * V;
-        if (live && c < a.cg && row + r < a.b) next[r][k].load(static_cast<const T*>(a.x) + (row + r) * a.n + c0 + c);
+        if (has[k] && row + r < a.b) next[r][k].load(x + (long long)r * a.n + k * lanes * V);
         else next[r][k].raw = {};
       }
   };
-  long long row = ((long long)blockIdx.y * kWarps + warp) * R;
   if (row < a.b) fetch(row);
-  for (; row < a.b; row += step) {
+  for (; row < a.b; row += step, y += step * a.n) {
     float v[R][K][V], mean[R], rstd[R];
 #pragma unroll
     for (int r = 0; r < R; r++) {
@@ -115,26 +120,24 @@ __global__ void __launch_bounds__(kThreads, K == 1 ? kBlocksAhead : 1) row_fwd_k
 #pragma unroll
       for (int k = 0; k < K; k++) {
         next[r][k].get(v[r][k]);
-#pragma unroll
-        for (int j = 0; j < V; j++) mean[r] += v[r][k][j];
+        mean[r] += sum_of(v[r][k]);
       }
     }
+    x += step * a.n;
     if (row + step < a.b) fetch(row + step);   // on their way while these rows are worked on
-    lanes_sums(mean, lanes);
+    lanes_sums<L>(mean, lanes);
 #pragma unroll
     for (int r = 0; r < R; r++) {
       mean[r] *= inv;
       rstd[r] = 0;
 #pragma unroll
-      for (int k = 0; k < K; k++)
-        if ((k * lanes + lane) * V < a.cg)
-#pragma unroll
-          for (int j = 0; j < V; j++) {
-            v[r][k][j] -= mean[r];
-            rstd[r] += v[r][k][j] * v[r][k][j];
-          }
+      for (int k = 0; k < K; k++) {
+        add_all(v[r][k], v[r][k], -mean[r]);
+        const float sq = dot_of(v[r][k], v[r][k]);
+        if (has[k]) rstd[r] += sq;
+      }
     }
-    lanes_sums(rstd, lanes);
+    lanes_sums<L>(rstd, lanes);
 #pragma unroll
     for (int r = 0; r < R; r++) {
       rstd[r] = rsqrtf(rstd[r] * inv + a.eps);
@@ -144,42 +147,45 @@ __global__ void __launch_bounds__(kThreads, K == 1 ? kBlocksAhead : 1) row_fwd_k
         a.rstd[(row + r) * a.groups + g] = rstd[r];
       }
 #pragma unroll
-      for (int k = 0; k < K; k++) {
-        const int c = (k * lanes + lane) * V;
-        if (c < a.cg) {
-#pragma unroll
-          for (int j = 0; j < V; j++) v[r][k][j] = v[r][k][j] * rstd[r] * w[k][j] + bias[k][j];
+      for (int k = 0; k < K; k++)
+        if (has[k]) {
+          mul_all(v[r][k], v[r][k], rstd[r]);
+          fma_all(v[r][k], v[r][k], w[k], bias[k]);
           activate(v[r][k], a.act);
-          store_vec<T, V>(static_cast<T*>(a.y) + (row + r) * a.n + c0 + c, v[r][k]);
+          store_vec<T, V>(y + (long long)r * a.n + k * lanes * V, v[r][k]);
         }
-      }
     }
   }
 }
 
 // The sums over rows stay in registers; a block's warps have the same groups and add theirs up at the end.
-template <class T, int V, int K, int R>
+template <class T, int V, int K, int R, int L>
 __global__ void __launch_bounds__(kThreads, K == 1 ? kBlocksBack : 1) row_bwd_kernel(Norm a, int lanes, int parts) {
   __shared__ float sums[kWarps][2][32 * V];
+  if (L > 0) lanes = L;
   const int per = 32 / lanes, lane = threadIdx.x % lanes, warp = threadIdx.x / 32;
-  const int g = blockIdx.x * per + (threadIdx.x & 31) / lanes, c0 = g * a.cg;
+  const int g = blockIdx.x * per + (threadIdx.x & 31) / lanes, c0 = g * a.cg + lane * V;
   const bool live = g < a.groups;
   const float inv = 1.f / a.cg;
+  bool has[K];
   float w[K][V], bias[K][V], gw[K][V], gb[K][V];
 #pragma unroll
   for (int k = 0; k < K; k++) {
-    const int c = (k * lanes + lane) * V;
+    has[k] = live && (k * lanes + lane) * V < a.cg;
 #pragma unroll
     for (int j = 0; j < V; j++) w[k][j] = bias[k][j] = gw[k][j] = gb[k][j] = 0;
-    if (live && c < a.cg) {
-      load_or<T, V>(a.w, c0 + c, 1.f, w[k]);
-      load_or<T, V>(a.bias, c0 + c, 0.f, bias[k]);
+    if (has[k]) {
+      load_or<T, V>(a.w, c0 + k * lanes * V, 1.f, w[k]);
+      load_or<T, V>(a.bias, c0 + k * lanes * V, 0.f, bias[k]);
     }
   }
   const long long step = (long long)gridDim.y * kWarps * R;
   Piece<T, V> px[R][K], pg[R][K];
   float pm[R], pr[R];
+  long long row = ((long long)blockIdx.y * kWarps + warp) * R;
+  long long at = row * a.n + c0, out = at;
   auto fetch = [&](long long row) {
+    const T *x = static_cast<const T*>(a.x) + at, *gy = static_cast<const T*>(a.gy) + at;
 #pragma unroll
     for (int r = 0; r < R; r++) {
       const bool there = live && row + r < a.b;
@@ -187,11 +193,9 @@ __global__ void __launch_bounds__(kThreads, K == 1 ? kBlocksBack : 1) row_bwd_ke
       pr[r] = there ? a.rstd[(row + r) * a.groups + g] : 0.f;
 #pragma unroll
       for (int k = 0; k < K; k++) {
-        const int c = (k * lanes + lane) * V;
-        const long long at = (row + r) * a.n + c0 + c;
-        if (there && c < a.cg) {
-          px[r][k].load(static_cast<const T*>(a.x) + at);
-          pg[r][k].load(static_cast<const T*>(a.gy) + at);
+        if (has[k] && row + r < a.b) {
+          px[r][k].load(x + (long long)r * a.n + k * lanes * V);
+          pg[r][k].load(gy + (long long)r * a.n + k * lanes * V);
         } else {
           px[r][k].raw = {};
           pg[r][k].raw = {};
@@ -199,9 +203,8 @@ __global__ void __launch_bounds__(kThreads, K == 1 ? kBlocksBack : 1) row_bwd_ke
       }
     }
   };
-  long long row = ((long long)blockIdx.y * kWarps + warp) * R;
   if (row < a.b) fetch(row);
-  for (; row < a.b; row += step) {
+  for (; row < a.b; row += step, out += step * a.n) {
     float h[R][K][V], gz[R][K][V], mean[R], rstd[R], s1[R], s2[R];
 #pragma unroll
     for (int r = 0; r < R; r++) {
@@ -209,6 +212,7 @@ __global__ void __launch_bounds__(kThreads, K == 1 ? kBlocksBack : 1) row_bwd_ke
 #pragma unroll
       for (int k = 0; k < K; k++) px[r][k].get(h[r][k]), pg[r][k].get(gz[r][k]);
     }
+    at += step * a.n;
     if (row + step < a.b) fetch(row + step);   // on their way while these rows are worked on
 #pragma unroll
     for (int r = 0; r < R; r++) {
@@ -216,37 +220,31 @@ __global__ void __launch_bounds__(kThreads, K == 1 ? kBlocksBack : 1) row_bwd_ke
 #pragma unroll
       for (int k = 0; k < K; k++) {
         float z[V];
-#pragma unroll
-        for (int j = 0; j < V; j++) {
-          h[r][k][j] = (h[r][k][j] - mean[r]) * rstd[r];
-          z[j] = h[r][k][j] * w[k][j] + bias[k][j];
-        }
+        add_all(h[r][k], h[r][k], -mean[r]);   // first the difference: a large mean costs no digits
+        mul_all(h[r][k], h[r][k], rstd[r]);
+        fma_all(z, h[r][k], w[k], bias[k]);
         activate_back(gz[r][k], z, a.act);
-#pragma unroll
-        for (int j = 0; j < V; j++) {
-          gb[k][j] += gz[r][k][j];
-          gw[k][j] += gz[r][k][j] * h[r][k][j];
-          gz[r][k][j] *= w[k][j];
-          s1[r] += gz[r][k][j];
-          s2[r] += gz[r][k][j] * h[r][k][j];
-        }
+        add_all(gb[k], gb[k], gz[r][k]);
+        fma_all(gw[k], gz[r][k], h[r][k], gw[k]);
+        mul_all(gz[r][k], gz[r][k], w[k]);
+        s1[r] += sum_of(gz[r][k]);
+        s2[r] += dot_of(gz[r][k], h[r][k]);
       }
     }
     if (a.y) {
-      lanes_sums(s1, lanes);
-      lanes_sums(s2, lanes);
+      lanes_sums<L>(s1, lanes);
+      lanes_sums<L>(s2, lanes);
 #pragma unroll
       for (int r = 0; r < R; r++) {
-        s1[r] *= inv, s2[r] *= inv;
+        s1[r] *= -inv, s2[r] *= -inv;
 #pragma unroll
-        for (int k = 0; k < K; k++) {
-          const int c = (k * lanes + lane) * V;
-          if (live && c < a.cg && row + r < a.b) {
-#pragma unroll
-            for (int j = 0; j < V; j++) gz[r][k][j] = rstd[r] * (gz[r][k][j] - s1[r] - h[r][k][j] * s2[r]);
-            store_vec<T, V>(static_cast<T*>(a.y) + (row + r) * a.n + c0 + c, gz[r][k]);
+        for (int k = 0; k < K; k++)
+          if (has[k] && row + r < a.b) {
+            add_all(gz[r][k], gz[r][k], s1[r]);
+            fma_all(gz[r][k], h[r][k], s2[r], gz[r][k]);
+            mul_all(gz[r][k], gz[r][k], rstd[r]);
+            store_vec<T, V>(static_cast<T*>(a.y) + out + (long long)r * a.n + k * lanes * V, gz[r][k]);
           }
-        }
       }
     }
   }
@@ -496,7 +494,7 @@ __global__ void __launch_bounds__(kThreads) tile_bwd_kernel(Norm a, int gpc, int
 
 // Sum, and sum of squares of differences from the piece's own mean, of every group of a piece: part (b, pieces, groups, 2).
 template <class T, int V>
-__global__ void __launch_bounds__(kThreads) piece_stats_kernel(Norm a, int pieces, int per) {
+__global__ void __launch_bounds__(kThreads, kPieceBlocks) piece_stats_kernel(Norm a, int pieces, int per) {
   extern __shared__ __align__(16) unsigned char memory[];
   const long long sample = blockIdx.x / pieces;
   const int piece = blockIdx.x % pieces;
@@ -581,7 +579,7 @@ __device__ __forceinline__ void join_pieces(const Norm& a, long long sample, int
 }
 
 template <class T, int V>
-__global__ void __launch_bounds__(kThreads) piece_apply_kernel(Norm a, int pieces, int per) {
+__global__ void __launch_bounds__(kThreads, kPieceBlocks) piece_apply_kernel(Norm a, int pieces, int per) {
   extern __shared__ __align__(16) unsigned char memory[];
   // the pieces that were read last may still be in L2: they are taken first
   const long long block = (long long)gridDim.x - 1 - blockIdx.x;
@@ -654,10 +652,9 @@ __device__ __forceinline__ void each_row(const Norm& a, long long base, int rows
         px[u].get(h);
         pg[u].get(g);
 #pragma unroll
-        for (int j = 0; j < V; j++) {
-          h[j] = (h[j] - mean[j]) * rstd[j];
-          z[j] = h[j] * w[j] + bias[j];
-        }
+        for (int j = 0; j < V; j++) h[j] -= mean[j];
+        mul_all(h, h, rstd);
+        fma_all(z, h, w, bias);
         activate_back(g, z, a.act);
         f(r + u * high, h, g);
       }
@@ -666,7 +663,7 @@ __device__ __forceinline__ void each_row(const Norm& a, long long base, int rows
 
 // gz xh and gz summed over a piece's rows, per channel: part (2, b * pieces, n); and times w, per group: back (b, pieces, groups, 2).
 template <class T, int V>
-__global__ void __launch_bounds__(kThreads) piece_back_sums_kernel(Norm a, int pieces, int per, float* back) {
+__global__ void __launch_bounds__(kThreads, kPieceBlocksBack) piece_back_sums_kernel(Norm a, int pieces, int per, float* back) {
   extern __shared__ __align__(16) unsigned char memory[];
   const long long sample = blockIdx.x / pieces;
   const int piece = blockIdx.x % pieces;
@@ -687,8 +684,8 @@ __global__ void __launch_bounds__(kThreads) piece_back_sums_kernel(Norm a, int p
         mean[j] = a.mean[g], rstd[j] = a.rstd[g], sw[j] = sb[j] = 0;
       }
       each_row<T, V>(a, base, rows, ty, cl.high, col, w, bias, mean, rstd, [&](int, const float (&h)[V], const float (&g)[V]) {
-#pragma unroll
-        for (int j = 0; j < V; j++) sb[j] += g[j], sw[j] += g[j] * h[j];
+        add_all(sb, sb, g);
+        fma_all(sw, g, h, sw);
       });
 #pragma unroll
       for (int j = 0; j < V; j++) {
@@ -718,7 +715,7 @@ __global__ void __launch_bounds__(kThreads) piece_back_sums_kernel(Norm a, int p
 }
 
 template <class T, int V>
-__global__ void __launch_bounds__(kThreads) piece_back_apply_kernel(Norm a, int pieces, int per, const float* back) {
+__global__ void __launch_bounds__(kThreads, kPieceBlocksBack) piece_back_apply_kernel(Norm a, int pieces, int per, const float* back) {
   extern __shared__ __align__(16) unsigned char memory[];
   const long long block = (long long)gridDim.x - 1 - blockIdx.x;   // what was read last first
   const long long sample = block / pieces;
@@ -854,7 +851,7 @@ Way choose(long long b, long long s, int n, int groups, int type, bool wide16, b
   const int high = high_of(n, w.V);
   w.shared = std::max(2LL * high * n, 2LL * groups) * 4;
   // as many blocks as the SMs hold at a time, so that all of them end together; rows enough in a piece that its sums are few beside it
-  const long long wanted = std::max(1LL, kSms * (backward ? 3 : 4) / b);
+  const long long wanted = std::max(1LL, kSms * (backward ? kPieceBlocksBack : kPieceBlocks) / b);
   w.per = (int)std::min((long long)1 << 24, std::max({(s + wanted - 1) / wanted, (long long)4 * high, std::min(s, (long long)16)}));
   w.pieces = (int)((s + w.per - 1) / w.per);
   w.parts = (int)std::min(b * w.pieces, 0x7fffffffLL);
@@ -933,10 +930,10 @@ int launch_group_norm(const GroupNormCall& c, cudaStream_t stream) {
       if (w.way == Way::kRow) {
         const dim3 grid(w.across, w.parts);
         if (!back) {
-          auto kernel = w.K == 1 ? row_fwd_kernel<T, V, 1, kRowsAhead> : row_fwd_kernel<T, V, 4, 1>;
+          auto kernel = w.K > 1 ? row_fwd_kernel<T, V, 4, 1, 32> : w.lanes == 32 ? row_fwd_kernel<T, V, 1, kRowsAhead, 32> : row_fwd_kernel<T, V, 1, kRowsAhead, 0>;
           kernel<<<grid, kThreads, 0, stream>>>(a, w.lanes);
         } else {
-          auto kernel = w.K == 1 ? row_bwd_kernel<T, V, 1, kRowsBack> : row_bwd_kernel<T, V, 4, 1>;
+          auto kernel = w.K > 1 ? row_bwd_kernel<T, V, 4, 1, 32> : w.lanes == 32 ? row_bwd_kernel<T, V, 1, kRowsBack, 32> : row_bwd_kernel<T, V, 1, kRowsBack, 0>;
           kernel<<<grid, kThreads, 0, stream>>>(a, w.lanes, w.parts);
         }
         return launched(fn);

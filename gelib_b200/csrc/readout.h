@@ -6,6 +6,9 @@
 #include <type_traits>
 
 #include "common.h"
+#ifdef __CUDACC__
+#include "f32x2.h"
+#endif
 
 namespace gelib_b200 {
 
@@ -106,14 +109,121 @@ __device__ __forceinline__ void store_vec(T* dst, const float (&x)[V]) {
   *reinterpret_cast<typename Raw<V * sizeof(T)>::type*>(dst) = pack<T, V>(x);
 }
 
-// 1 / (1 + exp(-z)) from the approximations of 2^x and 1 / x, without their treatment of subnormal numbers, which took most of the instructions: where
-// exp(-z) is subnormal it is nothing beside 1, and where 1 + exp(-z) is so large that the quotient is subnormal, that is 0 here.
-__device__ __forceinline__ float logistic(float z) {
-  float e, q;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z * -1.4426950408889634f));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(1.f + e));
-  return q;
+// V numbers at a time, in packed pairs: half the instructions.  d may be any of the operands.
+template <int V>
+__device__ __forceinline__ void fma_all(float (&d)[V], const float (&a)[V], const float (&b)[V], const float (&c)[V]) {
+  if constexpr (V % 2 == 0) {
+#pragma unroll
+    for (int k = 0; k < V; k += 2) unpack2(fma2(pack2(a[k], a[k + 1]), pack2(b[k], b[k + 1]), pack2(c[k], c[k + 1])), d[k], d[k + 1]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; k++) d[k] = fmaf(a[k], b[k], c[k]);
+  }
 }
+template <int V>
+__device__ __forceinline__ void fma_all(float (&d)[V], const float (&a)[V], float b, float c) {
+  if constexpr (V % 2 == 0) {
+#pragma unroll
+    for (int k = 0; k < V; k += 2) unpack2(fma2(pack2(a[k], a[k + 1]), pack2(b, b), pack2(c, c)), d[k], d[k + 1]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; k++) d[k] = fmaf(a[k], b, c);
+  }
+}
+template <int V>
+__device__ __forceinline__ void fma_all(float (&d)[V], const float (&a)[V], float b, const float (&c)[V]) {
+  if constexpr (V % 2 == 0) {
+#pragma unroll
+    for (int k = 0; k < V; k += 2) unpack2(fma2(pack2(a[k], a[k + 1]), pack2(b, b), pack2(c[k], c[k + 1])), d[k], d[k + 1]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; k++) d[k] = fmaf(a[k], b, c[k]);
+  }
+}
+template <int V>
+__device__ __forceinline__ void mul_all(float (&d)[V], const float (&a)[V], const float (&b)[V]) {
+  if constexpr (V % 2 == 0) {
+#pragma unroll
+    for (int k = 0; k < V; k += 2) unpack2(mul2(pack2(a[k], a[k + 1]), pack2(b[k], b[k + 1])), d[k], d[k + 1]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; k++) d[k] = a[k] * b[k];
+  }
+}
+template <int V>
+__device__ __forceinline__ void mul_all(float (&d)[V], const float (&a)[V], float b) {
+  if constexpr (V % 2 == 0) {
+#pragma unroll
+    for (int k = 0; k < V; k += 2) unpack2(mul2(pack2(a[k], a[k + 1]), pack2(b, b)), d[k], d[k + 1]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; k++) d[k] = a[k] * b;
+  }
+}
+template <int V>
+__device__ __forceinline__ void add_all(float (&d)[V], const float (&a)[V], const float (&b)[V]) {
+  if constexpr (V % 2 == 0) {
+#pragma unroll
+    for (int k = 0; k < V; k += 2) unpack2(add2(pack2(a[k], a[k + 1]), pack2(b[k], b[k + 1])), d[k], d[k + 1]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; k++) d[k] = a[k] + b[k];
+  }
+}
+template <int V>
+__device__ __forceinline__ void add_all(float (&d)[V], const float (&a)[V], float b) {
+  if constexpr (V % 2 == 0) {
+#pragma unroll
+    for (int k = 0; k < V; k += 2) unpack2(add2(pack2(a[k], a[k + 1]), pack2(b, b)), d[k], d[k + 1]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; k++) d[k] = a[k] + b;
+  }
+}
+template <int V>
+__device__ __forceinline__ float sum_of(const float (&a)[V]) {
+  if constexpr (V % 2 == 0) {
+    f32x2 s = pack2(a[0], a[1]);
+#pragma unroll
+    for (int k = 2; k < V; k += 2) s = add2(s, pack2(a[k], a[k + 1]));
+    float x, y;
+    unpack2(s, x, y);
+    return x + y;
+  } else {
+    float s = a[0];
+#pragma unroll
+    for (int k = 1; k < V; k++) s += a[k];
+    return s;
+  }
+}
+template <int V>
+__device__ __forceinline__ float dot_of(const float (&a)[V], const float (&b)[V]) {
+  if constexpr (V % 2 == 0) {
+    f32x2 s = mul2(pack2(a[0], a[1]), pack2(b[0], b[1]));
+#pragma unroll
+    for (int k = 2; k < V; k += 2) s = fma2(pack2(a[k], a[k + 1]), pack2(b[k], b[k + 1]), s);
+    float x, y;
+    unpack2(s, x, y);
+    return x + y;
+  } else {
+    float s = a[0] * b[0];
+#pragma unroll
+    for (int k = 1; k < V; k++) s = fmaf(a[k], b[k], s);
+    return s;
+  }
+}
+
+// q = 1 / (1 + 2^t), from the approximations of 2^x and 1 / x without their treatment of subnormal numbers, which took most of the instructions: where
+// 2^t is subnormal it is nothing beside 1, and where 1 + 2^t is so large that the quotient is subnormal, that is 0 here.
+template <int V>
+__device__ __forceinline__ void logistics(float (&q)[V], const float (&t)[V]) {
+#pragma unroll
+  for (int k = 0; k < V; k++) asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(q[k]) : "f"(t[k]));
+  add_all(q, q, 1.f);
+#pragma unroll
+  for (int k = 0; k < V; k++) asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q[k]) : "f"(q[k]));
+}
+constexpr float kLog2e = 1.4426950408889634f;
 
 constexpr float kGelu0 = 1.5957691216057308f;             // 2 sqrt(2 / pi): 0.5 (1 + tanh u) is the logistic function of 2u
 constexpr float kGelu1 = kGelu0 * 0.044715f;
@@ -125,36 +235,49 @@ __device__ __forceinline__ void activate(float (&x)[V], int act) {
   if (act == GELIB_ACT_RELU) {
 #pragma unroll
     for (int k = 0; k < V; k++) x[k] = x[k] < 0.f ? 0.f : x[k];     // NaN stays NaN
-  } else if (act == GELIB_ACT_SILU) {
-#pragma unroll
-    for (int k = 0; k < V; k++) x[k] *= logistic(x[k]);
-  } else {
-#pragma unroll
-    for (int k = 0; k < V; k++) x[k] *= logistic(x[k] * (kGelu0 + kGelu1 * x[k] * x[k]));
+    return;
   }
+  float t[V];
+  if (act == GELIB_ACT_SILU) {
+    mul_all(t, x, -kLog2e);
+  } else {
+    mul_all(t, x, x);
+    fma_all(t, t, -kLog2e * kGelu1, -kLog2e * kGelu0);
+    mul_all(t, t, x);
+  }
+  logistics(t, t);
+  mul_all(x, x, t);
 }
 
 // g = g act'(z)
 template <int V>
-__device__ __forceinline__ void activate_back(float (&g)[V], const float (&x)[V], int act) {
+__device__ __forceinline__ void activate_back(float (&g)[V], const float (&z)[V], int act) {
   if (act == GELIB_ACT_NONE) return;
   if (act == GELIB_ACT_RELU) {
 #pragma unroll
-    for (int k = 0; k < V; k++) g[k] = x[k] > 0.f ? g[k] : x[k] != x[k] ? x[k] : 0.f;
+    for (int k = 0; k < V; k++) g[k] = z[k] > 0.f ? g[k] : z[k] != z[k] ? z[k] : 0.f;
     return;
   }
-  const bool silu = act == GELIB_ACT_SILU;
+  float q[V], u[V];
+  if (act == GELIB_ACT_SILU) {   // q + z q (1 - q)
+    mul_all(q, z, -kLog2e);
+    logistics(q, q);
+    fma_all(u, q, -1.f, 1.f);
+    mul_all(u, u, z);
+  } else {                       // q + z q (1 - q) (k0 + 3 k1 z^2)
+    float z2[V];
 #pragma unroll
-  for (int k = 0; k < V; k++) {
-    const float z = x[k];
-    if (silu) {
-      const float q = logistic(z);
-      g[k] *= q * (1.f + z * (1.f - q));
-    } else {
-      const float z2 = fminf(z * z, 1e30f), q = logistic(z * (kGelu0 + kGelu1 * z2));   // finite: where q (1 - q) is 0 the product is
-      g[k] *= q + z * q * (1.f - q) * (kGelu0 + 3.f * kGelu1 * z2);
-    }
+    for (int k = 0; k < V; k++) z2[k] = fminf(z[k] * z[k], 1e30f);   // finite: where q (1 - q) is 0 the product is
+    fma_all(q, z2, -kLog2e * kGelu1, -kLog2e * kGelu0);
+    mul_all(q, q, z);
+    logistics(q, q);
+    fma_all(u, q, -1.f, 1.f);
+    mul_all(u, u, z);
+    fma_all(z2, z2, 3.f * kGelu1, kGelu0);
+    mul_all(u, u, z2);
   }
+  fma_all(q, q, u, q);
+  mul_all(g, g, q);
 }
 
 #endif
