@@ -37,7 +37,7 @@ int check_linear(const char* fn, const gelib_linear_args* p, bool back) {
   if (p->m < 0 || p->k < 0 || p->n < 0) return fail(GELIB_INVALID, fn, "negative size");
   if (!known_activation(p->act) || !known_type(p->type)) return fail(GELIB_INVALID, fn, "unknown activation or type");
   if (p->ldx < p->k || p->ldw < (p->w_transposed ? p->k : p->n)) return fail(GELIB_INVALID, fn, "rows overlap");
-  if (p->m > 0x7fffffffLL) return fail(GELIB_INVALID, fn, "too many rows");
+  if (p->m > 1LL << 30 || p->k > 1 << 30 || p->n > 1 << 30) return fail(GELIB_INVALID, fn, "more than 2^30 rows or columns");
   const int width = type_bytes(p->type);
   for (const void* q : {p->x, p->w, p->bias, p->residual, p->gy, (const void*)p->y, (const void*)p->z, (const void*)p->gx, (const void*)p->gw, (const void*)p->gb})
     if (!is_aligned(q, width)) return fail(GELIB_INVALID, fn, "data pointer not aligned to its type");
