@@ -109,6 +109,9 @@ def _adamw_step(params, grads, m, v, ms, vs, master, step, lr, beta1, beta2, eps
 def block8_values(codes, scale):
     """What an 8-bit state stands for (of exp_avg_sq: its root): codes times the scale of their block of 256, as a bfloat16 tensor of the codes'
     shape, exactly."""
+    out = native().block8_values(codes, scale)
+    if out is not None:
+        return out
     with torch.no_grad(), plain():
         device = codes.device
         if device.type != "cuda":

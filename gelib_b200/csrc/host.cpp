@@ -304,6 +304,19 @@ std::optional<bool> adamw_step(const Tensors& params, const Tensors& grads, cons
   return true;
 }
 
+std::optional<at::Tensor> block8_values(const at::Tensor& codes, const at::Tensor& scale) {
+  if (!codes.defined() || !codes.is_cuda()) return std::nullopt;
+  const auto device = codes.device();
+  if (!plain_dense(codes, device) || codes.scalar_type() != at::kFloat8_e4m3fn || !plain_dense(scale, device) || scale.scalar_type() != at::kFloat ||
+      scale.numel() != (codes.numel() + 255) / 256)
+    return std::nullopt;
+  c10::cuda::CUDAGuard guard(device);
+  at::Tensor out = at::empty(codes.sizes(), at::TensorOptions().dtype(at::kBFloat16).device(device));
+  void* s = stream_of(device);
+  call([&] { return gelib_block8_values(out.data_ptr(), codes.data_ptr(), scale.data_ptr<float>(), codes.numel(), s); });
+  return out;
+}
+
 // ---- readout ---------------------------------------------------------------------------------------------------------------------
 
 using OptTensor = std::optional<at::Tensor>;
@@ -515,6 +528,7 @@ PYBIND11_MODULE(_native, m) {
   m.def("part_backward", torch::wrap_pybind_function(&part_backward));
   m.def("linear", torch::wrap_pybind_function(&linear));
   m.def("group_norm", torch::wrap_pybind_function(&group_norm));
+  m.def("block8_values", torch::wrap_pybind_function(&block8_values));
   m.def("adamw_step", torch::wrap_pybind_function(&adamw_step));
   m.def("gather", torch::wrap_pybind_function(&gather));
 }

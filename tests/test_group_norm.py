@@ -283,3 +283,30 @@ def test_a_second_derivative_is_refused(native, monkeypatch):
     g, = torch.autograd.grad(G.group_norm(x, 2, activation="silu").square().sum(), x, create_graph=True)
     with pytest.raises(RuntimeError, match="once"):
         g.sum().backward()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("b,s,n,groups,dtype,offset", [(2, 90000, 112, 7, torch.float32, 0), (1, 90000, 111, 3, torch.float32, 1), (1, 170000, 112, 7, torch.bfloat16, 0)])
+def test_samples_larger_than_the_shared_memory_of_all_sms(b, s, n, groups, dtype, offset):
+    import gelib_b200 as G
+    x, w, bias, gy = make(b, s, n, dtype, offset)
+    got = run(G, x, groups, w, bias, "silu", gy)
+    for g, (want, size), what in zip(got, reference(x, groups, w, bias, 1e-5, "silu", gy), ("y", "gx", "gw", "gb")):
+        near(g, want, size, what)
+    again = run(G, x, groups, w, bias, "silu", gy)
+    assert all(torch.equal(p, q) for p, q in zip(got, again))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("b,s,n,groups", [(1, 9001, 64, 4), (3, 4003, 112, 7), (7, 2500, 200, 8), (40, 700, 333, 3), (150, 600, 256, 8), (2, 65536, 60, 5), (1, 37, 16384, 2), (5, 60, 12000, 3)])
+def test_samples_larger_than_the_shared_memory_of_one_sm(b, s, n, groups):
+    """Few and many of them, rows that do not divide among the blocks."""
+    import gelib_b200 as G
+    for dtype, offset in ((torch.float32, 0), (torch.bfloat16, 0), (torch.float32, 1)):
+        x, w, bias, gy = make(b, s, n, dtype, offset)
+        got = run(G, x, groups, w, bias, "gelu_tanh", gy)
+        for g, (want, size), what in zip(got, reference(x, groups, w, bias, 1e-5, "gelu_tanh", gy), ("y", "gx", "gw", "gb")):
+            near(g, want, size, (what, dtype, offset))
+        only_w = w.detach().requires_grad_()
+        G.group_norm(x, groups, only_w, bias, activation="gelu_tanh").backward(gy)
+        assert torch.equal(only_w.grad, got[2])
