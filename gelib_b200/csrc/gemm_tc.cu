@@ -351,6 +351,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_tc_kernel(const __grid_const
   tc::tc_fence_after();
   const uint32_t tmem = bars.tmem, ring_at = smem_u32(ring);
   bool ok = true;
+  let_next_begin();
+  await_previous();
 
   if (warp == 0 || warp == 2) {   // copies of A, of B
     const bool of_b = warp == 2;
@@ -685,7 +687,7 @@ bool encode(CUtensorMap* map, const Stored& s, int type, int box_x, int box_y) {
 }
 
 template <class T, int CG, int P>
-int launch_as(const TcMaps& maps, const TcArgs& a, cudaStream_t stream) {
+int launch_as(const TcMaps& maps, const TcArgs& a, bool follows, cudaStream_t stream) {
   static const char* fn = "linear";
   auto kernel = gemm_tc_kernel<T, CG, P>;
   constexpr int shared = Shape<CG, P>::kShared;
@@ -702,18 +704,20 @@ int launch_as(const TcMaps& maps, const TcArgs& a, cudaStream_t stream) {
   c.blockDim = dim3(kThreads);
   c.dynamicSmemBytes = shared;
   c.stream = stream;
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = CG, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
-  c.attrs = at;
-  c.numAttrs = CG > 1 ? 1 : 0;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  c.attrs = CG > 1 ? at : at + 1;
+  c.numAttrs = (CG > 1) + follows;
   GELIB_CUDA_TRY(fn, cudaLaunchKernelEx(&c, kernel, maps, a));
   return launched(fn);
 }
 
 template <class T, int P>
-int launch_config(int cg, const TcMaps& maps, const TcArgs& a, cudaStream_t stream) {
-  return cg == 2 ? launch_as<T, 2, P>(maps, a, stream) : launch_as<T, 1, P>(maps, a, stream);
+int launch_config(int cg, const TcMaps& maps, const TcArgs& a, bool follows, cudaStream_t stream) {
+  return cg == 2 ? launch_as<T, 2, P>(maps, a, follows, stream) : launch_as<T, 1, P>(maps, a, follows, stream);
 }
 
 }  // namespace
@@ -731,7 +735,7 @@ long long tc_gemm_workspace(const Gemm* g, int count) {
   return bytes;
 }
 
-int launch_tc_gemm(const Gemm* g, int count, void* workspace, Joins* joins, cudaStream_t stream) {
+int launch_tc_gemm(const Gemm* g, int count, bool follows, void* workspace, Joins* joins, cudaStream_t stream) {
   static const char* fn = "linear";
   const Plan plan = plan_of(g, count);
   TcMaps maps;
@@ -771,9 +775,9 @@ int launch_tc_gemm(const Gemm* g, int count, void* workspace, Joins* joins, cuda
   a.status = async_status_word(kStatusGemmTc);
   a.limit = inject_timeout() ? 0 : kWaitLimit;
   a.bf16 = g[0].type != GELIB_F16;
-  if (g[0].type == GELIB_F32) return launch_config<float, 3>(plan.cg, maps, a, stream);
-  if (g[0].type == GELIB_BF16) return launch_config<__nv_bfloat16, 1>(plan.cg, maps, a, stream);
-  return launch_config<__half, 1>(plan.cg, maps, a, stream);
+  if (g[0].type == GELIB_F32) return launch_config<float, 3>(plan.cg, maps, a, follows, stream);
+  if (g[0].type == GELIB_BF16) return launch_config<__nv_bfloat16, 1>(plan.cg, maps, a, follows, stream);
+  return launch_config<__half, 1>(plan.cg, maps, a, follows, stream);
 }
 
 }  // namespace gelib_b200

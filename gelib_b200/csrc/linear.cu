@@ -126,6 +126,7 @@ __device__ __forceinline__ void join_block(const Joins::Join& a, long long block
 template <class T>
 __global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ JoinArgs a) {
   __shared__ float t[8][32][5];
+  await_previous();
   long long block = blockIdx.x;
 #pragma unroll
   for (int i = 0; i < 2; i++) {
@@ -136,18 +137,20 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ 
     }
     block -= a.blocks[i];
   }
-  const int lane = threadIdx.x % 32, group = threadIdx.x / 32, n = a.joins.sum_n;
-  const long long c = block * 32 + lane;
+  // eight columns, 32 threads for each
+  float* sums = &t[0][0][0];
+  const int lane = threadIdx.x % 8, group = threadIdx.x / 8, n = a.joins.sum_n;
+  const long long c = block * 8 + lane;
   float s = 0;
   if (c < n)
-#pragma unroll 8
-    for (int i = group; i < a.joins.sum_parts; i += 8) s += a.joins.sums[(long long)i * n + c];
-  t[group][lane][0] = s;
+#pragma unroll 4
+    for (int i = group; i < a.joins.sum_parts; i += 32) s += a.joins.sums[(long long)i * n + c];
+  sums[threadIdx.x] = s;
   __syncthreads();
   if (group == 0 && c < n) {
     s = 0;
 #pragma unroll
-    for (int i = 0; i < 8; i++) s += t[i][lane][0];
+    for (int i = 0; i < 32; i++) s += sums[i * 8 + lane];
     static_cast<T*>(a.joins.gb)[c] = from_float<T>(s);
   }
 }
@@ -256,6 +259,7 @@ struct ActBack {
 template <class T, int V>
 __global__ void __launch_bounds__(kThreads) prepare_kernel(const __grid_constant__ ActBack a, const __grid_constant__ PlaneJobs jobs) {
   __shared__ float chan[kThreads * V];
+  let_next_begin();
   const int blocks = a.chunks * a.parts;
   if ((int)blockIdx.x >= blocks) {
     copy_planes<T>(jobs, blockIdx.x - blocks, gridDim.x - blocks);
@@ -409,8 +413,8 @@ long long products_workspace(const Gemm* g, int count, bool tc) {
   for (int i = 0; i < count; i++) bytes += simple_workspace(g[i]);
   return bytes;
 }
-int launch_products(const Gemm* g, int count, bool tc, char* at, Joins* joins, cudaStream_t stream) {
-  if (tc) return count ? launch_tc_gemm(g, count, at, joins, stream) : GELIB_OK;
+int launch_products(const Gemm* g, int count, bool tc, bool follows, char* at, Joins* joins, cudaStream_t stream) {
+  if (tc) return count ? launch_tc_gemm(g, count, follows, at, joins, stream) : GELIB_OK;
   for (int i = 0; i < count; i++) {
     const int st = launch_simple(g[i], at, joins, stream);
     if (st != GELIB_OK) return st;
@@ -437,13 +441,11 @@ int launch_joins(const Joins& joins, int type, cudaStream_t stream) {
     a.blocks[i] = (q.size + each - 1) / each;
     blocks += a.blocks[i];
   }
-  if (joins.gb) blocks += a.blocks[2] = (joins.sum_n + 31) / 32;
+  if (joins.gb) blocks += a.blocks[2] = (joins.sum_n + 7) / 8;
   if (blocks == 0) return GELIB_OK;
   if (blocks > 0x7fffffffLL) return fail(GELIB_INVALID, "linear", "too many elements");
-  if (type == GELIB_F32) join_kernel<float><<<(unsigned)blocks, kThreads, 0, stream>>>(a);
-  else if (type == GELIB_BF16) join_kernel<__nv_bfloat16><<<(unsigned)blocks, kThreads, 0, stream>>>(a);
-  else join_kernel<__half><<<(unsigned)blocks, kThreads, 0, stream>>>(a);
-  return launched("linear");
+  const auto kernel = type == GELIB_F32 ? join_kernel<float> : type == GELIB_BF16 ? join_kernel<__nv_bfloat16> : join_kernel<__half>;
+  return launch_after("linear", true, kernel, dim3((unsigned)blocks), kThreads, 0, stream, a);
 }
 
 long long linear_workspace(const gelib_linear_args& p, bool backward) {
@@ -465,15 +467,15 @@ int launch_linear(const gelib_linear_args& p, void* workspace, cudaStream_t stre
   const bool tc = takes_tc(p.m, p.k, p.n);
   char* at = (char*)workspace;
   int st;
+  PlaneJobs jobs = {};
   if (tc) {
-    PlaneJobs jobs = {};
     copy_if_needed(&x, p.type, at, &jobs);
     copy_if_needed(&w, p.type, at, &jobs);
     if ((st = launch_prepare({}, 1, jobs, p.type, stream)) != GELIB_OK) return st;
   }
   const Gemm g = forward_of(p, x, w);
   Joins joins;
-  if ((st = launch_products(&g, 1, tc, at, &joins, stream)) != GELIB_OK) return st;
+  if ((st = launch_products(&g, 1, tc, jobs.count > 0, at, &joins, stream)) != GELIB_OK) return st;
   return launch_joins(joins, p.type, stream);
 }
 
@@ -520,7 +522,7 @@ int launch_linear_back(const gelib_linear_args& p, void* workspace, cudaStream_t
   if (st != GELIB_OK) return st;
   Gemm g[2];
   const int count = backward_of(p, x, w, gz, g);
-  if ((st = launch_products(g, count, tc, at, &joins, stream)) != GELIB_OK) return st;
+  if ((st = launch_products(g, count, tc, jobs.count > 0 || back.chunks > 0, at, &joins, stream)) != GELIB_OK) return st;
   return launch_joins(joins, p.type, stream);
 }
 

@@ -53,7 +53,8 @@ int launch_joins(const Joins& joins, int type, cudaStream_t stream);
 // boundaries.
 bool tc_ready(const Stored& s, int type);
 long long tc_gemm_workspace(const Gemm* g, int count);
-int launch_tc_gemm(const Gemm* g, int count, void* workspace, Joins* joins, cudaStream_t stream);
+// `follows`: the launch before on the stream is one of this call's.
+int launch_tc_gemm(const Gemm* g, int count, bool follows, void* workspace, Joins* joins, cudaStream_t stream);
 
 // Products of at most eight rows (linear_rows.cu).
 bool takes_rows(const Gemm& g);

@@ -161,6 +161,7 @@ __global__ void __launch_bounds__(kThreads, K == 1 ? kBlocksAhead : 1) row_fwd_k
 // The sums over rows stay in registers; a block's warps have the same groups and add theirs up at the end.
 template <class T, int V, int K, int R, int L>
 __global__ void __launch_bounds__(kThreads, K == 1 ? kBlocksBack : 1) row_bwd_kernel(Norm a, int lanes, int parts) {
+  let_next_begin();
   __shared__ float sums[kWarps][2][32 * V];
   if (L > 0) lanes = L;
   const int per = 32 / lanes, lane = threadIdx.x % lanes, warp = threadIdx.x / 32;
@@ -383,6 +384,7 @@ __global__ void __launch_bounds__(kThreads) tile_fwd_kernel(Norm a, int gpc, int
 // Blocks of one chunk walk the samples; the chunk's parameter sums stay in shared memory.
 template <class T, int V>
 __global__ void __launch_bounds__(kThreads) tile_bwd_kernel(Norm a, int gpc, int parts) {
+  let_next_begin();
   extern __shared__ __align__(16) unsigned char memory[];
   const int chunk = blockIdx.x;
   const int g0 = chunk * gpc, ng = min(gpc, a.groups - g0), channels = ng * a.cg, c0 = g0 * a.cg, rows = (int)a.s;
@@ -495,6 +497,7 @@ __global__ void __launch_bounds__(kThreads) tile_bwd_kernel(Norm a, int gpc, int
 // Sum, and sum of squares of differences from the piece's own mean, of every group of a piece: part (b, pieces, groups, 2).
 template <class T, int V>
 __global__ void __launch_bounds__(kThreads, kPieceBlocks) piece_stats_kernel(Norm a, int pieces, int per) {
+  let_next_begin();
   extern __shared__ __align__(16) unsigned char memory[];
   const long long sample = blockIdx.x / pieces;
   const int piece = blockIdx.x % pieces;
@@ -580,6 +583,7 @@ __device__ __forceinline__ void join_pieces(const Norm& a, long long sample, int
 
 template <class T, int V>
 __global__ void __launch_bounds__(kThreads, kPieceBlocks) piece_apply_kernel(Norm a, int pieces, int per) {
+  await_previous();
   extern __shared__ __align__(16) unsigned char memory[];
   // the pieces that were read last may still be in L2: they are taken first
   const long long block = (long long)gridDim.x - 1 - blockIdx.x;
@@ -664,6 +668,7 @@ __device__ __forceinline__ void each_row(const Norm& a, long long base, int rows
 // gz xh and gz summed over a piece's rows, per channel: part (2, b * pieces, n); and times w, per group: back (b, pieces, groups, 2).
 template <class T, int V>
 __global__ void __launch_bounds__(kThreads, kPieceBlocksBack) piece_back_sums_kernel(Norm a, int pieces, int per, float* back) {
+  let_next_begin();
   extern __shared__ __align__(16) unsigned char memory[];
   const long long sample = blockIdx.x / pieces;
   const int piece = blockIdx.x % pieces;
@@ -716,6 +721,8 @@ __global__ void __launch_bounds__(kThreads, kPieceBlocksBack) piece_back_sums_ke
 
 template <class T, int V>
 __global__ void __launch_bounds__(kThreads, kPieceBlocksBack) piece_back_apply_kernel(Norm a, int pieces, int per, const float* back) {
+  let_next_begin();
+  await_previous();
   extern __shared__ __align__(16) unsigned char memory[];
   const long long block = (long long)gridDim.x - 1 - blockIdx.x;   // what was read last first
   const long long sample = block / pieces;
@@ -760,6 +767,7 @@ __global__ void __launch_bounds__(kThreads, kPieceBlocksBack) piece_back_apply_k
 template <class T>
 __global__ void __launch_bounds__(1024) sum_parts_kernel(T* gw, T* gb, const float* sums, int parts, int n) {
   __shared__ float t[32][33];
+  await_previous();
   const int c = blockIdx.x * 32 + threadIdx.x;
   T* out = blockIdx.y ? gb : gw;
   if (!out) return;
@@ -895,8 +903,7 @@ int launch_sum_parts(void* gw, void* gb, const float* sums, int parts, int n, in
   if (!gw && !gb) return GELIB_OK;
   return with_type(type, [&](auto* t) -> int {
     using T = std::remove_pointer_t<decltype(t)>;
-    sum_parts_kernel<T><<<dim3((n + 31) / 32, 2), dim3(32, 32), 0, stream>>>((T*)gw, (T*)gb, sums, parts, n);
-    return launched("sum_parts");
+    return launch_after("sum_parts", true, sum_parts_kernel<T>, dim3((n + 31) / 32, 2), dim3(32, 32), 0, stream, (T*)gw, (T*)gb, sums, parts, n);
   });
 }
 
@@ -955,8 +962,7 @@ int launch_group_norm(const GroupNormCall& c, cudaStream_t stream) {
         if ((st = launched(fn)) != GELIB_OK) return st;
         const size_t shared = 2ULL * c.groups * 4;
         if ((st = room(fn, piece_apply_kernel<T, V>, shared)) != GELIB_OK) return st;
-        piece_apply_kernel<T, V><<<(unsigned)samples, kThreads, shared, stream>>>(a, w.pieces, w.per);
-        return launched(fn);
+        return launch_after(fn, true, piece_apply_kernel<T, V>, dim3((unsigned)samples), kThreads, shared, stream, a, w.pieces, w.per);
       }
       if ((st = room(fn, piece_back_sums_kernel<T, V>, w.shared)) != GELIB_OK) return st;
       float* back = c.workspace + 2LL * w.parts * c.n;
@@ -964,8 +970,7 @@ int launch_group_norm(const GroupNormCall& c, cudaStream_t stream) {
       if ((st = launched(fn)) != GELIB_OK || !a.y) return st;
       const size_t shared = 2ULL * c.groups * 4;
       if ((st = room(fn, piece_back_apply_kernel<T, V>, shared)) != GELIB_OK) return st;
-      piece_back_apply_kernel<T, V><<<(unsigned)samples, kThreads, shared, stream>>>(a, w.pieces, w.per, back);
-      return launched(fn);
+      return launch_after(fn, true, piece_back_apply_kernel<T, V>, dim3((unsigned)samples), kThreads, shared, stream, a, w.pieces, w.per, (const float*)back);
     });
   });
   if (st != GELIB_OK || !back) return st;

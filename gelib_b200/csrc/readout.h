@@ -29,6 +29,24 @@ int launch_sum_parts(void* gw, void* gb, const float* sums, int parts, int n, in
 
 #ifdef __CUDACC__
 
+// Kernels of one call that follow one another: the later one is launched while the earlier one ends, and its blocks wait where they begin to read (or
+// write) what that one wrote.  Every block of it has to wait, so that nothing that comes after can begin before the earlier kernel has ended.
+__device__ __forceinline__ void let_next_begin() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void await_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <class... P, class... A>
+int launch_after(const char* fn, bool follows, void (*kernel)(P...), dim3 grid, dim3 block, size_t shared, cudaStream_t stream, const A&... args) {
+  cudaLaunchConfig_t c = {};
+  c.gridDim = grid, c.blockDim = block, c.dynamicSmemBytes = shared, c.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  c.attrs = at;
+  c.numAttrs = follows ? 1 : 0;
+  GELIB_CUDA_TRY(fn, cudaLaunchKernelEx(&c, kernel, args...));
+  return launched(fn);
+}
+
 template <class T>
 __device__ __forceinline__ float to_float(T v) {
   if constexpr (std::is_same_v<T, float>) return v;
