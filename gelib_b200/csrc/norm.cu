@@ -8,7 +8,8 @@
 // large mean costs no digits.  Memory bounds it: a read and a write forward, two reads and a write backward, if the elements that
 // share a statistic stay on the SM between its sum and its use.  Three ways of keeping them, by size:
 //
-//   row    s = 1 and a group of at most 1024 channels (512 in float32): a few lanes of a warp own a (row, group) in registers
+//   row    small samples (s = 1 and a group of at most 1024 channels, 512 in float32; or as many numbers in a group, whose row is 1, 2, 4, .. 32
+//          accesses): a few lanes of a warp own a (sample, group) in registers
 //   tile   a sample's rows of some groups fit a block's shared memory
 //   two    larger samples: sums over pieces of a sample, then a second pass over x (and gy) that applies them
 //
@@ -67,9 +68,17 @@ __device__ __forceinline__ void load_or(const void* p, long long at, float other
     for (int k = 0; k < V; k++) x[k] = other;
 }
 
-// ---- row: s = 1 ----------------------------------------------------------------------------------------------------------------
-// `lanes` lanes (a power of two) own a group: K accesses of V elements each.  A warp keeps its groups, whose weights it holds, and walks rows, R
-// at a time: their loads and the exchanges of their sums overlap.  Block (x, y): groups, and every gridDim.y-th set of 8 R rows.
+// ---- row: small samples ----------------------------------------------------------------------------------------------------------
+// `lanes` lanes (a power of two) own a group: K accesses of V elements each.  A warp keeps its groups, whose weights it holds, and walks samples, R
+// at a time: their loads and the exchanges of their sums overlap.  Block (x, y): groups, and every gridDim.y-th set of 8 R samples.
+// kMany: samples of several rows, whose group is `vpr` accesses wide, a power of two: a lane has the same channels in all of its rows.
+// (4096, 8, 512) in 32 groups, bfloat16: a block per sample took 78 us forward and 131 back.
+
+// Where a lane's k-th access lies from the group's first element, and whether there is one.
+struct Spot {
+  int row, vec;
+};
+__device__ __forceinline__ Spot spot_of(bool many, int i, int vpr) { return many ? Spot{i / vpr, i & (vpr - 1)} : Spot{0, i}; }
 
 template <class T, int V>
 struct Piece {   // an access as it lies
@@ -78,41 +87,48 @@ struct Piece {   // an access as it lies
   __device__ __forceinline__ void get(float (&x)[V]) const { unpack<T, V>(raw, x); }
 };
 
-template <class T, int V, int K, int R, int L>
-__global__ void __launch_bounds__(kThreads, K == 1 ? kBlocksAhead : 1) row_fwd_kernel(Norm a, int lanes) {
+template <class T, int V, int K, int R, int L, bool kMany>
+__global__ void __launch_bounds__(kThreads, K == 1 ? kBlocksAhead : 1) row_fwd_kernel(Norm a, int lanes, int vpr) {
   if (L > 0) lanes = L;
   const int per = 32 / lanes, lane = threadIdx.x % lanes, warp = threadIdx.x / 32;
-  const int g = blockIdx.x * per + (threadIdx.x & 31) / lanes, c0 = g * a.cg + lane * V;
+  const int g = blockIdx.x * per + (threadIdx.x & 31) / lanes, c0 = g * a.cg;
   const bool live = g < a.groups;
-  const float inv = 1.f / a.cg;
+  const long long sample = a.s * a.n;   // its elements
+  const float inv = 1.f / ((float)a.s * a.cg);
+  constexpr int W = kMany ? 1 : K;
   bool has[K];
-  float w[K][V], bias[K][V];
+  int off[K];
+  float w[W][V], bias[W][V];
 #pragma unroll
   for (int k = 0; k < K; k++) {
-    has[k] = live && (k * lanes + lane) * V < a.cg;
+    const Spot at = spot_of(kMany, k * lanes + lane, vpr);
+    has[k] = live && at.row < a.s && at.vec * V < a.cg;
+    off[k] = at.row * a.n + at.vec * V;
+    if (k < W) {
 #pragma unroll
-    for (int j = 0; j < V; j++) w[k][j] = bias[k][j] = 0;
-    if (has[k]) {
-      load_or<T, V>(a.w, c0 + k * lanes * V, 1.f, w[k]);
-      load_or<T, V>(a.bias, c0 + k * lanes * V, 0.f, bias[k]);
+      for (int j = 0; j < V; j++) w[k][j] = bias[k][j] = 0;
+      if (live && at.vec * V < a.cg) {
+        load_or<T, V>(a.w, c0 + at.vec * V, 1.f, w[k]);
+        load_or<T, V>(a.bias, c0 + at.vec * V, 0.f, bias[k]);
+      }
     }
   }
   const long long step = (long long)gridDim.y * kWarps * R;
   Piece<T, V> next[R][K];
   long long row = ((long long)blockIdx.y * kWarps + warp) * R;
-  const T* x = static_cast<const T*>(a.x) + row * a.n + c0;
-  T* y = static_cast<T*>(a.y) + row * a.n + c0;
+  const T* x = static_cast<const T*>(a.x) + row * sample + c0;
+  T* y = static_cast<T*>(a.y) + row * sample + c0;
   auto fetch = [&](long long row) {
 #pragma unroll
     for (int r = 0; r < R; r++)
 #pragma unroll
       for (int k = 0; k < K; k++) {
-        if (has[k] && row + r < a.b) next[r][k].load(x + (long long)r * a.n + k * lanes * V);
+        if (has[k] && row + r < a.b) next[r][k].load(x + r * sample + off[k]);
         else next[r][k].raw = {};
       }
   };
   if (row < a.b) fetch(row);
-  for (; row < a.b; row += step, y += step * a.n) {
+  for (; row < a.b; row += step, y += step * sample) {
     float v[R][K][V], mean[R], rstd[R];
 #pragma unroll
     for (int r = 0; r < R; r++) {
@@ -123,7 +139,7 @@ __global__ void __launch_bounds__(kThreads, K == 1 ? kBlocksAhead : 1) row_fwd_k
         mean[r] += sum_of(v[r][k]);
       }
     }
-    x += step * a.n;
+    x += step * sample;
     if (row + step < a.b) fetch(row + step);   // on their way while these rows are worked on
     lanes_sums<L>(mean, lanes);
 #pragma unroll
@@ -150,41 +166,48 @@ __global__ void __launch_bounds__(kThreads, K == 1 ? kBlocksAhead : 1) row_fwd_k
       for (int k = 0; k < K; k++)
         if (has[k]) {
           mul_all(v[r][k], v[r][k], rstd[r]);
-          fma_all(v[r][k], v[r][k], w[k], bias[k]);
+          fma_all(v[r][k], v[r][k], w[kMany ? 0 : k], bias[kMany ? 0 : k]);
           activate(v[r][k], a.act);
-          store_vec<T, V>(y + (long long)r * a.n + k * lanes * V, v[r][k]);
+          store_vec<T, V>(y + r * sample + off[k], v[r][k]);
         }
     }
   }
 }
 
 // The sums over rows stay in registers; a block's warps have the same groups and add theirs up at the end.
-template <class T, int V, int K, int R, int L>
-__global__ void __launch_bounds__(kThreads, K == 1 ? kBlocksBack : 1) row_bwd_kernel(Norm a, int lanes, int parts) {
+template <class T, int V, int K, int R, int L, bool kMany>
+__global__ void __launch_bounds__(kThreads, K == 1 ? kBlocksBack : 1) row_bwd_kernel(Norm a, int lanes, int vpr, int parts) {
   let_next_begin();
   __shared__ float sums[kWarps][2][32 * V];
   if (L > 0) lanes = L;
   const int per = 32 / lanes, lane = threadIdx.x % lanes, warp = threadIdx.x / 32;
-  const int g = blockIdx.x * per + (threadIdx.x & 31) / lanes, c0 = g * a.cg + lane * V;
+  const int g = blockIdx.x * per + (threadIdx.x & 31) / lanes, c0 = g * a.cg;
   const bool live = g < a.groups;
-  const float inv = 1.f / a.cg;
+  const long long sample = a.s * a.n;   // its elements
+  const float inv = 1.f / ((float)a.s * a.cg);
+  constexpr int W = kMany ? 1 : K;
   bool has[K];
-  float w[K][V], bias[K][V], gw[K][V], gb[K][V];
+  int off[K];
+  float w[W][V], bias[W][V], gw[W][V], gb[W][V];
 #pragma unroll
   for (int k = 0; k < K; k++) {
-    has[k] = live && (k * lanes + lane) * V < a.cg;
+    const Spot at = spot_of(kMany, k * lanes + lane, vpr);
+    has[k] = live && at.row < a.s && at.vec * V < a.cg;
+    off[k] = at.row * a.n + at.vec * V;
+    if (k < W) {
 #pragma unroll
-    for (int j = 0; j < V; j++) w[k][j] = bias[k][j] = gw[k][j] = gb[k][j] = 0;
-    if (has[k]) {
-      load_or<T, V>(a.w, c0 + k * lanes * V, 1.f, w[k]);
-      load_or<T, V>(a.bias, c0 + k * lanes * V, 0.f, bias[k]);
+      for (int j = 0; j < V; j++) w[k][j] = bias[k][j] = gw[k][j] = gb[k][j] = 0;
+      if (live && at.vec * V < a.cg) {
+        load_or<T, V>(a.w, c0 + at.vec * V, 1.f, w[k]);
+        load_or<T, V>(a.bias, c0 + at.vec * V, 0.f, bias[k]);
+      }
     }
   }
   const long long step = (long long)gridDim.y * kWarps * R;
   Piece<T, V> px[R][K], pg[R][K];
   float pm[R], pr[R];
   long long row = ((long long)blockIdx.y * kWarps + warp) * R;
-  long long at = row * a.n + c0, out = at;
+  long long at = row * sample + c0, out = at;
   auto fetch = [&](long long row) {
     const T *x = static_cast<const T*>(a.x) + at, *gy = static_cast<const T*>(a.gy) + at;
 #pragma unroll
@@ -195,8 +218,8 @@ __global__ void __launch_bounds__(kThreads, K == 1 ? kBlocksBack : 1) row_bwd_ke
 #pragma unroll
       for (int k = 0; k < K; k++) {
         if (has[k] && row + r < a.b) {
-          px[r][k].load(x + (long long)r * a.n + k * lanes * V);
-          pg[r][k].load(gy + (long long)r * a.n + k * lanes * V);
+          px[r][k].load(x + r * sample + off[k]);
+          pg[r][k].load(gy + r * sample + off[k]);
         } else {
           px[r][k].raw = {};
           pg[r][k].raw = {};
@@ -205,7 +228,7 @@ __global__ void __launch_bounds__(kThreads, K == 1 ? kBlocksBack : 1) row_bwd_ke
     }
   };
   if (row < a.b) fetch(row);
-  for (; row < a.b; row += step, out += step * a.n) {
+  for (; row < a.b; row += step, out += step * sample) {
     float h[R][K][V], gz[R][K][V], mean[R], rstd[R], s1[R], s2[R];
 #pragma unroll
     for (int r = 0; r < R; r++) {
@@ -213,21 +236,22 @@ __global__ void __launch_bounds__(kThreads, K == 1 ? kBlocksBack : 1) row_bwd_ke
 #pragma unroll
       for (int k = 0; k < K; k++) px[r][k].get(h[r][k]), pg[r][k].get(gz[r][k]);
     }
-    at += step * a.n;
+    at += step * sample;
     if (row + step < a.b) fetch(row + step);   // on their way while these rows are worked on
 #pragma unroll
     for (int r = 0; r < R; r++) {
       s1[r] = s2[r] = 0;
 #pragma unroll
       for (int k = 0; k < K; k++) {
+        const int q = kMany ? 0 : k;
         float z[V];
         add_all(h[r][k], h[r][k], -mean[r]);   // first the difference: a large mean costs no digits
         mul_all(h[r][k], h[r][k], rstd[r]);
-        fma_all(z, h[r][k], w[k], bias[k]);
-        activate_back(gz[r][k], z, a.act);
-        add_all(gb[k], gb[k], gz[r][k]);
-        fma_all(gw[k], gz[r][k], h[r][k], gw[k]);
-        mul_all(gz[r][k], gz[r][k], w[k]);
+        fma_all(z, h[r][k], w[q], bias[q]);
+        activate_back(gz[r][k], z, a.act);     // gy is zero where there is nothing
+        add_all(gb[q], gb[q], gz[r][k]);
+        fma_all(gw[q], gz[r][k], h[r][k], gw[q]);
+        mul_all(gz[r][k], gz[r][k], w[q]);
         s1[r] += sum_of(gz[r][k]);
         s2[r] += dot_of(gz[r][k], h[r][k]);
       }
@@ -244,14 +268,23 @@ __global__ void __launch_bounds__(kThreads, K == 1 ? kBlocksBack : 1) row_bwd_ke
             add_all(gz[r][k], gz[r][k], s1[r]);
             fma_all(gz[r][k], h[r][k], s2[r], gz[r][k]);
             mul_all(gz[r][k], gz[r][k], rstd[r]);
-            store_vec<T, V>(static_cast<T*>(a.y) + out + (long long)r * a.n + k * lanes * V, gz[r][k]);
+            store_vec<T, V>(static_cast<T*>(a.y) + out + r * sample + off[k], gz[r][k]);
           }
       }
     }
   }
   if (!a.part) return;
+  if constexpr (kMany) {   // lanes with the same channels
+    for (int d = vpr; d < lanes; d *= 2) {
 #pragma unroll
-  for (int k = 0; k < K; k++) {
+      for (int j = 0; j < V; j++) {
+        gw[0][j] += __shfl_xor_sync(0xffffffffu, gw[0][j], d);
+        gb[0][j] += __shfl_xor_sync(0xffffffffu, gb[0][j], d);
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < W; k++) {
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < V; j++) {
@@ -262,7 +295,7 @@ __global__ void __launch_bounds__(kThreads, K == 1 ? kBlocksBack : 1) row_bwd_ke
     for (int e = threadIdx.x; e < 2 * 32 * V; e += kThreads) {
       const int which = e / (32 * V), q = e % (32 * V), l = q / V;
       const int group = blockIdx.x * per + l / lanes, c = (k * lanes + l % lanes) * V + q % V;
-      if (group < a.groups && c < a.cg) {
+      if (group < a.groups && c < a.cg && (!kMany || l % lanes < vpr)) {
         float t = 0;
 #pragma unroll
         for (int i = 0; i < kWarps; i++) t += sums[i][which][q];
@@ -570,6 +603,7 @@ __device__ __forceinline__ void join_pieces(const Norm& a, long long sample, int
   const float* p = a.part + (sample * pieces * a.groups + g) * 2;
   const long long step = 2LL * a.groups;
   float t = 0;
+#pragma unroll 8
   for (int i = lane; i < pieces; i += 32) t += p[i * step] * (float)min((long long)per, a.s - (long long)i * per);
   const float mean = warp_total(t) / (float)a.s;
   t = 0;
@@ -734,6 +768,7 @@ __global__ void __launch_bounds__(kThreads, kPieceBlocksBack) piece_back_apply_k
   float* means = reinterpret_cast<float*>(memory);   // [2][groups]
   for (int g = warp; g < a.groups; g += kWarps) {
     float s1 = 0, s2 = 0;
+#pragma unroll 8
     for (int i = lane; i < pieces; i += 32) {
       const float2 q = *reinterpret_cast<const float2*>(back + ((sample * pieces + i) * a.groups + g) * 2);
       s1 += q.x, s2 += q.y;
@@ -794,7 +829,7 @@ constexpr int kSharedLimit = 200 * 1024;
 struct Way {
   enum { kRow, kTile, kTwo } way;
   int V;             // elements of an access
-  int lanes, K, R, across;   // row
+  int lanes, K, R, across, vpr;   // row
   int gpc, chunks;   // tile: groups of a chunk
   size_t shared;     // tile, two
   int parts;         // backward: rows of partial sums
@@ -807,14 +842,16 @@ Way choose(long long b, long long s, int n, int groups, int type, bool wide16, b
   Way w = {};
   const int cg = n / groups, size = type_bytes(type);
   auto fits = [&](int bytes) { return bytes >= size && cg * size % bytes == 0 && (bytes <= size || (bytes == 16 ? wide16 : wide8)); };
-  if (s == 1) {
+  if (s <= 512) {
     const int V = (fits(16) ? 16 : fits(8) ? 8 : size) / size;
-    const int need = (cg + V - 1) / V;
-    if (need <= 128) {
-      w.way = Way::kRow, w.V = V;
+    const int across = (cg + V - 1) / V;   // accesses of a row of a group
+    const bool even = across <= 32 && (across & (across - 1)) == 0;
+    const long long need = across * s;
+    if (need <= 128 && (s == 1 || even)) {
+      w.way = Way::kRow, w.V = V, w.vpr = across;
       w.lanes = 1;
       while (w.lanes < need && w.lanes < 32) w.lanes *= 2;
-      w.K = need <= 32 ? 1 : 4;
+      w.K = need <= 32 ? 1 : need <= 64 && s > 1 ? 2 : 4;
       const int across = (groups + 32 / w.lanes - 1) / (32 / w.lanes);
       w.across = across;
       w.R = w.K > 1 ? 1 : backward ? kRowsBack : kRowsAhead;
@@ -936,12 +973,21 @@ int launch_group_norm(const GroupNormCall& c, cudaStream_t stream) {
       int st;
       if (w.way == Way::kRow) {
         const dim3 grid(w.across, w.parts);
+        const bool many = c.s > 1;
         if (!back) {
-          auto kernel = w.K > 1 ? row_fwd_kernel<T, V, 4, 1, 32> : w.lanes == 32 ? row_fwd_kernel<T, V, 1, kRowsAhead, 32> : row_fwd_kernel<T, V, 1, kRowsAhead, 0>;
-          kernel<<<grid, kThreads, 0, stream>>>(a, w.lanes);
+          const auto kernel = many ? (w.K == 4   ? row_fwd_kernel<T, V, 4, 1, 32, true>
+                                      : w.K == 2 ? row_fwd_kernel<T, V, 2, 1, 32, true>
+                                      : w.lanes == 32 ? row_fwd_kernel<T, V, 1, kRowsAhead, 32, true> : row_fwd_kernel<T, V, 1, kRowsAhead, 0, true>)
+                                   : (w.K == 4 ? row_fwd_kernel<T, V, 4, 1, 32, false>
+                                      : w.lanes == 32 ? row_fwd_kernel<T, V, 1, kRowsAhead, 32, false> : row_fwd_kernel<T, V, 1, kRowsAhead, 0, false>);
+          kernel<<<grid, kThreads, 0, stream>>>(a, w.lanes, w.vpr);
         } else {
-          auto kernel = w.K > 1 ? row_bwd_kernel<T, V, 4, 1, 32> : w.lanes == 32 ? row_bwd_kernel<T, V, 1, kRowsBack, 32> : row_bwd_kernel<T, V, 1, kRowsBack, 0>;
-          kernel<<<grid, kThreads, 0, stream>>>(a, w.lanes, w.parts);
+          const auto kernel = many ? (w.K == 4   ? row_bwd_kernel<T, V, 4, 1, 32, true>
+                                      : w.K == 2 ? row_bwd_kernel<T, V, 2, 1, 32, true>
+                                      : w.lanes == 32 ? row_bwd_kernel<T, V, 1, kRowsBack, 32, true> : row_bwd_kernel<T, V, 1, kRowsBack, 0, true>)
+                                   : (w.K == 4 ? row_bwd_kernel<T, V, 4, 1, 32, false>
+                                      : w.lanes == 32 ? row_bwd_kernel<T, V, 1, kRowsBack, 32, false> : row_bwd_kernel<T, V, 1, kRowsBack, 0, false>);
+          kernel<<<grid, kThreads, 0, stream>>>(a, w.lanes, w.vpr, w.parts);
         }
         return launched(fn);
       }

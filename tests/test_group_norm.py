@@ -310,3 +310,17 @@ def test_samples_larger_than_the_shared_memory_of_one_sm(b, s, n, groups):
         only_w = w.detach().requires_grad_()
         G.group_norm(x, groups, only_w, bias, activation="gelu_tanh").backward(gy)
         assert torch.equal(only_w.grad, got[2])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("b,s,n,groups", [(50, 8, 512, 32), (9, 2, 64, 8), (300, 3, 32, 2), (41, 16, 64, 2), (5, 100, 24, 6), (17, 7, 128, 4), (3, 5, 4, 4), (70, 4, 1024, 4), (11, 64, 16, 2),
+                                          (6, 128, 8, 1), (5, 31, 96, 3)])
+def test_small_samples_of_several_rows(b, s, n, groups):
+    import gelib_b200 as G
+    for dtype, offset in ((torch.float32, 0), (torch.bfloat16, 0), (torch.float16, 1)):
+        x, w, bias, gy = make(b, s, n, dtype, offset)
+        got = run(G, x, groups, w, bias, "silu", gy)
+        for g, (want, size), what in zip(got, reference(x, groups, w, bias, 1e-5, "silu", gy), ("y", "gx", "gw", "gb")):
+            near(g, want, size, (what, dtype, offset))
+        again = run(G, x, groups, w, bias, "silu", gy)
+        assert all(torch.equal(p, q) for p, q in zip(got, again))
