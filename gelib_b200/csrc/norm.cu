@@ -321,15 +321,36 @@ __device__ __forceinline__ Columns columns_of(int channels, int V) {
   return c;
 }
 
+// The groups of a column's V channels: one division, not V.
+template <int V>
+__device__ __forceinline__ void groups_of(int channel, int cg, int (&g)[V]) {
+  int q = channel / cg, rest = channel - q * cg;
+#pragma unroll
+  for (int j = 0; j < V; j++) {
+    g[j] = q;
+    if (++rest == cg) rest = 0, q++;
+  }
+}
+
+// The sum over `high` rows of `channels` of a group's channels, by a warp.
+__device__ __forceinline__ float group_sum(const float* chan, int high, int channels, int g, int cg) {
+  const int lane = threadIdx.x % 32;
+  float t = 0;
+  for (int c = lane; c < cg; c += 32)
+    for (int i = 0; i < high; i++) t += chan[i * channels + g * cg + c];
+  return lanes_sum(t, 32);
+}
+
 // The sums of f over a column's rows, one per channel and row of threads, then per group: group[g] = sum.  chan has high * channels floats.
-template <int V, class F>
-__device__ __forceinline__ void channel_sums(const Columns& c, int rows, int channels, float* chan, F f) {
+template <int V, class P, class F>
+__device__ __forceinline__ void channel_sums(const Columns& c, int rows, int channels, float* chan, P prepare, F f) {
   const int tx = threadIdx.x % c.wide, ty = threadIdx.x / c.wide;
   if (ty < c.high)
     for (int col = tx; col < c.cols; col += c.wide) {
       float sum[V];
 #pragma unroll
       for (int j = 0; j < V; j++) sum[j] = 0;
+      prepare(col);
       for (int r = ty; r < rows; r += c.high) f(r, col, sum);
 #pragma unroll
       for (int j = 0; j < V; j++) chan[ty * channels + col * V + j] = sum[j];
@@ -350,37 +371,38 @@ __global__ void __launch_bounds__(kThreads) tile_fwd_kernel(Norm a, int gpc, int
   float* group = chan + max(cl.high * channels, 1);
   const T* x = static_cast<const T*>(a.x) + sample * a.s * a.n + c0;
   const float count = (float)rows * a.cg;
-  channel_sums<V>(cl, rows, channels, chan, [&](int r, int col, float (&sum)[V]) {
+  float mean[V];
+  channel_sums<V>(cl, rows, channels, chan, [](int) {}, [&](int r, int col, float (&sum)[V]) {
     using R = typename Raw<V * sizeof(T)>::type;
-    *reinterpret_cast<R*>(tile + r * channels + col * V) = *reinterpret_cast<const R*>(x + (long long)r * a.n + col * V);
+    const R raw = *reinterpret_cast<const R*>(x + (long long)r * a.n + col * V);
+    *reinterpret_cast<R*>(tile + r * channels + col * V) = raw;
     float v[V];
-    load_vec<T, V>(tile + r * channels + col * V, v);
-#pragma unroll
-    for (int j = 0; j < V; j++) sum[j] += v[j];
+    unpack<T, V>(raw, v);
+    add_all(sum, sum, v);
   });
   __syncthreads();
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   for (int g = warp; g < ng; g += kWarps) {
-    float t = 0;
-    for (int e = lane; e < cl.high * a.cg; e += 32) t += chan[e / a.cg * channels + g * a.cg + e % a.cg];
-    t = warp_total(t);
+    const float t = group_sum(chan, cl.high, channels, g, a.cg);
     if (lane == 0) group[g] = t / count;
   }
   __syncthreads();
-  channel_sums<V>(cl, rows, channels, chan, [&](int r, int col, float (&sum)[V]) {
+  auto of_column = [&](int col) {
+    int g[V];
+    groups_of<V>(col * V, a.cg, g);
+#pragma unroll
+    for (int j = 0; j < V; j++) mean[j] = group[g[j]];
+  };
+  channel_sums<V>(cl, rows, channels, chan, of_column, [&](int r, int col, float (&sum)[V]) {
     float v[V];
     load_vec<T, V>(tile + r * channels + col * V, v);
 #pragma unroll
-    for (int j = 0; j < V; j++) {
-      const float d = v[j] - group[(col * V + j) / a.cg];
-      sum[j] += d * d;
-    }
+    for (int j = 0; j < V; j++) v[j] -= mean[j];
+    fma_all(sum, v, v, sum);
   });
   __syncthreads();
   for (int g = warp; g < ng; g += kWarps) {
-    float t = 0;
-    for (int e = lane; e < cl.high * a.cg; e += 32) t += chan[e / a.cg * channels + g * a.cg + e % a.cg];
-    t = warp_total(t);
+    const float t = group_sum(chan, cl.high, channels, g, a.cg);
     if (lane == 0) {
       const float rstd = rsqrtf(t / count + a.eps);
       group[ng + g] = rstd;
@@ -394,20 +416,22 @@ __global__ void __launch_bounds__(kThreads) tile_fwd_kernel(Norm a, int gpc, int
   const int tx = threadIdx.x % cl.wide, ty = threadIdx.x / cl.wide;
   if (ty >= cl.high) return;
   for (int col = tx; col < cl.cols; col += cl.wide) {
-    float w[V], bias[V], mean[V];
+    float w[V], bias[V];
+    int g[V];
     load_or<T, V>(a.w, c0 + col * V, 1.f, w);
     load_or<T, V>(a.bias, c0 + col * V, 0.f, bias);
+    groups_of<V>(col * V, a.cg, g);
 #pragma unroll
     for (int j = 0; j < V; j++) {
-      const int g = (col * V + j) / a.cg;
-      mean[j] = group[g];
-      w[j] *= group[ng + g];
+      mean[j] = group[g[j]];
+      w[j] *= group[ng + g[j]];
     }
     for (int r = ty; r < rows; r += cl.high) {
       float v[V];
       load_vec<T, V>(tile + r * channels + col * V, v);
 #pragma unroll
-      for (int j = 0; j < V; j++) v[j] = (v[j] - mean[j]) * w[j] + bias[j];
+      for (int j = 0; j < V; j++) v[j] -= mean[j];
+      fma_all(v, v, w, bias);
       activate(v, a.act);
       store_vec<T, V>(static_cast<T*>(a.y) + (sample * a.s + r) * a.n + c0 + col * V, v);
     }
@@ -442,13 +466,12 @@ __global__ void __launch_bounds__(kThreads) tile_bwd_kernel(Norm a, int gpc, int
     if (ty < cl.high)
       for (int col = tx; col < cl.cols; col += cl.wide) {
         float w[V], bias[V], mean[V], rstd[V], sb[V], sw[V];
+        int gr[V];
         load_or<T, V>(a.w, c0 + col * V, 1.f, w);
         load_or<T, V>(a.bias, c0 + col * V, 0.f, bias);
+        groups_of<V>(col * V, a.cg, gr);
 #pragma unroll
-        for (int j = 0; j < V; j++) {
-          const int g = (col * V + j) / a.cg;
-          mean[j] = group[g], rstd[j] = group[ng + g], sb[j] = sw[j] = 0;
-        }
+        for (int j = 0; j < V; j++) mean[j] = group[gr[j]], rstd[j] = group[ng + gr[j]], sb[j] = sw[j] = 0;
         for (int r = ty; r < rows; r += cl.high) {
           using R = typename Raw<V * sizeof(T)>::type;
           const int at = r * channels + col * V;
@@ -457,16 +480,15 @@ __global__ void __launch_bounds__(kThreads) tile_bwd_kernel(Norm a, int gpc, int
           *reinterpret_cast<R*>(tx_ + at) = rx;
           *reinterpret_cast<R*>(tg_ + at) = rg;
           float h[V], g[V], z[V];
-          load_vec<T, V>(tx_ + at, h);
-          load_vec<T, V>(tg_ + at, g);
+          unpack<T, V>(rx, h);
+          unpack<T, V>(rg, g);
 #pragma unroll
-          for (int j = 0; j < V; j++) {
-            h[j] = (h[j] - mean[j]) * rstd[j];
-            z[j] = h[j] * w[j] + bias[j];
-          }
+          for (int j = 0; j < V; j++) h[j] -= mean[j];
+          mul_all(h, h, rstd);
+          fma_all(z, h, w, bias);
           activate_back(g, z, a.act);
-#pragma unroll
-          for (int j = 0; j < V; j++) sb[j] += g[j], sw[j] += g[j] * h[j];
+          add_all(sb, sb, g);
+          fma_all(sw, g, h, sw);
         }
 #pragma unroll
         for (int j = 0; j < V; j++) {
@@ -495,25 +517,26 @@ __global__ void __launch_bounds__(kThreads) tile_bwd_kernel(Norm a, int gpc, int
     if (a.y && ty < cl.high)
       for (int col = tx; col < cl.cols; col += cl.wide) {
         float w[V], bias[V], mean[V], rstd[V], s1[V], s2[V];
+        int gr[V];
         load_or<T, V>(a.w, c0 + col * V, 1.f, w);
         load_or<T, V>(a.bias, c0 + col * V, 0.f, bias);
+        groups_of<V>(col * V, a.cg, gr);
 #pragma unroll
-        for (int j = 0; j < V; j++) {
-          const int g = (col * V + j) / a.cg;
-          mean[j] = group[g], rstd[j] = group[ng + g], s1[j] = group[2 * ng + g], s2[j] = group[3 * ng + g];
-        }
+        for (int j = 0; j < V; j++) mean[j] = group[gr[j]], rstd[j] = group[ng + gr[j]], s1[j] = group[2 * ng + gr[j]], s2[j] = -group[3 * ng + gr[j]];
         for (int r = ty; r < rows; r += cl.high) {
           float h[V], g[V], z[V];
           load_vec<T, V>(tx_ + r * channels + col * V, h);
           load_vec<T, V>(tg_ + r * channels + col * V, g);
 #pragma unroll
-          for (int j = 0; j < V; j++) {
-            h[j] = (h[j] - mean[j]) * rstd[j];
-            z[j] = h[j] * w[j] + bias[j];
-          }
+          for (int j = 0; j < V; j++) h[j] -= mean[j];
+          mul_all(h, h, rstd);
+          fma_all(z, h, w, bias);
           activate_back(g, z, a.act);
+          mul_all(g, g, w);
 #pragma unroll
-          for (int j = 0; j < V; j++) g[j] = rstd[j] * (g[j] * w[j] - s1[j] - h[j] * s2[j]);
+          for (int j = 0; j < V; j++) g[j] -= s1[j];
+          fma_all(g, h, s2, g);
+          mul_all(g, g, rstd);
           store_vec<T, V>(static_cast<T*>(a.y) + base + (long long)r * a.n + col * V, g);
         }
       }
