@@ -12,6 +12,9 @@
 // The step is bound by memory: 28 bytes an element in 32 bits (p, m, v read and written, g read), 16 in 8 bits.  A network's weights
 // are many small tensors, so their addresses travel in the launch's parameters, a tensor is cut into pieces of as many elements as a block takes, and
 // a block finds its piece by bisection.
+//
+// Measured on 46.7 million weights: 190 us in 32 bits (28 bytes an element, 6.8 TB/s: the copy rate); 8 bits and a bfloat16 head 165 us, where the bytes take 114:
+// 75 instructions an element, most of them the two roundings, half of them on the integer pipe (57 % busy).  Two dozen small tensors 11 us a call, half of it Python's.
 #include <cuda_fp8.h>
 
 #include <algorithm>

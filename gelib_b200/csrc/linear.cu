@@ -6,6 +6,12 @@
 // Forward is one matrix product whose epilogue adds, activates and rounds once.  Backward is one pass over gy and z for gz and the
 // column sums, and two products.  Sums over rows are split over blocks when there are few tiles, as partial sums that are added
 // in a fixed order.
+//
+// The tensor cores (gemm_tc.cu) do the products of nine rows and more, at most eight go to linear_rows.cu, and a simple product of any layout does what
+// is left.  A backward call is three launches: what goes before the products (one pass over gy and z beside the operands'
+// copies), both products, and the joins of partial sums beside the bias's gradient.  With gradients, us a pass of the Python call: 777 x
+// 204 x 131 bfloat16 86 and 1000 x 1280 x 512 float32 87, of which autograd's own hand-over is about 50; 65536 x 112 x 112 float32 with
+// a residual 141, bound by memory (the float operands' copies are a third of the bytes); 4096 x 7168 x 2048 bfloat16 325, the products 260.
 #include <algorithm>
 
 #include "readout.h"
@@ -348,10 +354,18 @@ int launch_prepare(const ActBack& a, int V, const PlaneJobs& jobs, int type, cud
 
 long long up(long long bytes) { return (bytes + 255) / 256 * 256; }
 
-// Which product a layer's call takes: the tensor cores from `kTcWork` multiplications on, which is where their operands' copies (float, or
-// rows off their 16-byte boundaries) and a longer start are made up for.
-constexpr double kTcWork = 4e6;
-bool takes_tc(long long m, long long k, long long n) { return k > 0 && m > 16 && (double)m * k * n >= kTcWork && device_has_tcgen05(); }
+Stored x_of(const gelib_linear_args& p);
+Stored w_of(const gelib_linear_args& p);
+
+// Whether a layer's call takes the tensor cores.  At most eight rows do not: their forward and the gradient of x read the weights once
+// (linear_rows.cu), and the gradient of w is a sum of eight products.  More do, backward always (17 x 8 x 8 to 32 x 1280 x 1280, us: float32 13 to 23
+// against 21 to 60 of the simple product, bfloat16 11 to 21 against 27 to 72), forward unless operands have to be copied for less than 40000
+// multiplications (72 x 17 x 11 float32 8.7 simple, 11.3 with copies; 20 x 64 x 64 12.6 and 11.2; bfloat16 in place 6.6 whatever the size, 7.9 to 41).
+constexpr double kTcCopied = 4e4;
+bool takes_tc(const gelib_linear_args& p, bool backward) {
+  if (p.m <= 8 || p.k == 0 || !device_has_tcgen05()) return false;
+  return backward || (tc_ready(x_of(p), p.type) && tc_ready(w_of(p), p.type)) || (double)p.m * p.k * p.n >= kTcCopied;
+}
 
 Stored x_of(const gelib_linear_args& p) { return {p.x, p.m, p.k, p.ldx, 0, 1}; }
 Stored w_of(const gelib_linear_args& p) { return {p.w, p.w_transposed ? p.n : p.k, p.w_transposed ? p.k : p.n, p.ldw, 0, 1}; }
@@ -450,7 +464,7 @@ int launch_joins(const Joins& joins, int type, cudaStream_t stream) {
 
 long long linear_workspace(const gelib_linear_args& p, bool backward) {
   if (p.m == 0 || p.n == 0) return 0;
-  const bool tc = takes_tc(p.m, p.k, p.n);
+  const bool tc = takes_tc(p, backward);
   const Stored x = x_of(p), w = w_of(p), gz = {p.gy, p.m, p.n, p.n, 0, 1};
   const long long copies = tc ? copy_bytes(x, p.type) + copy_bytes(w, p.type) : 0;
   if (!backward) {
@@ -464,7 +478,7 @@ long long linear_workspace(const gelib_linear_args& p, bool backward) {
 
 int launch_linear(const gelib_linear_args& p, void* workspace, cudaStream_t stream) {
   Stored x = x_of(p), w = w_of(p);
-  const bool tc = takes_tc(p.m, p.k, p.n);
+  const bool tc = takes_tc(p, false);
   char* at = (char*)workspace;
   int st;
   PlaneJobs jobs = {};
@@ -488,7 +502,7 @@ int launch_linear_back(const gelib_linear_args& p, void* workspace, cudaStream_t
     if (p.gb && p.n) GELIB_CUDA_TRY(fn, cudaMemsetAsync(p.gb, 0, (size_t)p.n * width, stream));
     return GELIB_OK;
   }
-  const bool tc = takes_tc(p.m, p.k, p.n), products = (p.gx || p.gw) && p.k;
+  const bool tc = takes_tc(p, true), products = (p.gx || p.gw) && p.k;
   char* at = (char*)workspace;
   Joins joins;
   if (p.gb) {

@@ -5,7 +5,8 @@
 // The weights are read once, 16 bytes a lane.  Where a row of the weights holds all n of one k, a lane owns 16 bytes' worth of columns and
 // the lanes, warps and blocks of a cluster share k; where it holds all k of one n, a warp owns columns and its lanes share k.  The blocks of a
 // cluster add their sums through distributed shared memory in the order of their ranks, so that one launch does it and results repeat.
-// 1280 x 1280 bfloat16, one row: 4.1 us, of which the launch is most (3.3 MB).
+// 1280 x 1280 bfloat16, one row: 6.3 us a call of the Python function, nearly all of it the call and the launch (3.3 MB of weights take 0.5 us); by the simple product
+// with its sums joined by a second launch 37 us.
 #include <algorithm>
 
 #include "readout.h"
