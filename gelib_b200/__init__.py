@@ -2,8 +2,8 @@
 
 Drop-in for the ``gelib`` Python package on that path: ``SO3part`` / ``SO3vec`` (and the ``Arr``
 variants) with ``CGproduct``, ``DiagCGproduct``, ``spharm`` and autograd; ``gelib_b200.backend`` stands
-in for the pybind11 module ``gelib_base``.  All products run in hand-written CUDA kernels behind the
-C ABI of ``include/gelib_b200.h``; tensors must live on a CUDA device.
+in for the pybind11 module ``gelib_base``.  ``group_norm``, ``linear`` and ``AdamW`` are what a network needs after its last
+product.  All of it runs in hand-written CUDA kernels behind the C ABI of ``include/gelib_b200.h``; tensors must live on a CUDA device.
 """
 from . import backend
 from .backend import SO3CGmatrix, gather_map

@@ -11,10 +11,10 @@
 // five small products of a slab come first and a0 b0 last, and after every slab the sums leave tensor memory for registers, where
 // they are added with rounding: four cuts at full size and no more (7e-7).
 //
-// What bounds it: bfloat16, 4096 x 7168 x 2048 83 us (1440 TFLOP/s, 0.86 of the library's rate at 8192^3), 128 tiles on 74 pairs being two rounds; 8192^3 690 us
-// (1600); the slabs' way out of L2, 0.38 us for a pair's tile of 256 columns where the multiplications take 0.27.  float, 4096^3 620 us (222 TFLOP/s of float
-// products, six times as many on the tensor cores).  Steps of a 128 x 128 tile at that first size: one lane issuing in a branch 138 us, an elected lane of a converged warp 117, a
-// warp for A and one for B 105; the results of a tile by four warps, eight columns a store, held a row of 1152-long sums up (1152 wide: 62 us, the library 53).
+// What bounds it: bfloat16, 4096 x 7168 x 2048 83 us (1440 TFLOP/s; the library 80), where 128 tiles on 74 pairs are two rounds; 8192^3 690 us (1600; the
+// library 660).  A pair's slab for a tile of 256 columns takes 0.38 us, its multiplications 0.27: the rest is the slabs' way out of L2.  Sums of 1152 are short beside
+// the epilogue: 16384 x 1152 x 1152 62 us, the library 53.  float, 4096^3 650 us (210 TFLOP/s of float products, six times as many on the tensor cores).
+// Steps, first size in tiles of 128 x 128: one lane issuing in a branch 138 us, an elected lane of a converged warp 117, one warp for A and one for B 105.
 //
 // Every wait has a limit; a kernel that gives up says so in a status word, and ends.
 #include <cuda.h>
