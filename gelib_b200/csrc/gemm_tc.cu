@@ -601,6 +601,10 @@ double launch_time(const Work* w, int count, int slots) {
   return 3 + time + (join > 0 ? 2.5 + join : 0);
 }
 
+// A sum of 16-bit products stays in one accumulator, which the tensor cores cut off some 2e-8 of its size after every 16 products: beyond 131072
+// products that comes near float16's rounding, so longer sums are split, into 64 at most, whatever the number of tiles.
+constexpr int kLongSum = 2048;   // slabs
+
 // The tiles and splits of a launch's products with the least estimated time.
 Plan choose_plan(const Sizes* z, int count, int type) {
   Plan best = {1, 0, {{128, 1}, {128, 1}}};
@@ -614,9 +618,13 @@ Plan choose_plan(const Sizes* z, int count, int type) {
         const int next = bn - 16 * cg;
         if (bn > 32 * cg && (N + bn - 1) / bn == (N + next - 1) / next) continue;   // a narrower tile covers N as often
         const double tiles = (double)((z[i].M + 128 * cg - 1) / (128 * cg)) * ((N + bn - 1) / bn);
+        bool was_long = false;
         static const int kSplits[] = {1, 2, 3, 4, 5, 6, 8, 12, 16, 24, 32, 48, 64};
         for (int splits : kSplits) {
-          if (splits > 1 && (splits > slabs || tiles * splits > 2 * slots || slabs / splits < (type == GELIB_F32 ? 2 : 4))) break;
+          const bool long_sum = type != GELIB_F32 && slabs > (long long)kLongSum * splits && splits < 64;
+          if (splits > 1 && !was_long && (splits > slabs || tiles * splits > 2 * slots || slabs / splits < (type == GELIB_F32 ? 2 : 4))) break;
+          was_long = long_sum;
+          if (long_sum) continue;
           const long long per = (slabs + splits - 1) / splits;
           may[i].push_back({bn, (int)((slabs + per - 1) / per)});
         }
