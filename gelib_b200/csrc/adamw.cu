@@ -13,8 +13,8 @@
 // are many small tensors, so their addresses travel in the launch's parameters, a tensor is cut into pieces of as many elements as a block takes, and
 // a block finds its piece by bisection.
 //
-// Measured on 46.7 million weights: 190 us in 32 bits (28 bytes an element, 6.8 TB/s: the copy rate); 8 bits and a bfloat16 head 165 us, where the bytes take 114:
-// 75 instructions an element, most of them the two roundings, half of them on the integer pipe (57 % busy).  Two dozen small tensors 11 us a call, half of it Python's.
+// Measured on 46.7 million weights: 190 us in 32 bits (28 bytes an element, 6.8 TB/s: the copy rate); 8 bits and a bfloat16 head 141 us, where the bytes take 114:
+// 75 instructions an element, most of them the two roundings, half of them on the integer pipe.  Two dozen small tensors 11 us a call, half of it Python's.
 #include <cuda_fp8.h>
 
 #include <algorithm>
@@ -252,8 +252,9 @@ __device__ __forceinline__ void step_piece(const Entry& e, const Scalars& s, lon
   }
 }
 
+// Six blocks of an SM although a few registers spill: 8 bits 141 us, five 146, as many registers as it likes 166 to 222.
 template <int N, bool k8>
-__global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__ Args<N> a) {
+__global__ void __launch_bounds__(kThreads, k8 ? 6 : 4) adamw_kernel(const __grid_constant__ Args<N> a) {
   const Entry& e = find(a, (int)blockIdx.x);
   const long long i = (long long)((int)blockIdx.x - e.first) * kPiece + threadIdx.x * 8;
   static_assert(kPiece == kThreads * 8, "a lane takes eight elements");
@@ -291,18 +292,31 @@ constexpr int kMost = 350;   // entries of 88 bytes in the 32764 bytes that a la
 
 __global__ void __launch_bounds__(kThreads) block8_values_kernel(__nv_bfloat16* __restrict__ out, const unsigned char* __restrict__ codes,
                                                                 const float* __restrict__ scale, long long n, bool wide) {
-  const long long i = ((long long)blockIdx.x * kThreads + threadIdx.x) * 8;
-  if (i >= n) return;
-  unsigned short c[4];
-  float x[8];
-  wide ? load_codes<true>(codes, i, n, c) : load_codes<false>(codes, i, n, c);
-  const float s = scale[i / kBlock];
+  // two accesses a thread, asked for together
+  const long long i0 = ((long long)blockIdx.x * 2 * kThreads + threadIdx.x) * 8;
+  unsigned short c[2][4];
+  float s[2];
 #pragma unroll
-  for (int k = 0; k < 4; k++) {
-    const float2 f = values_of(c[k]);
-    x[2 * k] = f.x * s, x[2 * k + 1] = f.y * s;
+  for (int q = 0; q < 2; q++) {
+    const long long i = i0 + q * kThreads * 8;
+    if (i < n) {
+      wide ? load_codes<true>(codes, i, n, c[q]) : load_codes<false>(codes, i, n, c[q]);
+      s[q] = scale[i / kBlock];
+    }
   }
-  wide ? store_n<__nv_bfloat16, true>(out, i, n, x) : store_n<__nv_bfloat16, false>(out, i, n, x);
+#pragma unroll
+  for (int q = 0; q < 2; q++) {
+    const long long i = i0 + q * kThreads * 8;
+    if (i >= n) return;
+    float x[8];
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const float2 f = values_of(c[q][k]);
+      x[2 * k] = f.x, x[2 * k + 1] = f.y;
+    }
+    mul_all(x, x, s[q]);
+    wide ? store_n<__nv_bfloat16, true>(out, i, n, x) : store_n<__nv_bfloat16, false>(out, i, n, x);
+  }
 }
 
 }  // namespace
@@ -359,7 +373,7 @@ int launch_adamw(int count, const gelib_adamw_tensor* t, const gelib_adamw_optio
 int launch_block8_values(void* out, const void* codes, const float* scale, long long n, cudaStream_t stream) {
   if (n == 0) return GELIB_OK;
   const bool wide = is_aligned(out, 16) && is_aligned(codes, 8);
-  const long long per = kThreads * 8, blocks = (n + per - 1) / per;
+  const long long per = kThreads * 16, blocks = (n + per - 1) / per;
   if (blocks > 0x7fffffffLL) return fail(GELIB_INVALID, "block8_values", "too many elements");
   block8_values_kernel<<<(unsigned)blocks, kThreads, 0, stream>>>((__nv_bfloat16*)out, (const unsigned char*)codes, scale, n, wide);
   return launched("block8_values");
