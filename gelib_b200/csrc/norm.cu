@@ -18,7 +18,7 @@
 // Measured, forward / backward us (what the bytes take at 6.5 TB/s): rows of 7168 channels in 32 groups, 4096 of them, bfloat16 35 / 54 (18 / 27), bound by the
 // issue of instructions -- 240 for a warp's eight channels a lane in the first form, the packed pairs and the approximate logistic function without subnormal
 // numbers halved them; 4 x 65536 x 112 float32, in two passes, 70 / 113 (36 / 54 and half as much again for the second reading), memory at 0.75 of its
-// rate; 3000 x 19 x 204 bfloat16, in shared memory, 34 / 56 (7 / 11), the latency of a block's phases.
+// rate; 3000 x 19 x 204 bfloat16, in shared memory, 29 / 56 (7 / 11), the latency of a block's phases.
 #include <algorithm>
 
 #include "readout.h"
@@ -30,6 +30,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
+constexpr int kTileThreads = 128, kTileWarps = kTileThreads / 32;   // of a block that holds a sample: 3000 x 19 x 204 29 us forward, 34 with 256
 constexpr int kRowsAhead = 4, kRowsBack = 2;        // of a warp at a time, forward and backward
 constexpr int kBlocksAhead = 2, kBlocksBack = 2;    // of an SM
 constexpr int kPieceBlocks = 4, kPieceBlocksBack = 2;   // of an SM, where samples are taken in pieces
@@ -318,11 +319,11 @@ struct Columns {
   int wide;      // threads side by side: min(cols, kThreads)
   int high;      // rows worked on together
 };
-__device__ __forceinline__ Columns columns_of(int channels, int V) {
+__device__ __forceinline__ Columns columns_of(int channels, int V, int threads = kThreads) {
   Columns c;
   c.cols = channels / V;
-  c.wide = min(c.cols, kThreads);
-  c.high = kThreads / c.wide;
+  c.wide = min(c.cols, threads);
+  c.high = threads / c.wide;
   return c;
 }
 
@@ -365,12 +366,12 @@ __device__ __forceinline__ void channel_sums(const Columns& c, int rows, int cha
 __device__ __forceinline__ float warp_total(float v) { return lanes_sum(v, 32); }
 
 template <class T, int V>
-__global__ void __launch_bounds__(kThreads) tile_fwd_kernel(Norm a, int gpc, int chunks) {
+__global__ void __launch_bounds__(kTileThreads) tile_fwd_kernel(Norm a, int gpc, int chunks) {
   extern __shared__ __align__(16) unsigned char memory[];
   const int chunk = blockIdx.x % chunks;
   const long long sample = blockIdx.x / chunks;
   const int g0 = chunk * gpc, ng = min(gpc, a.groups - g0), channels = ng * a.cg, c0 = g0 * a.cg, rows = (int)a.s;
-  const Columns cl = columns_of(channels, V);
+  const Columns cl = columns_of(channels, V, kTileThreads);
   T* tile = reinterpret_cast<T*>(memory);
   float* chan = reinterpret_cast<float*>(memory + ((size_t)rows * channels * sizeof(T) + 15) / 16 * 16);
   float* group = chan + max(cl.high * channels, 1);
@@ -387,7 +388,7 @@ __global__ void __launch_bounds__(kThreads) tile_fwd_kernel(Norm a, int gpc, int
   });
   __syncthreads();
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  for (int g = warp; g < ng; g += kWarps) {
+  for (int g = warp; g < ng; g += kTileWarps) {
     const float t = group_sum(chan, cl.high, channels, g, a.cg);
     if (lane == 0) group[g] = t / count;
   }
@@ -406,7 +407,7 @@ __global__ void __launch_bounds__(kThreads) tile_fwd_kernel(Norm a, int gpc, int
     fma_all(sum, v, v, sum);
   });
   __syncthreads();
-  for (int g = warp; g < ng; g += kWarps) {
+  for (int g = warp; g < ng; g += kTileWarps) {
     const float t = group_sum(chan, cl.high, channels, g, a.cg);
     if (lane == 0) {
       const float rstd = rsqrtf(t / count + a.eps);
@@ -445,12 +446,12 @@ __global__ void __launch_bounds__(kThreads) tile_fwd_kernel(Norm a, int gpc, int
 
 // Blocks of one chunk walk the samples; the chunk's parameter sums stay in shared memory.
 template <class T, int V>
-__global__ void __launch_bounds__(kThreads) tile_bwd_kernel(Norm a, int gpc, int parts) {
+__global__ void __launch_bounds__(kTileThreads) tile_bwd_kernel(Norm a, int gpc, int parts) {
   let_next_begin();
   extern __shared__ __align__(16) unsigned char memory[];
   const int chunk = blockIdx.x;
   const int g0 = chunk * gpc, ng = min(gpc, a.groups - g0), channels = ng * a.cg, c0 = g0 * a.cg, rows = (int)a.s;
-  const Columns cl = columns_of(channels, V);
+  const Columns cl = columns_of(channels, V, kTileThreads);
   const size_t bytes = ((size_t)rows * channels * sizeof(T) + 15) / 16 * 16;
   T* tx_ = reinterpret_cast<T*>(memory);
   T* tg_ = reinterpret_cast<T*>(memory + bytes);
@@ -459,11 +460,11 @@ __global__ void __launch_bounds__(kThreads) tile_bwd_kernel(Norm a, int gpc, int
   float* group = total + 2 * channels;                           // [4][ng]: mean, rstd, two means of gradients
   const int tx = threadIdx.x % cl.wide, ty = threadIdx.x / cl.wide, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const float count = (float)rows * a.cg;
-  for (int c = threadIdx.x; c < 2 * channels; c += kThreads) total[c] = 0;
+  for (int c = threadIdx.x; c < 2 * channels; c += kTileThreads) total[c] = 0;
   for (long long sample = blockIdx.y; sample < a.b; sample += gridDim.y) {
     const long long base = sample * a.s * a.n + c0;
     __syncthreads();
-    for (int g = threadIdx.x; g < ng; g += kThreads) {
+    for (int g = threadIdx.x; g < ng; g += kTileThreads) {
       group[g] = a.mean[sample * a.groups + g0 + g];
       group[ng + g] = a.rstd[sample * a.groups + g0 + g];
     }
@@ -502,7 +503,7 @@ __global__ void __launch_bounds__(kThreads) tile_bwd_kernel(Norm a, int gpc, int
         }
       }
     __syncthreads();
-    for (int c = threadIdx.x; c < channels; c += kThreads) {
+    for (int c = threadIdx.x; c < channels; c += kTileThreads) {
       float sw = 0, sb = 0;
       for (int i = 0; i < cl.high; i++) sw += chan[i * channels + c], sb += chan[(cl.high + i) * channels + c];
       total[c] += sw;
@@ -512,7 +513,7 @@ __global__ void __launch_bounds__(kThreads) tile_bwd_kernel(Norm a, int gpc, int
       chan[cl.high * channels + c] = sb * w;
     }
     __syncthreads();
-    for (int g = warp; g < ng; g += kWarps) {
+    for (int g = warp; g < ng; g += kTileWarps) {
       float s1 = 0, s2 = 0;
       for (int c = lane; c < a.cg; c += 32) s2 += chan[g * a.cg + c], s1 += chan[cl.high * channels + g * a.cg + c];
       s1 = warp_total(s1), s2 = warp_total(s2);
@@ -548,7 +549,7 @@ __global__ void __launch_bounds__(kThreads) tile_bwd_kernel(Norm a, int gpc, int
   }
   __syncthreads();
   if (a.part)
-    for (int c = threadIdx.x; c < 2 * channels; c += kThreads)
+    for (int c = threadIdx.x; c < 2 * channels; c += kTileThreads)
       a.part[((long long)(c / channels) * parts + blockIdx.y) * a.n + c0 + c % channels] = total[c];
 }
 
@@ -864,7 +865,7 @@ struct Way {
   int pieces, per;   // two
 };
 
-int high_of(int channels, int V) { return kThreads / std::min(channels / V, kThreads); }
+int high_of(int channels, int V, int threads) { return threads / std::min(channels / V, threads); }
 
 Way choose(long long b, long long s, int n, int groups, int type, bool wide16, bool wide8, bool backward) {
   Way w = {};
@@ -895,7 +896,7 @@ Way choose(long long b, long long s, int n, int groups, int type, bool wide16, b
   auto vector = [&](int channels) { return (fits_row(channels, 16) ? 16 : fits_row(channels, 8) ? 8 : size) / size; };
   auto shared_of = [&](int gpc) {
     const long long channels = (long long)gpc * cg;
-    const int V = vector((int)channels), high = high_of((int)channels, V);
+    const int V = vector((int)channels), high = high_of((int)channels, V, kTileThreads);
     const long long tile = (s * channels * size + 15) / 16 * 16;
     return backward ? 2 * tile + (2LL * high * channels + 2 * channels + 4 * gpc) * 4 : tile + (high * channels + 2LL * gpc) * 4;
   };
@@ -910,18 +911,18 @@ Way choose(long long b, long long s, int n, int groups, int type, bool wide16, b
       w.way = Way::kTile, w.gpc = gpc, w.chunks = (groups + gpc - 1) / gpc;
       const int last = (groups - (w.chunks - 1) * gpc) * cg;
       w.V = std::min(vector(gpc * cg), vector(last));
-      const int high = std::max(high_of(gpc * cg, w.V), high_of(last, w.V));
+      const int high = std::max(high_of(gpc * cg, w.V, kTileThreads), high_of(last, w.V, kTileThreads));
       const long long channels = (long long)gpc * cg, tile = (s * channels * size + 15) / 16 * 16;
       w.shared = backward ? 2 * tile + (2LL * high * channels + 2 * channels + 4 * gpc) * 4 : tile + (high * channels + 2LL * gpc) * 4;
       if (w.shared <= (size_t)kSharedLimit) {
-        const long long resident = std::max(1LL, std::min(8LL, (long long)(220 * 1024) / (long long)(w.shared + 1024)));
+        const long long resident = std::max(1LL, std::min(2048LL / kTileThreads, (long long)(220 * 1024) / (long long)(w.shared + 1024)));
         w.parts = (int)std::max(1LL, std::min(b, (kSms * resident + w.chunks - 1) / w.chunks));
         return w;
       }
     }
   }
   w.way = Way::kTwo, w.V = vector(n);
-  const int high = high_of(n, w.V);
+  const int high = high_of(n, w.V, kThreads);
   w.shared = std::max(2LL * high * n, 2LL * groups) * 4;
   // as many blocks as the SMs hold at a time, so that all of them end together; rows enough in a piece that its sums are few beside it
   const long long wanted = std::max(1LL, kSms * (backward ? kPieceBlocksBack : kPieceBlocks) / b);
@@ -1022,10 +1023,10 @@ int launch_group_norm(const GroupNormCall& c, cudaStream_t stream) {
       if (w.way == Way::kTile) {
         if (!back) {
           if ((st = room(fn, tile_fwd_kernel<T, V>, w.shared)) != GELIB_OK) return st;
-          tile_fwd_kernel<T, V><<<(unsigned)samples, kThreads, w.shared, stream>>>(a, w.gpc, w.chunks);
+          tile_fwd_kernel<T, V><<<(unsigned)samples, kTileThreads, w.shared, stream>>>(a, w.gpc, w.chunks);
         } else {
           if ((st = room(fn, tile_bwd_kernel<T, V>, w.shared)) != GELIB_OK) return st;
-          tile_bwd_kernel<T, V><<<dim3(w.chunks, w.parts), kThreads, w.shared, stream>>>(a, w.gpc, w.parts);
+          tile_bwd_kernel<T, V><<<dim3(w.chunks, w.parts), kTileThreads, w.shared, stream>>>(a, w.gpc, w.parts);
         }
         return launched(fn);
       }
