@@ -13,8 +13,8 @@
 // are many small tensors, so their addresses travel in the launch's parameters, a tensor is cut into pieces of as many elements as a block takes, and
 // a block finds its piece by bisection.
 //
-// Measured on 46.7 million weights: 190 us in 32 bits (28 bytes an element, 6.8 TB/s: the copy rate); 8 bits and a bfloat16 head 141 us, where the bytes take 114:
-// 75 instructions an element, most of them the two roundings, half of them on the integer pipe.  Two dozen small tensors 11 us a call, half of it Python's.
+// Measured on 46.7 million weights: 190 us in 32 bits (28 bytes an element, 6.8 TB/s: the copy rate); 8 bits and a bfloat16 head 163 us, where the bytes take 114:
+// some 80 instructions an element, most of them the two roundings, half of them on the integer pipe.  Two dozen small tensors 11 us a call, half of it Python's.
 #include <cuda_fp8.h>
 
 #include <algorithm>
@@ -62,19 +62,42 @@ __device__ __forceinline__ unsigned random_bits(unsigned h) {
   return h ^ (h >> 15);
 }
 
-// Eight elements; r: the new root of v.  The approximate root and reciprocal are a unit or two in the last place off.
+// Eight elements.  The approximate root and reciprocal are a unit or two in the last place off, which the step may be too.
+//
+// kRoot: r becomes the new root of v, to be rounded to a code.  There a last place matters: where it moves a value over the point at which the
+// hash takes the other neighbour, the code is an eighth off.  So each product and sum is rounded by itself, in the formula's order (a packed product and
+// a packed sum were joined by the compiler: 8 codes of 2^24 differed), and one step of
+// Newton's method, r + (v - r^2) / 2r with the reciprocal at hand, rounds the root to nearest.
+template <bool kRoot>
 __device__ __forceinline__ void update(const Scalars& s, float (&g)[8], float (&p)[8], float (&m)[8], float (&v)[8], float (&r)[8]) {
   float t[8];
   mul_all(m, m, s.b1);
-  fma_all(m, g, s.one_b1, m);
-  mul_all(t, g, g);
   mul_all(v, v, s.b2);
-  fma_all(v, t, s.one_b2, v);
+  if constexpr (kRoot) {
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      m[k] = __fadd_rn(m[k], __fmul_rn(g[k], s.one_b1));
+      v[k] = __fadd_rn(v[k], __fmul_rn(__fmul_rn(g[k], s.one_b2), g[k]));
+    }
+  } else {
+    fma_all(m, g, s.one_b1, m);
+    mul_all(t, g, g);
+    fma_all(v, t, s.one_b2, v);
+  }
 #pragma unroll
   for (int k = 0; k < 8; k++) asm("sqrt.approx.f32 %0, %1;" : "=f"(r[k]) : "f"(v[k]));
   fma_all(t, r, s.root, s.eps);
 #pragma unroll
   for (int k = 0; k < 8; k++) asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t[k]) : "f"(t[k]));
+  if constexpr (kRoot) {
+    float h[8];
+    mul_all(h, r, -1.f);
+    fma_all(v, h, r, v);
+    mul_all(h, t, 0.5f * s.root);
+#pragma unroll
+    for (int k = 0; k < 8; k++) h[k] = fminf(h[k], 3.402823466e38f);   // v = 0 without an eps
+    fma_all(r, v, h, r);
+  }
   mul_all(t, t, m);
   mul_all(p, p, s.keep);
   fma_all(p, t, -s.step, p);
@@ -201,7 +224,7 @@ __device__ __forceinline__ void step_piece(const Entry& e, const Scalars& s, lon
   }
   if (s.grad_scale) mul_all(g, g, *s.grad_scale);
   float r[8];
-  update(s, g, p, m, v, r);
+  update<k8>(s, g, p, m, v, r);
   store_n<float, kWide>(master, i, n, p);
   if constexpr (sizeof(T) == 2) store_n<T, kWide>(static_cast<T*>(e.p), i, n, p);
   if constexpr (!k8) {
@@ -252,7 +275,7 @@ __device__ __forceinline__ void step_piece(const Entry& e, const Scalars& s, lon
   }
 }
 
-// Six blocks of an SM although a few registers spill: 8 bits 141 us, five 146, as many registers as it likes 166 to 222.
+// Six blocks of an SM although a few registers spill: 8 bits 141 us, five 146, as many registers as it likes 166 to 222 (before the root was rounded, which takes 22 more).
 template <int N, bool k8>
 __global__ void __launch_bounds__(kThreads, k8 ? 6 : 4) adamw_kernel(const __grid_constant__ Args<N> a) {
   const Entry& e = find(a, (int)blockIdx.x);

@@ -282,6 +282,38 @@ def test_lazily_conjugated_and_strided_gradients():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("eps", [1e-8, 0.0])
+def test_codes_are_those_of_moments_rounded_operation_by_operation(eps):
+    """A last place of a moment decides an eighth of its code once in 2^20 elements.  With each operation rounded to nearest by itself no code of 2^24
+    differs: the root's last step is off by 2^-43 of it at most, which would show once in 2^19 * 2^20 elements."""
+    import gelib_b200 as G
+    n, b1, b2, seed = 1 << 24, 0.9, 0.999, 29
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    size = torch.exp(torch.randn(n // 256, generator=gen, device="cuda")).repeat_interleave(256) * 1e-2
+    g = torch.randn(n, generator=gen, device="cuda") * size
+    old = [torch.randn(n, generator=gen, device="cuda") * size, (0.3 + torch.rand(n, generator=gen, device="cuda")) * size]
+    old[1][::1001] = 0
+    g[::1001] = 0
+    codes, scales = zip(*(_codes(x) for x in old))
+    m, r = (c.float() * k.repeat_interleave(256) for c, k in zip(codes, scales))
+    want = [m * b1 + g * (1 - b1), torch.sqrt(r * r * b2 + g * (1 - b2) * g)]
+    want[1][::1001] = 0
+    G.adamw_step([torch.zeros(n, device="cuda")], [g], [codes[0]], [codes[1]], step=1000, lr=1e-3, betas=(b1, b2), eps=eps, weight_decay=0.0,
+                 exp_avg_scale=[scales[0]], exp_avg_sq_scale=[scales[1]], seed=seed)
+    bits = _bits(seed, n).cuda()
+    for x, u, got, scale in ((want[0], bits & 0xffff, codes[0], scales[0]), (want[1], bits >> 16, codes[1], scales[1])):
+        b = x.view(-1, 256).double()
+        power = torch.exp2(torch.floor(torch.log2(b.abs().amax(1))) - 7)
+        assert torch.equal(power, scale.double())
+        y = (b / power[:, None]).abs().view(-1)
+        step = torch.exp2((torch.floor(torch.log2(y)) - 3).clamp(min=-9))
+        q = torch.floor(y / step + (u.double() * 16 + 8) / 2 ** 20) * step
+        if got is codes[1]:
+            q = torch.where((y > 0) & (q == 0), 2.0 ** -9, q)
+        assert torch.equal(got.double().abs(), q), (got.double().abs() != q).sum().item()
+
+
+@pytest.mark.gpu
 def test_saved_tensors_are_told_of_the_step():
     import gelib_b200 as G
     w = torch.nn.Parameter(torch.ones(4, 4, device="cuda"))
