@@ -13,7 +13,8 @@
 // are many small tensors, so their addresses travel in the launch's parameters, a tensor is cut into pieces of as many elements as a block takes, and
 // a block finds its piece by bisection.
 //
-// Measured on 46.7 million weights: 190 us in 32 bits (28 bytes an element, 6.8 TB/s: the copy rate); 8 bits and a bfloat16 head 163 us, where the bytes take 114:
+// Measured on 46.7 million weights: 190 us in 32 bits (28 bytes an element, 6.8 TB/s: the copy rate); 8 bits and a bfloat16 head 220 us with the values of both
+// moments written out (two launches of 27), where the step's bytes take 114:
 // some 80 instructions an element, most of them the two roundings, half of them on the integer pipe.  Two dozen small tensors 11 us a call, half of it Python's.
 #include <cuda_fp8.h>
 
@@ -74,10 +75,14 @@ __device__ __forceinline__ void update(const Scalars& s, float (&g)[8], float (&
   mul_all(m, m, s.b1);
   mul_all(v, v, s.b2);
   if constexpr (kRoot) {
+    float h[8];
+    mul_all(h, g, s.one_b1);
+    mul_all(t, g, s.one_b2);
+    mul_all(t, t, g);
 #pragma unroll
     for (int k = 0; k < 8; k++) {
-      m[k] = __fadd_rn(m[k], __fmul_rn(g[k], s.one_b1));
-      v[k] = __fadd_rn(v[k], __fmul_rn(__fmul_rn(g[k], s.one_b2), g[k]));
+      m[k] = __fadd_rn(m[k], h[k]);
+      v[k] = __fadd_rn(v[k], t[k]);
     }
   } else {
     fma_all(m, g, s.one_b1, m);
@@ -275,9 +280,9 @@ __device__ __forceinline__ void step_piece(const Entry& e, const Scalars& s, lon
   }
 }
 
-// Six blocks of an SM although a few registers spill: 8 bits 141 us, five 146, as many registers as it likes 166 to 222 (before the root was rounded, which takes 22 more).
+// Five blocks of an SM although registers spill: a pass over 46.7 million weights, with the values of both moments, 220 us in 8 bits; six 224.
 template <int N, bool k8>
-__global__ void __launch_bounds__(kThreads, k8 ? 6 : 4) adamw_kernel(const __grid_constant__ Args<N> a) {
+__global__ void __launch_bounds__(kThreads, k8 ? 5 : 4) adamw_kernel(const __grid_constant__ Args<N> a) {
   const Entry& e = find(a, (int)blockIdx.x);
   const long long i = (long long)((int)blockIdx.x - e.first) * kPiece + threadIdx.x * 8;
   static_assert(kPiece == kThreads * 8, "a lane takes eight elements");

@@ -3,6 +3,9 @@
 //   z = x w + bias,  y = act(z) + residual
 //   gz = gy act'(z),  gx = gz w^T,  gw = x^T gz,  gb = sum of gz's rows
 //
+// In 16 bits gz = gy act'(z) is rounded to the type it has as an operand of the matrix instructions, as the output is once more: a gradient is off by
+// the root of two times the output's own rounding (2.4e-3 of its norm against 1.7e-3 in bfloat16).
+//
 // Forward is one matrix product whose epilogue adds, activates and rounds once.  Backward is one pass over gy and z for gz and the
 // column sums, and two products.  Sums over rows are split over blocks when there are few tiles, as partial sums that are added
 // in a fixed order.
