@@ -282,19 +282,21 @@ __device__ __forceinline__ void activate_back(float (&g)[V], const float (&z)[V]
     logistics(q, q);
     fma_all(u, q, -1.f, 1.f);
     mul_all(u, u, z);
-  } else {                       // q + z q (1 - q) (k0 + 3 k1 z^2)
+    fma_all(q, q, u, q);
+  } else {                       // q + q (1 - q) z (k0 + 3 k1 z^2)
     float z2[V];
 #pragma unroll
-    for (int k = 0; k < V; k++) z2[k] = fminf(z[k] * z[k], 1e30f);   // finite: where q (1 - q) is 0 the product is
+    for (int k = 0; k < V; k++) z2[k] = fminf(z[k] * z[k], 1e30f);
     fma_all(q, z2, -kLog2e * kGelu1, -kLog2e * kGelu0);
     mul_all(q, q, z);
     logistics(q, q);
+    // q (1 - q) first: beyond |z| = 12 it is 0, and 0 times a finite z and the finite third factor stays 0; those two together may be an infinity
     fma_all(u, q, -1.f, 1.f);
+    mul_all(u, u, q);
     mul_all(u, u, z);
     fma_all(z2, z2, 3.f * kGelu1, kGelu0);
-    mul_all(u, u, z2);
+    fma_all(q, u, z2, q);
   }
-  fma_all(q, q, u, q);
   mul_all(g, g, q);
 }
 

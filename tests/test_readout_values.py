@@ -1,0 +1,58 @@
+"""Group norm and dense layers where values are extreme: arguments of activations far out, infinities, outliers, and gradients of few rows in 16 bits.
+
+Tolerances.  Where nothing is said, 64 * 2^-24 of the magnitudes that go into a result, as for the other tests of these operators, and half a unit in the last place
+of a 16-bit type.
+"""
+import math
+
+import pytest
+import torch
+
+EPS = 64 * 2.0 ** -24
+HALF = {torch.float32: 0.0, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+pytestmark = pytest.mark.gpu
+
+# the activations' derivatives are 0 below and 1 above, to the last bit of float32
+FAR = [-3e38, -1e37, -1e30, -1.9e28, -1e20, -1e18, -1e14, -2e13, -1e12, -1e9, -1e4, -200.0, 200.0, 1e4, 1e9, 1e12, 2e13, 1e14, 1e18, 1e20, 1e30, 1e37, 3e38]
+
+
+@pytest.mark.parametrize("act", ["relu", "silu", "gelu_tanh"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows", [1, 5, 23, 230])
+def test_layer_gradients_far_out(rows, dtype, act):
+    """x w = x for k = 1 and w = 1, in rows that hold every value in turn; eight columns, so gx = 8 act'."""
+    import gelib_b200 as G
+    for at in range(0, len(FAR), min(rows, len(FAR))):
+        values = [FAR[(at + i) % len(FAR)] for i in range(rows)]
+        x = torch.tensor(values, device="cuda").to(dtype).view(rows, 1).requires_grad_()
+        w = torch.ones(1, 8, dtype=dtype, device="cuda")
+        bias = torch.zeros(8, dtype=dtype, device="cuda", requires_grad=True)
+        y = G.linear(x, w, bias, activation=act)
+        gx, gb = torch.autograd.grad(y, (x, bias), torch.ones_like(y))
+        slope = (x.detach() > 0).double()
+        assert torch.equal(gx.double(), 8 * slope), gx[gx.double() != 8 * slope]
+        assert torch.equal(gb.double(), slope.sum().to(dtype).double().expand(8))
+
+
+@pytest.mark.parametrize("act", ["relu", "silu", "gelu_tanh"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("b,s", [(6, 1), (5, 4), (9, 37), (2, 3000)])
+def test_norm_gradients_far_out(b, s, dtype, act):
+    """The bias puts each channel far out, so the gradient is that of no activation for gy with the channels below zero left out."""
+    import gelib_b200 as G
+    n = 4 * len(FAR)
+    gen = torch.Generator(device="cuda").manual_seed(b + s)
+    x, gy = (torch.randn(b, s, n, generator=gen, device="cuda").to(dtype) for _ in range(2))
+    x.requires_grad_()
+    bias = torch.tensor(FAR * 4, device="cuda").to(dtype).requires_grad_()
+    gx, gb = torch.autograd.grad(G.group_norm(x, 4, None, bias, activation=act), (x, bias), gy)
+    none = torch.zeros(n, dtype=dtype, device="cuda", requires_grad=True)
+    masked = torch.where(bias.detach() > 0, gy, torch.zeros_like(gy))
+    want, wb = torch.autograd.grad(G.group_norm(x, 4, None, none), (x, none), masked)
+    half = HALF[dtype] or EPS
+    assert ((gx - want).double().abs() <= 2 * half * want.double().abs() + EPS * gy.double().abs().max() * 8).all()
+    assert torch.equal(gb, wb)
+
+
+def classes(t):
+    return torch.isnan(t), torch.isposinf(t), torch.isneginf(t)
