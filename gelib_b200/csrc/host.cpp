@@ -326,12 +326,17 @@ using torch::autograd::variable_list;
 void* ptr(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 at::Tensor or_none(const OptTensor& t) { return t ? *t : at::Tensor(); }
 
+// A forward-mode derivative, which these operators do not have: the Python code refuses it.  Asked of every operand, since a tensor with a
+// tangent need not ask for a gradient and would lose it here.
+bool has_tangent(const at::Tensor& t) { return t._fw_grad(/*level=*/0).defined(); }
+
 // Real, of x's type and device, of the given shape.
 bool goes_with(const at::Tensor& x, const OptTensor& t, at::IntArrayRef shape) {
-  return !t || (t->defined() && t->device() == x.device() && t->scalar_type() == x.scalar_type() && t->layout() == at::kStrided && t->sizes() == shape && !t->is_neg());
+  return !t || (t->defined() && t->device() == x.device() && t->scalar_type() == x.scalar_type() && t->layout() == at::kStrided && t->sizes() == shape && !t->is_neg() &&
+                !has_tangent(*t));
 }
 bool is_plain(const at::Tensor& x) {
-  return x.defined() && x.is_cuda() && x.layout() == at::kStrided && !x.is_neg() && !x.is_complex() && type_code(x.scalar_type()).has_value();
+  return x.defined() && x.is_cuda() && x.layout() == at::kStrided && !x.is_neg() && !x.is_complex() && type_code(x.scalar_type()).has_value() && !has_tangent(x);
 }
 
 at::Tensor workspace(int64_t bytes, const at::Tensor& like) {

@@ -2,7 +2,8 @@
 
 What the reference leaves to torch.nn (its Python layer ends with the products, python/src/gelib): the invariants of a network -- the l=0
 parts of its last product, (b, [grid...], channels) with the channels last as in every part -- are normalised and go through dense layers.
-Both operators compute on CUDA tensors in float32, bfloat16 or float16 with float32 sums, and have gradients; they can be differentiated once.  Calls whose operands need nothing special are made by the native host side.
+Both operators compute on CUDA tensors in float32, bfloat16 or float16 with float32 sums, and have gradients; they can be differentiated once, and
+not in forward mode, which is refused.  Calls whose operands need nothing special are made by the native host side.
 """
 import ctypes
 
