@@ -4,8 +4,8 @@
 //   xh = (x - mean) rstd,  z = xh w + bias,  y = act(z)
 //   gz = gy act'(z),  gw = sum gz xh,  gb = sum gz,  gx = rstd (gz w - mean(gz w) - xh mean(gz w xh))
 //
-// Statistics and sums are float32; the variance is a mean of squares of differences from the mean, not a difference of means, so a
-// large mean costs no digits.  Memory bounds it: a read and a write forward, two reads and a write backward, if the elements that
+// Statistics and sums are float32; the variance is a mean of squares of differences from the mean, not a difference of means, so neither a
+// large mean nor an outlier costs digits.  Memory bounds it: a read and a write forward, two reads and a write backward, if the elements that
 // share a statistic stay on the SM between its sum and its use.  Three ways of keeping them, by size:
 //
 //   row    small samples (s = 1 and a group of at most 1024 channels, 512 in float32; or as many numbers in a group, whose row is 1, 2, 4, .. 32
@@ -571,36 +571,53 @@ __global__ void __launch_bounds__(kThreads, kPieceBlocks) piece_stats_kernel(Nor
   const int tx = threadIdx.x % cl.wide, ty = threadIdx.x / cl.wide, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   if (ty < cl.high)
     for (int col = tx; col < cl.cols; col += cl.wide) {
-      // sums of differences from the thread's first row: what they lose to cancellation is of the size of the spread, not of the mean
-      float first[V], sum[V], sq[V];
+      // Each batch of rows has its mean first and its squared differences from that after, and joins those before by the difference of the means: no
+      // row is a point of reference for the others, so an outlier costs no digits wherever it lies.
+      float mean[V], sq[V];
 #pragma unroll
-      for (int j = 0; j < V; j++) first[j] = sum[j] = sq[j] = 0;
-      if (ty < rows) load_vec<T, V>(x + (long long)ty * a.n + col * V, first);
-      constexpr int U = 8;   // rows on their way together
-      for (int r = ty + cl.high; r < rows; r += U * cl.high) {
+      for (int j = 0; j < V; j++) mean[j] = sq[j] = 0;
+      const T* at = x + (long long)ty * a.n + col * V;
+      const long long step = (long long)cl.high * a.n;
+      float count = 0;
+      auto batch = [&](auto rows_of) {   // so many rows, on their way together
+        constexpr int U = decltype(rows_of)::value;
         Piece<T, V> p[U];
+        float m[V], q[V], v[V];
 #pragma unroll
-        for (int u = 0; u < U; u++)
-          if (r + u * cl.high < rows) p[u].load(x + (long long)(r + u * cl.high) * a.n + col * V);
+        for (int j = 0; j < V; j++) m[j] = q[j] = 0;
 #pragma unroll
-        for (int u = 0; u < U; u++)
-          if (r + u * cl.high < rows) {
-            float v[V];
-            p[u].get(v);
+        for (int u = 0; u < U; u++) p[u].load(at + u * step);
+        at += U * step;
 #pragma unroll
-            for (int j = 0; j < V; j++) {
-              const float d = v[j] - first[j];
-              sum[j] += d;
-              sq[j] += d * d;
-            }
-          }
-      }
-      const int mine = ty < rows ? (rows - ty + cl.high - 1) / cl.high : 0;
+        for (int u = 0; u < U; u++) {
+          p[u].get(v);
+          add_all(m, m, v);
+        }
+        mul_all(m, m, -1.f / U);   // less the mean
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+          p[u].get(v);
+          add_all(v, v, m);
+          fma_all(q, v, v, q);
+        }
+        const float share = __fdividef((float)U, count + U);
+        add_all(v, mean, m);                 // the means' difference
+        fma_all(mean, v, -share, mean);
+        mul_all(v, v, v);
+        add_all(sq, sq, q);
+        fma_all(sq, v, count * share, sq);
+        count += U;
+      };
+      int left = ty < rows ? (rows - ty + cl.high - 1) / cl.high : 0;
+      constexpr int kMost = V == 8 ? 4 : 8;   // eight times eight do not fit the registers of four blocks: 2 x 200000 x 512 bfloat16 241 us, 245 with spills
+      for (; left >= kMost; left -= kMost) batch(std::integral_constant<int, kMost>{});
+      if (left & 4) batch(std::integral_constant<int, 4>{});
+      if (left & 2) batch(std::integral_constant<int, 2>{});
+      if (left & 1) batch(std::integral_constant<int, 1>{});
 #pragma unroll
       for (int j = 0; j < V; j++) {
-        const float m = mine ? sum[j] / mine : 0;
-        chan[ty * a.n + col * V + j] = first[j] + m;                                   // mean of the thread's rows
-        chan[(cl.high + ty) * a.n + col * V + j] = mine ? fmaxf(sq[j] - sum[j] * m, 0.f) : 0;   // their squared differences
+        chan[ty * a.n + col * V + j] = mean[j];                // of the thread's rows
+        chan[(cl.high + ty) * a.n + col * V + j] = sq[j];      // their squared differences from it
       }
     }
   __syncthreads();

@@ -56,3 +56,21 @@ def test_norm_gradients_far_out(b, s, dtype, act):
 
 def classes(t):
     return torch.isnan(t), torch.isposinf(t), torch.isneginf(t)
+
+
+@pytest.mark.parametrize("outlier", [100.0, 1000.0, -30000.0])
+def test_an_outlier_in_the_first_row_costs_no_digits(outlier):
+    """A thread sums 4000 rows of one channel, which is a group of its own."""
+    import gelib_b200 as G
+    b, s, n = 300, 4000, 257
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    x = torch.randn(b, s, n, generator=gen, device="cuda")
+    x[:, 0] += outlier
+    y = G.group_norm(x, n)
+    for i in (0, b // 2, b - 1):
+        d = x[i].double()
+        mean, spread = d.mean(0), d.std(0, unbiased=False)
+        rstd = (spread ** 2 + 1e-5).rsqrt()
+        want, size = (d - mean) * rstd, (d.abs() + d.abs().mean(0)) * rstd
+        off = (y[i].double() - want).abs() / (EPS * (size + want.abs()))
+        assert (off <= 1).all(), off.max().item()
