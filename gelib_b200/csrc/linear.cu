@@ -237,11 +237,11 @@ __device__ __forceinline__ void copy_planes(const PlaneJobs& jobs, long long blo
       for (int j = 0; j < 8; j++) x[j] = j < live ? src[j] : from_float<T>(0.f);
     }
     if constexpr (sizeof(T) == 4) {
-      union { uint4 u; __nv_bfloat16 t[8]; } w[3];
+      union { uint4 u; uint32_t t[4]; } w[3];
 #pragma unroll
-      for (int j = 0; j < 8; j++) {
-        __nv_bfloat16 p[3];
-        split3(x[j], p);
+      for (int j = 0; j < 4; j++) {
+        uint32_t p[3];
+        split3(x[2 * j], x[2 * j + 1], p);
 #pragma unroll
         for (int i = 0; i < 3; i++) w[i].t[j] = p[i];
       }
@@ -295,12 +295,13 @@ __global__ void __launch_bounds__(kThreads) prepare_kernel(const __grid_constant
       }
       if (gz.base) {
         if (sizeof(T) == 4 && gz.planes == 3) {
-          union { __nv_bfloat16 t[V]; typename Raw<V * 2>::type raw; } w[3];
+          union { uint32_t t[(V + 1) / 2]; typename Raw<V * 2>::type raw; } w[3];
 #pragma unroll
-          for (int j = 0; j < V; j++) {
-            __nv_bfloat16 p[3];
-            split3(g[j], p);
-            w[0].t[j] = p[0], w[1].t[j] = p[1], w[2].t[j] = p[2];
+          for (int j = 0; j < V; j += 2) {
+            uint32_t p[3];
+            split3(g[j], j + 1 < V ? g[j + 1] : 0.f, p);
+#pragma unroll
+            for (int i = 0; i < 3; i++) w[i].t[j / 2] = p[i];
           }
 #pragma unroll
           for (int i = 0; i < 3; i++)

@@ -71,18 +71,29 @@ __device__ __forceinline__ T held(float z) {   // z as it is kept for the backwa
   return from_float<T>(z);
 }
 
-// x as the sum of three bfloat16 numbers, each the next eight bits, cut and not rounded: the sum is x to the last bit, and none of them is an infinity
-// that x is not.  An infinity or NaN is its first part, and the others are zero.
-__device__ __forceinline__ void split3(float x, __nv_bfloat16 (&p)[3]) {
-  float r = x;
-  const bool finite = fabsf(x) <= 3.402823466e38f;
+// Each of a pair of floats as the sum of three bfloat16 numbers (the first one's in the low halves), each the next eight bits, cut and not rounded: the sum is
+// x to the last bit, and none of them is an infinity that x is not.  NaN is its first part.  Where the second or third part would be zero it is the
+// smallest number of x's sign, 2^-133, unless the first is zero: so all products of an infinity with the parts of a number are infinities of one
+// sign, and with zero none is a number.
+__device__ __forceinline__ void split3(float x, float y, uint32_t (&p)[3]) {
+  float r[2] = {x, y};
+  const bool finite[2] = {fabsf(x) <= 3.402823466e38f, fabsf(y) <= 3.402823466e38f};
 #pragma unroll
   for (int i = 0; i < 3; i++) {
-    unsigned bits = __float_as_uint(r) & 0xffff0000u;
-    if (i == 0 && x != x) bits = 0x7fc00000u;
-    p[i] = __ushort_as_bfloat16((unsigned short)(bits >> 16));
-    r = finite ? r - __uint_as_float(bits) : 0.f;
+    uint32_t bits[2];
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+      bits[k] = __float_as_uint(r[k]) & 0xffff0000u;
+      if (i == 0 && r[k] != r[k]) bits[k] = 0x7fc00000u;
+      r[k] = finite[k] ? r[k] - __uint_as_float(bits[k]) : 0.f;
+    }
+    p[i] = __byte_perm(bits[0], bits[1], 0x7632);
   }
+  uint32_t least;   // of the two halves: 0 or 1, and the sign; a part has that sign or is zero, so the larger as a whole number is the part where there is one
+  asm("min.u16x2 %0, %1, %2;" : "=r"(least) : "r"(p[0] & 0x7fff7fffu), "r"(0x00010001u));
+  least |= p[0] & 0x80008000u;
+#pragma unroll
+  for (int i = 1; i < 3; i++) asm("max.u16x2 %0, %1, %2;" : "=r"(p[i]) : "r"(p[i]), "r"(least));
 }
 #endif
 

@@ -269,7 +269,7 @@ int gelib_group_norm_back(void* gx, void* gw, void* gb, const void* gy, const vo
  * Forward: y, and z where it is not NULL (a backward call with an activation needs it; in float16 it is held within that type's range).
  * Backward: of gy the gradients gx dense (m, k), gw dense and in w's own layout (k, n) or (n, k), gb (n); each may be NULL.
  * bias, residual may be NULL; m, k and n at most 2^30.  Sums are float; float operands are multiplied as three bfloat16 parts each, which keeps
- * float's precision for factors from 2^-109 on (an infinity among them gives infinity or NaN). */
+ * float's precision for factors from 2^-109 on, and an infinity times one of those an infinity. */
 typedef struct gelib_linear_args {
   const void *x, *w, *bias, *residual, *gy;
   void *y, *z, *gx, *gw, *gb;

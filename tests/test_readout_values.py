@@ -58,6 +58,40 @@ def classes(t):
     return torch.isnan(t), torch.isposinf(t), torch.isneginf(t)
 
 
+@pytest.mark.parametrize("m", [3, 40, 300])
+@pytest.mark.parametrize("wt", [False, True])
+def test_infinities_of_float32_layers(m, wt):
+    """An infinity times a number is an infinity of their signs, times 0 it is no number; what it does not meet stays."""
+    import gelib_b200 as G
+    inf, k, n = math.inf, 70, 48
+    gen = torch.Generator(device="cuda").manual_seed(m)
+    x, w, gy = (torch.randn(*shape, generator=gen, device="cuda") for shape in ((m, k), (k, n), (m, n)))
+    w[:, :8] = 1.0            # numbers of few bits
+    w[:, 8:12] = -0.375
+    w[5, 12] = 0.0
+    w[5, 13:16] = torch.tensor([1.5e-33, -1e-33, 2.0 ** -109], device="cuda")
+    w[5, 16:19] = torch.tensor([1e37, -1e37, 2.0 ** 120], device="cuda")
+    x[1, 5], x[2, 5], x[2, 6], x[0, 9] = inf, -inf, 2.0, 0.0
+    w[9, 20] = inf            # times x[0, 9] = 0
+    w[5, 21] = inf            # times both infinities
+    gy[0, 3] = -inf
+    # kept away from the infinities: rounding of huge sums
+    x[x[:, 5].isfinite(), 5] = 1e-3
+    w = (w.t().contiguous().t() if wt else w).requires_grad_()
+    x.requires_grad_()
+    y = G.linear(x, w)
+    want = x.detach().double() @ w.detach().double()
+    for got, ref in zip(classes(y), classes(want.float())):
+        assert torch.equal(got, ref), (got != ref).nonzero()[:8].tolist()
+    gx, gw = torch.autograd.grad(y, (x, w), gy)
+    for g, ref in ((gx, gy.double() @ w.detach().double().t()), (gw, x.detach().double().t() @ gy.double())):
+        for got, r in zip(classes(g), classes(ref.float())):
+            assert torch.equal(got, r), (got != r).nonzero()[:8].tolist()
+    fine = torch.isfinite(want.float())
+    size = x.detach().double().abs() @ w.detach().double().abs()
+    assert ((y.double() - want).abs()[fine] <= EPS * size[fine]).all()
+
+
 @pytest.mark.parametrize("outlier", [100.0, 1000.0, -30000.0])
 def test_an_outlier_in_the_first_row_costs_no_digits(outlier):
     """A thread sums 4000 rows of one channel, which is a group of its own."""
