@@ -38,7 +38,8 @@ class AdamwTensor(ctypes.Structure):
 class AdamwOptions(ctypes.Structure):
     """``gelib_adamw_options``"""
     _fields_ = [(name, ctypes.c_double) for name in ("lr", "beta1", "beta2", "eps", "weight_decay")]
-    _fields_ += [("step", ctypes.c_int64), ("seed", ctypes.c_uint64), ("grad_scale", ctypes.c_void_p), ("state_bits", ctypes.c_int)]
+    _fields_ += [("step", ctypes.c_int64), ("seed", ctypes.c_uint64), ("grad_scale", ctypes.c_void_p), ("state_bits", ctypes.c_int),
+                 ("refresh_master", ctypes.c_int)]
 
 
 class LinearArgs(ctypes.Structure):

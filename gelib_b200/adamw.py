@@ -36,7 +36,7 @@ def _dense(what, t, device, types, n):
 
 
 def adamw_step(params, grads, exp_avg, exp_avg_sq, *, step, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, exp_avg_scale=None,
-               exp_avg_sq_scale=None, master=None, seed=0, grad_scale=None):
+               exp_avg_sq_scale=None, master=None, seed=0, grad_scale=None, refresh_master=False):
     """One AdamW step, in place, on lists of tensors of one CUDA device:
 
         m = b1 m + (1 - b1) g,   v = b2 v + (1 - b2) g^2,   p = p (1 - lr weight_decay) - lr m / (1 - b1^step) / (sqrt(v / (1 - b2^step)) + eps)
@@ -46,8 +46,9 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, *, step, lr, betas=(0.9, 0.99
     exp_avg_sq_scale they are states in 8 bits: float8_e4m3fn codes, of which each 256 consecutive ones share a float32 scale; of v the
     root is held (:func:`block8_values` gives what they stand for).  They are rounded stochastically, by `seed` (another one each
     step) and an element's place in the lists, so the same call gives the same result.  master: float32 copies of the 16-bit parameters, which
-    take the step and of which these are the rounded values; None for the others.  grad_scale: a float32 tensor of one element on the device that
-    gradients are multiplied by (the inverse of a loss scale, the factor of a clipping).
+    take the step and of which these are the rounded values; None for the others.  refresh_master: a copy whose rounding is not its parameter
+    becomes the parameter before the step, element by element, so that what was written to parameters in between stays.  grad_scale: a float32
+    tensor of one element on the device that gradients are multiplied by (the inverse of a loss scale, the factor of a clipping).
 
     step, lr and the rest are numbers on the host: a captured graph would repeat them, so a stream that is being captured is refused.
     No two tensors of a call may overlap.
@@ -58,17 +59,17 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, *, step, lr, betas=(0.9, 0.99
     if len(params) == 0 and not (len(grads) or len(exp_avg) or len(exp_avg_sq)):
         return
     if native().adamw_step(params, grads, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, master, step, lr, beta1, beta2, eps, weight_decay,
-                           seed, grad_scale) is not None:
+                           seed, grad_scale, bool(refresh_master)) is not None:
         return
     with torch.no_grad(), plain():
         _adamw_step(list(params), list(grads), list(exp_avg), list(exp_avg_sq), exp_avg_scale, exp_avg_sq_scale, master, step, lr, beta1, beta2, eps,
-                    weight_decay, seed, grad_scale)
+                    weight_decay, seed, grad_scale, refresh_master)
         # what autograd has saved of these tensors is no longer what they hold
         for written in (params, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, master):
             torch.autograd.graph.increment_version([t for t in written or () if t is not None])
 
 
-def _adamw_step(params, grads, m, v, ms, vs, master, step, lr, beta1, beta2, eps, weight_decay, seed, grad_scale):
+def _adamw_step(params, grads, m, v, ms, vs, master, step, lr, beta1, beta2, eps, weight_decay, seed, grad_scale, refresh_master):
     k = len(params)
     if (ms is None) != (vs is None):
         raise RuntimeError("adamw_step: states in 8 bits need exp_avg_scale and exp_avg_sq_scale")
@@ -80,7 +81,7 @@ def _adamw_step(params, grads, m, v, ms, vs, master, step, lr, beta1, beta2, eps
         raise RuntimeError("gelib_b200 computes on CUDA tensors only (this build has no CPU path); got a %s tensor" % device.type)
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError("adamw_step: the step's number and its rate are host values, which a captured graph would repeat")
-    options = AdamwOptions(lr, beta1, beta2, eps, weight_decay, step, seed, None, 32 if ms is None else 8)
+    options = AdamwOptions(lr, beta1, beta2, eps, weight_decay, step, seed, None, 32 if ms is None else 8, bool(refresh_master))
     if grad_scale is not None:
         options.grad_scale = _dense("grad_scale", grad_scale, device, (torch.float32,), 1)
     real, codes = (torch.float32, torch.complex64), (torch.float8_e4m3fn,)
@@ -130,7 +131,8 @@ class AdamW(torch.optim.Optimizer):
     """torch.optim's AdamW on :func:`adamw_step`: one launch per param group and device.
 
     state_bits: 32, or 8 for moments of one byte an element (and 4 bytes per 256).  Parameters of 16 bits get float32 master
-    copies in the state.  seed: of the stochastic rounding of 8-bit states.
+    copies in the state; a step begins from the copies, and from the parameter where it was written since the last one.  seed: of the
+    stochastic rounding of 8-bit states.
     """
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, state_bits=32, seed=0):
@@ -173,7 +175,8 @@ class AdamW(torch.optim.Optimizer):
                 adamw_step([p for p, _ in members], [p.grad for p, _ in members], [s["exp_avg"] for s in states],
                            [s["exp_avg_sq"] for s in states], step=step + 1, lr=group["lr"], betas=group["betas"], eps=group["eps"],
                            weight_decay=group["weight_decay"], master=[s.get("master") for s in states],
-                           seed=group["seed"] + step + 1 + (number << 32), grad_scale=grad_scale, **scales)
+                           seed=group["seed"] + step + 1 + (number << 32), grad_scale=grad_scale, refresh_master=True,
+                           **scales)
                 for s in states:
                     s["step"] = step + 1
         return loss

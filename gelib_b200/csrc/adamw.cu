@@ -7,7 +7,8 @@
 // pairs of real ones.  The moments are held in 32 bits, or in 8: blocks of 256 elements share a power of two, codes are e4m3, and of v
 // the root is held, whose range is half of v's in powers of two.  A moment that changes by a thousandth of itself a step would never leave its
 // code if it were rounded to nearest, so rounding is stochastic, from a hash of the call's seed and the element's number; the root is
-// never rounded to zero while v is above it, which would divide by eps.
+// never rounded to zero while v is above it, which would divide by eps.  Where the caller asks for it a master copy whose rounding is not the parameter
+// becomes the parameter first, which is two bytes more to read.
 //
 // The step is bound by memory: 28 bytes an element in 32 bits (p, m, v read and written, g read), 16 in 8 bits.  A network's weights
 // are many small tensors, so their addresses travel in the launch's parameters, a tensor is cut into pieces of as many elements as a block takes, and
@@ -47,6 +48,7 @@ struct Scalars {
   float b1, one_b1, b2, one_b2, keep, step, root, eps;   // keep = 1 - lr wd, step = lr / (1 - b1^t), root = 1 / sqrt(1 - b2^t)
   const float* grad_scale;
   unsigned seed_mix;
+  int refresh;
 };
 
 template <int N>
@@ -208,6 +210,16 @@ __device__ __forceinline__ void step_piece(const Entry& e, const Scalars& s, lon
   float* master = sizeof(T) == 4 ? static_cast<float*>(e.p) : e.master;
   load_n<float, kWide>(master, i, n, p);
   load_n<T, kWide>(static_cast<const T*>(e.g), i, n, g);
+  if constexpr (sizeof(T) == 2) {
+    if (s.refresh) {   // what was written to a parameter since the last step is not its master copy's rounding
+      float q[8], held[8];
+      load_n<T, kWide>(static_cast<const T*>(e.p), i, n, q);
+      unpack<T, 8>(pack<T, 8>(p), held);
+#pragma unroll
+      for (int k = 0; k < 8; k++)
+        if (__float_as_uint(held[k]) != __float_as_uint(q[k])) p[k] = q[k];
+    }
+  }
   unsigned char *mc = static_cast<unsigned char*>(e.m), *vc = static_cast<unsigned char*>(e.v);
   const long long block = i / kBlock;
   if constexpr (k8) {
@@ -354,7 +366,7 @@ int launch_adamw(int count, const gelib_adamw_tensor* t, const gelib_adamw_optio
   const double c1 = 1 - std::pow(o.beta1, (double)o.step), c2 = 1 - std::pow(o.beta2, (double)o.step);
   s.b1 = (float)o.beta1, s.one_b1 = (float)(1 - o.beta1), s.b2 = (float)o.beta2, s.one_b2 = (float)(1 - o.beta2);
   s.keep = (float)(1 - o.lr * o.weight_decay), s.step = (float)(o.lr / c1), s.root = (float)(1 / std::sqrt(c2)), s.eps = (float)o.eps;
-  s.grad_scale = o.grad_scale;
+  s.grad_scale = o.grad_scale, s.refresh = o.refresh_master;
   s.seed_mix = (unsigned)o.seed * 0x6A09E667u + (unsigned)(o.seed >> 32) * 0x3C6EF373u;
   const bool k8 = o.state_bits == 8;
   std::vector<gelib_adamw_tensor> group;

@@ -251,12 +251,12 @@ int64_t reals(const at::Tensor& t) { return t.numel() * (t.is_complex() ? 2 : 1)
 // One step over lists of tensors; None when one of them is not plain, or does not go with the others.
 std::optional<bool> adamw_step(const Tensors& params, const Tensors& grads, const Tensors& m, const Tensors& v, const std::optional<Tensors>& ms,
                                const std::optional<Tensors>& vs, const std::optional<OptTensors>& master, int64_t step, double lr, double beta1, double beta2, double eps,
-                               double weight_decay, uint64_t seed, const std::optional<at::Tensor>& grad_scale) {
+                               double weight_decay, uint64_t seed, const std::optional<at::Tensor>& grad_scale, bool refresh_master) {
   const size_t k = params.size();
   if (k == 0 || grads.size() != k || m.size() != k || v.size() != k || ms.has_value() != vs.has_value()) return std::nullopt;
   if ((ms && (ms->size() != k || vs->size() != k)) || (master && master->size() != k) || !params[0].defined() || !params[0].is_cuda()) return std::nullopt;
   const auto device = params[0].device();
-  gelib_adamw_options o = {lr, beta1, beta2, eps, weight_decay, step, seed, nullptr, ms ? 8 : 32};
+  gelib_adamw_options o = {lr, beta1, beta2, eps, weight_decay, step, seed, nullptr, ms ? 8 : 32, refresh_master};
   if (grad_scale) {
     if (!plain_dense(*grad_scale, device) || grad_scale->scalar_type() != at::kFloat || grad_scale->numel() != 1) return std::nullopt;
     o.grad_scale = grad_scale->data_ptr<float>();

@@ -244,6 +244,7 @@ typedef struct gelib_adamw_options {
   uint64_t seed;           /* of the rounding to 8 bits: another one each step */
   const float* grad_scale; /* device memory, gradients are multiplied by it; NULL: 1 */
   int state_bits;          /* 32 or 8 */
+  int refresh_master;      /* nonzero: a master copy whose rounding is not the parameter becomes the parameter before the step */
 } gelib_adamw_options;
 
 /* m = b1 m + (1-b1) g, v = b2 v + (1-b2) g^2, p = p (1 - lr wd) - lr/(1-b1^t) m / (sqrt(v/(1-b2^t)) + eps) for every tensor, in one

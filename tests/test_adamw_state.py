@@ -1,0 +1,92 @@
+"""What AdamW keeps: master copies beside parameters that others write to."""
+import pytest
+import torch
+
+
+def _trained(dtype, bits, steps=3, lr=1e-2):
+    import gelib_b200 as G
+    gen = torch.Generator().manual_seed(5)
+    p = torch.nn.Parameter(torch.randn(700, generator=gen).to(dtype).cuda())
+    grads = [torch.randn(700, generator=gen).to(dtype).cuda() for _ in range(8)]
+    opt = G.AdamW([p], lr=lr, weight_decay=0.0, state_bits=bits)
+    for g in grads[:steps]:
+        p.grad = g
+        opt.step()
+    return p, opt, grads[steps:]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("how", ["data", "no_grad", "load_state_dict", "some"])
+def test_what_is_written_to_a_parameter_stays(how, dtype, bits, native, monkeypatch):
+    """A parameter that was written between two steps takes the next one from what it holds; a rate of zero leaves that as it is."""
+    import gelib_b200 as G
+    if not native:
+        monkeypatch.setattr(G._lib, "_native", G._lib._Declines())
+    p, opt, grads = _trained(dtype, bits)
+    old = p.detach().clone()
+    want = torch.linspace(-2, 2, 700, device="cuda").to(dtype)
+    if how == "data":
+        p.data.copy_(want)
+    elif how == "no_grad":
+        with torch.no_grad():
+            p.copy_(want)
+    elif how == "load_state_dict":
+        holder = torch.nn.Module()
+        holder.w = p
+        holder.load_state_dict({"w": want})
+    else:   # a clamp writes some elements only
+        p.data.clamp_(-0.5, 0.5)
+        want = old.clamp(-0.5, 0.5)
+        assert 0 < int((want != old).sum()) < 700
+    kept = opt.state[p].get("master", p.detach()).clone()
+    opt.param_groups[0]["lr"] = 0.0
+    p.grad = grads[0]
+    opt.step()
+    assert torch.equal(p.detach(), want)
+    if "master" in opt.state[p]:   # an element that was not written keeps its copy's further digits
+        same = want == old
+        master = opt.state[p]["master"]
+        assert torch.equal(master[same], kept[same]) and torch.equal(master[~same], want[~same].float())
+    opt.param_groups[0]["lr"] = 1e-1
+    p.grad = grads[1]
+    opt.step()
+    assert ((p.detach() - want).abs().float() < 0.5).all() and not torch.equal(p.detach(), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_steps_below_a_parameters_last_place_add_up(dtype):
+    p, opt, _ = _trained(dtype, 32, steps=0, lr=1e-6)
+    first = p.detach().float()
+    for _ in range(200):
+        p.grad = torch.ones_like(p)
+        opt.step()
+    moved = first - opt.state[p]["master"]
+    assert ((moved - 200e-6).abs() <= 200 * 16 * 2.0 ** -24 * (first.abs() + 1e-6)).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("offset", [0, 1])
+def test_refreshing_master_copies(offset, native, monkeypatch):
+    """adamw_step takes the step from the master copies; where it is told to, first from what the parameters hold where that is not their rounding."""
+    import gelib_b200 as G
+    if not native:
+        monkeypatch.setattr(G._lib, "_native", G._lib._Declines())
+    gen = torch.Generator().manual_seed(2)
+    for dtype in (torch.bfloat16, torch.float16):
+        copy = torch.randn(999 + offset, generator=gen).cuda()[offset:]
+        p = copy.to(dtype) if not offset else torch.cat([copy[:1], copy]).to(dtype)[1:]
+        p[::7] = 3.0
+        p[5], p[6] = float("nan"), -0.0
+        copy[6] = 0.0
+        for refresh in (False, True):
+            q, master = torch.cat([p[:offset], p])[offset:], torch.cat([copy[:offset], copy])[offset:]
+            m, v = (torch.zeros(999, device="cuda") for _ in range(2))
+            G.adamw_step([q], [torch.zeros_like(q)], [m], [v], step=1, lr=0.0, master=[master], refresh_master=refresh)
+            want = torch.where(p.view(torch.int16) == copy.to(dtype).view(torch.int16), copy, p.float()) if refresh else copy
+            assert torch.equal(master.view(torch.int32)[torch.arange(999) != 5], want.view(torch.int32)[torch.arange(999) != 5])
+            assert bool(master[5].isnan()) == refresh and torch.equal(q[7:], want[7:].to(dtype))
