@@ -4,7 +4,8 @@
 //   gz = gy act'(z),  gx = gz w^T,  gw = x^T gz,  gb = sum of gz's rows
 //
 // In 16 bits gz = gy act'(z) is rounded to the type it has as an operand of the matrix instructions, as the output is once more: a gradient is off by
-// the root of two times the output's own rounding (2.4e-3 of its norm against 1.7e-3 in bfloat16).
+// the root of two times the output's own rounding (2.4e-3 of its norm against 1.7e-3 in bfloat16).  Eight rows and fewer take no matrix
+// instructions, and gz stays in float.
 //
 // Forward is one matrix product whose epilogue adds, activates and rounds once.  Backward is one pass over gy and z for gz and the
 // column sums, and two products.  Sums over rows are split over blocks when there are few tiles, as partial sums that are added
@@ -49,15 +50,16 @@ __device__ __forceinline__ void finish(const Epilogue& e, long long at, int col,
   static_cast<T*>(e.y)[at] = from_float<T>(z[0]);
 }
 
-// Block (x, y): tile, columns fastest, and part y of the sum.  part: partial sums (parts, M, N), or null.
-template <class T>
+// Block (x, y): tile, columns fastest, and part y of the sum.  part: partial sums (parts, M, N), or null.  TA, TB: the operands' types, T or float.
+template <class T, class TA, class TB>
 __global__ void __launch_bounds__(kThreads) simple_gemm_kernel(Strided a, Strided b, Gemm g, float* part, long long depth) {
   __shared__ float sa[kDepth][kTile + 4], sb[kDepth][kTile + 4];
   const long long across = (g.N + kTile - 1) / kTile, m0 = blockIdx.x / across * kTile, n0 = blockIdx.x % across * kTile;
   const long long k0 = (long long)blockIdx.y * depth, k1 = min(g.K, k0 + depth);
   const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
   float d[4][4] = {};
-  const T *A = static_cast<const T*>(a.base), *B = static_cast<const T*>(b.base);
+  const TA* A = static_cast<const TA*>(a.base);
+  const TB* B = static_cast<const TB*>(b.base);
   for (long long k = k0; k < k1; k += kDepth) {
     for (int e = threadIdx.x; e < kTile * kDepth; e += kThreads) {
       // the index that is dense in memory runs fastest over the threads
@@ -191,9 +193,16 @@ int launch_simple(const Gemm& g, void* workspace, Joins* joins, cudaStream_t str
   if (tiles > 0x7fffffffLL) return fail(GELIB_INVALID, "linear", "too many elements");
   const dim3 grid((unsigned)tiles, s.parts);
   const Strided a = strided(g.a), b = strided(g.b);
-  if (g.type == GELIB_F32) simple_gemm_kernel<float><<<grid, kThreads, 0, stream>>>(a, b, g, part, s.depth);
-  else if (g.type == GELIB_BF16) simple_gemm_kernel<__nv_bfloat16><<<grid, kThreads, 0, stream>>>(a, b, g, part, s.depth);
-  else simple_gemm_kernel<__half><<<grid, kThreads, 0, stream>>>(a, b, g, part, s.depth);
+  const auto run = [&](auto kernel) { kernel<<<grid, kThreads, 0, stream>>>(a, b, g, part, s.depth); };
+  const auto run_type = [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    if (g.a.s.in_float) run(simple_gemm_kernel<T, float, T>);
+    else if (g.b.s.in_float) run(simple_gemm_kernel<T, T, float>);
+    else run(simple_gemm_kernel<T, T, T>);
+  };
+  if (g.type == GELIB_F32) run(simple_gemm_kernel<float, float, float>);
+  else if (g.type == GELIB_BF16) run_type((__nv_bfloat16*)nullptr);
+  else run_type((__half*)nullptr);
   return launched("linear");
 }
 
@@ -306,6 +315,14 @@ __global__ void __launch_bounds__(kThreads) prepare_kernel(const __grid_constant
 #pragma unroll
           for (int i = 0; i < 3; i++)
             *reinterpret_cast<typename Raw<V * 2>::type*>((__nv_bfloat16*)gz.base + i * gz.plane + r * gz.ld + c) = w[i].raw;
+        } else if (sizeof(T) == 2 && gz.in_float) {
+          float* to = (float*)gz.base + r * gz.ld + c;
+          if constexpr (V % 4 == 0)
+#pragma unroll
+            for (int j = 0; j < V; j += 4) *reinterpret_cast<float4*>(to + j) = make_float4(g[j], g[j + 1], g[j + 2], g[j + 3]);
+          else
+#pragma unroll
+            for (int j = 0; j < V; j++) to[j] = g[j];
         } else {
           store_vec<T, V>((T*)gz.base + r * gz.ld + c, g);
         }
@@ -390,6 +407,9 @@ void copy_if_needed(Stored* s, int type, char*& at, PlaneJobs* jobs) {
   jobs->add(*s, to, type);
   *s = to;
 }
+
+// gz = gy act'(z): in the type that the tensor cores take, in float for the other products.
+long long gz_bytes(const gelib_linear_args& p, bool tc) { return tc ? planes_bytes(p.m, p.n, p.type) : up(4LL * p.m * p.n); }
 
 long long sums_bytes(const gelib_linear_args& p) {
   return up(4LL * p.n * std::max(pieces_of(p.m, p.n, p.type, false).parts, pieces_of(p.m, p.n, p.type, true).parts));
@@ -477,7 +497,7 @@ long long linear_workspace(const gelib_linear_args& p, bool backward) {
   }
   Gemm g[2];
   const int count = backward_of(p, x, w, gz, g);
-  return planes_bytes(p.m, p.n, p.type) + copies + sums_bytes(p) + products_workspace(g, count, tc);
+  return gz_bytes(p, tc) + copies + sums_bytes(p) + products_workspace(g, count, tc);
 }
 
 int launch_linear(const gelib_linear_args& p, void* workspace, cudaStream_t stream) {
@@ -523,7 +543,8 @@ int launch_linear_back(const gelib_linear_args& p, void* workspace, cudaStream_t
     if (tc) gz = planes_at(gz, p.type, at);
     else {
       gz.base = at;
-      at += planes_bytes(p.m, p.n, p.type);
+      gz.in_float = true;
+      at += gz_bytes(p, tc);
     }
     back.gz = gz;
   }

@@ -13,11 +13,13 @@ struct Epilogue {
 };
 
 // A matrix as it lies in memory: rows of dense columns, `ld` elements apart.  planes 3: a float matrix as the sum of three bfloat16
-// ones, `plane` elements apart (each holds the next eight bits of the significand).
+// ones, `plane` elements apart (each holds the next eight bits of the significand).  in_float: it is float although the call's type is another, which
+// only the products without tensor cores take.
 struct Stored {
   const void* base;
   long long rows, cols, ld, plane;
   int planes;
+  bool in_float = false;
 };
 
 // One operand of D = A B, M x K or K x N: its rows are the sum's index, or (by_sum false) M's or N's.

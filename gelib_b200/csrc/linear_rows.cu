@@ -64,15 +64,16 @@ __device__ __forceinline__ void join_and_store(const RowsArgs& a, const float* s
   if (ranks > 1) cluster_sync();   // nobody leaves while its sums are read
 }
 
-// Rows of w are k's.  A warp has eight lanes side by side and four k's.
-template <class T, int V, int M>
+// Rows of w are k's.  A warp has eight lanes side by side and four k's.  X: x's type, T or float.
+template <class T, class X, int V, int M>
 __global__ void __launch_bounds__(kThreads) rows_by_sum_kernel(RowsArgs a) {
   constexpr int kWidth = 8 * V;
   __shared__ __align__(16) float xs[kKept * M];             // [k][m]
   __shared__ float sums[kWarps * M * kWidth];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, n0 = blockIdx.x * kWidth, n = n0 + lane % 8 * V, mine = warp * 4 + lane / 8;
   const int k0 = blockIdx.y * a.per, k1 = min(a.K, k0 + a.per);
-  const T *x = static_cast<const T*>(a.x), *w = static_cast<const T*>(a.w);
+  const X* x = static_cast<const X*>(a.x);
+  const T* w = static_cast<const T*>(a.w);
   float s[M][V];
 #pragma unroll
   for (int m = 0; m < M; m++)
@@ -129,14 +130,15 @@ __global__ void __launch_bounds__(kThreads) rows_by_sum_kernel(RowsArgs a) {
 }
 
 // Rows of w are n's.  A warp has C of them; its lanes take V neighbouring k's each.
-template <class T, int V, int M, int C>
+template <class T, class X, int V, int M, int C>
 __global__ void __launch_bounds__(kThreads) rows_across_kernel(RowsArgs a) {
   constexpr int kWidth = kWarps * C;
-  __shared__ __align__(16) T xs[M * kKept];                 // [m][k]
+  __shared__ __align__(16) X xs[M * kKept];                 // [m][k]
   __shared__ float sums[M * kWidth];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, n0 = blockIdx.x * kWidth, n = n0 + warp * C;
   const int k0 = blockIdx.y * a.per, k1 = min(a.K, k0 + a.per);
-  const T *x = static_cast<const T*>(a.x), *w = static_cast<const T*>(a.w);
+  const X* x = static_cast<const X*>(a.x);
+  const T* w = static_cast<const T*>(a.w);
   float s[C][M];
 #pragma unroll
   for (int c = 0; c < C; c++)
@@ -147,7 +149,7 @@ __global__ void __launch_bounds__(kThreads) rows_across_kernel(RowsArgs a) {
     __syncthreads();
     for (int e = threadIdx.x; e < kept * M; e += kThreads) {
       const int q = e % kept, m = e / kept;
-      xs[m * kKept + q] = m < a.M ? x[m * a.ldx + k + q] : from_float<T>(0.f);
+      xs[m * kKept + q] = m < a.M ? x[m * a.ldx + k + q] : from_float<X>(0.f);
     }
     __syncthreads();
     if (n < a.N)
@@ -164,7 +166,9 @@ __global__ void __launch_bounds__(kThreads) rows_across_kernel(RowsArgs a) {
 #pragma unroll
         for (int m = 0; m < M; m++) {
           float f[V];
-          load_vec<T, V>(xs + m * kKept + q, f);
+          constexpr int kOne = V * sizeof(X) > 16 ? 16 / sizeof(X) : V;   // of an access
+#pragma unroll
+          for (int j = 0; j < V; j += kOne) load_vec<X, kOne>(xs + m * kKept + q + j, reinterpret_cast<float(&)[kOne]>(f[j]));
 #pragma unroll
           for (int c = 0; c < C; c++)
 #pragma unroll
@@ -204,25 +208,25 @@ int launch_rows_as(K kernel, RowsArgs a, int width, int step, cudaStream_t strea
   return launched(fn);
 }
 
-template <class T, int V, int M>
+template <class T, class X, int V, int M>
 int launch_rows_of(const RowsArgs& a, bool by_sum, cudaStream_t stream) {
   constexpr int C = M >= 4 ? 4 : 1;
-  if (by_sum) return launch_rows_as(rows_by_sum_kernel<T, V, M>, a, 8 * V, 32, stream);
-  return launch_rows_as(rows_across_kernel<T, V, M, C>, a, kWarps * C, 32 * V, stream);
+  if (by_sum) return launch_rows_as(rows_by_sum_kernel<T, X, V, M>, a, 8 * V, 32, stream);
+  return launch_rows_as(rows_across_kernel<T, X, V, M, C>, a, kWarps * C, 32 * V, stream);
 }
 
-template <class T, int V>
+template <class T, class X, int V>
 int launch_rows_wide(const RowsArgs& a, bool by_sum, cudaStream_t stream) {
-  if (a.M == 1) return launch_rows_of<T, V, 1>(a, by_sum, stream);
-  if (a.M <= 4) return launch_rows_of<T, V, 4>(a, by_sum, stream);
-  return launch_rows_of<T, V, 8>(a, by_sum, stream);
+  if (a.M == 1) return launch_rows_of<T, X, V, 1>(a, by_sum, stream);
+  if (a.M <= 4) return launch_rows_of<T, X, V, 4>(a, by_sum, stream);
+  return launch_rows_of<T, X, V, 8>(a, by_sum, stream);
 }
 
-template <class T>
+template <class T, class X>
 int launch_rows_type(const RowsArgs& a, const Operand& w, cudaStream_t stream) {
   constexpr int V = 16 / sizeof(T);
   const bool wide = is_aligned(a.w, 16) && a.ldw % V == 0 && (w.by_sum ? a.N : a.K) % V == 0;
-  return wide ? launch_rows_wide<T, V>(a, w.by_sum, stream) : launch_rows_wide<T, 1>(a, w.by_sum, stream);
+  return wide ? launch_rows_wide<T, X, V>(a, w.by_sum, stream) : launch_rows_wide<T, X, 1>(a, w.by_sum, stream);
 }
 
 }  // namespace
@@ -231,8 +235,10 @@ bool takes_rows(const Gemm& g) { return g.M <= 8 && !g.a.by_sum && g.K > 0 && g.
 
 int launch_rows(const Gemm& g, cudaStream_t stream) {
   const RowsArgs a = {g.e, g.a.s.base, g.b.s.base, g.a.s.ld, g.b.s.ld, (int)g.M, (int)g.N, (int)g.K, 0};
-  return g.type == GELIB_F32 ? launch_rows_type<float>(a, g.b, stream)
-         : g.type == GELIB_BF16 ? launch_rows_type<__nv_bfloat16>(a, g.b, stream) : launch_rows_type<__half>(a, g.b, stream);
+  if (g.type == GELIB_F32) return launch_rows_type<float, float>(a, g.b, stream);
+  if (g.type == GELIB_BF16)
+    return g.a.s.in_float ? launch_rows_type<__nv_bfloat16, float>(a, g.b, stream) : launch_rows_type<__nv_bfloat16, __nv_bfloat16>(a, g.b, stream);
+  return g.a.s.in_float ? launch_rows_type<__half, float>(a, g.b, stream) : launch_rows_type<__half, __half>(a, g.b, stream);
 }
 
 }  // namespace gelib_b200

@@ -108,3 +108,28 @@ def test_an_outlier_in_the_first_row_costs_no_digits(outlier):
         want, size = (d - mean) * rstd, (d.abs() + d.abs().mean(0)) * rstd
         off = (y[i].double() - want).abs() / (EPS * (size + want.abs()))
         assert (off <= 1).all(), off.max().item()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("wt", [False, True])
+@pytest.mark.parametrize("act", ["relu", "silu", "gelu_tanh"])
+@pytest.mark.parametrize("m,k,n", [(1, 40, 24), (2, 33, 65), (5, 256, 520), (8, 70, 1030)])
+def test_gradients_of_few_rows_are_rounded_once(m, k, n, act, wt, dtype):
+    """At most eight rows are multiplied in float32: gx and gw are off by their own rounding alone, given x w + bias as it is kept."""
+    import gelib_b200 as G
+    gen = torch.Generator(device="cuda").manual_seed(m + k + n)
+    x, gy = (torch.randn(m, q, generator=gen, device="cuda").to(dtype) for q in (k, n))
+    w = (torch.randn(k, n, generator=gen, device="cuda") * k ** -0.5).to(dtype)
+    w = w.t().contiguous().t() if wt else w
+    kept = G.linear(x, w)     # x w, rounded as it is for the backward call
+    x.requires_grad_(), w.requires_grad_()
+    gx, gw = torch.autograd.grad(G.linear(x, w, activation=act), (x, w), gy)
+    z = kept.double().requires_grad_()
+    f = {"relu": torch.relu, "silu": torch.nn.functional.silu, "gelu_tanh": lambda t: torch.nn.functional.gelu(t, approximate="tanh")}[act](z)
+    gz, = torch.autograd.grad(f, z, gy.double())
+    slope = gy.double().abs() * 1.2 * (1 + z.detach().abs())   # what an error of a few units in float32 of the derivative's terms does
+    x64, w64 = x.detach().double(), w.detach().double()
+    tiny = 2.0 ** -24 if dtype == torch.float16 else 1e-37
+    for got, want, size in ((gx, gz @ w64.t(), slope @ w64.abs().t()), (gw, x64.t() @ gz, x64.abs().t() @ slope)):
+        off, allowed = (got.double() - want).abs(), EPS * size + HALF[dtype] * (want.abs() + EPS * size) + tiny
+        assert (off <= allowed).all(), (off / allowed).max().item()
