@@ -65,12 +65,11 @@ __device__ __forceinline__ unsigned random_bits(unsigned h) {
   return h ^ (h >> 15);
 }
 
-// Eight elements.  The approximate root and reciprocal are a unit or two in the last place off, which the step may be too.
+// Eight elements.  The approximate reciprocal, and the approximate root where it is not kept, are a unit or two in the last place off, which the step may be too.
 //
 // kRoot: r becomes the new root of v, to be rounded to a code.  There a last place matters: where it moves a value over the point at which the
 // hash takes the other neighbour, the code is an eighth off.  So each product and sum is rounded by itself, in the formula's order (a packed product and
-// a packed sum were joined by the compiler: 8 codes of 2^24 differed), and one step of
-// Newton's method, r + (v - r^2) / 2r with the reciprocal at hand, rounds the root to nearest.
+// a packed sum were joined by the compiler: 8 codes of 2^24 differed), and the root is the one rounded to nearest.
 template <bool kRoot>
 __device__ __forceinline__ void update(const Scalars& s, float (&g)[8], float (&p)[8], float (&m)[8], float (&v)[8], float (&r)[8]) {
   float t[8];
@@ -92,19 +91,13 @@ __device__ __forceinline__ void update(const Scalars& s, float (&g)[8], float (&
     fma_all(v, t, s.one_b2, v);
   }
 #pragma unroll
-  for (int k = 0; k < 8; k++) asm("sqrt.approx.f32 %0, %1;" : "=f"(r[k]) : "f"(v[k]));
+  for (int k = 0; k < 8; k++) {
+    if constexpr (kRoot) r[k] = __fsqrt_rn(v[k]);
+    else asm("sqrt.approx.f32 %0, %1;" : "=f"(r[k]) : "f"(v[k]));
+  }
   fma_all(t, r, s.root, s.eps);
 #pragma unroll
   for (int k = 0; k < 8; k++) asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t[k]) : "f"(t[k]));
-  if constexpr (kRoot) {
-    float h[8];
-    mul_all(h, r, -1.f);
-    fma_all(v, h, r, v);
-    mul_all(h, t, 0.5f * s.root);
-#pragma unroll
-    for (int k = 0; k < 8; k++) h[k] = fminf(h[k], 3.402823466e38f);   // v = 0 without an eps
-    fma_all(r, v, h, r);
-  }
   mul_all(t, t, m);
   mul_all(p, p, s.keep);
   fma_all(p, t, -s.step, p);

@@ -1,6 +1,8 @@
-"""What AdamW keeps: master copies beside parameters that others write to."""
+"""What AdamW keeps: master copies beside parameters that others write to, and roots of the second moment for any eps."""
 import pytest
 import torch
+
+from test_adamw import _bits, _codes
 
 
 def _trained(dtype, bits, steps=3, lr=1e-2):
@@ -90,3 +92,28 @@ def test_refreshing_master_copies(offset, native, monkeypatch):
             want = torch.where(p.view(torch.int16) == copy.to(dtype).view(torch.int16), copy, p.float()) if refresh else copy
             assert torch.equal(master.view(torch.int32)[torch.arange(999) != 5], want.view(torch.int32)[torch.arange(999) != 5])
             assert bool(master[5].isnan()) == refresh and torch.equal(q[7:], want[7:].to(dtype))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size,eps", [(1e-2, 1e-2), (1e-2, 1e2), (1e-9, 1e-8), (1e-13, 1e-8), (1e-13, 0.0), (1e12, 1e-8)])
+def test_codes_of_the_root_whatever_eps_is(size, eps):
+    """The root that is held does not depend on eps.  Rounded to nearest it has the codes of torch's root, all of 2^24 elements."""
+    import gelib_b200 as G
+    n, b1, b2, seed = 1 << 24, 0.9, 0.999, 31
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    sizes = torch.exp(torch.randn(n // 256, generator=gen, device="cuda")).repeat_interleave(256) * size
+    g = torch.randn(n, generator=gen, device="cuda") * sizes
+    code, scale = _codes((0.3 + torch.rand(n, generator=gen, device="cuda")) * sizes)
+    r = code.float() * scale.repeat_interleave(256)
+    root = torch.sqrt(r * r * b2 + g * (1 - b2) * g)
+    m, ms = torch.zeros(n, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn), torch.ones(n // 256, device="cuda")
+    G.adamw_step([torch.zeros(n, device="cuda")], [g], [m], [code], step=1000, lr=1e-3, betas=(b1, b2), eps=eps, weight_decay=0.0,
+                 exp_avg_scale=[ms], exp_avg_sq_scale=[scale], seed=seed)
+    b = root.view(-1, 256).double()
+    power = torch.exp2((torch.floor(torch.log2(b.amax(1))) - 7).clamp(min=-100))
+    assert torch.equal(power, scale.double())
+    y = (b / power[:, None]).view(-1)
+    step = torch.exp2((torch.floor(torch.log2(y)) - 3).clamp(min=-9))
+    q = torch.floor(y / step + ((_bits(seed, n).cuda() >> 16).double() * 16 + 8) / 2 ** 20) * step
+    q = torch.where((y > 0) & (q == 0), 2.0 ** -9, q)
+    assert torch.equal(code.double(), q), (code.double() != q).sum().item()
