@@ -20,6 +20,7 @@
 // numbers halved them; 4 x 65536 x 112 float32, in two passes, 70 / 113 (36 / 54 and half as much again for the second reading), memory at 0.75 of its
 // rate; 3000 x 19 x 204 bfloat16, in shared memory, 29 / 56 (7 / 11), the latency of a block's phases.
 #include <algorithm>
+#include <atomic>
 
 #include "readout.h"
 #include "norm.h"
@@ -974,9 +975,18 @@ int with_type(int type, F f) {
   return f((__half*)nullptr);
 }
 
-template <class K>
-int room(const char* fn, K kernel, size_t bytes) {
-  if (bytes > 48 * 1024) GELIB_CUDA_TRY(fn, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+// More shared memory than a block has by itself.  The limit belongs to the kernel, in every thread of the process: it is set once on a device, to the most
+// that any call takes, and never lowered under another thread's launch.
+template <auto kernel>
+int room(const char* fn, size_t bytes) {
+  if (bytes <= 48 * 1024) return GELIB_OK;
+  static std::atomic<uint64_t> allowed{0};   // devices on which it is set
+  int device = 0;
+  GELIB_CUDA_TRY(fn, cudaGetDevice(&device));
+  const uint64_t bit = device < 64 ? 1ull << device : 0;
+  if (allowed.load(std::memory_order_relaxed) & bit) return GELIB_OK;
+  GELIB_CUDA_TRY(fn, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedLimit));
+  allowed.fetch_or(bit, std::memory_order_relaxed);
   return GELIB_OK;
 }
 
@@ -1039,29 +1049,29 @@ int launch_group_norm(const GroupNormCall& c, cudaStream_t stream) {
       }
       if (w.way == Way::kTile) {
         if (!back) {
-          if ((st = room(fn, tile_fwd_kernel<T, V>, w.shared)) != GELIB_OK) return st;
+          if ((st = room<tile_fwd_kernel<T, V>>(fn, w.shared)) != GELIB_OK) return st;
           tile_fwd_kernel<T, V><<<(unsigned)samples, kTileThreads, w.shared, stream>>>(a, w.gpc, w.chunks);
         } else {
-          if ((st = room(fn, tile_bwd_kernel<T, V>, w.shared)) != GELIB_OK) return st;
+          if ((st = room<tile_bwd_kernel<T, V>>(fn, w.shared)) != GELIB_OK) return st;
           tile_bwd_kernel<T, V><<<dim3(w.chunks, w.parts), kTileThreads, w.shared, stream>>>(a, w.gpc, w.parts);
         }
         return launched(fn);
       }
       if (w.shared > (size_t)kSharedLimit) return fail(GELIB_INVALID, fn, "too many channels");  // not up to GELIB_NORM_MAX_CHANNELS
       if (!back) {
-        if ((st = room(fn, piece_stats_kernel<T, V>, w.shared)) != GELIB_OK) return st;
+        if ((st = room<piece_stats_kernel<T, V>>(fn, w.shared)) != GELIB_OK) return st;
         piece_stats_kernel<T, V><<<(unsigned)samples, kThreads, w.shared, stream>>>(a, w.pieces, w.per);
         if ((st = launched(fn)) != GELIB_OK) return st;
         const size_t shared = 2ULL * c.groups * 4;
-        if ((st = room(fn, piece_apply_kernel<T, V>, shared)) != GELIB_OK) return st;
+        if ((st = room<piece_apply_kernel<T, V>>(fn, shared)) != GELIB_OK) return st;
         return launch_after(fn, true, piece_apply_kernel<T, V>, dim3((unsigned)samples), kThreads, shared, stream, a, w.pieces, w.per);
       }
-      if ((st = room(fn, piece_back_sums_kernel<T, V>, w.shared)) != GELIB_OK) return st;
+      if ((st = room<piece_back_sums_kernel<T, V>>(fn, w.shared)) != GELIB_OK) return st;
       float* back = c.workspace + 2LL * w.parts * c.n;
       piece_back_sums_kernel<T, V><<<(unsigned)samples, kThreads, w.shared, stream>>>(a, w.pieces, w.per, back);
       if ((st = launched(fn)) != GELIB_OK || !a.y) return st;
       const size_t shared = 2ULL * c.groups * 4;
-      if ((st = room(fn, piece_back_apply_kernel<T, V>, shared)) != GELIB_OK) return st;
+      if ((st = room<piece_back_apply_kernel<T, V>>(fn, shared)) != GELIB_OK) return st;
       return launch_after(fn, true, piece_back_apply_kernel<T, V>, dim3((unsigned)samples), kThreads, shared, stream, a, w.pieces, w.per, (const float*)back);
     });
   });
