@@ -746,57 +746,93 @@ __device__ __forceinline__ void each_row(const Norm& a, long long base, int rows
   }
 }
 
-// gz xh and gz summed over a piece's rows, per channel: part (2, b * pieces, n); and times w, per group: back (b, pieces, groups, 2).
-template <class T, int V>
+// V consecutive floats, V 1 or a multiple of 2.
+template <int V>
+__device__ __forceinline__ void load_floats(const float* src, float (&x)[V]) {
+  constexpr int kOne = V > 4 ? 4 : V;
+#pragma unroll
+  for (int j = 0; j < V; j += kOne) load_vec<float, kOne>(src + j, reinterpret_cast<float(&)[kOne]>(x[j]));
+}
+template <int V>
+__device__ __forceinline__ void store_floats(float* dst, const float (&x)[V]) {
+  constexpr int kOne = V > 4 ? 4 : V;
+#pragma unroll
+  for (int j = 0; j < V; j += kOne) store_vec<float, kOne>(dst + j, reinterpret_cast<const float(&)[kOne]>(x[j]));
+}
+
+// gz xh and gz summed over the rows of a block's pieces, per channel: part (2, blocks, n), or null; and over each piece, times w, per group: back (b, pieces,
+// groups, 2).  kWalk: a block takes every gridDim.x-th piece and adds their sums up, else it has one piece.
+template <class T, int V, bool kWalk>
 __global__ void __launch_bounds__(kThreads, kPieceBlocksBack) piece_back_sums_kernel(Norm a, int pieces, int per, float* back) {
   let_next_begin();
   extern __shared__ __align__(16) unsigned char memory[];
-  const long long sample = blockIdx.x / pieces;
-  const int piece = blockIdx.x % pieces;
-  const long long r0 = (long long)piece * per;
-  const int rows = (int)min((long long)per, a.s - r0);
   const Columns cl = columns_of(a.n, V);
   float* chan = reinterpret_cast<float*>(memory);   // [2][high][n]
   const int tx = threadIdx.x % cl.wide, ty = threadIdx.x / cl.wide, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const long long base = (sample * a.s + r0) * a.n;
-  if (ty < cl.high)
-    for (int col = tx; col < cl.cols; col += cl.wide) {
-      float w[V], bias[V], mean[V], rstd[V], sw[V], sb[V];
-      load_or<T, V>(a.w, col * V, 1.f, w);
-      load_or<T, V>(a.bias, col * V, 0.f, bias);
+  const unsigned items = (unsigned)(a.b * pieces);
+  for (unsigned item = blockIdx.x; item < items; item += gridDim.x) {
+    const bool first = !kWalk || item == blockIdx.x;
+    if (!first) __syncthreads();   // the sums of the piece before have been read
+    const long long sample = item / pieces, r0 = (long long)(item % pieces) * per;
+    const int rows = (int)min((long long)per, a.s - r0);
+    const long long base = (sample * a.s + r0) * a.n;
+    if (ty < cl.high)
+      for (int col = tx; col < cl.cols; col += cl.wide) {
+        float w[V], bias[V], mean[V], rstd[V], sw[V], sb[V];
+        load_or<T, V>(a.w, col * V, 1.f, w);
+        load_or<T, V>(a.bias, col * V, 0.f, bias);
 #pragma unroll
-      for (int j = 0; j < V; j++) {
-        const long long g = sample * a.groups + (col * V + j) / a.cg;
-        mean[j] = a.mean[g], rstd[j] = a.rstd[g], sw[j] = sb[j] = 0;
+        for (int j = 0; j < V; j++) {
+          const long long g = sample * a.groups + (col * V + j) / a.cg;
+          mean[j] = a.mean[g], rstd[j] = a.rstd[g], sw[j] = sb[j] = 0;
+        }
+        each_row<T, V>(a, base, rows, ty, cl.high, col, w, bias, mean, rstd, [&](int, const float (&h)[V], const float (&g)[V]) {
+          add_all(sb, sb, g);
+          fma_all(sw, g, h, sw);
+        });
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+          chan[ty * a.n + col * V + j] = sw[j];
+          chan[(cl.high + ty) * a.n + col * V + j] = sb[j];
+        }
       }
-      each_row<T, V>(a, base, rows, ty, cl.high, col, w, bias, mean, rstd, [&](int, const float (&h)[V], const float (&g)[V]) {
-        add_all(sb, sb, g);
-        fma_all(sw, g, h, sw);
-      });
+    __syncthreads();
+    for (int e = threadIdx.x; e < 2 * cl.cols; e += kThreads) {
+      const int which = e >= cl.cols, q = (e - which * cl.cols) * V;
+      float* total = a.part + ((long long)which * gridDim.x + blockIdx.x) * a.n + q;   // this thread's own place, of every piece
+      float old[V], t[V];
 #pragma unroll
-      for (int j = 0; j < V; j++) {
-        chan[ty * a.n + col * V + j] = sw[j];
-        chan[(cl.high + ty) * a.n + col * V + j] = sb[j];
+      for (int j = 0; j < V; j++) old[j] = t[j] = 0;
+      if (a.part && !first) load_floats(total, old);
+      for (int i = 0; i < cl.high; i++) {
+        float v[V];
+        load_floats(chan + (which * cl.high + i) * a.n + q, v);
+        add_all(t, t, v);
+      }
+      if (a.part) {
+        add_all(old, old, t);
+        store_floats(total, old);
+      }
+      if (a.w) {
+        float w[V];
+        load_vec<T, V>(static_cast<const T*>(a.w) + q, w);
+        mul_all(t, t, w);
+      }
+      store_floats(chan + which * cl.high * a.n + q, t);   // row 0 of its part: read by this thread alone so far
+    }
+    if (a.y) {
+      __syncthreads();
+      for (int g = warp; g < a.groups; g += kWarps) {
+        float s1 = 0, s2 = 0;
+        for (int c = lane; c < a.cg; c += 32) s2 += chan[g * a.cg + c], s1 += chan[cl.high * a.n + g * a.cg + c];
+        s1 = warp_total(s1), s2 = warp_total(s2);
+        if (lane == 0) {
+          float* out = back + ((long long)item * a.groups + g) * 2;
+          out[0] = s1, out[1] = s2;
+        }
       }
     }
-  __syncthreads();
-  for (int c = threadIdx.x; c < 2 * a.n; c += kThreads) {
-    const int which = c / a.n, q = c % a.n;
-    float t = 0;
-    for (int i = 0; i < cl.high; i++) t += chan[(which * cl.high + i) * a.n + q];
-    a.part[((long long)which * (a.b * pieces) + blockIdx.x) * a.n + q] = t;
-    chan[which * cl.high * a.n + q] = t * (a.w ? to_float(static_cast<const T*>(a.w)[q]) : 1.f);   // row 0 of its part: read by this thread alone so far
-  }
-  if (!a.y) return;
-  __syncthreads();
-  for (int g = warp; g < a.groups; g += kWarps) {
-    float s1 = 0, s2 = 0;
-    for (int c = lane; c < a.cg; c += 32) s2 += chan[g * a.cg + c], s1 += chan[cl.high * a.n + g * a.cg + c];
-    s1 = warp_total(s1), s2 = warp_total(s2);
-    if (lane == 0) {
-      float* out = back + ((sample * pieces + piece) * a.groups + g) * 2;
-      out[0] = s1, out[1] = s2;
-    }
+    if (!kWalk) return;
   }
 }
 
@@ -881,6 +917,7 @@ struct Way {
   size_t shared;     // tile, two
   int parts;         // backward: rows of partial sums
   int pieces, per;   // two
+  bool walk;         // two, backward: blocks take several pieces
 };
 
 int high_of(int channels, int V, int threads) { return threads / std::min(channels / V, threads); }
@@ -946,7 +983,13 @@ Way choose(long long b, long long s, int n, int groups, int type, bool wide16, b
   const long long wanted = std::max(1LL, kSms * (backward ? kPieceBlocksBack : kPieceBlocks) / b);
   w.per = (int)std::min((long long)1 << 24, std::max({(s + wanted - 1) / wanted, (long long)4 * high, std::min(s, (long long)16)}));
   w.pieces = (int)((s + w.per - 1) / w.per);
-  w.parts = (int)std::min(b * w.pieces, 0x7fffffffLL);
+  // Partial sums of the parameters' gradients are 8 bytes a channel: a row of them for each piece, or for each of as many blocks as the SMs hold, which then walk
+  // the pieces.  They walk where a row would be more than a sixteenth of its piece (4000 x 4 x 7168 bfloat16 backward 452 us, 683 with a row each), and where
+  // there are so many pieces that the workspace would grow with the batch.  Else the walk costs more than the rows (500 x 900 x 520 bfloat16
+  // 710 us, 686 with a row each).
+  const long long samples = b * w.pieces, wave = (long long)kSms * kPieceBlocksBack;
+  w.walk = samples > 8 * wave || (samples > wave && std::min(s, (long long)w.per) * size < 128);
+  w.parts = (int)std::min(w.walk ? wave : samples, 0x7fffffffLL);
   return w;
 }
 
@@ -1019,7 +1062,7 @@ int launch_group_norm(const GroupNormCall& c, cudaStream_t stream) {
   const Way w = choose(c.b, c.s, c.n, c.groups, c.type, wide_at({c.x, c.w, c.bias, c.gy, c.y}, 16), wide_at({c.x, c.w, c.bias, c.gy, c.y}, 8), back);
   Norm a = {c.x, c.w, c.bias, c.gy, c.y, c.mean, c.rstd, c.workspace, c.b, c.s, c.n, c.groups, c.n / c.groups, c.eps, c.act};
   const bool sums = c.gw || c.gb;
-  if (w.way != Way::kTwo && !sums) a.part = nullptr;
+  if ((back || w.way != Way::kTwo) && !sums) a.part = nullptr;   // the forward in two passes keeps its statistics there
   const long long samples = w.way == Way::kTwo ? c.b * w.pieces : w.way == Way::kTile ? c.b * w.chunks : 1;
   if (samples > 0x7fffffffLL || (back && c.b * c.groups > 0x7fffffffLL)) return fail(GELIB_INVALID, fn, "too many samples");
   const int st = with_type(c.type, [&](auto* t) -> int {
@@ -1066,9 +1109,14 @@ int launch_group_norm(const GroupNormCall& c, cudaStream_t stream) {
         if ((st = room<piece_apply_kernel<T, V>>(fn, shared)) != GELIB_OK) return st;
         return launch_after(fn, true, piece_apply_kernel<T, V>, dim3((unsigned)samples), kThreads, shared, stream, a, w.pieces, w.per);
       }
-      if ((st = room<piece_back_sums_kernel<T, V>>(fn, w.shared)) != GELIB_OK) return st;
       float* back = c.workspace + 2LL * w.parts * c.n;
-      piece_back_sums_kernel<T, V><<<(unsigned)samples, kThreads, w.shared, stream>>>(a, w.pieces, w.per, back);
+      if (w.walk) {
+        if ((st = room<piece_back_sums_kernel<T, V, true>>(fn, w.shared)) != GELIB_OK) return st;
+        piece_back_sums_kernel<T, V, true><<<w.parts, kThreads, w.shared, stream>>>(a, w.pieces, w.per, back);
+      } else {
+        if ((st = room<piece_back_sums_kernel<T, V, false>>(fn, w.shared)) != GELIB_OK) return st;
+        piece_back_sums_kernel<T, V, false><<<w.parts, kThreads, w.shared, stream>>>(a, w.pieces, w.per, back);
+      }
       if ((st = launched(fn)) != GELIB_OK || !a.y) return st;
       const size_t shared = 2ULL * c.groups * 4;
       if ((st = room<piece_back_apply_kernel<T, V>>(fn, shared)) != GELIB_OK) return st;

@@ -1,4 +1,4 @@
-"""How group norm and dense layers are called: forward-mode derivatives, several threads at a time."""
+"""How group norm and dense layers are called: forward-mode derivatives, several threads at a time, workspaces."""
 import threading
 
 import pytest
@@ -63,3 +63,46 @@ def test_two_threads_with_different_sizes(cabi, sizes, backward):
     for t in threads:
         t.join()
     assert not errors, errors[0]
+
+
+@pytest.mark.parametrize("s,n,groups,kind", [(2, 16384, 1, 1), (4, 7168, 1, 1), (2, 7168, 1, 0), (600, 4096, 4, 0)])
+def test_workspace_of_the_gradient_stays_small(cabi, s, n, groups, kind):
+    """Parameter gradients are partial sums per block that an SM holds, whatever the batch: at most two blocks on each of 148 SMs."""
+    size = 4 if kind == 0 else 2
+    for b in (1, 100, 4096, 100000):
+        most = 2 * 296 * n * 4 + 64 * b * groups * max(1, s // 16)
+        assert cabi.gelib_group_norm_workspace(b, s, n, groups, kind, 1) <= most, b
+    b = 100000
+    assert cabi.gelib_group_norm_workspace(b, s, n, groups, kind, 1) < b * s * n * size / 16
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("b,s,n,groups", [(700, 2, 16384, 1), (700, 4, 7168, 1), (500, 900, 520, 4), (3, 3000, 520, 4)])
+def test_gradients_of_more_pieces_than_blocks(b, s, n, groups, dtype):
+    import gelib_b200 as G
+    gen = torch.Generator(device="cuda").manual_seed(b + s)
+    x, gy = (torch.randn(b, s, n, generator=gen, device="cuda").to(dtype) for _ in range(2))
+    w, bias = (torch.randn(n, generator=gen, device="cuda").to(dtype) for _ in range(2))
+    leaves = [t.requires_grad_() for t in (x, w, bias)]
+    got = torch.autograd.grad(G.group_norm(x, groups, w, bias, activation="silu"), leaves, gy)
+    for alone in range(3):   # each by itself, and the same when it is asked for again
+        again, = torch.autograd.grad(G.group_norm(x, groups, w, bias, activation="silu"), leaves[alone], gy)
+        assert torch.equal(again, got[alone])
+    wants, sizes = [torch.zeros(n, dtype=torch.float64, device="cuda") for _ in range(2)], [torch.zeros(n, dtype=torch.float64, device="cuda") for _ in range(2)]
+    for at in range(0, b, 100):
+        with torch.no_grad():
+            v = x[at:at + 100].double().view(-1, s, groups, n // groups)
+            var, mean = torch.var_mean(v, (1, 3), correction=0, keepdim=True)
+            h = ((v - mean) * (var + 1e-5).rsqrt()).reshape(-1, s, n)
+            z = h * w.double() + bias.double()
+            q = torch.sigmoid(z)
+            g = gy[at:at + 100].double()
+            gz = g * q * (1 + z * (1 - q))
+            more = g.abs() * 1.2 * (1 + h.abs() * w.double().abs() + z.abs())
+            for i, (a, c) in enumerate(((gz * h, more * (h.abs() + 1)), (gz, more))):
+                wants[i] += a.sum((0, 1))
+                sizes[i] += c.sum((0, 1))
+    half = 2.0 ** -8 if dtype == torch.bfloat16 else 0.0
+    for g, want, size in zip(got[1:], wants, sizes):
+        assert ((g.double() - want).abs() <= 64 * 2.0 ** -24 * size + half * (want.abs() + 64 * 2.0 ** -24 * size)).all()
