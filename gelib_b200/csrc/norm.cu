@@ -1064,7 +1064,7 @@ int launch_group_norm(const GroupNormCall& c, cudaStream_t stream) {
   const bool sums = c.gw || c.gb;
   if ((back || w.way != Way::kTwo) && !sums) a.part = nullptr;   // the forward in two passes keeps its statistics there
   const long long samples = w.way == Way::kTwo ? c.b * w.pieces : w.way == Way::kTile ? c.b * w.chunks : 1;
-  if (samples > 0x7fffffffLL || (back && c.b * c.groups > 0x7fffffffLL)) return fail(GELIB_INVALID, fn, "too many samples");
+  if (samples > 0x7fffffffLL) return fail(GELIB_INVALID, fn, "too many samples");
   const int st = with_type(c.type, [&](auto* t) -> int {
     using T = std::remove_pointer_t<decltype(t)>;
     return with_vector<T>(w.V, [&](auto v) -> int {

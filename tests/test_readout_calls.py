@@ -1,4 +1,4 @@
-"""How group norm and dense layers are called: forward-mode derivatives, several threads at a time, workspaces."""
+"""How group norm and dense layers are called: forward-mode derivatives, several threads at a time, workspaces, very many statistics."""
 import threading
 
 import pytest
@@ -106,3 +106,21 @@ def test_gradients_of_more_pieces_than_blocks(b, s, n, groups, dtype):
     half = 2.0 ** -8 if dtype == torch.bfloat16 else 0.0
     for g, want, size in zip(got[1:], wants, sizes):
         assert ((g.double() - want).abs() <= 64 * 2.0 ** -24 * size + half * (want.abs() + 64 * 2.0 ** -24 * size)).all()
+
+
+@pytest.mark.gpu
+def test_more_than_2_to_31_statistics():
+    import gelib_b200 as G
+    if torch.cuda.get_device_properties(0).total_memory < 100 * 2 ** 30:
+        pytest.skip("needs 100 GB of device memory")
+    b, n, groups = 262200, 16384, 8192
+    assert b * groups > 2 ** 31
+    x = torch.empty(b, n, dtype=torch.float16, device="cuda").normal_().requires_grad_()
+    y = G.group_norm(x, groups, activation="relu")
+    gx, = torch.autograd.grad(y, x, x.detach())
+    for at in (0, b - 1):
+        one = x[at:at + 1].detach().clone().requires_grad_()
+        want = G.group_norm(one, groups, activation="relu")
+        gone, = torch.autograd.grad(want, one, one.detach())
+        for got, ref in ((y[at:at + 1], want), (gx[at:at + 1], gone)):
+            assert torch.allclose(got.float(), ref.float(), rtol=2.0 ** -10, atol=1e-4)
