@@ -182,11 +182,28 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def load_state_dict(self, state_dict):
-        """As torch's, but states keep their own types: torch would turn codes and master copies into the parameter's type."""
-        super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
-        numbers = [i for group in state_dict["param_groups"] for i in group["params"]]
-        params = [p for group in self.param_groups for p in group["params"]]
-        for i, p in zip(numbers, params):
-            if i in state_dict["state"]:
-                self.state[p] = {name: value.detach().to(p.device, copy=True) if isinstance(value, torch.Tensor) else value
-                                 for name, value in state_dict["state"][i].items()}
+        """As torch's, but states keep their own types: torch would turn codes and master copies into the parameter's type.
+
+        Hooks see what they would of torch's: those before it the whole dict, which they may replace, those after it the loaded state.  So the state is taken
+        out behind the last hook before torch loads, and put in ahead of the first one after.
+        """
+        held = {}
+
+        def take(_, given):
+            held.update(given)
+            return {"state": {}, "param_groups": given["param_groups"]}
+
+        def put(_):
+            numbers = [i for group in held["param_groups"] for i in group["params"]]
+            params = [p for group in self.param_groups for p in group["params"]]
+            for i, p in zip(numbers, params):
+                if i in held["state"]:
+                    self.state[p] = {name: value.detach().to(p.device, copy=True) if isinstance(value, torch.Tensor) else value
+                                     for name, value in held["state"][i].items()}
+
+        hooks = [self.register_load_state_dict_pre_hook(take), self.register_load_state_dict_post_hook(put, prepend=True)]
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()

@@ -1,4 +1,4 @@
-"""What AdamW keeps: master copies beside parameters that others write to, and roots of the second moment for any eps."""
+"""What AdamW keeps: master copies beside parameters that others write to, roots of the second moment for any eps, and states that come back from a dict."""
 import pytest
 import torch
 
@@ -117,3 +117,64 @@ def test_codes_of_the_root_whatever_eps_is(size, eps):
     q = torch.floor(y / step + ((_bits(seed, n).cuda() >> 16).double() * 16 + 8) / 2 ** 20) * step
     q = torch.where((y > 0) & (q == 0), 2.0 ** -9, q)
     assert torch.equal(code.double(), q), (code.double() != q).sum().item()
+
+
+def _with_state(value=2.0):
+    import gelib_b200 as G
+    p = torch.nn.Parameter(torch.ones(300, dtype=torch.bfloat16))
+    opt = G.AdamW([p], state_bits=8)
+    state = opt._state_of(p, 8)
+    state["step"] = 4
+    state["master"].fill_(value + 2.0 ** -12)
+    state["exp_avg"].view(torch.uint8).fill_(9)
+    state["exp_avg_scale"].fill_(0.25)
+    return p, opt
+
+
+def test_hooks_see_the_state_that_is_loaded():
+    _, opt = _with_state()
+    p, other = _with_state(1.0)
+    seen = {}
+
+    def before(o, d):
+        seen["before"] = {k: dict(v) for k, v in d["state"].items()}
+
+    def after(o):
+        seen["after"] = dict(o.state[p])
+
+    other.register_load_state_dict_pre_hook(before)
+    other.register_load_state_dict_post_hook(after)
+    for _ in range(2):   # nothing of the first call is left for the second
+        seen.clear()
+        other.load_state_dict(opt.state_dict())
+        assert seen["before"][0]["step"] == 4 and float(seen["before"][0]["master"][0]) == 2.0 + 2.0 ** -12
+        assert seen["after"]["step"] == 4 and seen["after"]["exp_avg"].dtype == torch.float8_e4m3fn
+        assert seen["after"]["master"].dtype == torch.float32 and float(seen["after"]["master"][7]) == 2.0 + 2.0 ** -12
+        assert (seen["after"]["exp_avg"].view(torch.uint8) == 9).all() and (seen["after"]["exp_avg_scale"] == 0.25).all()
+    assert seen["after"]["master"] is not opt.state[opt.param_groups[0]["params"][0]]["master"]
+    assert len(other._optimizer_load_state_dict_pre_hooks) == 1 and len(other._optimizer_load_state_dict_post_hooks) == 1
+
+
+def test_a_hook_may_give_another_state():
+    _, opt = _with_state()
+    p, other = _with_state(1.0)
+
+    def before(o, d):
+        new = dict(d)
+        new["state"] = {0: dict(d["state"][0], step=11)}
+        return new
+
+    other.register_load_state_dict_pre_hook(before)
+    other.load_state_dict(opt.state_dict())
+    assert other.state[p]["step"] == 11
+
+
+def test_a_state_that_does_not_fit_changes_nothing():
+    import gelib_b200 as G
+    _, opt = _with_state()
+    p, q = (torch.nn.Parameter(torch.ones(3)) for _ in range(2))
+    other = G.AdamW([p, q])
+    other._state_of(p, 32)
+    with pytest.raises(ValueError):
+        other.load_state_dict(opt.state_dict())
+    assert p in other.state and not other._optimizer_load_state_dict_pre_hooks and not other._optimizer_load_state_dict_post_hooks
