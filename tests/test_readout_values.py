@@ -133,3 +133,24 @@ def test_gradients_of_few_rows_are_rounded_once(m, k, n, act, wt, dtype):
     for got, want, size in ((gx, gz @ w64.t(), slope @ w64.abs().t()), (gw, x64.t() @ gz, x64.abs().t() @ slope)):
         off, allowed = (got.double() - want).abs(), EPS * size + HALF[dtype] * (want.abs() + EPS * size) + tiny
         assert (off <= allowed).all(), (off / allowed).max().item()
+
+
+@pytest.mark.parametrize("m", [5, 40])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_gradients_of_an_empty_sum(m, dtype):
+    """k = 0: y = act(bias) + residual, and the bias's gradient is a sum over the rows."""
+    import gelib_b200 as G
+    n = 12
+    gen = torch.Generator(device="cuda").manual_seed(m)
+    x, w = torch.zeros(m, 0, dtype=dtype, device="cuda", requires_grad=True), torch.zeros(0, n, dtype=dtype, device="cuda", requires_grad=True)
+    bias, gy = (torch.randn(*shape, generator=gen, device="cuda").to(dtype) for shape in ((n,), (m, n)))
+    bias.requires_grad_()
+    y = G.linear(x, w, bias, activation="silu")
+    gx, gw, gb = torch.autograd.grad(y, (x, w, bias), gy)
+    z = bias.detach().double().requires_grad_()
+    f = torch.nn.functional.silu(z)
+    slope, = torch.autograd.grad(f.sum(), z)
+    assert ((y.double() - f.detach()).abs() <= (EPS + HALF[dtype]) * f.detach().abs() + EPS).all()
+    want, size = slope * gy.double().sum(0), gy.double().abs().sum(0) * 1.2 * (1 + z.detach().abs())
+    assert ((gb.double() - want).abs() <= EPS * size + HALF[dtype] * want.abs()).all()
+    assert gx.shape == (m, 0) and gw.shape == (0, n)
