@@ -14,9 +14,10 @@
 // are many small tensors, so their addresses travel in the launch's parameters, a tensor is cut into pieces of as many elements as a block takes, and
 // a block finds its piece by bisection.
 //
-// Measured on 46.7 million weights: 190 us in 32 bits (28 bytes an element, 6.8 TB/s: the copy rate); 8 bits and a bfloat16 head 220 us with the values of both
-// moments written out (two launches of 27), where the step's bytes take 114:
-// some 80 instructions an element, most of them the two roundings, half of them on the integer pipe.  Two dozen small tensors 11 us a call, half of it Python's.
+// Measured on 46.7 million weights: 190 us in 32 bits (28 bytes an element, 6.8 TB/s: the copy rate); 8 bits and a bfloat16 head 222 us with the values of both
+// moments written out (two launches of 27), where the step's bytes take 114.  Its 85 instructions an element, most of them the two roundings, fill 65 % of the issue
+// slots and 56 % of the integer pipe, DRAM is at 48 %: loads and arithmetic of a piece follow one another, and 36 warps of an SM do not cover
+// that.  Two dozen small tensors 11 us a call, half of it Python's.
 #include <cuda_fp8.h>
 
 #include <algorithm>
@@ -285,7 +286,7 @@ __device__ __forceinline__ void step_piece(const Entry& e, const Scalars& s, lon
   }
 }
 
-// Five blocks of an SM although registers spill: a pass over 46.7 million weights, with the values of both moments, 220 us in 8 bits; six 224.
+// Five blocks of an SM although registers spill: a pass over 46.7 million weights, with the values of both moments, 222 us in 8 bits; six took 4 us more.
 template <int N, bool k8>
 __global__ void __launch_bounds__(kThreads, k8 ? 5 : 4) adamw_kernel(const __grid_constant__ Args<N> a) {
   const Entry& e = find(a, (int)blockIdx.x);
@@ -321,7 +322,8 @@ int launch(const gelib_adamw_tensor* t, const long long* first_block, int count,
   return launched("adamw_step");
 }
 
-constexpr int kMost = 350;   // entries of 88 bytes in the 32764 bytes that a launch's parameters may have
+constexpr int kMost = 350;   // entries of 80 bytes
+static_assert(sizeof(Args<kMost>) <= 32764, "what a launch's parameters may have");
 
 __global__ void __launch_bounds__(kThreads) block8_values_kernel(__nv_bfloat16* __restrict__ out, const unsigned char* __restrict__ codes,
                                                                 const float* __restrict__ scale, long long n, bool wide) {

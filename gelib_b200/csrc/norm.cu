@@ -15,10 +15,10 @@
 //
 // Parameter gradients are partial sums per block, added up in a fixed order by a second kernel: results repeat bit for bit.
 //
-// Measured, forward / backward us (what the bytes take at 6.5 TB/s): rows of 7168 channels in 32 groups, 4096 of them, bfloat16 35 / 54 (18 / 27), bound by the
-// issue of instructions -- 240 for a warp's eight channels a lane in the first form, the packed pairs and the approximate logistic function without subnormal
-// numbers halved them; 4 x 65536 x 112 float32, in two passes, 70 / 113 (36 / 54 and half as much again for the second reading), memory at 0.75 of its
-// rate; 3000 x 19 x 204 bfloat16, in shared memory, 29 / 56 (7 / 11), the latency of a block's phases.
+// Measured, forward / backward us (what the bytes take at 6.5 TB/s): rows of 7168 channels in 32 groups, 4096 of them, bfloat16 35 / 54 (18 / 27); no unit is
+// full there -- issue slots 56 / 61 %, special functions 52 / 31 % --, the fixed latency of dependent instructions is what 14 warps of an SM wait for.
+// 4 x 65536 x 112 float32, in two passes, 70 / 113 (36 / 54 and half as much again for the second reading), memory at 0.75 of its
+// rate, a batch of rows on its way at a time; 3000 x 19 x 204 bfloat16, in shared memory, 29 / 56 (7 / 11), the latency of a block's phases.
 #include <algorithm>
 #include <atomic>
 
