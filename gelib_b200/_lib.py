@@ -49,6 +49,13 @@ class LinearArgs(ctypes.Structure):
     _fields_ += [(name, ctypes.c_int) for name in ("w_transposed", "act", "type")]
 
 
+class LinearLossArgs(ctypes.Structure):
+    """``gelib_linear_loss_args``"""
+    _fields_ = [(name, ctypes.c_void_p) for name in ("x", "w", "bias", "target", "teacher", "gy", "loss", "state", "gx", "gw", "gb")]
+    _fields_ += [(name, ctypes.c_int64) for name in ("m", "ldx", "ldw", "ignore_index")] + [("temperature", ctypes.c_double)]
+    _fields_ += [(name, ctypes.c_int) for name in ("k", "n", "top", "w_transposed", "reduction", "type", "teacher_type", "index_bytes")]
+
+
 _P5 = ctypes.POINTER(Tensor5)
 _lib = None
 
@@ -108,6 +115,15 @@ SYMBOLS = {
     "gelib_linear_workspace": (ctypes.c_longlong, [ctypes.POINTER(LinearArgs), ctypes.c_int]),
     "gelib_linear": (ctypes.c_int, [ctypes.POINTER(LinearArgs), ctypes.c_void_p, ctypes.c_void_p]),
     "gelib_linear_back": (ctypes.c_int, [ctypes.POINTER(LinearArgs), ctypes.c_void_p, ctypes.c_void_p]),
+    "gelib_embedding": (ctypes.c_int, [ctypes.c_void_p] * 3 + [ctypes.c_longlong, ctypes.c_int, ctypes.c_int, ctypes.c_longlong, ctypes.c_double]
+                        + [ctypes.c_int] * 2 + [ctypes.c_void_p]),
+    "gelib_embedding_workspace": (ctypes.c_longlong, [ctypes.c_longlong] + [ctypes.c_int] * 3),
+    "gelib_embedding_back": (ctypes.c_int, [ctypes.c_void_p] * 3 + [ctypes.c_longlong, ctypes.c_int, ctypes.c_int, ctypes.c_double, ctypes.c_longlong]
+                             + [ctypes.c_int] * 2 + [ctypes.c_void_p] * 2),
+    "gelib_linear_loss_state_bytes": (ctypes.c_longlong, [ctypes.POINTER(LinearLossArgs)]),
+    "gelib_linear_loss_workspace": (ctypes.c_longlong, [ctypes.POINTER(LinearLossArgs), ctypes.c_int]),
+    "gelib_linear_loss": (ctypes.c_int, [ctypes.POINTER(LinearLossArgs), ctypes.c_void_p, ctypes.c_void_p]),
+    "gelib_linear_loss_back": (ctypes.c_int, [ctypes.POINTER(LinearLossArgs), ctypes.c_void_p, ctypes.c_void_p]),
     "gelib_kernel_launch_count": (ctypes.c_longlong, []),
     "gelib_set_option": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_char_p]),
     "gelib_async_status": (ctypes.c_int, []),

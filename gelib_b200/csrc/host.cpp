@@ -1,4 +1,4 @@
-// The host side of the Python products, in native code: what SO3part.py, SO3vec.py, readout.py and adamw.py do around one C-ABI call --
+// The host side of the Python products, in native code: what SO3part.py, SO3vec.py, readout.py, heads.py and adamw.py do around one C-ABI call --
 // output type, output tensors, zero-filled gradients, descriptors, device, stream -- for operands that need nothing special.  Each
 // function returns None, having done nothing, when an operand is not plain (not on a CUDA device, not complex64, lazily
 // conjugated, more than two grid dimensions, two parts of one l, ...), when sizes do not fit together, and when the library
@@ -523,6 +523,159 @@ std::optional<at::Tensor> group_norm(const at::Tensor& x, int groups, const OptT
   return norm_call(x, w, b, groups, eps, act, at::Tensor());
 }
 
+// ---- embedding tables and losses ---------------------------------------------------------------------------------------------------
+
+bool plain_numbers(const at::Tensor& t, c10::Device device) {
+  return t.defined() && t.device() == device && t.layout() == at::kStrided && (t.scalar_type() == at::kLong || t.scalar_type() == at::kInt);
+}
+
+at::Tensor embedding_call(const at::Tensor& ids, const at::Tensor& w, double scale) {
+  c10::cuda::CUDAGuard guard(w.device());
+  const int64_t n = ids.numel(), d = w.size(1);
+  c10::SmallVector<int64_t, 6> shape(ids.sizes().begin(), ids.sizes().end());
+  shape.push_back(d);
+  const at::Tensor y = at::empty(shape, w.options());
+  void* s = stream_of(w.device());
+  const int type = *type_code(w.scalar_type()), bytes = static_cast<int>(ids.element_size());
+  call([&] { return gelib_embedding(ptr(y), ptr(ids), ptr(w), n, static_cast<int>(w.size(0)), static_cast<int>(d), std::max(w.stride(0), d), scale, bytes, type, s); });
+  return y;
+}
+
+struct EmbeddingFunction : torch::autograd::Function<EmbeddingFunction> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& ids, const at::Tensor& w, double scale, int64_t padding) {
+    ctx->save_for_backward({ids});
+    ctx->saved_data["v"] = w.size(0);
+    ctx->saved_data["d"] = w.size(1);
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["padding"] = padding;
+    return embedding_call(ids, w, scale);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list out(4);
+    if (!grads[0].defined()) return out;
+    {
+      const at::NoGradGuard off;
+      const at::Tensor ids = ctx->get_saved_variables()[0], gy = grads[0].resolve_neg().contiguous();
+      c10::cuda::CUDAGuard guard(gy.device());
+      const int64_t n = ids.numel(), padding = ctx->saved_data["padding"].toInt();
+      const int v = static_cast<int>(ctx->saved_data["v"].toInt()), d = static_cast<int>(ctx->saved_data["d"].toInt());
+      const int type = *type_code(gy.scalar_type()), bytes = static_cast<int>(ids.element_size());
+      const double scale = ctx->saved_data["scale"].toDouble();
+      out[1] = at::empty({v, d}, gy.options());
+      const at::Tensor space = workspace(gelib_embedding_workspace(n, v, d, type), gy);
+      void* s = stream_of(gy.device());
+      call([&] { return gelib_embedding_back(ptr(out[1]), ptr(gy), ptr(ids), n, v, d, scale, padding, bytes, type, ptr(space), s); });
+    }
+    return differentiable_once(std::move(out), "embedding");
+  }
+};
+
+std::optional<at::Tensor> embedding(const at::Tensor& ids, const at::Tensor& w, double scale, std::optional<int64_t> padding_idx) {
+  if (!is_plain(w) || w.dim() != 2 || !plain_numbers(ids, w.device()) || !ids.is_contiguous() || ids.numel() == 0 || w.numel() == 0) return std::nullopt;
+  const int64_t v = w.size(0), d = w.size(1);
+  if (v > INT_MAX || d > INT_MAX || (w.stride(1) != 1 && d > 1) || (w.stride(0) < d && v > 1)) return std::nullopt;
+  if (padding_idx && (*padding_idx < -v || *padding_idx >= v)) return std::nullopt;
+  const int64_t padding = padding_idx ? (*padding_idx < 0 ? *padding_idx + v : *padding_idx) : -1;
+  if (at::GradMode::is_enabled() && w.requires_grad()) return EmbeddingFunction::apply(ids, w, scale, padding);
+  return embedding_call(ids, w, scale);
+}
+
+struct LossCall {
+  gelib_linear_loss_args a = {};
+  at::Tensor x, w;
+};
+// x and w as they lie, or copies; the rest is dense.
+void describe_loss(LossCall* l, const at::Tensor& x, const at::Tensor& w, const at::Tensor& bias, const at::Tensor& target, const at::Tensor& teacher) {
+  l->a.k = static_cast<int>(w.size(0));
+  l->a.n = static_cast<int>(w.size(1));
+  l->a.m = 1;
+  for (int64_t d = 0; d + 1 < x.dim(); d++) l->a.m *= x.size(d);
+  l->x = as_rows(x, l->a.k, &l->a.ldx);
+  l->a.w_transposed = w.stride(0) == 1 && w.stride(1) != 1 && w.stride(1) >= l->a.k;
+  if (l->a.w_transposed) l->w = w, l->a.ldw = w.stride(1);
+  else l->w = as_rows(w, l->a.n, &l->a.ldw);
+  l->a.x = ptr(l->x), l->a.w = ptr(l->w), l->a.bias = ptr(bias), l->a.target = ptr(target), l->a.teacher = ptr(teacher);
+  l->a.top = teacher.defined() ? static_cast<int>(teacher.size(-1)) : 1;
+  l->a.type = *type_code(x.scalar_type()), l->a.teacher_type = teacher.defined() ? *type_code(teacher.scalar_type()) : 0;
+  l->a.index_bytes = static_cast<int>(target.element_size());
+}
+
+// state: what the backward call needs of it.
+at::Tensor loss_call(LossCall* l, const at::Tensor& x, const at::Tensor& w, const at::Tensor& bias, const at::Tensor& target, const at::Tensor& teacher, at::Tensor* state) {
+  c10::cuda::CUDAGuard guard(x.device());
+  describe_loss(l, x, w, bias, target, teacher);
+  const at::Tensor loss = at::empty(l->a.reduction == GELIB_LOSS_NONE ? x.sizes().slice(0, x.dim() - 1) : at::IntArrayRef{}, x.options().dtype(at::kFloat));
+  *state = at::empty({gelib_linear_loss_state_bytes(&l->a)}, x.options().dtype(at::kByte));
+  l->a.loss = ptr(loss), l->a.state = ptr(*state);
+  const at::Tensor space = workspace(gelib_linear_loss_workspace(&l->a, 0), x);
+  void* s = stream_of(x.device());
+  call([&] { return gelib_linear_loss(&l->a, ptr(space), s); });
+  return loss;
+}
+
+struct LinearLossFunction : torch::autograd::Function<LinearLossFunction> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, const OptTensor& bias, const at::Tensor& target, const OptTensor& teacher,
+                            int64_t reduction, int64_t ignore_index, double temperature) {
+    LossCall l;
+    l.a.reduction = static_cast<int>(reduction), l.a.ignore_index = ignore_index, l.a.temperature = temperature;
+    at::Tensor state, loss = loss_call(&l, x, w, or_none(bias), target, or_none(teacher), &state);
+    ctx->save_for_backward({x, w, or_none(bias), target, or_none(teacher), state});
+    ctx->saved_data["reduction"] = reduction;
+    ctx->saved_data["ignore_index"] = ignore_index;
+    ctx->saved_data["temperature"] = temperature;
+    return loss;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list out(8);
+    if (!grads[0].defined()) return out;
+    {
+      const at::NoGradGuard off;
+      const auto saved = ctx->get_saved_variables();
+      const at::Tensor &x = saved[0], gy = grads[0].resolve_neg().contiguous();
+      c10::cuda::CUDAGuard guard(x.device());
+      LossCall l;
+      l.a.reduction = static_cast<int>(ctx->saved_data["reduction"].toInt()), l.a.ignore_index = ctx->saved_data["ignore_index"].toInt();
+      l.a.temperature = ctx->saved_data["temperature"].toDouble();
+      describe_loss(&l, x, saved[1], saved[2], saved[3], saved[4]);
+      // edges are counted over the tensors that were given
+      if (ctx->needs_input_grad(0)) out[0] = at::empty(x.sizes(), x.options());
+      if (ctx->needs_input_grad(1)) out[1] = at::empty(l.a.w_transposed ? std::vector<int64_t>{l.a.n, l.a.k} : std::vector<int64_t>{l.a.k, l.a.n}, x.options());
+      if (saved[2].defined() && ctx->needs_input_grad(2)) out[2] = at::empty({l.a.n}, x.options());
+      l.a.gy = ptr(gy), l.a.state = ptr(saved[5]), l.a.gx = ptr(out[0]), l.a.gw = ptr(out[1]), l.a.gb = ptr(out[2]);
+      const at::Tensor space = workspace(gelib_linear_loss_workspace(&l.a, 1), x);
+      void* s = stream_of(x.device());
+      call([&] { return gelib_linear_loss_back(&l.a, ptr(space), s); });
+      if (out[1].defined() && l.a.w_transposed) out[1] = out[1].t();
+    }
+    return differentiable_once(std::move(out), saved_name(ctx));
+  }
+  static const char* saved_name(AutogradContext* ctx) { return ctx->get_saved_variables()[4].defined() ? "linear_distillation" : "linear_cross_entropy"; }
+};
+
+std::optional<at::Tensor> linear_loss(const at::Tensor& x, const at::Tensor& w, const OptTensor& bias, const at::Tensor& target, const OptTensor& teacher, int reduction,
+                                      int64_t ignore_index, double temperature) {
+  if (!is_plain(x) || x.dim() < 1 || x.numel() == 0 || !w.defined() || w.dim() != 2 || w.numel() == 0 || x.size(-1) != w.size(0) || !goes_with(x, w, w.sizes()))
+    return std::nullopt;
+  if (w.size(0) > INT_MAX || w.size(1) > INT_MAX || !goes_with(x, bias, {w.size(1)}) || (bias && !bias->is_contiguous())) return std::nullopt;
+  if (!plain_numbers(target, x.device()) || !target.is_contiguous()) return std::nullopt;
+  const auto lead = x.sizes().slice(0, x.dim() - 1);
+  if (teacher) {
+    const at::Tensor& t = *teacher;
+    if (!is_plain(t) || t.device() != x.device() || !t.is_contiguous() || t.requires_grad() || t.dim() != x.dim() || t.sizes().slice(0, lead.size()) != lead) return std::nullopt;
+    if (target.sizes() != t.sizes() || t.size(-1) < 1 || t.size(-1) > GELIB_LOSS_MAX_TOP) return std::nullopt;
+  } else if (target.sizes() != lead) {
+    return std::nullopt;
+  }
+  const at::Tensor b = or_none(bias);
+  const auto wants = [](const at::Tensor& t) { return t.defined() && t.requires_grad(); };
+  if (at::GradMode::is_enabled() && (wants(x) || wants(w) || wants(b)))
+    return LinearLossFunction::apply(x, w, bias, target, teacher, static_cast<int64_t>(reduction), ignore_index, temperature);
+  LossCall l;
+  l.a.reduction = reduction, l.a.ignore_index = ignore_index, l.a.temperature = temperature;
+  at::Tensor state;
+  return loss_call(&l, x, w, b, target, or_none(teacher), &state);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_native, m) {
@@ -533,6 +686,8 @@ PYBIND11_MODULE(_native, m) {
   m.def("part_backward", torch::wrap_pybind_function(&part_backward));
   m.def("linear", torch::wrap_pybind_function(&linear));
   m.def("group_norm", torch::wrap_pybind_function(&group_norm));
+  m.def("embedding", torch::wrap_pybind_function(&embedding));
+  m.def("linear_loss", torch::wrap_pybind_function(&linear_loss));
   m.def("block8_values", torch::wrap_pybind_function(&block8_values));
   m.def("adamw_step", torch::wrap_pybind_function(&adamw_step));
   m.def("gather", torch::wrap_pybind_function(&gather));

@@ -283,6 +283,45 @@ long long gelib_linear_workspace(const gelib_linear_args* args, int backward);
 int gelib_linear(const gelib_linear_args* args, void* workspace, void* stream);
 int gelib_linear_back(const gelib_linear_args* args, void* workspace, void* stream);
 
+/* ---- embedding tables and losses -------------------------------------------------------------------------------
+ * Both ends of a network over discrete things (species of atoms, entries of a vocabulary).  Numbers of entries and classes are int64 or
+ * int32 (index_bytes 8 or 4) in device memory; those that name no row are never used as an address.  Workspaces as above. */
+
+/* y[i] = scale * weight[ids[i]]: weight (v, d) with rows of ldw elements, y dense (n, d), both of `type`.  A row whose id is outside [0, v) is NaN. */
+int gelib_embedding(void* y, const void* ids, const void* weight, long long n, int v, int d, long long ldw, double scale, int index_bytes, int type,
+                    void* stream);
+/* gw[r] = scale * the sum of gy's rows i with ids[i] = r, in their order and in float, rounded once; zero where there is none and in row
+ * `padding` (negative: none).  gy dense (n, d), gw dense (v, d), overwritten.  ids outside [0, v) are left out. */
+long long gelib_embedding_workspace(long long n, int v, int d, int type);
+int gelib_embedding_back(void* gw, const void* gy, const void* ids, long long n, int v, int d, double scale, long long padding, int index_bytes,
+                         int type, void* workspace, void* stream);
+
+/* Losses of the rows of z = x w + bias, which is never kept: x (m, k) with rows of ldx elements, w (k, n) with rows of ldw or with w_transposed
+ * (n, k), bias (n) or NULL, all of `type`.
+ *   teacher NULL (top 1): cross entropy, loss = log sum_j exp z_j - z_t, t = target[row]; rows with t = ignore_index have no loss.
+ *   otherwise: divergence from a teacher's `top` logits per row, teacher (m, top) dense of teacher_type at the classes target (m, top): with q =
+ *   softmax(teacher / T) over the entries whose class is not negative and p = softmax(z / T), loss = T^2 sum q (log q - log p); rows without entries
+ *   have no loss.  At most GELIB_LOSS_MAX_TOP entries.
+ * Rows without a loss count as 0, their gradients are zero, and no number of x there has any effect.  A class of n or more (for cross entropy any
+ * other negative one too) makes its row's loss and gradients NaN.
+ * reduction: GELIB_LOSS_NONE (loss (m)), GELIB_LOSS_SUM or GELIB_LOSS_MEAN over the rows that have a loss (loss (1); 0 when none has).  Losses are float.
+ * `state`: gelib_linear_loss_state_bytes of the caller's memory, 256-byte aligned, written by the forward call and read by the backward call, with the
+ * other arguments as they were.  Backward: of gy (float, (m) or (1) like loss) the gradients gx dense (m, k), gw dense and in w's layout, gb (n); each
+ * may be NULL.  k is at most 65536; m and n at most 2^30. */
+#define GELIB_LOSS_MAX_TOP 1024
+enum { GELIB_LOSS_NONE = 0, GELIB_LOSS_SUM = 1, GELIB_LOSS_MEAN = 2 };
+typedef struct gelib_linear_loss_args {
+  const void *x, *w, *bias, *target, *teacher, *gy;
+  void *loss, *state, *gx, *gw, *gb;
+  int64_t m, ldx, ldw, ignore_index;
+  double temperature;
+  int k, n, top, w_transposed, reduction, type, teacher_type, index_bytes;
+} gelib_linear_loss_args;
+long long gelib_linear_loss_state_bytes(const gelib_linear_loss_args* args);
+long long gelib_linear_loss_workspace(const gelib_linear_loss_args* args, int backward);
+int gelib_linear_loss(const gelib_linear_loss_args* args, void* workspace, void* stream);
+int gelib_linear_loss_back(const gelib_linear_loss_args* args, void* workspace, void* stream);
+
 /* ---- introspection ------------------------------------------------------------------------------- */
 
 /* Number of kernels this library has launched in the calling process (all threads, all devices). */
