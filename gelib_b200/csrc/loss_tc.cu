@@ -1,0 +1,466 @@
+// The products of the losses on the tensor cores: three epilogues of the kernel in gemm_tc.cuh.
+//
+//   forward   z = x w + bias; of z only the largest of a row's columns, the sum of exp2(c (z - largest)) and z at the row's classes are kept.
+//   slope     z again; dz = up g (exp2(c (z - largest) - log2 sum) - q), the operand of the gradients.
+//   gradients dz w^T and x^T dz by one launch, added up over the pieces of the classes in float.
+//
+// A lane of the epilogue's warps has 16 columns of a row at a time, so that a row's maximum and sum stay in its registers over a tile.
+#include "loss.h"
+
+#include "gemm_tc.cuh"
+
+namespace gelib_b200 {
+
+namespace {
+
+// Sixteen columns of z from class n on, of `end`: the sums and the bias.
+template <class T>
+__device__ __forceinline__ void logits_of(float (&v)[kChunk], const uint32_t (&r)[kChunk], const T* bias, bool wide, int n, int end) {
+#pragma unroll
+  for (int j = 0; j < kChunk; j++) v[j] = __uint_as_float(r[j]);
+  if (!bias) return;
+  float b[kChunk];
+  if (wide && n + kChunk <= end) {
+    constexpr int V = 16 / sizeof(T);
+#pragma unroll
+    for (int j = 0; j < kChunk; j += V) {
+      float w[V];
+      load_vec<T, V>(bias + n + j, w);
+#pragma unroll
+      for (int k = 0; k < V; k++) b[j + k] = w[k];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < kChunk; j++) b[j] = n + j < end ? to_float(bias[n + j]) : 0.f;
+  }
+  add_all(v, v, b);
+}
+
+struct ForwardProblem : TcShape {
+  const void* bias;
+  int wide;          // the bias begins on a 16-byte boundary
+  Entries e;
+  float c;
+  float2* part;
+  float* at_entry;
+};
+
+template <class T>
+struct ForwardEnd {
+  using Problem = ForwardProblem;
+  static constexpr bool kTwo = false;
+  float2 sum;
+  Next next;
+  long long row;
+  int tile;
+
+  template <int kChunks>
+  __device__ __forceinline__ void ahead(const Problem& g, const Item& it, long long m0, int n0, int lane, bool second) {
+    row = m0 + lane;
+    tile = it.n * 2 + second;
+    sum = {-INFINITY, 0.f};
+    next.begin(g.e, row, row < g.M, n0);
+  }
+  __device__ __forceinline__ void take(const Problem& g, int, int n, int, uint32_t, const uint32_t (&r)[kChunk], bool) {
+    float v[kChunk];
+    logits_of<T>(v, r, static_cast<const T*>(g.bias), g.wide, n, g.N);
+    if (n + kChunk > g.N)
+#pragma unroll
+      for (int j = 0; j < kChunk; j++)
+        if (n + j >= g.N) v[j] = -INFINITY;
+    while (next.cls < n + kChunk) {
+      if (next.cls >= n) {
+        float z = 0;
+#pragma unroll
+        for (int j = 0; j < kChunk; j++)
+          if (next.cls == n + j) z = v[j];
+        g.at_entry[row * g.e.top + next.at] = z;
+      }
+      next.advance(g.e, row);
+    }
+    __syncwarp();   // the next read of tensor memory is the whole warp's
+    float top = v[0];
+#pragma unroll
+    for (int j = 1; j < kChunk; j++) top = fmaxf(top, v[j]);
+    top = fmaxf(top, sum.x);
+    const float from = top == -INFINITY ? 0.f : top;
+    add_all(v, v, -from);
+    mul_all(v, v, g.c);
+#pragma unroll
+    for (int j = 0; j < kChunk; j++) v[j] = exp2_of(v[j]);
+    sum.y = fmaf(sum.y, exp2_of(g.c * (sum.x - from)), sum_of(v));
+    sum.x = top;
+  }
+  __device__ __forceinline__ void end(const Problem& g, int) {
+    if (row < g.M) g.part[(long long)tile * g.M + row] = sum;
+  }
+};
+
+struct SlopeProblem : TcShape {
+  const void* bias;  // of the piece's classes
+  int wide;
+  Entries e;
+  float c, up;
+  const float2* lse;
+  const float *gy, *most;
+  void* dz;
+  long long ld, plane;
+  float* sums;
+  int first;
+};
+
+__device__ __forceinline__ void take_from_shared(uint32_t at, float x) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(v - x) : "memory");
+}
+
+template <class T>
+struct SlopeEnd {
+  using Problem = SlopeProblem;
+  static constexpr bool kTwo = false;
+  Next next;
+  long long m0;
+  float2 lse;
+  float g_up;
+  bool out, some_out;   // the lane's row has no loss; one of the warp's has none
+
+  template <int kChunks>
+  __device__ __forceinline__ void ahead(const Problem& g, const Item&, long long m, int n0, int lane, bool) {
+    m0 = m;
+    const long long row = m0 + lane;
+    lse = row < g.M ? g.lse[row] : float2{0.f, INFINITY};
+    out = lse.y == INFINITY;
+    some_out = __any_sync(0xffffffffu, out);
+    g_up = g.up;
+    if (g.gy && row < g.M) g_up *= g.most ? g.gy[row] / *g.most : g.gy[row];
+    next.begin(g.e, row, !out, g.first + n0);
+  }
+  __device__ __forceinline__ void take(const Problem& g, int, int n, int lane, uint32_t block, const uint32_t (&r)[kChunk], bool) {
+    float v[kChunk];
+    logits_of<T>(v, r, static_cast<const T*>(g.bias), g.wide, n, g.N);
+    add_all(v, v, -lse.x);
+    fma_all(v, v, g.c, -lse.y);
+#pragma unroll
+    for (int j = 0; j < kChunk; j++) v[j] = exp2_of(v[j]);
+    mul_all(v, v, g_up);
+    if (some_out)
+#pragma unroll
+      for (int j = 0; j < kChunk; j++) v[j] = out ? 0.f : v[j];
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < kAcross; j++)
+      tc::sts128(block + (lane * kPitch + 4 * j) * 4, __float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]), __float_as_uint(v[4 * j + 2]), __float_as_uint(v[4 * j + 3]));
+    const int cls = g.first + n;
+    while (next.cls < cls + kChunk) {
+      const long long row = m0 + lane;
+      if (next.cls >= cls) take_from_shared(block + (lane * kPitch + next.cls - cls) * 4, g_up * (g.e.q ? g.e.q[row * g.e.top + next.at] : 1.f));
+      next.advance(g.e, row);
+    }
+    __syncwarp();
+    const int col = lane % kAcross * 4, live = min(4, g.N - n - col);
+    float s[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int pass = 0; pass < kPasses; pass++) {
+      const float4 f = tc::lds128(block + ((pass * kRows + lane / kAcross) * kPitch + col) * 4);
+      const float d[4] = {f.x, f.y, f.z, f.w};
+      add_all(s, s, d);   // rows that are not there are zero
+      const long long m = m0 + pass * kRows + lane / kAcross, at = m * g.ld + n + col;
+      if (m >= g.M || live <= 0) continue;
+      if constexpr (sizeof(T) == 4) {
+        uint32_t p[3], q[3];
+        split3(d[0], d[1], p);
+        split3(d[2], d[3], q);
+#pragma unroll
+        for (int i = 0; i < 3; i++) {
+          __nv_bfloat16* to = static_cast<__nv_bfloat16*>(g.dz) + i * g.plane + at;
+          *reinterpret_cast<uint2*>(to) = make_uint2(p[i], q[i]);   // rows have room for a multiple of eight
+        }
+      } else {
+        store_vec<T, 4>(static_cast<T*>(g.dz) + at, d);
+      }
+    }
+    if (!g.sums) return;
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+#pragma unroll
+      for (int d = kAcross; d < 32; d *= 2) s[j] += __shfl_xor_sync(0xffffffffu, s[j], d);
+    if (lane < kAcross && m0 < g.M) {
+      float* to = g.sums + m0 / 32 * g.N + n + col;
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        if (j < live) to[j] = s[j];
+    }
+  }
+  __device__ __forceinline__ void end(const Problem&, int) {}
+};
+
+struct GradProblem : TcShape {
+  float* part;            // partial sums (splits, M, N), or null
+  float* sum;
+  void* y;                // null: not finished yet
+  long long ldy;
+  int begun;              // something has been added to `sum`
+  int vec_f, vec_y;       // four columns at a time: in `part` and `sum`, in y
+  const float *a0, *a1;
+  float a2;
+};
+
+__device__ __forceinline__ float scale_of(const float* a0, const float* a1, float a2) { return a2 * (a0 ? *a0 : 1.f) * (a1 ? *a1 : 1.f); }
+
+// v (+ what is in `sum`) to y, times `scale`, or to `sum`.
+template <class T, int V>
+__device__ __forceinline__ void finish_grad(T* y, float* sum, bool begun, float scale, float (&v)[V]) {
+  if (sum && begun) {
+    float w[V];
+    load_vec<float, V>(sum, w);
+    add_all(v, v, w);
+  }
+  if (y) {
+    mul_all(v, v, scale);
+    store_vec<T, V>(y, v);
+  } else {
+    store_vec<float, V>(sum, v);
+  }
+}
+
+template <class T>
+struct GradEnd {
+  using Problem = GradProblem;
+  static constexpr bool kTwo = true;
+  long long m0;
+  int split;
+  float scale;
+
+  template <int kChunks>
+  __device__ __forceinline__ void ahead(const Problem& g, const Item& it, long long m, int, int, bool) {
+    m0 = m, split = it.split;
+    scale = scale_of(g.a0, g.a1, g.a2);
+  }
+  __device__ __forceinline__ void take(const Problem& g, int, int n0, int lane, uint32_t block, const uint32_t (&r)[kChunk], bool) {
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < kAcross; j++) tc::sts128(block + (lane * kPitch + 4 * j) * 4, r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+    __syncwarp();
+    const int col = lane % kAcross * 4, n = n0 + col, live = min(4, g.N - n);
+#pragma unroll
+    for (int pass = 0; pass < kPasses; pass++) {
+      const float4 f = tc::lds128(block + ((pass * kRows + lane / kAcross) * kPitch + col) * 4);
+      const long long m = m0 + pass * kRows + lane / kAcross, at = m * g.N + n;
+      if (m >= g.M || live <= 0) continue;
+      float d[4] = {f.x, f.y, f.z, f.w};
+      if (g.part) {
+        float* to = g.part + (long long)split * g.M * g.N + at;
+        if (g.vec_f) *reinterpret_cast<float4*>(to) = f;
+        else
+#pragma unroll
+          for (int j = 0; j < 4; j++)
+            if (j < live) to[j] = d[j];
+        continue;
+      }
+      T* y = g.y ? static_cast<T*>(g.y) + m * g.ldy + n : nullptr;
+      float* sum = g.sum ? g.sum + at : nullptr;
+      if ((!sum || g.vec_f) && (!y || g.vec_y)) {
+        finish_grad<T, 4>(y, sum, g.begun, scale, d);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+          if (j < live) {
+            float one[1] = {d[j]};
+            finish_grad<T, 1>(y ? y + j : nullptr, sum ? sum + j : nullptr, g.begun, scale, one);
+          }
+      }
+    }
+  }
+  __device__ __forceinline__ void end(const Problem&, int) {}
+};
+
+// Partial sums added up in their order, and columns' sums in the last blocks.
+constexpr int kJoinThreads = 256;
+struct GradJoins {
+  struct Join {
+    const float* part;
+    float* sum;
+    void* y;
+    long long ldy, M, blocks;
+    int parts, N, begun, vec;
+  } j[2];
+  const float *a0, *a1;
+  float a2;
+  const float* sums;
+  void* gb;
+  long long sum_parts;
+  int sum_n;
+};
+
+template <class T, int V>
+__device__ __forceinline__ void join_grad(const GradJoins::Join& a, long long block, float scale, float (&t)[8][32][5]) {
+  const int lane = threadIdx.x % 32, group = threadIdx.x / 32;
+  const long long size = a.M * a.N, at = (block * 32 + lane) * V;
+  float d[V];
+#pragma unroll
+  for (int j = 0; j < V; j++) d[j] = 0;
+  if (at < size)
+#pragma unroll 4
+    for (int i = group; i < a.parts; i += 8) {
+      float v[V];
+      load_vec<float, V>(a.part + i * size + at, v);
+      add_all(d, d, v);
+    }
+#pragma unroll
+  for (int j = 0; j < V; j++) t[group][lane][j] = d[j];
+  __syncthreads();
+  if (group > 0 || at >= size) return;
+#pragma unroll
+  for (int j = 0; j < V; j++) {
+    d[j] = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) d[j] += t[i][lane][j];
+  }
+  const long long m = at / a.N, n = at - m * a.N;
+  finish_grad<T, V>(a.y ? static_cast<T*>(a.y) + m * a.ldy + n : nullptr, a.sum ? a.sum + at : nullptr, a.begun, scale, d);
+}
+
+template <class T>
+__global__ void __launch_bounds__(kJoinThreads) grad_join_kernel(const __grid_constant__ GradJoins a) {
+  __shared__ float t[8][32][5];
+  let_next_begin();
+  await_previous();
+  const float scale = scale_of(a.a0, a.a1, a.a2);
+  long long block = blockIdx.x;
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    if (block < a.j[i].blocks) {
+      if (a.j[i].vec) join_grad<T, 4>(a.j[i], block, scale, t);
+      else join_grad<T, 1>(a.j[i], block, scale, t);
+      return;
+    }
+    block -= a.j[i].blocks;
+  }
+  // eight columns, 32 threads for each
+  float* sums = &t[0][0][0];
+  const int lane = threadIdx.x % 8, group = threadIdx.x / 8;
+  const long long c = block * 8 + lane;
+  float s = 0;
+  if (c < a.sum_n)
+#pragma unroll 4
+    for (long long i = group; i < a.sum_parts; i += 32) s += a.sums[i * a.sum_n + c];
+  sums[threadIdx.x] = s;
+  __syncthreads();
+  if (group == 0 && c < a.sum_n) {
+    s = 0;
+#pragma unroll
+    for (int i = 0; i < 32; i++) s += sums[i * 8 + lane];
+    static_cast<T*>(a.gb)[c] = from_float<T>(s * scale);
+  }
+}
+
+// ---- host ---------------------------------------------------------------------------------------------------------------------
+
+// One product whose sums may not be split.
+template <template <class> class E, class Problem>
+int launch_whole(const char* fn, const Sizes& z, const Operand& x, const Operand& w, int type, const Problem& more, bool follows, cudaStream_t stream) {
+  const Plan plan = plan_of(&z, 1, type, true);
+  TcMaps maps;
+  TcArgs<Problem> a = {};
+  a.p[0] = more;
+  const int st = shape_of(fn, plan, plan.c[0], z, x, w, type, &a.p[0], &maps.a[0], &maps.b[0]);
+  if (st != GELIB_OK) return st;
+  a.items = a.p[0].items;
+  maps.a[1] = maps.a[0], maps.b[1] = maps.b[0];
+  finish_args(&a, plan, type);
+  if (type == GELIB_F32) return launch_config<E<float>, 3>(fn, plan.cg, maps, a, follows, stream);
+  if (type == GELIB_BF16) return launch_config<E<__nv_bfloat16>, 1>(fn, plan.cg, maps, a, follows, stream);
+  return launch_config<E<__half>, 1>(fn, plan.cg, maps, a, follows, stream);
+}
+
+Plan plan_for(const Grads& g, Sizes (&z)[kProblems]) {
+  for (int i = 0; i < g.count; i++) z[i] = {g.g[i].M, g.g[i].N, g.g[i].K};
+  return plan_of(z, g.count, g.type, false);
+}
+
+}  // namespace
+
+int forward_parts(long long M, int N, int K, int type) {
+  const Sizes z = {M, N, K};
+  const int bn = plan_of(&z, 1, type, true).c[0].bn;
+  return 2 * ((N + bn - 1) / bn);
+}
+
+int launch_forward_product(const char* fn, const ForwardProduct& p, bool follows, cudaStream_t stream) {
+  ForwardProblem g = {};
+  g.bias = p.bias, g.wide = is_aligned(p.bias, 16);
+  g.e = p.e, g.c = p.c, g.part = p.part, g.at_entry = p.at_entry;
+  return launch_whole<ForwardEnd>(fn, {p.M, p.N, p.K}, {p.x, false}, {p.w, p.w_by_sum}, p.type, g, follows, stream);
+}
+
+int launch_slope_product(const char* fn, const SlopeProduct& p, bool follows, cudaStream_t stream) {
+  SlopeProblem g = {};
+  g.bias = p.bias ? (const char*)p.bias + (long long)p.first * type_bytes(p.type) : nullptr;
+  g.wide = is_aligned(g.bias, 16);
+  g.e = p.e, g.c = p.c, g.up = p.up, g.lse = p.lse, g.gy = p.gy, g.most = p.most;
+  g.dz = const_cast<void*>(p.dz.base), g.ld = p.dz.ld, g.plane = p.dz.plane;
+  g.sums = p.sums, g.first = p.first;
+  return launch_whole<SlopeEnd>(fn, {p.M, p.N, p.K}, {p.x, false}, {p.w, p.w_by_sum}, p.type, g, follows, stream);
+}
+
+long long grads_workspace(const Grads& g) {
+  if (g.count == 0) return 0;
+  Sizes z[kProblems];
+  const Plan p = plan_for(g, z);
+  long long bytes = 0;
+  for (int i = 0; i < g.count; i++)
+    if (p.c[i].splits > 1) bytes += (p.c[i].splits * g.g[i].M * g.g[i].N * 4 + 255) / 256 * 256;
+  return bytes;
+}
+
+int launch_grads(const char* fn, const Grads& q, bool follows, void* workspace, cudaStream_t stream) {
+  GradJoins joins = {};
+  joins.a0 = q.a0, joins.a1 = q.a1, joins.a2 = q.a2;
+  int joined = 0;
+  if (q.count) {
+    Sizes z[kProblems];
+    const Plan plan = plan_for(q, z);
+    TcMaps maps;
+    TcArgs<GradProblem> a = {};
+    char* at = (char*)workspace;
+    const bool other = swapped(plan, z, q.count, q.type);
+    for (int i = 0; i < q.count; i++) {
+      const GradProduct& g = q.g[i];
+      const Config& c = plan.c[i];
+      const int k = other ? 1 - i : i;
+      GradProblem& p = a.p[k];
+      const int st = shape_of(fn, plan, c, z[i], g.a, g.b, q.type, &p, &maps.a[k], &maps.b[k]);
+      if (st != GELIB_OK) return st;
+      p.sum = g.sum, p.begun = !g.first, p.y = g.last ? g.y : nullptr, p.ldy = g.ldy;
+      p.a0 = q.a0, p.a1 = q.a1, p.a2 = q.a2;
+      p.vec_f = g.N % 4 == 0;
+      p.vec_y = g.N % 4 == 0 && g.ldy % 4 == 0 && is_aligned(g.y, 4 * type_bytes(q.type));
+      if (c.splits > 1) {
+        p.part = (float*)at;
+        at += (c.splits * g.M * g.N * 4 + 255) / 256 * 256;
+        GradJoins::Join& j = joins.j[joined++];
+        j = {p.part, g.sum, p.y, g.ldy, g.M, 0, c.splits, (int)g.N, p.begun, p.vec_f && (!p.y || p.vec_y)};
+        j.blocks = (g.M * g.N / (j.vec ? 4 : 1) + 31) / 32;
+      }
+      a.items += p.items;
+    }
+    if (q.count == 1) maps.a[1] = maps.a[0], maps.b[1] = maps.b[0];
+    finish_args(&a, plan, q.type);
+    const int st = q.type == GELIB_F32    ? launch_config<GradEnd<float>, 3>(fn, plan.cg, maps, a, follows, stream)
+                   : q.type == GELIB_BF16 ? launch_config<GradEnd<__nv_bfloat16>, 1>(fn, plan.cg, maps, a, follows, stream)
+                                          : launch_config<GradEnd<__half>, 1>(fn, plan.cg, maps, a, follows, stream);
+    if (st != GELIB_OK) return st;
+  }
+  long long blocks = joins.j[0].blocks + joins.j[1].blocks;
+  if (q.gb) {
+    joins.sums = q.sums, joins.gb = q.gb, joins.sum_parts = q.sum_parts, joins.sum_n = q.sum_n;
+    blocks += (q.sum_n + 7) / 8;
+  }
+  if (blocks == 0) return GELIB_OK;
+  if (blocks > 0x7fffffffLL) return fail(GELIB_INVALID, fn, "too many elements");
+  const auto kernel = q.type == GELIB_F32 ? grad_join_kernel<float> : q.type == GELIB_BF16 ? grad_join_kernel<__nv_bfloat16> : grad_join_kernel<__half>;
+  return launch_after(fn, true, kernel, dim3((unsigned)blocks), kJoinThreads, 0, stream, joins);
+}
+
+}  // namespace gelib_b200
