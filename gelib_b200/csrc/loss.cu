@@ -119,55 +119,77 @@ struct RowSum {
   double loss;
   long long count;
 };
-constexpr int kRows = 32, kGroups = kThreads / kRows;
+struct Total {
+  int reduction;
+  float *loss, *scale;
 
-// A block takes 32 rows; eight groups of lanes share a row's tiles, then a warp takes four rows' entries.
-__global__ void __launch_bounds__(kThreads) rows_kernel(Entries e, State s, const float2* part, const float* at_entry, int parts, long long M, float c, float temperature,
-                                                        int reduction, float* loss, RowSum* sums) {
-  __shared__ float2 of[kGroups][kRows];
-  __shared__ float losses[kRows];
-  __shared__ int counts[kRows];
+  __device__ __forceinline__ void put(const RowSum& all) const {
+    const double by = reduction == GELIB_LOSS_SUM ? 1.0 : all.count ? 1.0 / (double)all.count : 0.0;
+    *loss = (float)(all.loss * by);
+    *scale = (float)by;
+  }
+};
+constexpr int kRows = 32, kRowThreads = 32 * kRows, kBatch = 4;
+
+// A block takes 32 rows at a time: 32 warps share the rows' tiles, a row a lane, then every warp joins one row and adds up its entries.  What there is
+// is a few numbers a row, so that a handful of blocks waits for memory and little else: kBatch tiles are asked for at a time.
+__global__ void __launch_bounds__(kRowThreads) rows_kernel(Entries e, State s, const float2* part, const float* at_entry, int parts, long long M, float c, float temperature,
+                                                           Total total, RowSum* sums) {
+  __shared__ float2 of[kRows][kRows + 1];
+  __shared__ RowSum rows[kRows];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  const long long m0 = (long long)blockIdx.x * kRows, m = m0 + lane;
-  float2 v = {-INFINITY, 0.f};
+  RowSum mine = {0, 0};
   let_next_begin();
   await_previous();
-  if (m < M)
-    for (int i = warp; i < parts; i += kGroups) v = joined(v, part[(long long)i * M + m], c);
-  of[warp][lane] = v;
-  __syncthreads();
-  for (int r = warp; r < kRows; r += kGroups) {
-    const long long row = m0 + r;
-    if (row >= M) {
-      if (lane == 0) losses[r] = 0, counts[r] = 0;
-      continue;
+  for (long long m0 = (long long)blockIdx.x * kRows; m0 < M; m0 += (long long)gridDim.x * kRows) {
+    const long long m = m0 + lane, row = m0 + warp;
+    float2 v = {-INFINITY, 0.f};
+    if (m < M)
+      for (int i = warp; i < parts; i += 32 * kBatch) {
+        float2 w[kBatch];
+#pragma unroll
+        for (int j = 0; j < kBatch; j++) w[j] = i + 32 * j < parts ? part[(long long)(i + 32 * j) * M + m] : float2{-INFINITY, 0.f};
+#pragma unroll
+        for (int j = 0; j < kBatch; j++) v = joined(v, w[j], c);
+      }
+    of[warp][lane] = v;
+    __syncthreads();
+    v = of[lane][warp];
+    __syncthreads();
+#pragma unroll
+    for (int d = 16; d; d /= 2) {
+      const float2 w = {__shfl_xor_sync(0xffffffffu, v.x, d), __shfl_xor_sync(0xffffffffu, v.y, d)};
+      v = joined(v, w, c);
     }
-    float2 sum = of[0][r];
-    for (int i = 1; i < kGroups; i++) sum = joined(sum, of[i][r], c);
+    if (row >= M) continue;
     const int t = first_class(e, row);
     float d = 0;
     for (int k = lane; k < e.top; k += 32) {
       if (t == kInvalid || (k == 0 ? t : e.ids[row * e.top + k]) == kNone) continue;
-      const float q = e.q ? e.q[row * e.top + k] : 1.f, to = (sum.x - at_entry[row * e.top + k]) / temperature;
+      const float q = e.q ? e.q[row * e.top + k] : 1.f, to = (v.x - at_entry[row * e.top + k]) / temperature;
       d += q == 1.f ? to : q * (logf(q) + to);
     }
 #pragma unroll
     for (int i = 16; i; i /= 2) d += __shfl_xor_sync(0xffffffffu, d, i);
-    if (lane) continue;
-    d = t == kNone ? 0.f : t == kInvalid ? NAN : temperature * temperature * (d + logf(sum.y));
-    // a row of -infinity alone has no softmax
-    s.lse[row] = {sum.x, t == kNone ? INFINITY : t == kInvalid || sum.x == -INFINITY ? NAN : log2f(sum.y)};
-    if (reduction == GELIB_LOSS_NONE) loss[row] = d;
-    losses[r] = d, counts[r] = t != kNone;
+    d = t == kNone ? 0.f : t == kInvalid ? NAN : temperature * temperature * (d + logf(v.y));
+    if (lane == 0) {
+      // a row of -infinity alone has no softmax
+      s.lse[row] = {v.x, t == kNone ? INFINITY : t == kInvalid || v.x == -INFINITY ? NAN : log2f(v.y)};
+      if (total.reduction == GELIB_LOSS_NONE) total.loss[row] = d;
+    }
+    mine.loss += d, mine.count += t != kNone;
   }
+  if (total.reduction == GELIB_LOSS_NONE) return;
+  if (lane == 0) rows[warp] = mine;
   __syncthreads();
-  if (reduction == GELIB_LOSS_NONE || threadIdx.x) return;
+  if (threadIdx.x) return;
   RowSum all = {0, 0};
-  for (int r = 0; r < kRows; r++) all.loss += losses[r], all.count += counts[r];
-  sums[blockIdx.x] = all;
+  for (int r = 0; r < kRows; r++) all.loss += rows[r].loss, all.count += rows[r].count;
+  if (gridDim.x == 1) total.put(all);
+  else sums[blockIdx.x] = all;
 }
 
-__global__ void __launch_bounds__(kThreads) total_kernel(const RowSum* sums, int parts, int reduction, float* loss, float* scale) {
+__global__ void __launch_bounds__(kThreads) total_kernel(const RowSum* sums, int parts, Total total) {
   __shared__ RowSum of[kThreads];
   RowSum v = {0, 0};
   await_previous();
@@ -178,10 +200,7 @@ __global__ void __launch_bounds__(kThreads) total_kernel(const RowSum* sums, int
     if (threadIdx.x < d) of[threadIdx.x].loss += of[threadIdx.x + d].loss, of[threadIdx.x].count += of[threadIdx.x + d].count;
     __syncthreads();
   }
-  if (threadIdx.x) return;
-  const double by = reduction == GELIB_LOSS_SUM ? 1.0 : of[0].count ? 1.0 / (double)of[0].count : 0.0;
-  *loss = (float)(of[0].loss * by);
-  *scale = (float)by;
+  if (threadIdx.x == 0) total.put(of[0]);
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------------
@@ -209,6 +228,9 @@ int piece_of(const gelib_linear_loss_args& p) {
 
 long long groups_of(long long m) { return (m + 31) / 32; }
 
+// Blocks of rows: one for a few rows, which then adds them all up without another launch.
+int row_blocks(long long m) { return m <= 4 * kRows ? 1 : (int)std::min<long long>((m + kRows - 1) / kRows, 148 * 2); }
+
 int forward(const gelib_linear_loss_args& p, char* at, cudaStream_t stream) {
   static const char* fn = "linear_loss";
   const State s = state_of(p);
@@ -227,14 +249,15 @@ int forward(const gelib_linear_loss_args& p, char* at, cudaStream_t stream) {
   copy_if_needed(&f.x, p.type, at, &jobs);
   copy_if_needed(&f.w, p.type, at, &jobs);
   if ((st = launch_copies(fn, jobs, nullptr, p.type, stream)) != GELIB_OK) return st;
-  const int parts = forward_parts(p.m, p.n, p.k, p.type), blocks = (int)((p.m + kRows - 1) / kRows);
+  const int parts = forward_parts(p.m, p.n, p.k, p.type), blocks = row_blocks(p.m);
   f.part = (float2*)at, at += up(8LL * parts * p.m);
   f.at_entry = (float*)at, at += up(4 * p.m * p.top);
   if ((st = launch_forward_product(fn, f, jobs.count > 0, stream)) != GELIB_OK) return st;
-  st = launch_after(fn, true, rows_kernel, dim3(blocks), kThreads, 0, stream, e, s, (const float2*)f.part, (const float*)f.at_entry, parts, (long long)p.m, c, temperature_of(p),
-                    p.reduction, (float*)p.loss, (RowSum*)at);
-  if (st != GELIB_OK || p.reduction == GELIB_LOSS_NONE) return st;
-  return launch_after(fn, true, total_kernel, dim3(1), kThreads, 0, stream, (const RowSum*)at, blocks, p.reduction, (float*)p.loss, s.scale);
+  const Total total = {p.reduction, (float*)p.loss, s.scale};
+  st = launch_after(fn, true, rows_kernel, dim3(blocks), kRowThreads, 0, stream, e, s, (const float2*)f.part, (const float*)f.at_entry, parts, (long long)p.m, c,
+                    temperature_of(p), total, (RowSum*)at);
+  if (st != GELIB_OK || p.reduction == GELIB_LOSS_NONE || blocks == 1) return st;
+  return launch_after(fn, true, total_kernel, dim3(1), kThreads, 0, stream, (const RowSum*)at, blocks, total);
 }
 
 // What a backward call does with a piece of `width` classes from `first` on; addresses in the workspace where `at` is one.
@@ -332,7 +355,7 @@ long long linear_loss_state_bytes(const gelib_linear_loss_args& p) { return 256 
 long long linear_loss_workspace(const gelib_linear_loss_args& p, bool backward) {
   if (backward) return p.gx || p.gw || p.gb ? room_of(p, nullptr).bytes : 0;
   return copy_bytes(x_of(p), p.type) + copy_bytes(w_of(p), p.type) + up(8LL * forward_parts(p.m, p.n, p.k, p.type) * p.m) + up(4 * p.m * p.top) +
-         up((p.m + kRows - 1) / kRows * (long long)sizeof(RowSum));
+         up(row_blocks(p.m) * (long long)sizeof(RowSum));
 }
 
 int launch_linear_loss(const gelib_linear_loss_args& p, void* workspace, cudaStream_t stream) {
