@@ -211,7 +211,7 @@ constexpr int kLongSum = 2048;   // slabs
 
 // The tiles and splits of a launch's products with the least estimated time.
 Plan choose_plan(const Sizes* z, int count, int type, bool whole) {
-  Plan best = {1, 0, {{128, 1}, {128, 1}}};
+  Plan best = {1, 0, 0, {{128, 1}, {128, 1}}};
   double best_time = 1e30;
   for (int cg = 1; cg <= 2; cg++) {
     const int slots = kSms / cg;
@@ -239,20 +239,20 @@ Plan choose_plan(const Sizes* z, int count, int type, bool whole) {
       Work w[kProblems] = {work_of(z[0], cg, c0, type), {}};
       if (count == 1) {
         const double t = launch_time(w, 1, slots);
-        if (t < best_time) best_time = t, best = {cg, 0, {c0, c0}};
+        if (t < best_time) best_time = t, best = {cg, 0, 0, {c0, c0}};
         continue;
       }
       for (const Config& c1 : may[1]) {
         w[1] = work_of(z[1], cg, c1, type);
         const double t = launch_time(w, 2, slots);
-        if (t < best_time) best_time = t, best = {cg, 0, {c0, c1}};
+        if (t < best_time) best_time = t, best = {cg, 0, 0, {c0, c1}};
       }
     }
   }
-  if (count == 2) {   // whether handing every other round out backwards evens the blocks' times out
+  if (count == 2) {   // the way of handing items out that evens the blocks' times out: as they come, every other round backwards, or the longer ones' last round first
     Work w[kProblems] = {work_of(z[0], best.cg, best.c[0], type), work_of(z[1], best.cg, best.c[1], type)};
     if (w[1].each > w[0].each) std::swap(w[0], w[1]);
-    const int slots = kSms / best.cg;
+    const int slots = kSms / best.cg, longer = (int)w[0].items % slots;
     const double items = w[0].items + w[1].items;
     if (items <= 16.0 * slots) {
       double most[2] = {0, 0};
@@ -266,6 +266,14 @@ Plan choose_plan(const Sizes* z, int count, int type, bool whole) {
         }
       }
       best.flip = most[1] < most[0];
+      best_time = std::min(most[0], most[1]);
+    } else {
+      best_time = std::ceil(w[0].items / slots) * w[0].each + std::ceil((items - slots * std::ceil(w[0].items / slots)) / slots) * w[1].each;
+    }
+    const int lead = (int)(w[0].each / w[1].each + 0.5), spare = slots - longer;
+    if (longer > 0 && lead > 0 && w[1].items > (double)lead * spare) {
+      const double time = std::ceil(w[0].items / slots) * w[0].each + std::ceil((w[1].items - (double)lead * spare) / slots) * w[1].each;
+      if (time < 0.97 * best_time) best.flip = 0, best.lead = lead;
     }
   }
   return best;

@@ -39,7 +39,7 @@ struct Config {
   int bn, splits;
 };
 struct Plan {
-  int cg, flip;
+  int cg, flip, lead;
   Config c[kProblems];
 };
 struct Sizes {
@@ -75,6 +75,7 @@ struct TcArgs {
   Problem p[kProblems];               // those with longer items first
   int items;                          // of all
   int flip;                           // every other round of items is handed out from the last block on
+  int lead;                           // not 0: so many of the second product's items go to each block that has one of the first's less, before the others get any
   int* status;
   int limit;                          // of the first waits: kWaitLimit, or 0 where a test makes them run out
   int bf16;
@@ -197,11 +198,19 @@ struct Walk {
   int round, at, which;
   template <class Args>
   __device__ __forceinline__ bool next(const Args& a, int mine, int blocks) {
-    at = round * blocks + (a.flip && (round & 1) ? blocks - 1 - mine : mine);
+    const int first = a.p[0].items;
+    if (a.lead == 0) {
+      at = round * blocks + (a.flip && (round & 1) ? blocks - 1 - mine : mine);
+    } else {
+      const int whole = first / blocks, more = first - whole * blocks, r = round - whole - (mine < more);   // r: number of the block's item of the second
+      if (r < 0) at = round * blocks + mine;
+      else if (mine >= more && r < a.lead) at = first + r * (blocks - more) + mine - more;
+      else at = first + a.lead * (blocks - more) + (mine >= more ? r - a.lead : r) * blocks + mine;
+    }
     round++;
     if (at >= a.items) return false;
-    which = at >= a.p[0].items;
-    if (which) at -= a.p[0].items;
+    which = at >= first;
+    if (which) at -= first;
     return true;
   }
 };
@@ -488,7 +497,7 @@ inline int shape_of(const char* fn, const Plan& plan, const Config& c, const Siz
 }
 template <class Args>
 void finish_args(Args* a, const Plan& plan, int type) {
-  a->flip = plan.flip;
+  a->flip = plan.flip, a->lead = plan.lead;
   a->status = async_status_word(kStatusGemmTc);
   a->limit = inject_timeout() ? 0 : kWaitLimit;
   a->bf16 = type != GELIB_F16;

@@ -231,6 +231,15 @@ long long groups_of(long long m) { return (m + 31) / 32; }
 // Blocks of rows: one for a few rows, which then adds them all up without another launch.
 int row_blocks(long long m) { return m <= 4 * kRows ? 1 : (int)std::min<long long>((m + kRows - 1) / kRows, 148 * 2); }
 
+ForwardProduct forward_of(const gelib_linear_loss_args& p) {
+  return {x_of(p), w_of(p), !p.w_transposed, p.bias, p.m, p.n, p.k, p.type, entries_of(p, state_of(p)), slope_of(p), nullptr, nullptr};
+}
+// Partial sums of a row.
+int parts_of(const gelib_linear_loss_args& p) {
+  const ForwardProduct f = forward_of(p);
+  return takes_few(f) ? few_parts(f) : forward_parts(p.m, p.n, p.k, p.type);
+}
+
 int forward(const gelib_linear_loss_args& p, char* at, cudaStream_t stream) {
   static const char* fn = "linear_loss";
   const State s = state_of(p);
@@ -244,15 +253,18 @@ int forward(const gelib_linear_loss_args& p, char* at, cudaStream_t stream) {
     else teacher_kernel<<<blocks, 128, 0, stream>>>(s, e, (const __half*)p.teacher, p.m, c);
     if ((st = launched(fn)) != GELIB_OK) return st;
   }
-  ForwardProduct f = {x_of(p), w_of(p), !p.w_transposed, p.bias, p.m, p.n, p.k, p.type, e, c};
+  ForwardProduct f = forward_of(p);
+  const bool few = takes_few(f);
   PlaneJobs jobs = {};
-  copy_if_needed(&f.x, p.type, at, &jobs);
-  copy_if_needed(&f.w, p.type, at, &jobs);
-  if ((st = launch_copies(fn, jobs, nullptr, p.type, stream)) != GELIB_OK) return st;
-  const int parts = forward_parts(p.m, p.n, p.k, p.type), blocks = row_blocks(p.m);
+  if (!few) {
+    copy_if_needed(&f.x, p.type, at, &jobs);
+    copy_if_needed(&f.w, p.type, at, &jobs);
+    if ((st = launch_copies(fn, jobs, nullptr, p.type, stream)) != GELIB_OK) return st;
+  }
+  const int parts = parts_of(p), blocks = row_blocks(p.m);
   f.part = (float2*)at, at += up(8LL * parts * p.m);
   f.at_entry = (float*)at, at += up(4 * p.m * p.top);
-  if ((st = launch_forward_product(fn, f, jobs.count > 0, stream)) != GELIB_OK) return st;
+  if ((st = few ? launch_few(fn, f, false, stream) : launch_forward_product(fn, f, jobs.count > 0, stream)) != GELIB_OK) return st;
   const Total total = {p.reduction, (float*)p.loss, s.scale};
   st = launch_after(fn, true, rows_kernel, dim3(blocks), kRowThreads, 0, stream, e, s, (const float2*)f.part, (const float*)f.at_entry, parts, (long long)p.m, c,
                     temperature_of(p), total, (RowSum*)at);
@@ -354,7 +366,8 @@ long long linear_loss_state_bytes(const gelib_linear_loss_args& p) { return 256 
 
 long long linear_loss_workspace(const gelib_linear_loss_args& p, bool backward) {
   if (backward) return p.gx || p.gw || p.gb ? room_of(p, nullptr).bytes : 0;
-  return copy_bytes(x_of(p), p.type) + copy_bytes(w_of(p), p.type) + up(8LL * forward_parts(p.m, p.n, p.k, p.type) * p.m) + up(4 * p.m * p.top) +
+  const long long copies = takes_few(forward_of(p)) ? 0 : copy_bytes(x_of(p), p.type) + copy_bytes(w_of(p), p.type);
+  return copies + up(8LL * parts_of(p) * p.m) + up(4 * p.m * p.top) +
          up(row_blocks(p.m) * (long long)sizeof(RowSum));
 }
 

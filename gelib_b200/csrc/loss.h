@@ -44,6 +44,11 @@ struct ForwardProduct {
 int forward_parts(long long M, int N, int K, int type);
 int launch_forward_product(const char* fn, const ForwardProduct& p, bool follows, cudaStream_t stream);
 
+// The same for a few rows (loss_rows.cu), of x and w as the caller has them.
+bool takes_few(const ForwardProduct& p);
+int few_parts(const ForwardProduct& p);
+int launch_few(const char* fn, const ForwardProduct& p, bool follows, cudaStream_t stream);
+
 // z again, of the N classes from `first` on, and of it dz = up g (p - q), which the tensor cores take: 16-bit, or three planes.
 struct SlopeProduct {
   Stored x, w;          // w: of these classes
@@ -103,28 +108,39 @@ __device__ __forceinline__ float2 joined(float2 a, float2 b, float c) {
   return {top, a.y * exp2_of(c * (a.x - from)) + b.y * exp2_of(c * (b.x - from))};
 }
 
-// A row's classes from some column on, in ascending order.
+// A row's classes from some column on, in ascending order, with their shares.  The one after the next is asked for when the next is, so that nobody
+// waits for it unless two are close together.
 struct Next {
-  int cls;   // the next one, or kNone
-  int at;    // its place
+  int cls, after;     // or kNone
+  float q, q_after;
+  int at;             // the next one's place
 
+  __device__ __forceinline__ void look(const Entries& e, long long row, int place, int& c, float& share) {
+    const bool there = place < e.top;
+    c = there ? e.ids[row * e.top + place] : kNone;
+    share = there ? e.q[row * e.top + place] : 0.f;
+  }
   __device__ __forceinline__ void begin(const Entries& e, long long row, bool live, int from) {
-    at = 0;
+    at = 0, q = 1.f, after = kNone, q_after = 0.f;
     cls = live ? first_class(e, row) : kNone;
     if (cls == kInvalid) cls = kNone;
-    if (e.top == 1 || cls >= from) return;
-    int high = e.top;   // the first place whose class is not below `from`: in (at, high]
-    while (high - at > 1) {
-      const int mid = (at + high) / 2;
-      if (e.ids[row * e.top + mid] < from) at = mid;
-      else high = mid;
+    if (!e.ids || cls == kNone) return;
+    if (cls < from) {
+      int high = e.top;   // the first place whose class is not below `from`: in (at, high]
+      while (high - at > 1) {
+        const int mid = (at + high) / 2;
+        if (e.ids[row * e.top + mid] < from) at = mid;
+        else high = mid;
+      }
+      at = high;
     }
-    at = high;
-    cls = at < e.top ? e.ids[row * e.top + at] : kNone;
+    look(e, row, at, cls, q);
+    look(e, row, at + 1, after, q_after);
   }
   __device__ __forceinline__ void advance(const Entries& e, long long row) {
     at++;
-    cls = at < e.top ? e.ids[row * e.top + at] : kNone;
+    cls = after, q = q_after;
+    if (cls != kNone) look(e, row, at + 1, after, q_after);
   }
 };
 #endif

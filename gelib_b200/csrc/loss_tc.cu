@@ -154,7 +154,7 @@ struct SlopeEnd {
     const int cls = g.first + n;
     while (next.cls < cls + kChunk) {
       const long long row = m0 + lane;
-      if (next.cls >= cls) take_from_shared(block + (lane * kPitch + next.cls - cls) * 4, g_up * (g.e.q ? g.e.q[row * g.e.top + next.at] : 1.f));
+      if (next.cls >= cls) take_from_shared(block + (lane * kPitch + next.cls - cls) * 4, g_up * next.q);
       next.advance(g.e, row);
     }
     __syncwarp();
