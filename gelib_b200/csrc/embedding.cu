@@ -4,6 +4,7 @@
 //
 // Both are bound by memory: forward reads the rows that are met and writes y, backward reads gy and writes all of gw.
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <initializer_list>
 #include <type_traits>
@@ -61,16 +62,20 @@ __global__ void __launch_bounds__(kThreads) embedding_kernel(const EmbeddingCall
 
 // ---- the numbers in order -----------------------------------------------------------------------------------------------------
 //
-// Stable radix passes, least significant digit first: a block counts the digits of its stretch of the numbers, the next launch has every block add up what
-// others have of each digit, and place its own.  Within a block a warp ranks 32 numbers at a time by the lanes that have the same digit, so
-// that equal numbers keep their order whatever the timing.  Few numbers are sorted by one block, all passes in one launch.
+// Stable radix passes, least significant digit first.  A block ranks a tile of numbers, a warp 32 of them at a time by the lanes that have the same digit, so
+// that equal numbers keep their order whatever the timing; puts them in order in shared memory, and writes runs of equal digits: written as they
+// come, 65536 numbers on eight SMs took 22 us a pass, a line of the cache for every number.  Where a block's runs go follows from what all blocks have of each
+// digit.  Up to 65536 numbers are sorted by the blocks of one cluster, all passes in one launch, which tell each other through shared memory; for more there
+// is a launch that counts before each that places.
 
-constexpr int kSortThreads = 512, kSortWarps = kSortThreads / 32;
-constexpr int kEach = 8;                              // numbers of a lane
+constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
+constexpr int kEach = 8;                              // numbers of a thread
 constexpr int kTile = kSortThreads * kEach;           // of a block at a time
-constexpr int kMaxBits = 10;
-constexpr int kOneBlock = 2 * kTile;                  // numbers that one block sorts
+constexpr int kMaxBits = 10;                          // of a digit, a thread each
+constexpr int kClusterMost = 8;
+constexpr int kClusterNumbers = kClusterMost * kTile; // that a cluster sorts
 constexpr int kSortBlocks = 148;                      // at most, otherwise
+static_assert(1 << kMaxBits == kSortThreads, "a thread owns a digit");
 
 struct Sort {
   const void* ids;          // of the first pass
@@ -80,165 +85,198 @@ struct Sort {
   long long n, padding, per;   // per: numbers of a block
   int index_bytes, v, passes, bits, blocks;
 };
-// What does not count has the number v, behind all rows.
+__device__ __forceinline__ unsigned* of_pass(unsigned* const (&two)[2], int pass) { return pass & 1 ? two[1] : two[0]; }
+// What does not count has the number v, behind all rows.  What other blocks of a cluster have put down the first cache knows nothing of.
 __device__ __forceinline__ unsigned key_of(const Sort& s, int pass, long long i) {
-  if (pass > 0) return s.keys[(pass - 1) & 1][i];
+  if (pass > 0) return __ldcg(of_pass(s.keys, pass - 1) + i);
   const long long id = index_at(s.ids, i, s.index_bytes);
   return id < 0 || id >= s.v || id == s.padding ? (unsigned)s.v : (unsigned)id;
 }
 
 struct SortShared {
   unsigned short rank[kSortWarps][1 << kMaxBits];
-  int base[1 << kMaxBits];
+  unsigned key[kTile], place[kTile];
+  int start[1 << kMaxBits], to[1 << kMaxBits];   // of a digit: its first place in the tile, and how far from there it goes
+  int counts[kClusterMost][1 << kMaxBits];       // of every block of a cluster
   int warp_sum[kSortWarps];
 };
 
-// sh.base becomes, of every digit, how many numbers have a lower one.
-__device__ __forceinline__ void scan_digits(SortShared& sh, int digits) {
-  const int t = threadIdx.x, lane = t % 32;
-  const int a = 2 * t < digits ? sh.base[2 * t] : 0, b = 2 * t + 1 < digits ? sh.base[2 * t + 1] : 0;
-  int sum = a + b;
+// The lanes that are live and have this digit.
+__device__ __forceinline__ unsigned lanes_with(unsigned digit, bool live, int bits) {
+  unsigned same = __ballot_sync(0xffffffffu, live);
+#pragma unroll
+  for (int b = 0; b < kMaxBits; b++)
+    if (b < bits) {
+      const unsigned set = __ballot_sync(0xffffffffu, digit >> b & 1);
+      same &= digit >> b & 1 ? set : ~set;
+    }
+  return same;
+}
+
+// The sum of the v of lower threads.
+__device__ __forceinline__ int sum_of_lower(SortShared& sh, int v) {
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  int sum = v;
 #pragma unroll
   for (int d = 1; d < 32; d *= 2) {
     const int o = __shfl_up_sync(0xffffffffu, sum, d);
     if (lane >= d) sum += o;
   }
-  if (lane == 31) sh.warp_sum[t / 32] = sum;
+  if (lane == 31) sh.warp_sum[warp] = sum;
   __syncthreads();
-  int before = sum - a - b;
-  for (int w = 0; w < t / 32; w++) before += sh.warp_sum[w];
-  if (2 * t < digits) sh.base[2 * t] = before;
-  if (2 * t + 1 < digits) sh.base[2 * t + 1] = before + a;
+  int lower = lane < warp ? sh.warp_sum[lane] : 0;
+#pragma unroll
+  for (int d = 16; d; d /= 2) lower += __shfl_xor_sync(0xffffffffu, lower, d);
   __syncthreads();
+  return lower + sum - v;
 }
 
-__device__ __forceinline__ void count_digits(const Sort& s, int pass, long long i0, long long i1, int* hist) {
-  const int digits = 1 << s.bits, shift = pass * s.bits;
-  for (int d = threadIdx.x; d < digits; d += kSortThreads) hist[d] = 0;
-  __syncthreads();
-  for (long long i = i0 + threadIdx.x; i < i1; i += kSortThreads) atomicAdd(&hist[key_of(s, pass, i) >> shift & (digits - 1)], 1);
-  __syncthreads();
-}
-
-// Numbers i0 to i1 to their places; sh.base says where the next one of every digit goes.
-__device__ __forceinline__ void place_digits(const Sort& s, int pass, long long i0, long long i1, SortShared& sh) {
-  const int digits = 1 << s.bits, shift = pass * s.bits, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  unsigned *keys = s.keys[pass & 1], *places = s.places[pass & 1];
-  const unsigned* from = s.places[(pass - 1) & 1];
-  for (long long t0 = i0; t0 < i1; t0 += kTile) {
-    for (int d = threadIdx.x; d < kSortWarps * digits / 2; d += kSortThreads) {
-      const int w = d / (digits / 2), at = d % (digits / 2);
-      reinterpret_cast<unsigned*>(sh.rank[w])[at] = 0;
-    }
-    __syncthreads();
-    unsigned key[kEach], place[kEach], rank[kEach];
+// Numbers i0 to i1 of a pass, in a thread's registers.
+struct Tile {
+  unsigned key[kEach], place[kEach], rank[kEach];   // rank: among the warp's with the same digit
+};
+// Returns how many of the tile have the thread's digit.
+__device__ __forceinline__ int rank_tile(const Sort& s, int pass, long long i0, int count, SortShared& sh, Tile& t) {
+  const int digits = 1 << s.bits, shift = pass * s.bits, warp = threadIdx.x / 32, lane = threadIdx.x % 32, each = (count + kSortThreads - 1) / kSortThreads;
+  for (int d = lane; d < digits / 2; d += 32) reinterpret_cast<unsigned*>(sh.rank[warp])[d] = 0;
+  __syncwarp();
 #pragma unroll
-    for (int r = 0; r < kEach; r++) {
-      const long long i = t0 + (warp * kEach + r) * 32 + lane;
-      key[r] = i < i1 ? key_of(s, pass, i) : 0;
-      place[r] = i < i1 ? (pass > 0 ? from[i] : (unsigned)i) : 0;
+  for (int r = 0; r < kEach; r++) {
+    const int i = (warp * each + r) * 32 + lane;
+    t.key[r] = t.place[r] = t.rank[r] = 0;
+    if (r < each && i < count) {
+      t.key[r] = key_of(s, pass, i0 + i);
+      t.place[r] = pass > 0 ? __ldcg(of_pass(s.places, pass - 1) + i0 + i) : (unsigned)(i0 + i);
     }
-#pragma unroll
-    for (int r = 0; r < kEach; r++) {
-      const bool live = t0 + (warp * kEach + r) * 32 + lane < i1;
-      const unsigned digit = key[r] >> shift & (digits - 1);
-      unsigned same = __ballot_sync(0xffffffffu, live);   // the lanes that have this digit
-#pragma unroll
-      for (int b = 0; b < kMaxBits; b++)
-        if (b < s.bits) {
-          const unsigned set = __ballot_sync(0xffffffffu, digit >> b & 1);
-          same &= digit >> b & 1 ? set : ~set;
-        }
-      const unsigned short before = live ? sh.rank[warp][digit] : 0;
-      rank[r] = before + __popc(same & ((1u << lane) - 1));
-      __syncwarp();
-      if (live && lane == __ffs(same) - 1) sh.rank[warp][digit] = before + (unsigned short)__popc(same);
-      __syncwarp();
-    }
-    __syncthreads();
-    // over the warps: where each one's begin, and how many there are in all
-    int total[(1 << kMaxBits) / kSortThreads];
-#pragma unroll
-    for (int k = 0; k < (1 << kMaxBits) / kSortThreads; k++) {
-      const int d = threadIdx.x + k * kSortThreads;
-      int sum = 0;
-      if (d < digits)
-        for (int w = 0; w < kSortWarps; w++) {
-          const int c = sh.rank[w][d];
-          sh.rank[w][d] = (unsigned short)sum;
-          sum += c;
-        }
-      total[k] = sum;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int r = 0; r < kEach; r++) {
-      if (t0 + (warp * kEach + r) * 32 + lane >= i1) continue;
-      const unsigned digit = key[r] >> shift & (digits - 1);
-      const int to = sh.base[digit] + sh.rank[warp][digit] + rank[r];
-      keys[to] = key[r], places[to] = place[r];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < (1 << kMaxBits) / kSortThreads; k++) {
-      const int d = threadIdx.x + k * kSortThreads;
-      if (d < digits) sh.base[d] += total[k];
-    }
-    __syncthreads();
   }
+#pragma unroll
+  for (int r = 0; r < kEach; r++)
+    if (r < each) {
+      const bool live = (warp * each + r) * 32 + lane < count;
+      const unsigned digit = t.key[r] >> shift & (digits - 1), same = lanes_with(digit, live, s.bits);
+      const int before = live ? sh.rank[warp][digit] : 0;
+      t.rank[r] = before + __popc(same & ((1u << lane) - 1));
+      __syncwarp();
+      if (live && lane == __ffs(same) - 1) sh.rank[warp][digit] = (unsigned short)(before + __popc(same));
+      __syncwarp();
+    }
+  __syncthreads();
+  int sum = 0;
+  if ((int)threadIdx.x < digits) {   // over the warps: where each one's begin
+#pragma unroll
+    for (int w0 = 0; w0 < kSortWarps; w0 += 8) {
+      int c[8];
+#pragma unroll
+      for (int w = 0; w < 8; w++) c[w] = sh.rank[w0 + w][threadIdx.x];
+#pragma unroll
+      for (int w = 0; w < 8; w++) {
+        sh.rank[w0 + w][threadIdx.x] = (unsigned short)sum;
+        sum += c[w];
+      }
+    }
+  }
+  return sum;
 }
 
-__global__ void __launch_bounds__(kSortThreads) sort_kernel(const Sort s) {
-  __shared__ SortShared sh;
+// The tile to its places; `sum` as above, `base`: where the first of the thread's digit goes.
+__device__ __forceinline__ void place_tile(const Sort& s, int pass, int count, int sum, int base, SortShared& sh, const Tile& t) {
+  const int digits = 1 << s.bits, shift = pass * s.bits, warp = threadIdx.x / 32, lane = threadIdx.x % 32, each = (count + kSortThreads - 1) / kSortThreads;
+  const int start = sum_of_lower(sh, sum);
+  sh.start[threadIdx.x] = start, sh.to[threadIdx.x] = base - start;
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < kEach; r++)
+    if (r < each && (warp * each + r) * 32 + lane < count) {
+      const unsigned digit = t.key[r] >> shift & (digits - 1);
+      const int at = sh.start[digit] + sh.rank[warp][digit] + t.rank[r];
+      sh.key[at] = t.key[r], sh.place[at] = t.place[r];
+    }
+  __syncthreads();
+  unsigned *keys = of_pass(s.keys, pass), *places = of_pass(s.places, pass);
+  for (int i = threadIdx.x; i < count; i += kSortThreads) {
+    const unsigned key = sh.key[i];
+    const int to = sh.to[key >> shift & (digits - 1)] + i;
+    keys[to] = key, places[to] = sh.place[i];
+  }
+  __syncthreads();
+}
+
+__device__ __forceinline__ uint32_t at_rank(uint32_t local, uint32_t rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(local), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+__global__ void __launch_bounds__(kSortThreads) cluster_sort_kernel(const Sort s) {   // the cluster is the grid
+  extern __shared__ __align__(16) unsigned char raw[];
+  SortShared& sh = *reinterpret_cast<SortShared*>(raw);
+  const int blocks = gridDim.x, block = blockIdx.x, digit = threadIdx.x, digits = 1 << s.bits;
+  const long long i0 = min(s.n, block * s.per);
+  const int count = (int)(min(s.n, i0 + s.per) - i0);
   let_next_begin();
-  if (threadIdx.x == 0) *s.heads = 0;
+  if (block == 0 && threadIdx.x == 0) *s.heads = 0;
+  cluster_sync();   // all blocks are there
   for (int pass = 0; pass < s.passes; pass++) {
-    count_digits(s, pass, 0, s.n, sh.base);
-    scan_digits(sh, 1 << s.bits);
-    place_digits(s, pass, 0, s.n, sh);
+    Tile t;
+    const int sum = rank_tile(s, pass, i0, count, sh, t);
+    if (digit < digits) {
+      const uint32_t mine = (uint32_t)__cvta_generic_to_shared(&sh.counts[block][digit]);
+      for (int b = 0; b < blocks; b++) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at_rank(mine, b)), "r"(sum) : "memory");
+    }
+    cluster_sync();
+    int before = 0, all = 0;
+    if (digit < digits)
+      for (int b = 0; b < blocks; b++) {
+        const int c = sh.counts[b][digit];
+        before += b < block ? c : 0;
+        all += c;
+      }
+    place_tile(s, pass, count, sum, sum_of_lower(sh, all) + before, sh, t);
+    __threadfence();
+    cluster_sync();
   }
 }
 
 __global__ void __launch_bounds__(kSortThreads) count_kernel(const Sort s, int pass) {
   __shared__ int hist[1 << kMaxBits];
+  const int digits = 1 << s.bits, shift = pass * s.bits;
   let_next_begin();
   await_previous();
   if (pass == 0 && blockIdx.x == 0 && threadIdx.x == 0) *s.heads = 0;
-  const long long i0 = blockIdx.x * s.per;
-  count_digits(s, pass, i0, min(s.n, i0 + s.per), hist);
-  for (int d = threadIdx.x; d < 1 << s.bits; d += kSortThreads) s.counts[(blockIdx.x << s.bits) + d] = hist[d];
+  hist[threadIdx.x] = 0;
+  __syncthreads();
+  const long long i0 = blockIdx.x * s.per, i1 = min(s.n, i0 + s.per);
+  for (long long i = i0 + threadIdx.x; i < i1; i += kSortThreads) atomicAdd(&hist[key_of(s, pass, i) >> shift & (digits - 1)], 1);
+  __syncthreads();
+  if ((int)threadIdx.x < digits) s.counts[(blockIdx.x << s.bits) + threadIdx.x] = hist[threadIdx.x];
 }
 
 __global__ void __launch_bounds__(kSortThreads) place_kernel(const Sort s, int pass) {
-  __shared__ SortShared sh;
-  const int digits = 1 << s.bits;
+  extern __shared__ __align__(16) unsigned char raw[];
+  SortShared& sh = *reinterpret_cast<SortShared*>(raw);
+  const int digit = threadIdx.x;
   let_next_begin();
   await_previous();
-  int before[(1 << kMaxBits) / kSortThreads];
-#pragma unroll
-  for (int k = 0; k < (1 << kMaxBits) / kSortThreads; k++) {
-    const int d = threadIdx.x + k * kSortThreads;
-    int mine = 0, all = 0;
-    if (d < digits)
+  int before = 0, all = 0;
+  if (digit < 1 << s.bits)
 #pragma unroll 8
-      for (int b = 0; b < s.blocks; b++) {
-        const int c = s.counts[(b << s.bits) + d];
-        mine += b < (int)blockIdx.x ? c : 0;
-        all += c;
-      }
-    before[k] = mine;
-    if (d < digits) sh.base[d] = all;
+    for (int b = 0; b < s.blocks; b++) {
+      const int c = s.counts[(b << s.bits) + digit];
+      before += b < (int)blockIdx.x ? c : 0;
+      all += c;
+    }
+  int base = sum_of_lower(sh, all) + before;
+  const long long i1 = min(s.n, (blockIdx.x + 1) * s.per);
+  for (long long i0 = blockIdx.x * s.per; i0 < i1; i0 += kTile) {
+    const int count = (int)min((long long)kTile, i1 - i0);
+    Tile t;
+    const int sum = rank_tile(s, pass, i0, count, sh, t);
+    place_tile(s, pass, count, sum, base, sh, t);
+    base += sum;
   }
-  __syncthreads();
-  scan_digits(sh, digits);
-#pragma unroll
-  for (int k = 0; k < (1 << kMaxBits) / kSortThreads; k++) {
-    const int d = threadIdx.x + k * kSortThreads;
-    if (d < digits) sh.base[d] += before[k];
-  }
-  __syncthreads();
-  const long long i0 = blockIdx.x * s.per;
-  place_digits(s, pass, i0, min(s.n, i0 + s.per), sh);
 }
 
 // ---- sums of equal numbers ----------------------------------------------------------------------------------------------------
@@ -409,18 +447,20 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Reduce a) {
     const long long stretch = a.heads[1 + h / slabs], i1 = (stretch + 1) * a.per;
     const int col = ((int)(h % slabs) * 32 + lane) * V;
     const unsigned cur = a.keys[i1];
-    long long low = i1, high = a.n;   // the first place that is not the row's
-    while (low < high) {
-      const long long mid = (low + high) / 2;
-      if (a.keys[mid] == cur) low = mid + 1;
-      else high = mid;
+    long long low = i1, high = a.n;   // the first place that is not the row's, by 32 places at a time: low is the row's, high is not
+    while (high - low > 1) {
+      const long long step = (high - low + 32) / 33, at = low + (lane + 1) * step;
+      const int same = __popc(__ballot_sync(0xffffffffu, at < high && a.keys[min(at, a.n - 1)] == cur));
+      const long long past = low + (same + 1) * step;
+      low += same * step;
+      high = min(high, past);
     }
-    const long long last = (low - 1) / a.per;
+    const long long last = low / a.per;
     float s[V];
 #pragma unroll
     for (int k = 0; k < V; k++) s[k] = 0;
     if (col < a.d)
-#pragma unroll 4
+#pragma unroll 8
       for (long long p = stretch + warp; p <= last; p += kJoinWarps) {
         float g[V];
         load_part<V>(a.part + (p * 2 + (p == stretch)) * a.d + col, g);
@@ -480,7 +520,44 @@ void digits_of(int v, int* passes, int* bits) {
   *bits = std::max(1, (all + *passes - 1) / *passes);
 }
 
-long long sort_blocks(long long n) { return n <= kOneBlock ? 1 : std::min<long long>(kSortBlocks, (n + kTile - 1) / kTile); }
+// Blocks of the sort: of a cluster for few numbers, one number a thread at the least; otherwise half a tile.
+long long sort_blocks(long long n) {
+  if (n <= kClusterNumbers) return std::max(1LL, std::min<long long>(kClusterMost, n / kSortThreads));
+  return std::min<long long>(kSortBlocks, 2 * ((n + kTile - 1) / kTile));
+}
+
+template <class... P>
+int allow_shared(const char* fn, void (*kernel)(P...), std::atomic<uint64_t>* allowed) {   // allowed: devices on which the kernel may have this much shared memory
+  int device = 0;
+  GELIB_CUDA_TRY(fn, cudaGetDevice(&device));
+  const uint64_t bit = device < 64 ? 1ull << device : 0;
+  if (allowed->load(std::memory_order_relaxed) & bit) return GELIB_OK;
+  GELIB_CUDA_TRY(fn, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(SortShared)));
+  allowed->fetch_or(bit, std::memory_order_relaxed);
+  return GELIB_OK;
+}
+
+int launch_sort(const char* fn, const Sort& s, cudaStream_t stream) {
+  static std::atomic<uint64_t> cluster_allowed{0}, place_allowed{0};
+  int st;
+  if (s.n <= kClusterNumbers) {
+    if ((st = allow_shared(fn, cluster_sort_kernel, &cluster_allowed)) != GELIB_OK) return st;
+    cudaLaunchConfig_t c = {};
+    c.gridDim = dim3(s.blocks), c.blockDim = dim3(kSortThreads), c.dynamicSmemBytes = sizeof(SortShared), c.stream = stream;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = s.blocks, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
+    c.attrs = at, c.numAttrs = 1;
+    GELIB_CUDA_TRY(fn, cudaLaunchKernelEx(&c, cluster_sort_kernel, s));
+    return launched(fn);
+  }
+  if ((st = allow_shared(fn, place_kernel, &place_allowed)) != GELIB_OK) return st;
+  for (int pass = 0; pass < s.passes; pass++) {
+    if ((st = launch_after(fn, pass > 0, count_kernel, dim3(s.blocks), kSortThreads, 0, stream, s, pass)) != GELIB_OK) return st;
+    if ((st = launch_after(fn, true, place_kernel, dim3(s.blocks), kSortThreads, sizeof(SortShared), stream, s, pass)) != GELIB_OK) return st;
+  }
+  return GELIB_OK;
+}
 
 // Numbers of a stretch: enough stretches to fill the machine, of whole batches.
 template <int V>
@@ -499,7 +576,7 @@ Room room_of(long long n, int d, int v, int per) {
   const long long blocks = sort_blocks(n), stretches = (n + per - 1) / per;
   Room r;
   r.keys = up(4 * (n + kBatch));
-  r.counts = blocks > 1 ? up((4LL << bits) * blocks) : 0;
+  r.counts = n > kClusterNumbers ? up((4LL << bits) * blocks) : 0;
   r.heads = up(4 * (1 + stretches));
   r.part = up(stretches * 2 * d * 4);
   r.bytes = 4 * r.keys + r.counts + r.heads + r.part;
@@ -523,16 +600,8 @@ int launch_backward_as(const EmbeddingCall& c, char* at, cudaStream_t stream) {
     digits_of(c.v, &s.passes, &s.bits);
     s.blocks = (int)sort_blocks(c.n);
     s.per = (c.n + s.blocks - 1) / s.blocks;
-    int st;
-    if (s.blocks == 1) {
-      sort_kernel<<<1, kSortThreads, 0, stream>>>(s);
-      if ((st = launched(fn)) != GELIB_OK) return st;
-    } else {
-      for (int pass = 0; pass < s.passes; pass++) {
-        if ((st = launch_after(fn, pass > 0, count_kernel, dim3(s.blocks), kSortThreads, 0, stream, s, pass)) != GELIB_OK) return st;
-        if ((st = launch_after(fn, true, place_kernel, dim3(s.blocks), kSortThreads, 0, stream, s, pass)) != GELIB_OK) return st;
-      }
-    }
+    int st = launch_sort(fn, s, stream);
+    if (st != GELIB_OK) return st;
     a.keys = s.keys[(s.passes - 1) & 1], a.places = s.places[(s.passes - 1) & 1], a.heads = s.heads;
     a.gw = c.gw, a.gy = c.gy, a.part = (float*)(at + 4 * r.keys + r.counts + r.heads);
     a.n = c.n, a.stretches = (c.n + a.per - 1) / a.per, a.v = c.v, a.d = c.d, a.scale = c.scale;
