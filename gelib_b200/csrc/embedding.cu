@@ -392,10 +392,21 @@ __device__ __forceinline__ void add_stretch(const Reduce& a, long long team, int
   const bool goes_on = i1 < a.n && a.keys[i1] == cur;
   if (goes_on && whole) {
     if (!is_long(a, i1, cur)) {   // the rest of it too
-      for (long long p = i1; p < a.n && a.keys[p] == cur; p++) {
-        float g[V];
-        load_vec<T, V>(gy + (long long)a.places[p] * a.d, g);
-        add_all(s, s, g);
+      for (int i = count; i0 + i < a.n; i += kBatch) {
+        R raw[kBatch];
+        ask(i);
+        int live = 0;
+#pragma unroll
+        for (int j = 0; j < kBatch; j++)
+          if (live == j && i0 + i + j < a.n && key[j] == cur) raw[j] = *reinterpret_cast<const R*>(gy + (long long)place[j] * a.d), live++;
+#pragma unroll
+        for (int j = 0; j < kBatch; j++)
+          if (j < live) {
+            float g[V];
+            unpack<T, V>(raw[j], g);
+            add_all(s, s, g);
+          }
+        if (live < kBatch) break;
       }
       put(false);
       return;

@@ -270,11 +270,13 @@ Plan choose_plan(const Sizes* z, int count, int type, bool whole) {
     } else {
       best_time = std::ceil(w[0].items / slots) * w[0].each + std::ceil((items - slots * std::ceil(w[0].items / slots)) / slots) * w[1].each;
     }
-    const int lead = (int)(w[0].each / w[1].each + 0.5), spare = slots - longer;
-    if (longer > 0 && lead > 0 && w[1].items > (double)lead * spare) {
-      const double time = std::ceil(w[0].items / slots) * w[0].each + std::ceil((w[1].items - (double)lead * spare) / slots) * w[1].each;
-      if (time < 0.97 * best_time) best.flip = 0, best.lead = lead;
-    }
+    const double whole = std::floor(w[0].items / slots);
+    if (longer > 0)
+      for (int lead = 1; lead <= 2 * w[0].each / w[1].each + 1; lead++) {
+        const double rest = std::max(0.0, w[1].items - (double)lead * (slots - longer));
+        const double time = whole * w[0].each + std::max(w[0].each, lead * w[1].each) + std::ceil(rest / slots) * w[1].each;
+        if (time < 0.97 * best_time) best.flip = 0, best.lead = lead, best_time = time;
+      }
   }
   return best;
 }

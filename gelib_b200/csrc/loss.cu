@@ -264,7 +264,7 @@ int forward(const gelib_linear_loss_args& p, char* at, cudaStream_t stream) {
   const int parts = parts_of(p), blocks = row_blocks(p.m);
   f.part = (float2*)at, at += up(8LL * parts * p.m);
   f.at_entry = (float*)at, at += up(4 * p.m * p.top);
-  if ((st = few ? launch_few(fn, f, false, stream) : launch_forward_product(fn, f, jobs.count > 0, stream)) != GELIB_OK) return st;
+  if ((st = few ? launch_few(fn, f, stream) : launch_forward_product(fn, f, jobs.count > 0, stream)) != GELIB_OK) return st;
   const Total total = {p.reduction, (float*)p.loss, s.scale};
   st = launch_after(fn, true, rows_kernel, dim3(blocks), kRowThreads, 0, stream, e, s, (const float2*)f.part, (const float*)f.at_entry, parts, (long long)p.m, c,
                     temperature_of(p), total, (RowSum*)at);

@@ -12,6 +12,7 @@ namespace gelib_b200 {
 namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kAcrossThreads = 512, kAcrossWarps = kAcrossThreads / 32;
 constexpr int kSms = 148;
 
 struct RowsArgs {
@@ -47,12 +48,13 @@ __device__ __forceinline__ void take(const RowsArgs& a, float z, int cls, int ro
 }
 
 // Partial sums of a block's warps, (warp, row), to the block's part.
-__device__ __forceinline__ void join_warps(const RowsArgs& a, const float2 (&of)[kWarps][8]) {
+template <int kCount>
+__device__ __forceinline__ void join_warps(const RowsArgs& a, const float2 (&of)[kCount][8]) {
   __syncthreads();
   if ((int)threadIdx.x < a.M) {
     float2 s = of[0][threadIdx.x];
 #pragma unroll
-    for (int w = 1; w < kWarps; w++) s = joined(s, of[w][threadIdx.x], a.c);
+    for (int w = 1; w < kCount; w++) s = joined(s, of[w][threadIdx.x], a.c);
     a.part[(long long)blockIdx.x * a.M + threadIdx.x] = s;
   }
 }
@@ -117,11 +119,11 @@ __global__ void __launch_bounds__(kThreads) along_kernel(const RowsArgs a) {
   join_warps(a, of);
 }
 
-// w (K, N): a block's classes are 32 V that follow one another; its warps take every eighth k, and their sums meet in shared memory row by row.
+// w (K, N): a block's classes are 32 V that follow one another; its warps take every sixteenth k, and their sums meet in shared memory row by row.
 template <class T, int V, int M>
-__global__ void __launch_bounds__(kThreads) across_kernel(const RowsArgs a) {
-  __shared__ float2 of[kWarps][8];
-  __shared__ float sums[kWarps][32 * V + 1];
+__global__ void __launch_bounds__(kAcrossThreads) across_kernel(const RowsArgs a) {
+  __shared__ float2 of[8][8];
+  __shared__ float sums[kAcrossWarps][32 * V + 1];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, n0 = blockIdx.x * 32 * V, n = n0 + lane * V;
   const T *x = static_cast<const T*>(a.x), *w = static_cast<const T*>(a.w);
   let_next_begin();
@@ -132,8 +134,8 @@ __global__ void __launch_bounds__(kThreads) across_kernel(const RowsArgs a) {
 #pragma unroll
     for (int j = 0; j < V; j++) s[m][j] = 0;
   if (n < a.N)
-#pragma unroll 4
-    for (int k = warp; k < a.K; k += kWarps) {
+#pragma unroll 8
+    for (int k = warp; k < a.K; k += kAcrossWarps) {
       float u[V];
       load_vec<T, V>(w + k * a.ldw + n, u);
 #pragma unroll
@@ -152,7 +154,7 @@ __global__ void __launch_bounds__(kThreads) across_kernel(const RowsArgs a) {
     if (at < 32 * V && cls < a.N) {
       float z = a.bias ? to_float(static_cast<const T*>(a.bias)[cls]) : 0.f;
 #pragma unroll
-      for (int q = 0; q < kWarps; q++) z += sums[q][at % V * 32 + at / V];
+      for (int q = 0; q < kAcrossWarps; q++) z += sums[q][at % V * 32 + at / V];
       take(a, z, cls, m, next, sum);
     }
     __syncwarp();
@@ -161,31 +163,27 @@ __global__ void __launch_bounds__(kThreads) across_kernel(const RowsArgs a) {
       const float2 o = {__shfl_xor_sync(0xffffffffu, sum.x, d), __shfl_xor_sync(0xffffffffu, sum.y, d)};
       sum = joined(sum, o, a.c);
     }
-    if (lane == 0) of[warp][m] = sum;
+    if (lane == 0 && warp < 8) of[warp][m] = sum;   // 256 classes at the most
     __syncthreads();
   }
   join_warps(a, of);
 }
 
-template <class T, int V, int M>
-int launch_rows_as(const char* fn, RowsArgs& a, bool along, int blocks, bool follows, cudaStream_t stream) {
-  return launch_after(fn, follows, along ? along_kernel<T, V, M> : across_kernel<T, V, M>, dim3(blocks), kThreads, 0, stream, a);
-}
-template <class T, int V>
-int launch_rows_of(const char* fn, RowsArgs& a, bool along, int blocks, bool follows, cudaStream_t stream) {
-  return a.M == 1  ? launch_rows_as<T, V, 1>(fn, a, along, blocks, follows, stream)
-         : a.M <= 2 ? launch_rows_as<T, V, 2>(fn, a, along, blocks, follows, stream)
-         : a.M <= 4 ? launch_rows_as<T, V, 4>(fn, a, along, blocks, follows, stream) : launch_rows_as<T, V, 8>(fn, a, along, blocks, follows, stream);
-}
-
-// Whether 16 bytes of the weights can be taken at a time.
-bool takes_wide(const ForwardProduct& p) {
-  const int V = 16 / type_bytes(p.type);
-  return is_aligned(p.w.base, 16) && (p.w_by_sum ? p.N : p.K) % V == 0 && (p.w.ld % V == 0 || p.w.rows <= 1) && is_aligned(p.x.base, p.w_by_sum ? 1 : 16);
+// How many classes of a lane, or numbers of one class, go in one access: 16 bytes of them or one; where a row has all classes also 8 or 4 bytes, so that
+// few classes make more blocks.
+int width_of(const ForwardProduct& p) {
+  const auto fits = [&](int V) {
+    return is_aligned(p.w.base, V * type_bytes(p.type)) && (p.w_by_sum ? p.N : p.K) % V == 0 && (p.w.ld % V == 0 || p.w.rows <= 1) &&
+           (p.w_by_sum || is_aligned(p.x.base, 16));
+  };
+  int V = 16 / type_bytes(p.type);
+  if (!p.w_by_sum) return fits(V) ? V : 1;
+  while (V > 1 && (!fits(V) || (p.N + 32 * V - 1) / (32 * V) < kSms)) V /= 2;
+  return V;
 }
 int blocks_of(const ForwardProduct& p, int* per) {
   if (p.w_by_sum) {
-    *per = 32 * (takes_wide(p) ? 16 / type_bytes(p.type) : 1);
+    *per = 32 * width_of(p);
     return (p.N + *per - 1) / *per;
   }
   // four blocks of an SM, four classes of a warp at the least
@@ -193,23 +191,45 @@ int blocks_of(const ForwardProduct& p, int* per) {
   return (int)((p.N + (long long)*per * kWarps - 1) / ((long long)*per * kWarps));
 }
 
+template <class T, int V, int M>
+int launch_rows_as(const char* fn, const RowsArgs& a, bool along, int blocks, cudaStream_t stream) {
+  if (along) {
+    if constexpr (V == 1 || V * sizeof(T) == 16) return launch_after(fn, false, along_kernel<T, V, M>, dim3(blocks), kThreads, 0, stream, a);
+  }
+  return launch_after(fn, false, across_kernel<T, V, M>, dim3(blocks), kAcrossThreads, 0, stream, a);
+}
+template <class T, int V>
+int launch_rows_of(const char* fn, const RowsArgs& a, bool along, int blocks, cudaStream_t stream) {
+  if (a.M == 1) return launch_rows_as<T, V, 1>(fn, a, along, blocks, stream);
+  if (a.M == 2) return launch_rows_as<T, V, 2>(fn, a, along, blocks, stream);
+  if constexpr (sizeof(T) == 4) return a.M <= 4 ? launch_rows_as<T, V, 4>(fn, a, along, blocks, stream) : launch_rows_as<T, V, 8>(fn, a, along, blocks, stream);
+  return fail(GELIB_INVALID, fn, "too many rows");
+}
+template <class T>
+int launch_rows_type(const char* fn, const RowsArgs& a, bool along, int blocks, int V, cudaStream_t stream) {
+  if constexpr (sizeof(T) == 2)
+    if (V == 8) return launch_rows_of<T, 8>(fn, a, along, blocks, stream);
+  if (V == 4) return launch_rows_of<T, 4>(fn, a, along, blocks, stream);
+  if (V == 2) return launch_rows_of<T, 2>(fn, a, along, blocks, stream);
+  return launch_rows_of<T, 1>(fn, a, along, blocks, stream);
+}
+
 }  // namespace
 
-bool takes_few(const ForwardProduct& p) { return p.M <= 8; }
+// Rows that are few.
+bool takes_few(const ForwardProduct& p) { return p.M <= (p.type == GELIB_F32 ? 8 : 2); }
 
 int few_parts(const ForwardProduct& p) {
   int per;
   return blocks_of(p, &per);
 }
 
-int launch_few(const char* fn, const ForwardProduct& p, bool follows, cudaStream_t stream) {
+int launch_few(const char* fn, const ForwardProduct& p, cudaStream_t stream) {
   RowsArgs a = {p.x.base, p.w.base, p.bias, p.x.ld, p.w.ld, (int)p.M, p.N, p.K, p.e, p.c, p.part, p.at_entry, 0};
-  const int blocks = blocks_of(p, &a.per);
-  const bool wide = takes_wide(p), along = !p.w_by_sum;
-  if (p.type == GELIB_F32) return wide ? launch_rows_of<float, 4>(fn, a, along, blocks, follows, stream) : launch_rows_of<float, 1>(fn, a, along, blocks, follows, stream);
-  if (p.type == GELIB_BF16)
-    return wide ? launch_rows_of<__nv_bfloat16, 8>(fn, a, along, blocks, follows, stream) : launch_rows_of<__nv_bfloat16, 1>(fn, a, along, blocks, follows, stream);
-  return wide ? launch_rows_of<__half, 8>(fn, a, along, blocks, follows, stream) : launch_rows_of<__half, 1>(fn, a, along, blocks, follows, stream);
+  const int blocks = blocks_of(p, &a.per), V = width_of(p);
+  const bool along = !p.w_by_sum;
+  return p.type == GELIB_F32    ? launch_rows_type<float>(fn, a, along, blocks, V, stream)
+         : p.type == GELIB_BF16 ? launch_rows_type<__nv_bfloat16>(fn, a, along, blocks, V, stream) : launch_rows_type<__half>(fn, a, along, blocks, V, stream);
 }
 
 }  // namespace gelib_b200
