@@ -91,7 +91,7 @@ int gelib_embedding_back(void* gw, const void* gy, const void* ids, long long n,
 }
 
 long long gelib_linear_loss_state_bytes(const gelib_linear_loss_args* p) {
-  return p && p->m >= 0 && p->m <= 1LL << 30 && p->top >= 1 && p->top <= GELIB_LOSS_MAX_TOP ? linear_loss_state_bytes(*p) : 0;
+  return p && p->m >= 0 && p->m <= 1LL << 30 && p->n >= 1 && p->n <= 1 << 30 && p->top >= 1 && p->top <= GELIB_LOSS_MAX_TOP ? linear_loss_state_bytes(*p) : 0;
 }
 
 long long gelib_linear_loss_workspace(const gelib_linear_loss_args* p, int backward) {

@@ -26,25 +26,36 @@ namespace gelib_b200 {
 namespace {
 
 constexpr int kThreads = 256;
-State state_of(const gelib_linear_loss_args& p) {
+
+// Buckets of a row's classes: 128 at the most.
+int bucket_of(int n) { return (n / 128 + 256) / 256 * 256; }
+int buckets_of(int n) { return (n + bucket_of(n) - 1) / bucket_of(n); }
+
+// The state and its bytes; p.state may be null.
+State state_of(const gelib_linear_loss_args& p, long long* bytes = nullptr) {
   char* at = (char*)p.state;
-  State s;
+  State s = {};
   s.scale = (float*)at, at += 256;
   s.lse = (float2*)at, at += up(p.m * 8);
-  s.ids = (int*)at, at += up(p.m * p.top * 4);
-  s.q = (float*)at;
+  if (p.teacher) {
+    s.ids = (int*)at, at += up(p.m * p.top * 4);
+    s.q = (float*)at, at += up(p.m * p.top * 4);
+    s.starts = (unsigned short*)at, at += up(p.m * (buckets_of(p.n) + 1) * 2);
+  }
+  if (bytes) *bytes = at - (char*)p.state;
   return s;
 }
 
 Entries entries_of(const gelib_linear_loss_args& p, const State& s) {
-  return {p.target, p.teacher ? s.ids : nullptr, p.teacher ? s.q : nullptr, p.ignore_index, p.top, p.index_bytes, p.n};
+  return {p.target, s.ids, s.q, s.starts, p.ignore_index, p.top, p.index_bytes, p.n, bucket_of(p.n), buckets_of(p.n)};
 }
+
 // ---- the teacher -------------------------------------------------------------------------------------------------------------
 
 // A warp per row: q = softmax(logits / T) over the entries, in ascending order of their classes.
 template <class T>
 __global__ void __launch_bounds__(128) teacher_kernel(State s, Entries e, const T* logits, long long m, float c) {
-  __shared__ int ids[4][GELIB_LOSS_MAX_TOP];
+  __shared__ int ids[4][GELIB_LOSS_MAX_TOP], sorted[4][GELIB_LOSS_MAX_TOP];
   __shared__ float share[4][GELIB_LOSS_MAX_TOP];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, top = e.top;
   const long long row = (long long)blockIdx.x * 4 + warp;
@@ -74,12 +85,26 @@ __global__ void __launch_bounds__(128) teacher_kernel(State s, Entries e, const 
 #pragma unroll
   for (int d = 16; d; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
   __syncwarp();
+  int live = 0;
   for (int i = lane; i < top; i += 32) {
     const int id = ids[warp][i];
     int place = 0;
     for (int j = 0; j < top; j++) place += ids[warp][j] < id || (ids[warp][j] == id && j < i);
+    live += id != kNone;
+    sorted[warp][place] = id;
     s.ids[row * top + place] = invalid && place == 0 ? kInvalid : id;
     s.q[row * top + place] = id == kNone ? 0.f : share[warp][i] / sum;
+  }
+  live = invalid ? 0 : __reduce_add_sync(0xffffffffu, live);
+  __syncwarp();
+  for (int b = lane; b <= e.buckets; b += 32) {
+    int low = 0, high = live;   // the first place whose class is in bucket b or above
+    while (low < high && b < e.buckets) {
+      const int mid = (low + high) / 2;
+      if (sorted[warp][mid] < b * e.bucket) low = mid + 1;
+      else high = mid;
+    }
+    s.starts[row * (e.buckets + 1) + b] = (unsigned short)(b < e.buckets ? low : live);
   }
 }
 
@@ -362,7 +387,11 @@ int backward(const gelib_linear_loss_args& p, char* workspace, cudaStream_t stre
 
 }  // namespace
 
-long long linear_loss_state_bytes(const gelib_linear_loss_args& p) { return 256 + up(p.m * 8) + (p.teacher ? 2 * up(p.m * p.top * 4) : 0); }
+long long linear_loss_state_bytes(const gelib_linear_loss_args& p) {
+  long long bytes;
+  state_of(p, &bytes);
+  return bytes;
+}
 
 long long linear_loss_workspace(const gelib_linear_loss_args& p, bool backward) {
   if (backward) return p.gx || p.gw || p.gb ? room_of(p, nullptr).bytes : 0;

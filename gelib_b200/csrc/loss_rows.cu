@@ -70,7 +70,7 @@ __global__ void __launch_bounds__(kThreads) along_kernel(const RowsArgs a) {
   let_next_begin();
   await_previous();
   Next next;
-  next.begin(a.e, row, row < a.M && c0 < c1, (int)min(c0, (long long)INT_MAX));
+  next.begin(a.e, row, row < a.M && c0 < c1, (int)c0, (int)c1);
   float2 sum = {-INFINITY, 0.f};
   for (long long c = c0; c < c1; c += 4) {
     float s[M][4];
@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(kAcrossThreads) across_kernel(const RowsArgs a
     float2 sum = {-INFINITY, 0.f};
     Next next;
     const int at = (int)threadIdx.x, cls = n0 + at;   // class `at` of the block lies at [at % V][at / V]
-    next.begin(a.e, m, at < 32 * V && cls < a.N, cls);
+    next.begin(a.e, m, at < 32 * V && cls < a.N, cls, cls + 1);
     if (at < 32 * V && cls < a.N) {
       float z = a.bias ? to_float(static_cast<const T*>(a.bias)[cls]) : 0.f;
 #pragma unroll

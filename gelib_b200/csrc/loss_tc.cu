@@ -59,7 +59,7 @@ struct ForwardEnd {
     row = m0 + lane;
     tile = it.n * 2 + second;
     sum = {-INFINITY, 0.f};
-    next.begin(g.e, row, row < g.M, n0);
+    next.begin(g.e, row, row < g.M, n0, min(g.N, it.n * g.bn + g.bn));
   }
   __device__ __forceinline__ void take(const Problem& g, int, int n, int, uint32_t, const uint32_t (&r)[kChunk], bool) {
     float v[kChunk];
@@ -126,7 +126,7 @@ struct SlopeEnd {
   bool out, some_out;   // the lane's row has no loss; one of the warp's has none
 
   template <int kChunks>
-  __device__ __forceinline__ void ahead(const Problem& g, const Item&, long long m, int n0, int lane, bool) {
+  __device__ __forceinline__ void ahead(const Problem& g, const Item& it, long long m, int n0, int lane, bool) {
     m0 = m;
     const long long row = m0 + lane;
     lse = row < g.M ? g.lse[row] : float2{0.f, INFINITY};
@@ -134,7 +134,7 @@ struct SlopeEnd {
     some_out = __any_sync(0xffffffffu, out);
     g_up = g.up;
     if (g.gy && row < g.M) g_up *= g.most ? g.gy[row] / *g.most : g.gy[row];
-    next.begin(g.e, row, !out, g.first + n0);
+    next.begin(g.e, row, !out, g.first + n0, g.first + min(g.N, it.n * g.bn + g.bn));
   }
   __device__ __forceinline__ void take(const Problem& g, int, int n, int lane, uint32_t block, const uint32_t (&r)[kChunk], bool) {
     float v[kChunk];
@@ -159,32 +159,39 @@ struct SlopeEnd {
     }
     __syncwarp();
     const int col = lane % kAcross * 4, live = min(4, g.N - n - col);
-    float s[4] = {0, 0, 0, 0};
+    const long long m = m0 + lane / kAcross;
+    float d[kPasses][4];
 #pragma unroll
     for (int pass = 0; pass < kPasses; pass++) {
       const float4 f = tc::lds128(block + ((pass * kRows + lane / kAcross) * kPitch + col) * 4);
-      const float d[4] = {f.x, f.y, f.z, f.w};
-      add_all(s, s, d);   // rows that are not there are zero
-      const long long m = m0 + pass * kRows + lane / kAcross, at = m * g.ld + n + col;
-      if (m >= g.M || live <= 0) continue;
-      if constexpr (sizeof(T) == 4) {
-        uint32_t p[3], q[3];
-        split3(d[0], d[1], p);
-        split3(d[2], d[3], q);
+      d[pass][0] = f.x, d[pass][1] = f.y, d[pass][2] = f.z, d[pass][3] = f.w;
+    }
+    if (live > 0) {
+      const long long at = m * g.ld + n + col, step = kRows * g.ld;   // rows have room for a multiple of eight
 #pragma unroll
-        for (int i = 0; i < 3; i++) {
-          __nv_bfloat16* to = static_cast<__nv_bfloat16*>(g.dz) + i * g.plane + at;
-          *reinterpret_cast<uint2*>(to) = make_uint2(p[i], q[i]);   // rows have room for a multiple of eight
+      for (int pass = 0; pass < kPasses; pass++) {
+        if (m + pass * kRows >= g.M) break;
+        if constexpr (sizeof(T) == 4) {
+          uint32_t p[3], q[3];
+          split3(d[pass][0], d[pass][1], p);
+          split3(d[pass][2], d[pass][3], q);
+#pragma unroll
+          for (int i = 0; i < 3; i++)
+            *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(g.dz) + i * g.plane + at + pass * step) = make_uint2(p[i], q[i]);
+        } else {
+          store_vec<T, 4>(static_cast<T*>(g.dz) + at + pass * step, d[pass]);
         }
-      } else {
-        store_vec<T, 4>(static_cast<T*>(g.dz) + at, d);
       }
     }
+    __syncwarp();
     if (!g.sums) return;
+    float s[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int pass = 0; pass < kPasses; pass++) add_all(s, s, d[pass]);   // rows that are not there are zero
 #pragma unroll
     for (int j = 0; j < 4; j++)
 #pragma unroll
-      for (int d = kAcross; d < 32; d *= 2) s[j] += __shfl_xor_sync(0xffffffffu, s[j], d);
+      for (int o = kAcross; o < 32; o *= 2) s[j] += __shfl_xor_sync(0xffffffffu, s[j], o);
     if (lane < kAcross && m0 < g.M) {
       float* to = g.sums + m0 / 32 * g.N + n + col;
 #pragma unroll
@@ -243,34 +250,51 @@ struct GradEnd {
     for (int j = 0; j < kAcross; j++) tc::sts128(block + (lane * kPitch + 4 * j) * 4, r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
     __syncwarp();
     const int col = lane % kAcross * 4, n = n0 + col, live = min(4, g.N - n);
+    const long long m = m0 + lane / kAcross;
+    float d[kPasses][4];
 #pragma unroll
     for (int pass = 0; pass < kPasses; pass++) {
       const float4 f = tc::lds128(block + ((pass * kRows + lane / kAcross) * kPitch + col) * 4);
-      const long long m = m0 + pass * kRows + lane / kAcross, at = m * g.N + n;
-      if (m >= g.M || live <= 0) continue;
-      float d[4] = {f.x, f.y, f.z, f.w};
-      if (g.part) {
-        float* to = g.part + (long long)split * g.M * g.N + at;
-        if (g.vec_f) *reinterpret_cast<float4*>(to) = f;
-        else
+      d[pass][0] = f.x, d[pass][1] = f.y, d[pass][2] = f.z, d[pass][3] = f.w;
+    }
+    const bool inside = m0 + 32 <= g.M && n0 + kChunk <= g.N;
+    float* sum = g.part ? g.part + (long long)split * g.M * g.N : g.sum;   // partial sums go like those of a first piece
+    const bool adds = !g.part && g.begun;
+    T* y = g.part ? nullptr : static_cast<T*>(g.y);
+    if (inside && (!sum || g.vec_f) && (!y || g.vec_y)) {
+      // nothing to be left out: the lane's four accesses one after the other
+      if (sum) sum += m * g.N + n;
+      const long long step = (long long)kRows * g.N;
+      if (sum && adds)
 #pragma unroll
-          for (int j = 0; j < 4; j++)
-            if (j < live) to[j] = d[j];
-        continue;
-      }
-      T* y = g.y ? static_cast<T*>(g.y) + m * g.ldy + n : nullptr;
-      float* sum = g.sum ? g.sum + at : nullptr;
-      if ((!sum || g.vec_f) && (!y || g.vec_y)) {
-        finish_grad<T, 4>(y, sum, g.begun, scale, d);
+        for (int pass = 0; pass < kPasses; pass++) {
+          float w[4];
+          load_vec<float, 4>(sum + pass * step, w);
+          add_all(d[pass], d[pass], w);
+        }
+      if (y) {
+        y += m * g.ldy + n;
+#pragma unroll
+        for (int pass = 0; pass < kPasses; pass++) {
+          mul_all(d[pass], d[pass], scale);
+          store_vec<T, 4>(y + pass * kRows * g.ldy, d[pass]);
+        }
       } else {
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-          if (j < live) {
-            float one[1] = {d[j]};
-            finish_grad<T, 1>(y ? y + j : nullptr, sum ? sum + j : nullptr, g.begun, scale, one);
-          }
+        for (int pass = 0; pass < kPasses; pass++) store_vec<float, 4>(sum + pass * step, d[pass]);
       }
+      return;
     }
+#pragma unroll
+    for (int pass = 0; pass < kPasses; pass++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const long long row = m + pass * kRows;
+        if (row >= g.M || j >= live) continue;
+        float one[1] = {d[pass][j]};
+        finish_grad<T, 1>(y ? y + row * g.ldy + n + j : nullptr, sum ? sum + row * g.N + n + j : nullptr, adds, scale, one);
+      }
+    __syncwarp();
   }
   __device__ __forceinline__ void end(const Problem&, int) {}
 };
