@@ -14,6 +14,7 @@ namespace {
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kAcrossThreads = 512, kAcrossWarps = kAcrossThreads / 32;
 constexpr int kSms = 148;
+constexpr int blocks_of_sm(int rows) { return rows == 1 ? 4 : rows == 2 ? 3 : 2; }   // that its registers have room for
 
 struct RowsArgs {
   const void *x, *w, *bias;
@@ -61,7 +62,7 @@ __device__ __forceinline__ void join_warps(const RowsArgs& a, const float2 (&of)
 
 // w (N, K): a warp's classes are a.per that follow one another; lane 4 r + j of it keeps the sums of row r over every fourth.
 template <class T, int V, int M>
-__global__ void __launch_bounds__(kThreads) along_kernel(const RowsArgs a) {
+__global__ void __launch_bounds__(kThreads, blocks_of_sm(M)) along_kernel(const RowsArgs a) {
   __shared__ float2 of[kWarps][8];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, row = lane / 4;
   const long long c0 = ((long long)blockIdx.x * kWarps + warp) * a.per, c1 = min((long long)a.N, c0 + a.per);
@@ -80,7 +81,7 @@ __global__ void __launch_bounds__(kThreads) along_kernel(const RowsArgs a) {
       for (int j = 0; j < 4; j++) s[m][j] = 0;
     const T* of_class[4];
 #pragma unroll
-    for (int j = 0; j < 4; j++) of_class[j] = w + min(c + j, (long long)a.N - 1) * a.ldw;
+    for (int j = 0; j < 4; j++) of_class[j] = w + min(c + j, c1 - 1) * a.ldw;
 #pragma unroll 2
     for (int k = lane * V; k < a.K; k += 32 * V) {
       float u[4][V];
@@ -186,8 +187,8 @@ int blocks_of(const ForwardProduct& p, int* per) {
     *per = 32 * width_of(p);
     return (p.N + *per - 1) / *per;
   }
-  // four blocks of an SM, four classes of a warp at the least
-  *per = std::max(4, (int)((p.N / (kSms * 4LL * kWarps) + 3) / 4 * 4));
+  const long long warps = kSms * blocks_of_sm((int)p.M) * kWarps;   // of one round
+  *per = (int)std::max(4LL, (p.N + warps - 1) / warps);
   return (int)((p.N + (long long)*per * kWarps - 1) / ((long long)*per * kWarps));
 }
 

@@ -317,30 +317,36 @@ struct GradJoins {
   int sum_n;
 };
 
+// Many parts are shared by the warps of a block, whose sums are added in a fixed order.
+constexpr int kSharedParts = 8;
 template <class T, int V>
 __device__ __forceinline__ void join_grad(const GradJoins::Join& a, long long block, float scale, float (&t)[8][32][5]) {
   const int lane = threadIdx.x % 32, group = threadIdx.x / 32;
-  const long long size = a.M * a.N, at = (block * 32 + lane) * V;
+  const bool shared = a.parts >= kSharedParts;
+  const long long size = a.M * a.N, at = (shared ? block * 32 + lane : block * kJoinThreads + threadIdx.x) * V;
   float d[V];
 #pragma unroll
   for (int j = 0; j < V; j++) d[j] = 0;
   if (at < size)
 #pragma unroll 4
-    for (int i = group; i < a.parts; i += 8) {
+    for (int i = shared ? group : 0; i < a.parts; i += shared ? 8 : 1) {
       float v[V];
       load_vec<float, V>(a.part + i * size + at, v);
       add_all(d, d, v);
     }
+  if (shared) {
 #pragma unroll
-  for (int j = 0; j < V; j++) t[group][lane][j] = d[j];
-  __syncthreads();
-  if (group > 0 || at >= size) return;
+    for (int j = 0; j < V; j++) t[group][lane][j] = d[j];
+    __syncthreads();
+    if (group > 0) return;
 #pragma unroll
-  for (int j = 0; j < V; j++) {
-    d[j] = 0;
+    for (int j = 0; j < V; j++) {
+      d[j] = 0;
 #pragma unroll
-    for (int i = 0; i < 8; i++) d[j] += t[i][lane][j];
+      for (int i = 0; i < 8; i++) d[j] += t[i][lane][j];
+    }
   }
+  if (at >= size) return;
   const long long m = at / a.N, n = at - m * a.N;
   finish_grad<T, V>(a.y ? static_cast<T*>(a.y) + m * a.ldy + n : nullptr, a.sum ? a.sum + at : nullptr, a.begun, scale, d);
 }
@@ -465,7 +471,8 @@ int launch_grads(const char* fn, const Grads& q, bool follows, void* workspace, 
         at += (c.splits * g.M * g.N * 4 + 255) / 256 * 256;
         GradJoins::Join& j = joins.j[joined++];
         j = {p.part, g.sum, p.y, g.ldy, g.M, 0, c.splits, (int)g.N, p.begun, p.vec_f && (!p.y || p.vec_y)};
-        j.blocks = (g.M * g.N / (j.vec ? 4 : 1) + 31) / 32;
+        const int side = c.splits >= kSharedParts ? 32 : kJoinThreads;   // accesses of a block
+        j.blocks = (g.M * g.N / (j.vec ? 4 : 1) + side - 1) / side;
       }
       a.items += p.items;
     }
