@@ -562,6 +562,94 @@ def test_module():
     assert same.abs() < 1e-5
 
 
+@pytest.mark.gpu
+def test_a_wait_that_runs_out_is_reported():
+    """On the host's side alone: the kernel is told not to wait, gives up, and says so to the next call and to async_status."""
+    import gelib_b200 as G
+    x, w, bias, target, _ = make(200, 64, 300, torch.bfloat16)
+    want = run(x, w, bias, target, None, torch.tensor(1.0, device="cuda"))
+    for part in ("forward", "backward"):
+        leaf = x.clone().requires_grad_()
+        loss = None if part == "forward" else call(leaf, w, bias, target, None)
+        G._lib.set_option("inject_timeout", "1")
+        try:
+            if part == "forward":
+                call(x, w, bias, target, None)
+            else:
+                torch.autograd.grad(loss, leaf)
+            torch.cuda.synchronize()
+        finally:
+            G._lib.set_option("inject_timeout", "0")
+        with pytest.raises(RuntimeError, match="wait"):
+            G._lib.async_status()
+    got = run(x, w, bias, target, None, torch.tensor(1.0, device="cuda"))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("wt", [False, True])
+def test_weights_of_more_than_2_to_31_elements(wt):
+    """The last classes of a vocabulary of a million: their logits, and their gradients, against those of these classes alone."""
+    import gelib_b200 as G
+    if torch.cuda.get_device_properties(0).total_memory < 60 * 2 ** 30:
+        pytest.skip("needs 60 GB of device memory")
+    k, n, m, tail = 2056, (1 << 20) + 264, 20, 520
+    assert k * n > 2 ** 31
+    w = torch.zeros((n, k) if wt else (k, n), dtype=torch.bfloat16, device="cuda")
+    w = w.t() if wt else w
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    w[:, -tail:] = (torch.randn(k, tail, generator=gen, device="cuda") * k ** -0.5).to(w.dtype)
+    x = torch.randn(m, k, generator=gen, device="cuda").to(w.dtype)
+    target = n - 1 - torch.arange(m, device="cuda") % tail
+    gy = torch.ones(m, device="cuda")
+    loss, gx, gw = run(x, w, None, target, None, gy, reduction="none")
+    # all other classes have z = 0: as one class with a bias of log of their number
+    small = torch.cat([torch.zeros(k, 1, dtype=w.dtype, device="cuda"), w[:, -tail:]], 1).double()
+    z = x.double() @ small
+    z[:, 0] += math.log(n - tail)
+    lse = torch.logsumexp(z, 1, keepdim=True)
+    want = lse[:, 0] - z[torch.arange(m, device="cuda"), target - (n - tail) + 1]
+    off = EPS * (x.double().abs() @ small.abs() + z.abs()).amax(1) * 2 + EPS * (1 + lse[:, 0].abs())
+    assert ((loss.double() - want).abs() <= off).all()
+    dz = (z - lse).exp()
+    dz[torch.arange(m, device="cuda"), target - (n - tail) + 1] -= 1
+    want_gx, want_gw = dz[:, 1:] @ small[:, 1:].t(), x.double().t() @ dz[:, 1:]
+    # dz and the result are rounded to 16 bits
+    size = dz[:, 1:].abs() + off[:, None]
+    assert ((gx.double() - want_gx).abs() <= 2.0 ** -8 * (size @ small[:, 1:].abs().t() + want_gx.abs()) * 1.1 + 1e-6).all()
+    assert ((gw[:, -tail:].double() - want_gw).abs() <= 2.0 ** -8 * (x.double().abs().t() @ size + want_gw.abs()) * 1.1 + 1e-6).all()
+    first = x.double().t() @ ((z[:, :1] - lse).exp() / (n - tail)).expand(m, 8)   # a class of the many
+    assert ((gw[:, :8].double() - first).abs() <= 2.0 ** -6 * first.abs() + 1e-9).all()
+
+
+@pytest.mark.gpu
+def test_more_than_2_to_31_numbers_of_dz():
+    """A piece of dz beyond 2^31 elements: rows far down have the gradients that they have by themselves."""
+    if torch.cuda.get_device_properties(0).total_memory < 60 * 2 ** 30:
+        pytest.skip("needs 60 GB of device memory")
+    m, k, n = 1100000, 16, 2048
+    assert m * n > 2 ** 31
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    x = torch.randn(m, k, generator=gen, device="cuda").to(torch.bfloat16)
+    w = (torch.randn(k, n, generator=gen, device="cuda") * 0.3).to(torch.bfloat16)
+    target = torch.randint(n, (m,), generator=gen, device="cuda")
+    loss, gx, gw = run(x, w, None, target, None, torch.ones(m, device="cuda"), reduction="none")
+    for at in (0, m // 2 + 77, m - 300):
+        rows = slice(at, at + 300)
+        wants = reference(x[rows], w, None, target[rows], None, 1.0, torch.ones(300, device="cuda"), "none")
+        near(loss[rows], wants[0], "loss")
+        near(gx[rows], wants[1], "gx")
+    want = torch.zeros(k, n, dtype=torch.float64, device="cuda")
+    allowed = torch.zeros_like(want)
+    for at in range(0, m, 110000):
+        rows = slice(at, at + 110000)
+        p = torch.softmax(x[rows].double() @ w.double(), 1)
+        p[torch.arange(p.size(0), device="cuda"), target[rows]] -= 1
+        want += x[rows].double().t() @ p
+        allowed += x[rows].double().abs().t() @ p.abs()
+    assert ((gw.double() - want).abs() <= (2.0 ** -8 + EPS) * allowed * 1.01 + 2.0 ** -8 * want.abs()).all()
+
+
 def test_cpu_tensors_are_refused(cabi):
     import gelib_b200 as G
     with pytest.raises(RuntimeError, match="CUDA tensors only"):
