@@ -50,26 +50,35 @@ Entries entries_of(const gelib_linear_loss_args& p, const State& s) {
   return {p.target, s.ids, s.q, s.starts, p.ignore_index, p.top, p.index_bytes, p.n, bucket_of(p.n), buckets_of(p.n)};
 }
 
-// ---- the teacher -------------------------------------------------------------------------------------------------------------
+// ---- before the products ------------------------------------------------------------------------------------------------------
 
-// A warp per row: q = softmax(logits / T) over the entries, in ascending order of their classes.
-template <class T>
-__global__ void __launch_bounds__(128) teacher_kernel(State s, Entries e, const T* logits, long long m, float c) {
-  __shared__ int ids[4][GELIB_LOSS_MAX_TOP], sorted[4][GELIB_LOSS_MAX_TOP];
-  __shared__ float share[4][GELIB_LOSS_MAX_TOP];
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, top = e.top;
-  const long long row = (long long)blockIdx.x * 4 + warp;
-  if (row >= m) return;
+struct Teacher {
+  const void* logits;   // null: none
+  int type;
+  long long m;
+  float c;
+};
+constexpr int kTeacherRows = kCopyThreads / 32;   // of a block
+long long teacher_shared(int top) { return kTeacherRows * top * 12LL; }
+
+__device__ __forceinline__ float logit_at(const Teacher& t, long long i) {
+  if (t.type == GELIB_F32) return static_cast<const float*>(t.logits)[i];
+  return t.type == GELIB_BF16 ? to_float(static_cast<const __nv_bfloat16*>(t.logits)[i]) : to_float(static_cast<const __half*>(t.logits)[i]);
+}
+
+// A warp per row: q = softmax(logits / T) over the entries, in ascending order of their classes, and where its buckets begin.
+__device__ __forceinline__ void prepare_row(const State& s, const Entries& e, const Teacher& t, long long row, int* ids, int* sorted, float* share) {
+  const int lane = threadIdx.x % 32, top = e.top;
   bool invalid = false, number = true;
   float most = -INFINITY;
   for (int i = lane; i < top; i += 32) {
     const long long id = index_at(e.target, row * top + i, e.index_bytes);
-    const float t = id < 0 ? -INFINITY : to_float(logits[row * top + i]);
+    const float v = id < 0 ? -INFINITY : logit_at(t, row * top + i);
     invalid |= id >= e.n;
-    number &= t == t;
-    ids[warp][i] = id < 0 || id >= e.n ? kNone : (int)id;
-    share[warp][i] = t;
-    most = fmaxf(most, t);
+    number &= v == v;
+    ids[i] = id < 0 || id >= e.n ? kNone : (int)id;
+    share[i] = v;
+    most = fmaxf(most, v);
   }
   invalid = __any_sync(0xffffffffu, invalid), number = __all_sync(0xffffffffu, number);
 #pragma unroll
@@ -77,9 +86,9 @@ __global__ void __launch_bounds__(128) teacher_kernel(State s, Entries e, const 
   float sum = 0;
   for (int i = lane; i < top; i += 32) {
     // a logit of -infinity is no entry; one of +infinity or NaN leaves no number of the row
-    const float q = share[warp][i] == -INFINITY ? 0.f : number ? exp2_of(c * (share[warp][i] - most)) : NAN;
-    share[warp][i] = q;
-    if (q == 0.f) ids[warp][i] = kNone;
+    const float q = share[i] == -INFINITY ? 0.f : number ? exp2_of(t.c * (share[i] - most)) : NAN;
+    share[i] = q;
+    if (q == 0.f) ids[i] = kNone;
     sum += q;
   }
 #pragma unroll
@@ -87,13 +96,13 @@ __global__ void __launch_bounds__(128) teacher_kernel(State s, Entries e, const 
   __syncwarp();
   int live = 0;
   for (int i = lane; i < top; i += 32) {
-    const int id = ids[warp][i];
+    const int id = ids[i];
     int place = 0;
-    for (int j = 0; j < top; j++) place += ids[warp][j] < id || (ids[warp][j] == id && j < i);
+    for (int j = 0; j < top; j++) place += ids[j] < id || (ids[j] == id && j < i);
     live += id != kNone;
-    sorted[warp][place] = id;
+    sorted[place] = id;
     s.ids[row * top + place] = invalid && place == 0 ? kInvalid : id;
-    s.q[row * top + place] = id == kNone ? 0.f : share[warp][i] / sum;
+    s.q[row * top + place] = id == kNone ? 0.f : share[i] / sum;
   }
   live = invalid ? 0 : __reduce_add_sync(0xffffffffu, live);
   __syncwarp();
@@ -101,27 +110,44 @@ __global__ void __launch_bounds__(128) teacher_kernel(State s, Entries e, const 
     int low = 0, high = live;   // the first place whose class is in bucket b or above
     while (low < high && b < e.buckets) {
       const int mid = (low + high) / 2;
-      if (sorted[warp][mid] < b * e.bucket) low = mid + 1;
+      if (sorted[mid] < b * e.bucket) low = mid + 1;
       else high = mid;
     }
     s.starts[row * (e.buckets + 1) + b] = (unsigned short)(b < e.buckets ? low : live);
   }
 }
 
-// ---- before the products ------------------------------------------------------------------------------------------------------
+// The teacher's rows in the first blocks, the operands' copies in the others.
+template <class T>
+__global__ void __launch_bounds__(kCopyThreads) prepare_kernel(const State s, const Entries e, const Teacher t, int teachers, const __grid_constant__ PlaneJobs jobs,
+                                                               const float2* rows_out) {
+  extern __shared__ int shared[];
+  let_next_begin();
+  if ((int)blockIdx.x >= teachers) {
+    copy_planes<T, true>(jobs, blockIdx.x - teachers, gridDim.x - teachers, rows_out);
+    return;
+  }
+  const int warp = threadIdx.x / 32;
+  const long long row = (long long)blockIdx.x * kTeacherRows + warp;
+  int* mine = shared + warp * e.top * 3;
+  if (row < t.m) prepare_row(s, e, t, row, mine, mine + e.top, reinterpret_cast<float*>(mine + 2 * e.top));
+}
 
 template <class T>
-__global__ void __launch_bounds__(kCopyThreads) copy_kernel(const __grid_constant__ PlaneJobs jobs, const float2* rows_out) {
-  let_next_begin();
-  copy_planes<T, true>(jobs, blockIdx.x, gridDim.x, rows_out);
-}
-int launch_copies(const char* fn, const PlaneJobs& jobs, const float2* rows_out, int type, cudaStream_t stream) {
-  if (jobs.count == 0) return GELIB_OK;
-  const unsigned blocks = (unsigned)std::min((jobs.first[jobs.count] + kCopyThreads - 1) / kCopyThreads, 148LL * 8);
-  if (type == GELIB_F32) copy_kernel<float><<<blocks, kCopyThreads, 0, stream>>>(jobs, rows_out);
-  else if (type == GELIB_BF16) copy_kernel<__nv_bfloat16><<<blocks, kCopyThreads, 0, stream>>>(jobs, rows_out);
-  else copy_kernel<__half><<<blocks, kCopyThreads, 0, stream>>>(jobs, rows_out);
+int launch_prepare_as(const char* fn, const State& s, const Entries& e, const Teacher& t, const PlaneJobs& jobs, const float2* rows_out, cudaStream_t stream) {
+  const long long teachers = t.logits ? (t.m + kTeacherRows - 1) / kTeacherRows : 0;
+  const long long blocks = teachers + std::min((jobs.first[jobs.count] + kCopyThreads - 1) / kCopyThreads, 148LL * 8);
+  const size_t shared = t.logits ? (size_t)teacher_shared(e.top) : 0;
+  if (shared > 48 * 1024) {   // asked for anew each time: it is the device's, and the largest is the same for all
+    GELIB_CUDA_TRY(fn, cudaFuncSetAttribute(prepare_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)teacher_shared(GELIB_LOSS_MAX_TOP)));
+  }
+  prepare_kernel<T><<<(unsigned)blocks, kCopyThreads, shared, stream>>>(s, e, t, (int)teachers, jobs, rows_out);
   return launched(fn);
+}
+int launch_prepare(const char* fn, const State& s, const Entries& e, const Teacher& t, const PlaneJobs& jobs, const float2* rows_out, int type, cudaStream_t stream) {
+  if (jobs.count == 0 && !t.logits) return GELIB_OK;
+  return type == GELIB_F32    ? launch_prepare_as<float>(fn, s, e, t, jobs, rows_out, stream)
+         : type == GELIB_BF16 ? launch_prepare_as<__nv_bfloat16>(fn, s, e, t, jobs, rows_out, stream) : launch_prepare_as<__half>(fn, s, e, t, jobs, rows_out, stream);
 }
 
 // The largest |gy|; 1 where that is zero or no finite number.
@@ -271,25 +297,19 @@ int forward(const gelib_linear_loss_args& p, char* at, cudaStream_t stream) {
   const Entries e = entries_of(p, s);
   const float c = slope_of(p);
   int st;
-  if (p.teacher) {
-    const unsigned blocks = (unsigned)((p.m + 3) / 4);
-    if (p.teacher_type == GELIB_F32) teacher_kernel<<<blocks, 128, 0, stream>>>(s, e, (const float*)p.teacher, p.m, c);
-    else if (p.teacher_type == GELIB_BF16) teacher_kernel<<<blocks, 128, 0, stream>>>(s, e, (const __nv_bfloat16*)p.teacher, p.m, c);
-    else teacher_kernel<<<blocks, 128, 0, stream>>>(s, e, (const __half*)p.teacher, p.m, c);
-    if ((st = launched(fn)) != GELIB_OK) return st;
-  }
   ForwardProduct f = forward_of(p);
   const bool few = takes_few(f);
   PlaneJobs jobs = {};
   if (!few) {
     copy_if_needed(&f.x, p.type, at, &jobs);
     copy_if_needed(&f.w, p.type, at, &jobs);
-    if ((st = launch_copies(fn, jobs, nullptr, p.type, stream)) != GELIB_OK) return st;
   }
+  if ((st = launch_prepare(fn, s, e, {p.teacher, p.teacher_type, p.m, c}, jobs, nullptr, p.type, stream)) != GELIB_OK) return st;
+  const bool follows = p.teacher || jobs.count > 0;
   const int parts = parts_of(p), blocks = row_blocks(p.m);
   f.part = (float2*)at, at += up(8LL * parts * p.m);
   f.at_entry = (float*)at, at += up(4 * p.m * p.top);
-  if ((st = few ? launch_few(fn, f, stream) : launch_forward_product(fn, f, jobs.count > 0, stream)) != GELIB_OK) return st;
+  if ((st = few ? launch_few(fn, f, follows, stream) : launch_forward_product(fn, f, follows, stream)) != GELIB_OK) return st;
   const Total total = {p.reduction, (float*)p.loss, s.scale};
   st = launch_after(fn, true, rows_kernel, dim3(blocks), kRowThreads, 0, stream, e, s, (const float2*)f.part, (const float*)f.at_entry, parts, (long long)p.m, c,
                     temperature_of(p), total, (RowSum*)at);
@@ -371,7 +391,7 @@ int backward(const gelib_linear_loss_args& p, char* workspace, cudaStream_t stre
     most_kernel<<<1, 1024, 0, stream>>>((const float*)p.gy, p.m, r.most);
     if ((st = launched(fn)) != GELIB_OK) return st;
   }
-  if ((st = launch_copies(fn, r.jobs, r.rows_out, p.type, stream)) != GELIB_OK) return st;
+  if ((st = launch_prepare(fn, s, entries_of(p, s), {}, r.jobs, r.rows_out, p.type, stream)) != GELIB_OK) return st;
   bool follows = r.jobs.count > 0;
   for (int first = 0; first < p.n; first += r.piece) {
     const int width = std::min(r.piece, p.n - first);

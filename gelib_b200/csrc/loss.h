@@ -50,7 +50,7 @@ int launch_forward_product(const char* fn, const ForwardProduct& p, bool follows
 // The same for a few rows (loss_rows.cu), of x and w as the caller has them.
 bool takes_few(const ForwardProduct& p);
 int few_parts(const ForwardProduct& p);
-int launch_few(const char* fn, const ForwardProduct& p, cudaStream_t stream);
+int launch_few(const char* fn, const ForwardProduct& p, bool follows, cudaStream_t stream);
 
 // z again, of the N classes from `first` on, and of it dz = up g (p - q), which the tensor cores take: 16-bit, or three planes.
 struct SlopeProduct {

@@ -193,26 +193,26 @@ int blocks_of(const ForwardProduct& p, int* per) {
 }
 
 template <class T, int V, int M>
-int launch_rows_as(const char* fn, const RowsArgs& a, bool along, int blocks, cudaStream_t stream) {
+int launch_rows_as(const char* fn, const RowsArgs& a, bool along, int blocks, bool follows, cudaStream_t stream) {
   if (along) {
-    if constexpr (V == 1 || V * sizeof(T) == 16) return launch_after(fn, false, along_kernel<T, V, M>, dim3(blocks), kThreads, 0, stream, a);
+    if constexpr (V == 1 || V * sizeof(T) == 16) return launch_after(fn, follows, along_kernel<T, V, M>, dim3(blocks), kThreads, 0, stream, a);
   }
-  return launch_after(fn, false, across_kernel<T, V, M>, dim3(blocks), kAcrossThreads, 0, stream, a);
+  return launch_after(fn, follows, across_kernel<T, V, M>, dim3(blocks), kAcrossThreads, 0, stream, a);
 }
 template <class T, int V>
-int launch_rows_of(const char* fn, const RowsArgs& a, bool along, int blocks, cudaStream_t stream) {
-  if (a.M == 1) return launch_rows_as<T, V, 1>(fn, a, along, blocks, stream);
-  if (a.M == 2) return launch_rows_as<T, V, 2>(fn, a, along, blocks, stream);
-  if constexpr (sizeof(T) == 4) return a.M <= 4 ? launch_rows_as<T, V, 4>(fn, a, along, blocks, stream) : launch_rows_as<T, V, 8>(fn, a, along, blocks, stream);
+int launch_rows_of(const char* fn, const RowsArgs& a, bool along, int blocks, bool follows, cudaStream_t stream) {
+  if (a.M == 1) return launch_rows_as<T, V, 1>(fn, a, along, blocks, follows, stream);
+  if (a.M == 2) return launch_rows_as<T, V, 2>(fn, a, along, blocks, follows, stream);
+  if constexpr (sizeof(T) == 4) return a.M <= 4 ? launch_rows_as<T, V, 4>(fn, a, along, blocks, follows, stream) : launch_rows_as<T, V, 8>(fn, a, along, blocks, follows, stream);
   return fail(GELIB_INVALID, fn, "too many rows");
 }
 template <class T>
-int launch_rows_type(const char* fn, const RowsArgs& a, bool along, int blocks, int V, cudaStream_t stream) {
+int launch_rows_type(const char* fn, const RowsArgs& a, bool along, int blocks, int V, bool follows, cudaStream_t stream) {
   if constexpr (sizeof(T) == 2)
-    if (V == 8) return launch_rows_of<T, 8>(fn, a, along, blocks, stream);
-  if (V == 4) return launch_rows_of<T, 4>(fn, a, along, blocks, stream);
-  if (V == 2) return launch_rows_of<T, 2>(fn, a, along, blocks, stream);
-  return launch_rows_of<T, 1>(fn, a, along, blocks, stream);
+    if (V == 8) return launch_rows_of<T, 8>(fn, a, along, blocks, follows, stream);
+  if (V == 4) return launch_rows_of<T, 4>(fn, a, along, blocks, follows, stream);
+  if (V == 2) return launch_rows_of<T, 2>(fn, a, along, blocks, follows, stream);
+  return launch_rows_of<T, 1>(fn, a, along, blocks, follows, stream);
 }
 
 }  // namespace
@@ -225,12 +225,12 @@ int few_parts(const ForwardProduct& p) {
   return blocks_of(p, &per);
 }
 
-int launch_few(const char* fn, const ForwardProduct& p, cudaStream_t stream) {
+int launch_few(const char* fn, const ForwardProduct& p, bool follows, cudaStream_t stream) {
   RowsArgs a = {p.x.base, p.w.base, p.bias, p.x.ld, p.w.ld, (int)p.M, p.N, p.K, p.e, p.c, p.part, p.at_entry, 0};
   const int blocks = blocks_of(p, &a.per), V = width_of(p);
   const bool along = !p.w_by_sum;
-  return p.type == GELIB_F32    ? launch_rows_type<float>(fn, a, along, blocks, V, stream)
-         : p.type == GELIB_BF16 ? launch_rows_type<__nv_bfloat16>(fn, a, along, blocks, V, stream) : launch_rows_type<__half>(fn, a, along, blocks, V, stream);
+  return p.type == GELIB_F32    ? launch_rows_type<float>(fn, a, along, blocks, V, follows, stream)
+         : p.type == GELIB_BF16 ? launch_rows_type<__nv_bfloat16>(fn, a, along, blocks, V, follows, stream) : launch_rows_type<__half>(fn, a, along, blocks, V, follows, stream);
 }
 
 }  // namespace gelib_b200
