@@ -115,11 +115,12 @@ SYMBOLS = {
     "gelib_linear_workspace": (ctypes.c_longlong, [ctypes.POINTER(LinearArgs), ctypes.c_int]),
     "gelib_linear": (ctypes.c_int, [ctypes.POINTER(LinearArgs), ctypes.c_void_p, ctypes.c_void_p]),
     "gelib_linear_back": (ctypes.c_int, [ctypes.POINTER(LinearArgs), ctypes.c_void_p, ctypes.c_void_p]),
-    "gelib_embedding": (ctypes.c_int, [ctypes.c_void_p] * 3 + [ctypes.c_longlong, ctypes.c_int, ctypes.c_int, ctypes.c_longlong, ctypes.c_double]
-                        + [ctypes.c_int] * 2 + [ctypes.c_void_p]),
+    "gelib_embedding_state_bytes": (ctypes.c_longlong, [ctypes.c_longlong, ctypes.c_int]),
+    "gelib_embedding": (ctypes.c_int, [ctypes.c_void_p] * 3 + [ctypes.c_longlong, ctypes.c_int, ctypes.c_int, ctypes.c_longlong, ctypes.c_double, ctypes.c_longlong]
+                        + [ctypes.c_int] * 2 + [ctypes.c_void_p] * 2),
     "gelib_embedding_workspace": (ctypes.c_longlong, [ctypes.c_longlong] + [ctypes.c_int] * 3),
-    "gelib_embedding_back": (ctypes.c_int, [ctypes.c_void_p] * 3 + [ctypes.c_longlong, ctypes.c_int, ctypes.c_int, ctypes.c_double, ctypes.c_longlong]
-                             + [ctypes.c_int] * 2 + [ctypes.c_void_p] * 2),
+    "gelib_embedding_back": (ctypes.c_int, [ctypes.c_void_p] * 3 + [ctypes.c_longlong, ctypes.c_int, ctypes.c_int, ctypes.c_double, ctypes.c_int]
+                             + [ctypes.c_void_p] * 2),
     "gelib_linear_loss_state_bytes": (ctypes.c_longlong, [ctypes.POINTER(LinearLossArgs)]),
     "gelib_linear_loss_workspace": (ctypes.c_longlong, [ctypes.POINTER(LinearLossArgs), ctypes.c_int]),
     "gelib_linear_loss": (ctypes.c_int, [ctypes.POINTER(LinearLossArgs), ctypes.c_void_p, ctypes.c_void_p]),

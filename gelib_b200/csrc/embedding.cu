@@ -32,12 +32,8 @@ Teams teams_of(int d) {
 // A team looks up kRows rows that follow one another, so that as many are on their way at a time.
 constexpr int kRows = 4;
 template <class T, int V>
-__global__ void __launch_bounds__(kThreads) embedding_kernel(const EmbeddingCall c, Teams t) {
+__device__ __forceinline__ void look_up(const EmbeddingCall& c, long long i0, int col) {
   using R = typename Raw<V * sizeof(T)>::type;
-  const long long team = ((long long)blockIdx.x * kThreads + threadIdx.x) / t.lanes, group = team / t.slabs;
-  const int col = ((int)(team - group * t.slabs) * t.lanes + threadIdx.x % t.lanes) * V;
-  const long long i0 = group * kRows;
-  if (i0 >= c.n || col >= c.d) return;
   long long id[kRows];
   R raw[kRows];
 #pragma unroll
@@ -58,6 +54,14 @@ __global__ void __launch_bounds__(kThreads) embedding_kernel(const EmbeddingCall
     }
     store_vec<T, V>(static_cast<T*>(c.y) + (i0 + j) * c.d + col, x);
   }
+}
+
+template <class T, int V>
+__global__ void __launch_bounds__(kThreads) embedding_kernel(const EmbeddingCall c, Teams t) {
+  const long long team = ((long long)blockIdx.x * kThreads + threadIdx.x) / t.lanes, group = team / t.slabs, i0 = group * kRows;
+  const int col = ((int)(team - group * t.slabs) * t.lanes + threadIdx.x % t.lanes) * V;
+  if (i0 < c.n && col < c.d) look_up<T, V>(c, i0, col);
+  await_previous();   // the sort that this kernel runs beside: what comes after the two follows this one
 }
 
 // ---- the numbers in order -----------------------------------------------------------------------------------------------------
@@ -81,7 +85,6 @@ struct Sort {
   const void* ids;          // of the first pass
   unsigned *keys[2], *places[2];
   int* counts;              // (blocks, digits)
-  int* heads;               // its first is set to zero
   long long n, padding, per;   // per: numbers of a block
   int index_bytes, v, passes, bits, blocks;
 };
@@ -217,7 +220,6 @@ __global__ void __launch_bounds__(kSortThreads) cluster_sort_kernel(const Sort s
   const long long i0 = min(s.n, block * s.per);
   const int count = (int)(min(s.n, i0 + s.per) - i0);
   let_next_begin();
-  if (block == 0 && threadIdx.x == 0) *s.heads = 0;
   cluster_sync();   // all blocks are there
   for (int pass = 0; pass < s.passes; pass++) {
     Tile t;
@@ -245,7 +247,6 @@ __global__ void __launch_bounds__(kSortThreads) count_kernel(const Sort s, int p
   const int digits = 1 << s.bits, shift = pass * s.bits;
   let_next_begin();
   await_previous();
-  if (pass == 0 && blockIdx.x == 0 && threadIdx.x == 0) *s.heads = 0;
   hist[threadIdx.x] = 0;
   __syncthreads();
   const long long i0 = blockIdx.x * s.per, i1 = min(s.n, i0 + s.per);
@@ -293,7 +294,7 @@ struct Reduce {
   void* gw;
   const void* gy;
   float* part;            // (stretches, 2, d): of what came before the stretch, of what goes on behind it
-  int* heads;             // a count, then the stretches in which something begins that is cut
+  int* heads;             // of every stretch: whether something begins there that is cut
   long long n, stretches;
   int v, d, per;          // per: numbers of a stretch, a multiple of kBatch
   Teams teams;
@@ -333,6 +334,9 @@ __device__ __forceinline__ void add_stretch(const Reduce& a, long long team, int
   const T* gy = static_cast<const T*>(a.gy) + col;
   T* gw = static_cast<T*>(a.gw) + col;
   const int count = (int)min((long long)a.per, a.n - i0);
+  const auto head = [&](int cut) {
+    if (slab == 0 && lane == 0) a.heads[stretch] = cut;
+  };
   const unsigned* keys = a.keys + i0;
   unsigned cur = keys[0];
   bool whole = true, skip = false;    // what is being added began here; it is another team's
@@ -387,10 +391,10 @@ __device__ __forceinline__ void add_stretch(const Reduce& a, long long team, int
       }
     }
   }
-  if (cur >= (unsigned)a.v || skip) return;
   const long long i1 = i0 + count;
   const bool goes_on = i1 < a.n && a.keys[i1] == cur;
-  if (goes_on && whole) {
+  int cut = 0;
+  if (goes_on && whole && !skip && cur < (unsigned)a.v) {
     if (!is_long(a, i1, cur)) {   // the rest of it too
       for (int i = count; i0 + i < a.n; i += kBatch) {
         R raw[kBatch];
@@ -409,11 +413,13 @@ __device__ __forceinline__ void add_stretch(const Reduce& a, long long team, int
         if (live < kBatch) break;
       }
       put(false);
+      head(0);
       return;
     }
-    if (slab == 0 && lane == 0) a.heads[1 + atomicAdd(a.heads, 1)] = (int)stretch;
+    cut = 1;
   }
   put(goes_on);
+  head(cut);
 }
 
 template <class T, int V>
@@ -445,53 +451,67 @@ __global__ void __launch_bounds__(kThreads) reduce_kernel(const Reduce a) {
   }
 }
 
-// A block joins the parts of a row and 32 V of its columns, for one after another of what was cut (in whatever order: each is added up by itself): 32
-// warps take parts in turn, their sums are added in order.
+// A block joins the parts of a row and 32 V of its columns: 32 warps take parts in turn, their sums are added in order.  Blocks take every so many-th of
+// the stretches, a thousand at a time, and of these what is cut.
 constexpr int kJoinThreads = 1024, kJoinWarps = kJoinThreads / 32;
 template <class T, int V>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Reduce a) {
   __shared__ float of[kJoinWarps / 2][32 * V];
+  __shared__ int heads[kJoinThreads], found[kJoinWarps];
   await_previous();
   const int slabs = (a.d + 32 * V - 1) / (32 * V), lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  const long long all = (long long)*a.heads * slabs;
-  for (long long h = blockIdx.x; h < all; h += gridDim.x) {
-    const long long stretch = a.heads[1 + h / slabs], i1 = (stretch + 1) * a.per;
-    const int col = ((int)(h % slabs) * 32 + lane) * V;
-    const unsigned cur = a.keys[i1];
-    long long low = i1, high = a.n;   // the first place that is not the row's, by 32 places at a time: low is the row's, high is not
-    while (high - low > 1) {
-      const long long step = (high - low + 32) / 33, at = low + (lane + 1) * step;
-      const int same = __popc(__ballot_sync(0xffffffffu, at < high && a.keys[min(at, a.n - 1)] == cur));
-      const long long past = low + (same + 1) * step;
-      low += same * step;
-      high = min(high, past);
-    }
-    const long long last = low / a.per;
-    float s[V];
-#pragma unroll
-    for (int k = 0; k < V; k++) s[k] = 0;
-    if (col < a.d)
-#pragma unroll 8
-      for (long long p = stretch + warp; p <= last; p += kJoinWarps) {
-        float g[V];
-        load_part<V>(a.part + (p * 2 + (p == stretch)) * a.d + col, g);
-        add_all(s, s, g);
+  const long long all = a.stretches * slabs;
+  for (long long h0 = blockIdx.x; h0 < all; h0 += (long long)gridDim.x * kJoinThreads) {
+    // what is cut among the next thousand of the block's, in order
+    const long long mine = h0 + (long long)threadIdx.x * gridDim.x;
+    const bool cut = mine < all && a.heads[mine / slabs];
+    const unsigned cuts = __ballot_sync(0xffffffffu, cut);
+    if (lane == 0) found[warp] = __popc(cuts);
+    __syncthreads();
+    int before = 0, count = 0;
+    for (int w = 0; w < kJoinWarps; w++) before += w < warp ? found[w] : 0, count += found[w];
+    if (cut) heads[before + __popc(cuts & ((1u << lane) - 1))] = threadIdx.x;
+    __syncthreads();
+    for (int k = 0; k < count; k++) {
+      const long long h = h0 + (long long)heads[k] * gridDim.x, stretch = h / slabs, i1 = (stretch + 1) * a.per;
+      const int col = ((int)(h % slabs) * 32 + lane) * V;
+      const unsigned cur = a.keys[i1];
+      long long low = i1, high = a.n;   // the first place that is not the row's, by 32 places at a time: low is the row's, high is not
+      while (high - low > 1) {
+        const long long step = (high - low + 32) / 33, at = low + (lane + 1) * step;
+        const int same = __popc(__ballot_sync(0xffffffffu, at < high && a.keys[min(at, a.n - 1)] == cur));
+        const long long past = low + (same + 1) * step;
+        low += same * step;
+        high = min(high, past);
       }
+      const long long last = low / a.per;
+      float s[V];
 #pragma unroll
-    for (int half = kJoinWarps / 2; half; half /= 2) {
-      if (warp >= half && warp < 2 * half)
+      for (int k = 0; k < V; k++) s[k] = 0;
+      if (col < a.d)
+#pragma unroll 8
+        for (long long p = stretch + warp; p <= last; p += kJoinWarps) {
+          float g[V];
+          load_part<V>(a.part + (p * 2 + (p == stretch)) * a.d + col, g);
+          add_all(s, s, g);
+        }
 #pragma unroll
-        for (int k = 0; k < V; k++) of[warp - half][k * 32 + lane] = s[k];
-      __syncthreads();
-      if (warp < half)
+      for (int half = kJoinWarps / 2; half; half /= 2) {
+        if (warp >= half && warp < 2 * half)
 #pragma unroll
-        for (int k = 0; k < V; k++) s[k] += of[warp][k * 32 + lane];
-      __syncthreads();
+          for (int k = 0; k < V; k++) of[warp - half][k * 32 + lane] = s[k];
+        __syncthreads();
+        if (warp < half)
+#pragma unroll
+          for (int k = 0; k < V; k++) s[k] += of[warp][k * 32 + lane];
+        __syncthreads();
+      }
+      if (warp == 0 && col < a.d) {
+        mul_all(s, s, a.scale);
+        store_vec<T, V>(static_cast<T*>(a.gw) + (long long)cur * a.d + col, s);
+      }
     }
-    if (warp == 0 && col < a.d) {
-      mul_all(s, s, a.scale);
-      store_vec<T, V>(static_cast<T*>(a.gw) + (long long)cur * a.d + col, s);
-    }
+    __syncthreads();
   }
 }
 
@@ -510,14 +530,14 @@ int with_width(long long d, long long ld, std::initializer_list<const void*> p, 
 }
 
 template <class T>
-int launch_forward_as(const EmbeddingCall& c, cudaStream_t stream) {
+int launch_forward_as(const EmbeddingCall& c, bool beside, cudaStream_t stream) {
+  if (c.d == 0) return GELIB_OK;
   return with_width<T>(c.d, c.ldw, {c.y, c.weight}, [&](auto width) -> int {
     constexpr int V = decltype(width)::value;
     const Teams t = teams_of<V>(c.d);
     const long long blocks = ((c.n + kRows - 1) / kRows * t.slabs * t.lanes + kThreads - 1) / kThreads;
     if (blocks > 0x7fffffffLL) return fail(GELIB_INVALID, "embedding", "too many elements");
-    embedding_kernel<T, V><<<(unsigned)blocks, kThreads, 0, stream>>>(c, t);
-    return launched("embedding");
+    return launch_after("embedding", beside, embedding_kernel<T, V>, dim3((unsigned)blocks), kThreads, 0, stream, c, t);
   });
 }
 
@@ -578,48 +598,43 @@ int stretch_of(long long n, int d) {
   return (int)std::min(256LL, std::max<long long>(16, (n / std::max(1LL, teams) + kBatch - 1) / kBatch * kBatch));
 }
 
-struct Room {
-  long long keys, counts, heads, part, bytes;
-};
-Room room_of(long long n, int d, int v, int per) {
-  int passes, bits;
-  digits_of(v, &passes, &bits);
-  const long long blocks = sort_blocks(n), stretches = (n + per - 1) / per;
-  Room r;
-  r.keys = up(4 * (n + kBatch));
-  r.counts = n > kClusterNumbers ? up((4LL << bits) * blocks) : 0;
-  r.heads = up(4 * (1 + stretches));
-  r.part = up(stretches * 2 * d * 4);
-  r.bytes = 4 * r.keys + r.counts + r.heads + r.part;
-  return r;
+// The state: twice two arrays of numbers, of which the last pass's stay, and the blocks' counts.
+Sort sort_of(long long n, int v, void* state, long long* bytes) {
+  Sort s = {};
+  s.n = n, s.v = v;
+  digits_of(v, &s.passes, &s.bits);
+  s.blocks = (int)sort_blocks(n);
+  s.per = (n + s.blocks - 1) / s.blocks;
+  char* at = (char*)state;
+  const long long each = up(4 * (n + kBatch));
+  for (int i = 0; i < 2; i++) s.keys[i] = (unsigned*)(at + 2 * i * each), s.places[i] = (unsigned*)(at + (2 * i + 1) * each);
+  s.counts = (int*)(at + 4 * each);
+  if (bytes) *bytes = 4 * each + (n > kClusterNumbers ? up((4LL << s.bits) * s.blocks) : 0);
+  return s;
+}
+
+long long workspace_of(long long n, int d, int per) {
+  const long long stretches = (n + per - 1) / per;
+  return up(4 * stretches) + up(stretches * 2 * d * 4);
 }
 
 template <class T>
-int launch_backward_as(const EmbeddingCall& c, char* at, cudaStream_t stream) {
+int launch_backward_as(const EmbeddingCall& c, const void* state, char* at, cudaStream_t stream) {
   static const char* fn = "embedding_back";
   return with_width<T>(c.d, c.d, {c.gw, c.gy}, [&](auto width) -> int {
     constexpr int V = decltype(width)::value;
     Reduce a = {};
     a.teams = teams_of<V>(c.d);
     a.per = stretch_of<V>(c.n, c.d);
-    const Room r = room_of(c.n, c.d, c.v, a.per);
-    Sort s = {};
-    s.ids = c.ids, s.n = c.n, s.padding = c.padding, s.index_bytes = c.index_bytes, s.v = c.v;
-    for (int i = 0; i < 2; i++) s.keys[i] = (unsigned*)(at + 2 * i * r.keys), s.places[i] = (unsigned*)(at + (2 * i + 1) * r.keys);
-    s.counts = (int*)(at + 4 * r.keys);
-    s.heads = (int*)(at + 4 * r.keys + r.counts);
-    digits_of(c.v, &s.passes, &s.bits);
-    s.blocks = (int)sort_blocks(c.n);
-    s.per = (c.n + s.blocks - 1) / s.blocks;
-    int st = launch_sort(fn, s, stream);
-    if (st != GELIB_OK) return st;
-    a.keys = s.keys[(s.passes - 1) & 1], a.places = s.places[(s.passes - 1) & 1], a.heads = s.heads;
-    a.gw = c.gw, a.gy = c.gy, a.part = (float*)(at + 4 * r.keys + r.counts + r.heads);
+    const Sort s = sort_of(c.n, c.v, const_cast<void*>(state), nullptr);
+    a.keys = s.keys[(s.passes - 1) & 1], a.places = s.places[(s.passes - 1) & 1];
     a.n = c.n, a.stretches = (c.n + a.per - 1) / a.per, a.v = c.v, a.d = c.d, a.scale = c.scale;
+    a.heads = (int*)at;
+    a.gw = c.gw, a.gy = c.gy, a.part = (float*)(at + up(4 * a.stretches));
     a.blocks = (a.stretches * a.teams.slabs * a.teams.lanes + kThreads - 1) / kThreads;
     const long long blocks = a.blocks + ((long long)c.v + kThreads - 1) / kThreads, cuts = c.n / kShort * ((c.d + 32 * V - 1) / (32 * V));
     if (blocks > 0x7fffffffLL) return fail(GELIB_INVALID, fn, "too many elements");
-    st = launch_after(fn, true, reduce_kernel<T, V>, dim3((unsigned)blocks), kThreads, 0, stream, a);
+    int st = launch_after(fn, false, reduce_kernel<T, V>, dim3((unsigned)blocks), kThreads, 0, stream, a);
     if (st != GELIB_OK || c.n <= kShort || a.stretches == 1) return st;   // nothing is cut
     return launch_after(fn, true, join_kernel<T, V>, dim3((unsigned)std::min(cuts, 296LL)), kJoinThreads, 0, stream, a);
   });
@@ -627,22 +642,37 @@ int launch_backward_as(const EmbeddingCall& c, char* at, cudaStream_t stream) {
 
 }  // namespace
 
-long long embedding_workspace(long long n, int v, int d, int type) {
-  long long bytes = 0;
-  // the alignment of the call is not known here
-  for (int per : {stretch_of<1>(n, d), stretch_of<2>(n, d), stretch_of<4>(n, d), type == GELIB_F32 ? 256 : stretch_of<8>(n, d)})
-    bytes = std::max(bytes, room_of(n, d, v, per).bytes);
+long long embedding_state_bytes(long long n, int v) {
+  long long bytes;
+  sort_of(n, v, nullptr, &bytes);
   return bytes;
 }
 
-int launch_embedding(const EmbeddingCall& c, cudaStream_t stream) {
-  return c.type == GELIB_F32 ? launch_forward_as<float>(c, stream) : c.type == GELIB_BF16 ? launch_forward_as<__nv_bfloat16>(c, stream) : launch_forward_as<__half>(c, stream);
+long long embedding_workspace(long long n, int, int d, int type) {
+  long long bytes = 0;
+  // the alignment of the call is not known here
+  for (int per : {stretch_of<1>(n, d), stretch_of<2>(n, d), stretch_of<4>(n, d), type == GELIB_F32 ? 256 : stretch_of<8>(n, d)})
+    bytes = std::max(bytes, workspace_of(n, d, per));
+  return bytes;
 }
 
-int launch_embedding_back(const EmbeddingCall& c, void* workspace, cudaStream_t stream) {
+// The sort takes eight SMs and has nothing to do with the rows, so the two run side by side.
+int launch_embedding(const EmbeddingCall& c, void* state, cudaStream_t stream) {
+  if (state) {
+    Sort s = sort_of(c.n, c.v, state, nullptr);
+    s.ids = c.ids, s.padding = c.padding, s.index_bytes = c.index_bytes;
+    const int st = launch_sort("embedding", s, stream);
+    if (st != GELIB_OK) return st;
+  }
+  const bool beside = state != nullptr;
+  return c.type == GELIB_F32    ? launch_forward_as<float>(c, beside, stream)
+         : c.type == GELIB_BF16 ? launch_forward_as<__nv_bfloat16>(c, beside, stream) : launch_forward_as<__half>(c, beside, stream);
+}
+
+int launch_embedding_back(const EmbeddingCall& c, const void* state, void* workspace, cudaStream_t stream) {
   char* at = (char*)workspace;
-  return c.type == GELIB_F32    ? launch_backward_as<float>(c, at, stream)
-         : c.type == GELIB_BF16 ? launch_backward_as<__nv_bfloat16>(c, at, stream) : launch_backward_as<__half>(c, at, stream);
+  return c.type == GELIB_F32    ? launch_backward_as<float>(c, state, at, stream)
+         : c.type == GELIB_BF16 ? launch_backward_as<__nv_bfloat16>(c, state, at, stream) : launch_backward_as<__half>(c, state, at, stream);
 }
 
 }  // namespace gelib_b200

@@ -13,9 +13,10 @@ struct EmbeddingCall {
   int v, d, index_bytes, type;
   float scale;
 };
+long long embedding_state_bytes(long long n, int v);
 long long embedding_workspace(long long n, int v, int d, int type);
-int launch_embedding(const EmbeddingCall& c, cudaStream_t stream);
-int launch_embedding_back(const EmbeddingCall& c, void* workspace, cudaStream_t stream);
+int launch_embedding(const EmbeddingCall& c, void* state, cudaStream_t stream);
+int launch_embedding_back(const EmbeddingCall& c, const void* state, void* workspace, cudaStream_t stream);
 
 long long linear_loss_state_bytes(const gelib_linear_loss_args& p);
 long long linear_loss_workspace(const gelib_linear_loss_args& p, bool backward);

@@ -20,11 +20,10 @@ int guarded(const char* fn, F f) {
   }
 }
 
-int check_embedding(const char* fn, long long n, int v, int d, int index_bytes, int type) {
+int check_embedding(const char* fn, long long n, int v, int d, int type) {
   if (n < 0 || v < 0 || d < 0) return fail(GELIB_INVALID, fn, "negative size");
   if (n > 1LL << 30 || v > 1 << 30 || d > 1 << 20) return fail(GELIB_INVALID, fn, "more than 2^30 rows, or more than 2^20 columns");
   if (!known_type(type)) return fail(GELIB_INVALID, fn, "unknown type");
-  if (index_bytes != 8 && index_bytes != 4) return fail(GELIB_INVALID, fn, "numbers of rows have 8 or 4 bytes");
   return GELIB_OK;
 }
 
@@ -53,17 +52,21 @@ int check_loss(const char* fn, const gelib_linear_loss_args* p, bool back) {
 
 extern "C" {
 
-int gelib_embedding(void* y, const void* ids, const void* weight, long long n, int v, int d, long long ldw, double scale, int index_bytes, int type,
-                    void* stream) {
+long long gelib_embedding_state_bytes(long long n, int v) { return n > 0 && v > 0 && n <= 1LL << 30 && v <= 1 << 30 ? embedding_state_bytes(n, v) : 0; }
+
+int gelib_embedding(void* y, const void* ids, const void* weight, long long n, int v, int d, long long ldw, double scale, long long padding, int index_bytes,
+                    int type, void* state, void* stream) {
   static const char* fn = "embedding";
   return guarded(fn, [&]() -> int {
-    const int st = check_embedding(fn, n, v, d, index_bytes, type);
-    if (st != GELIB_OK || n == 0 || d == 0) return st;
-    if (!y || !ids || (v && !weight)) return fail(GELIB_INVALID, fn, "null pointer");
+    const int st = check_embedding(fn, n, v, d, type);
+    if (st != GELIB_OK || n == 0) return st;
+    if (index_bytes != 8 && index_bytes != 4) return fail(GELIB_INVALID, fn, "numbers of rows have 8 or 4 bytes");
+    if (!ids || (d && (!y || (v && !weight)))) return fail(GELIB_INVALID, fn, "null pointer");
     if (ldw < d) return fail(GELIB_INVALID, fn, "rows overlap");
     if (!is_aligned(y, type_bytes(type)) || !is_aligned(weight, type_bytes(type)) || !is_aligned(ids, index_bytes))
       return fail(GELIB_INVALID, fn, "data pointer not aligned to its type");
-    return launch_embedding({y, nullptr, ids, weight, nullptr, n, ldw, -1, v, d, index_bytes, type, (float)scale}, (cudaStream_t)stream);
+    if (!is_aligned(state, 256)) return fail(GELIB_INVALID, fn, "the state is not 256-byte aligned");
+    return launch_embedding({y, nullptr, ids, weight, nullptr, n, ldw, padding, v, d, index_bytes, type, (float)scale}, v ? state : nullptr, (cudaStream_t)stream);
   });
 }
 
@@ -72,21 +75,20 @@ long long gelib_embedding_workspace(long long n, int v, int d, int type) {
   return embedding_workspace(n, v, d, type);
 }
 
-int gelib_embedding_back(void* gw, const void* gy, const void* ids, long long n, int v, int d, double scale, long long padding, int index_bytes, int type,
-                         void* workspace, void* stream) {
+int gelib_embedding_back(void* gw, const void* gy, const void* state, long long n, int v, int d, double scale, int type, void* workspace, void* stream) {
   static const char* fn = "embedding_back";
   return guarded(fn, [&]() -> int {
-    const int st = check_embedding(fn, n, v, d, index_bytes, type);
+    const int st = check_embedding(fn, n, v, d, type);
     if (st != GELIB_OK || v == 0 || d == 0) return st;
-    if (!gw || (n && (!gy || !ids))) return fail(GELIB_INVALID, fn, "null pointer");
-    if (!is_aligned(gw, type_bytes(type)) || !is_aligned(gy, type_bytes(type)) || !is_aligned(ids, index_bytes) || !is_aligned(workspace, 256))
-      return fail(GELIB_INVALID, fn, "data pointer not aligned to its type");
+    if (!gw || (n && (!gy || !state))) return fail(GELIB_INVALID, fn, "null pointer");
+    if (!is_aligned(gw, type_bytes(type)) || !is_aligned(gy, type_bytes(type))) return fail(GELIB_INVALID, fn, "data pointer not aligned to its type");
+    if (!is_aligned(workspace, 256) || !is_aligned(state, 256)) return fail(GELIB_INVALID, fn, "the workspace or the state is not 256-byte aligned");
     if (n == 0) {
       GELIB_CUDA_TRY(fn, cudaMemsetAsync(gw, 0, (size_t)v * d * type_bytes(type), (cudaStream_t)stream));
       return GELIB_OK;
     }
     if (!workspace && embedding_workspace(n, v, d, type) > 0) return fail(GELIB_INVALID, fn, "no workspace");
-    return launch_embedding_back({nullptr, gw, ids, nullptr, gy, n, 0, padding, v, d, index_bytes, type, (float)scale}, workspace, (cudaStream_t)stream);
+    return launch_embedding_back({nullptr, gw, nullptr, nullptr, gy, n, 0, -1, v, d, 8, type, (float)scale}, state, workspace, (cudaStream_t)stream);
   });
 }
 

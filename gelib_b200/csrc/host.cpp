@@ -529,42 +529,45 @@ bool plain_numbers(const at::Tensor& t, c10::Device device) {
   return t.defined() && t.device() == device && t.layout() == at::kStrided && (t.scalar_type() == at::kLong || t.scalar_type() == at::kInt);
 }
 
-at::Tensor embedding_call(const at::Tensor& ids, const at::Tensor& w, double scale) {
+// state: for the gradient, or undefined.
+at::Tensor embedding_call(const at::Tensor& ids, const at::Tensor& w, double scale, int64_t padding, at::Tensor* state) {
   c10::cuda::CUDAGuard guard(w.device());
   const int64_t n = ids.numel(), d = w.size(1);
+  const int v = static_cast<int>(w.size(0));
   c10::SmallVector<int64_t, 6> shape(ids.sizes().begin(), ids.sizes().end());
   shape.push_back(d);
   const at::Tensor y = at::empty(shape, w.options());
-  void* s = stream_of(w.device());
+  if (state) *state = workspace(gelib_embedding_state_bytes(n, v), w);
+  void *s = stream_of(w.device()), *kept = state ? ptr(*state) : nullptr;
   const int type = *type_code(w.scalar_type()), bytes = static_cast<int>(ids.element_size());
-  call([&] { return gelib_embedding(ptr(y), ptr(ids), ptr(w), n, static_cast<int>(w.size(0)), static_cast<int>(d), std::max(w.stride(0), d), scale, bytes, type, s); });
+  call([&] { return gelib_embedding(ptr(y), ptr(ids), ptr(w), n, v, static_cast<int>(d), std::max(w.stride(0), d), scale, padding, bytes, type, kept, s); });
   return y;
 }
 
 struct EmbeddingFunction : torch::autograd::Function<EmbeddingFunction> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& ids, const at::Tensor& w, double scale, int64_t padding) {
-    ctx->save_for_backward({ids});
+    at::Tensor state, y = embedding_call(ids, w, scale, padding, &state);
+    ctx->save_for_backward({state});
+    ctx->saved_data["n"] = ids.numel();
     ctx->saved_data["v"] = w.size(0);
     ctx->saved_data["d"] = w.size(1);
     ctx->saved_data["scale"] = scale;
-    ctx->saved_data["padding"] = padding;
-    return embedding_call(ids, w, scale);
+    return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     variable_list out(4);
     if (!grads[0].defined()) return out;
     {
       const at::NoGradGuard off;
-      const at::Tensor ids = ctx->get_saved_variables()[0], gy = grads[0].resolve_neg().contiguous();
+      const at::Tensor state = ctx->get_saved_variables()[0], gy = grads[0].resolve_neg().contiguous();
       c10::cuda::CUDAGuard guard(gy.device());
-      const int64_t n = ids.numel(), padding = ctx->saved_data["padding"].toInt();
-      const int v = static_cast<int>(ctx->saved_data["v"].toInt()), d = static_cast<int>(ctx->saved_data["d"].toInt());
-      const int type = *type_code(gy.scalar_type()), bytes = static_cast<int>(ids.element_size());
+      const int64_t n = ctx->saved_data["n"].toInt();
+      const int v = static_cast<int>(ctx->saved_data["v"].toInt()), d = static_cast<int>(ctx->saved_data["d"].toInt()), type = *type_code(gy.scalar_type());
       const double scale = ctx->saved_data["scale"].toDouble();
       out[1] = at::empty({v, d}, gy.options());
       const at::Tensor space = workspace(gelib_embedding_workspace(n, v, d, type), gy);
       void* s = stream_of(gy.device());
-      call([&] { return gelib_embedding_back(ptr(out[1]), ptr(gy), ptr(ids), n, v, d, scale, padding, bytes, type, ptr(space), s); });
+      call([&] { return gelib_embedding_back(ptr(out[1]), ptr(gy), ptr(state), n, v, d, scale, type, ptr(space), s); });
     }
     return differentiable_once(std::move(out), "embedding");
   }
@@ -577,7 +580,7 @@ std::optional<at::Tensor> embedding(const at::Tensor& ids, const at::Tensor& w, 
   if (padding_idx && (*padding_idx < -v || *padding_idx >= v)) return std::nullopt;
   const int64_t padding = padding_idx ? (*padding_idx < 0 ? *padding_idx + v : *padding_idx) : -1;
   if (at::GradMode::is_enabled() && w.requires_grad()) return EmbeddingFunction::apply(ids, w, scale, padding);
-  return embedding_call(ids, w, scale);
+  return embedding_call(ids, w, scale, padding, nullptr);
 }
 
 struct LossCall {

@@ -28,7 +28,7 @@ namespace {
 constexpr int kThreads = 256;
 
 // Buckets of a row's classes: 128 at the most.
-int bucket_of(int n) { return (n / 128 + 256) / 256 * 256; }
+int bucket_of(int n) { return (int)((n + 32767LL) / 32768) * 256; }
 int buckets_of(int n) { return (n + bucket_of(n) - 1) / bucket_of(n); }
 
 // The state and its bytes; p.state may be null.

@@ -45,12 +45,14 @@ class EmbeddingFn(torch.autograd.Function):
     def forward(ctx, ids, weight, scale, padding):
         ids, weight = ids.contiguous(), _rows(weight)
         v, d = weight.shape
-        y = torch.empty(ids.numel(), d, dtype=weight.dtype, device=weight.device)
+        n = ids.numel()
+        y = torch.empty(n, d, dtype=weight.dtype, device=weight.device)
+        state = _workspace(lib().gelib_embedding_state_bytes(n, v), weight) if ctx.needs_input_grad[1] else None
         with device_guard(weight):
-            check(lib().gelib_embedding(_ptr(y), _ptr(ids), _ptr(weight), ids.numel(), v, d, max(weight.stride(0), d), scale, ids.element_size(),
-                                        _TYPES[weight.dtype], stream_of(weight)))
-        ctx.save_for_backward(ids)
-        ctx.sizes, ctx.scale, ctx.padding = (v, d), scale, padding
+            check(lib().gelib_embedding(_ptr(y), _ptr(ids), _ptr(weight), n, v, d, max(weight.stride(0), d), scale, padding, ids.element_size(),
+                                        _TYPES[weight.dtype], _ptr(state), stream_of(weight)))
+        ctx.save_for_backward(state)
+        ctx.sizes, ctx.scale = (n, v, d), scale
         return y
 
     @staticmethod
@@ -61,14 +63,13 @@ class EmbeddingFn(torch.autograd.Function):
 
     @staticmethod
     def gradient(ctx, gy):
-        ids, = ctx.saved_tensors
+        state, = ctx.saved_tensors
         gy = _dense(gy)
-        v, d = ctx.sizes
+        n, v, d = ctx.sizes
         gw = torch.empty(v, d, dtype=gy.dtype, device=gy.device)
         with device_guard(gy):
-            w = _workspace(lib().gelib_embedding_workspace(ids.numel(), v, d, _TYPES[gy.dtype]), gy)
-            check(lib().gelib_embedding_back(_ptr(gw), _ptr(gy), _ptr(ids), ids.numel(), v, d, ctx.scale, ctx.padding, ids.element_size(),
-                                             _TYPES[gy.dtype], _ptr(w), stream_of(gy)))
+            w = _workspace(lib().gelib_embedding_workspace(n, v, d, _TYPES[gy.dtype]), gy)
+            check(lib().gelib_embedding_back(_ptr(gw), _ptr(gy), _ptr(state), n, v, d, ctx.scale, _TYPES[gy.dtype], _ptr(w), stream_of(gy)))
         return gw
 
 

@@ -287,14 +287,16 @@ int gelib_linear_back(const gelib_linear_args* args, void* workspace, void* stre
  * Both ends of a network over discrete things (species of atoms, entries of a vocabulary).  Numbers of entries and classes are int64 or
  * int32 (index_bytes 8 or 4) in device memory; those that name no row are never used as an address.  Workspaces as above. */
 
-/* y[i] = scale * weight[ids[i]]: weight (v, d) with rows of ldw elements, y dense (n, d), both of `type`.  A row whose id is outside [0, v) is NaN. */
-int gelib_embedding(void* y, const void* ids, const void* weight, long long n, int v, int d, long long ldw, double scale, int index_bytes, int type,
-                    void* stream);
-/* gw[r] = scale * the sum of gy's rows i with ids[i] = r, in their order and in float, rounded once; zero where there is none and in row
- * `padding` (negative: none).  gy dense (n, d), gw dense (v, d), overwritten.  ids outside [0, v) are left out. */
+/* y[i] = scale * weight[ids[i]]: weight (v, d) with rows of ldw elements, y dense (n, d), both of `type`.  A row whose id is outside [0, v) is NaN.
+ * state: gelib_embedding_state_bytes of the caller's memory, 256-byte aligned, for a backward call: the numbers in order, sorted while the rows are looked
+ * up, without those outside [0, v) and without `padding` (negative: none); or NULL. */
+long long gelib_embedding_state_bytes(long long n, int v);
+int gelib_embedding(void* y, const void* ids, const void* weight, long long n, int v, int d, long long ldw, double scale, long long padding, int index_bytes,
+                    int type, void* state, void* stream);
+/* gw[r] = scale * the sum of gy's rows i with ids[i] = r, in their order and in float, rounded once; zero where there is none.  gy dense (n, d), gw
+ * dense (v, d), overwritten; state as the forward call left it, n and v as they were there. */
 long long gelib_embedding_workspace(long long n, int v, int d, int type);
-int gelib_embedding_back(void* gw, const void* gy, const void* ids, long long n, int v, int d, double scale, long long padding, int index_bytes,
-                         int type, void* workspace, void* stream);
+int gelib_embedding_back(void* gw, const void* gy, const void* state, long long n, int v, int d, double scale, int type, void* workspace, void* stream);
 
 /* Losses of the rows of z = x w + bias, which is never kept: x (m, k) with rows of ldx elements, w (k, n) with rows of ldw or with w_transposed
  * (n, k), bias (n) or NULL, all of `type`.

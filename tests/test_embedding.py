@@ -198,6 +198,27 @@ def test_offsets_beyond_32_bits():
 
 
 @pytest.mark.gpu
+def test_several_gradients_of_one_call_and_numbers_that_change_after_it():
+    """The numbers are those of the forward call; its gradients can be had again, on two streams at a time."""
+    import gelib_b200 as G
+    for n, v in ((5000, 40), (90000, 300)):
+        ids, weight, gy = make(n, v, 48, torch.float32)
+        weight.requires_grad_()
+        want = reference(ids, weight.detach(), gy, 1.0)[1]
+        y = G.embedding(ids, weight)
+        ids.zero_()
+        streams = [torch.cuda.Stream() for _ in range(2)]
+        torch.cuda.synchronize()
+        got = []
+        for turn in range(6):
+            with torch.cuda.stream(streams[turn % 2]):
+                got.append(torch.autograd.grad(y, weight, gy, retain_graph=True)[0])
+        torch.cuda.synchronize()
+        near(got[0], want)
+        assert all(torch.equal(g, got[0]) for g in got)
+
+
+@pytest.mark.gpu
 def test_two_captured_graphs_and_eager_calls_in_between():
     """Both graphs replay after either has changed its inputs; nothing in them waits for the host."""
     import gelib_b200 as G
@@ -313,29 +334,29 @@ C_REFUSALS = {
     "null pointer": dict(y=0),
     "rows overlap": dict(ldw=7),
     "not aligned": dict(weight=4098),
+    "state is not": dict(state=4100),
 }
 
 
 @pytest.mark.parametrize("message", list(C_REFUSALS))
 def test_arguments_of_the_c_abi(cabi, message):
     """No kernel is launched: the addresses stand for nothing."""
-    a = dict(y=4096, ids=4096, weight=4096, n=2, v=5, d=8, ldw=8, scale=1.0, index_bytes=8, type=0)
+    a = dict(y=4096, ids=4096, weight=4096, n=2, v=5, d=8, ldw=8, scale=1.0, padding=-1, index_bytes=8, type=0, state=4096)
     a.update(C_REFUSALS[message])
-    status = cabi.gelib_embedding(a["y"], a["ids"], a["weight"], a["n"], a["v"], a["d"], a["ldw"], a["scale"], a["index_bytes"], a["type"], None)
-    assert status == 2 and message in cabi.gelib_last_error().decode()
+    assert cabi.gelib_embedding(*a.values(), None) == 2 and message in cabi.gelib_last_error().decode()
 
 
-@pytest.mark.parametrize("message,change", [("negative size", dict(v=-1)), ("null pointer", dict(gy=0)), ("not aligned", dict(gw=4098)), ("not aligned", dict(space=4100))])
+@pytest.mark.parametrize("message,change", [("negative size", dict(v=-1)), ("null pointer", dict(gy=0)), ("null pointer", dict(state=0)), ("not aligned", dict(gw=4098)),
+                                            ("not 256-byte", dict(space=4100)), ("not 256-byte", dict(state=4100)), ("no workspace", dict(space=0))])
 def test_arguments_of_the_c_abi_backward(cabi, message, change):
-    a = dict(gw=4096, gy=4096, ids=4096, n=2, v=5, d=8, space=4096)
+    a = dict(gw=4096, gy=4096, state=4096, n=2, v=5, d=8, scale=1.0, type=0, space=4096)
     a.update(change)
-    status = cabi.gelib_embedding_back(a["gw"], a["gy"], a["ids"], a["n"], a["v"], a["d"], 1.0, -1, 8, 0, a["space"], None)
-    assert status == 2 and message in cabi.gelib_last_error().decode()
+    assert cabi.gelib_embedding_back(*a.values(), None) == 2 and message in cabi.gelib_last_error().decode()
 
 
-def test_workspace_of_the_gradient(cabi):
-    """Numbers in order and partial sums of rows that lie in several pieces: some 32 bytes a number, and at most two rows for each of the pieces."""
-    for n, v, d, kind in ((1, 1, 1, 0), (64, 100, 192, 0), (65536, 100, 112, 0), (32768, 65536, 2048, 1), (1 << 20, 262144, 128, 2)):
-        got = cabi.gelib_embedding_workspace(n, v, d, kind)
-        assert 0 <= got <= 40 * n + 16 * v + (1 << 22) + 8 * d * (n // 4 + 148 * 64)
-    assert cabi.gelib_embedding_workspace(0, 5, 4, 0) == 0 and cabi.gelib_embedding_workspace(5, 5, 4, 9) == 0
+def test_state_and_workspace(cabi):
+    """Numbers in order, twice, and blocks' counts of digits; at most two rows of partial sums for every 16 numbers."""
+    for n, v, d, kind in ((1, 1, 1, 0), (64, 100, 192, 0), (65536, 100, 112, 0), (65537, 100, 112, 0), (32768, 65536, 2048, 1), (1 << 20, 262144, 128, 2)):
+        assert 16 * n <= cabi.gelib_embedding_state_bytes(n, v) <= 16 * n + (1 << 20)
+        assert 0 < cabi.gelib_embedding_workspace(n, v, d, kind) <= 8 * (d + 1) * (n // 16 + 1) + 1024
+    assert cabi.gelib_embedding_workspace(0, 5, 4, 0) == 0 and cabi.gelib_embedding_workspace(5, 5, 4, 9) == 0 and cabi.gelib_embedding_state_bytes(0, 5) == 0
