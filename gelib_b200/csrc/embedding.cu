@@ -423,7 +423,7 @@ __device__ __forceinline__ void add_stretch(const Reduce& a, long long team, int
 }
 
 template <class T, int V>
-__global__ void __launch_bounds__(kThreads) reduce_kernel(const Reduce a) {
+__global__ void __launch_bounds__(kThreads, V == 8 ? 2 : 3) reduce_kernel(const Reduce a) {   // eight columns in 80 registers spill: 158 in place of 147 us
   let_next_begin();
   await_previous();
   if (blockIdx.x < a.blocks) {
@@ -451,16 +451,51 @@ __global__ void __launch_bounds__(kThreads) reduce_kernel(const Reduce a) {
   }
 }
 
-// A block joins the parts of a row and 32 V of its columns: 32 warps take parts in turn, their sums are added in order.  Blocks take every so many-th of
-// the stretches, a thousand at a time, and of these what is cut.
+// What was cut is joined, a row and 32 V of its columns by a warp, or, with many parts, by a block whose warps take parts in turn; either way in the order
+// of the parts.  Blocks take every so many-th of the stretches, a thousand at a time.
 constexpr int kJoinThreads = 1024, kJoinWarps = kJoinThreads / 32;
+constexpr int kFewParts = 16;   // that a warp joins
+
+// The stretch in which what begins in `stretch` and is cut ends; the warp looks at 32 places at a time.
+__device__ __forceinline__ long long last_stretch(const Reduce& a, long long stretch, int lane) {
+  long long low = (stretch + 1) * a.per, high = a.n;   // low is the row's, high is not
+  const unsigned cur = a.keys[low];
+  while (high - low > 1) {
+    const long long step = (high - low + 32) / 33, at = low + (lane + 1) * step;
+    const int same = __popc(__ballot_sync(0xffffffffu, at < high && a.keys[min(at, a.n - 1)] == cur));
+    high = min(high, low + (same + 1) * step);
+    low += same * step;
+  }
+  return low / a.per;
+}
+
+template <int V>
+__device__ __forceinline__ void add_parts(const Reduce& a, long long stretch, long long first, long long last, int step, int col, float (&s)[V]) {
+#pragma unroll
+  for (int k = 0; k < V; k++) s[k] = 0;
+  if (col >= a.d) return;
+#pragma unroll 8
+  for (long long p = first; p <= last; p += step) {
+    float g[V];
+    load_part<V>(a.part + (p * 2 + (p == stretch)) * a.d + col, g);
+    add_all(s, s, g);
+  }
+}
+
 template <class T, int V>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Reduce a) {
   __shared__ float of[kJoinWarps / 2][32 * V];
   __shared__ int heads[kJoinThreads], found[kJoinWarps];
+  __shared__ long long last[kJoinThreads];   // of those with many parts
   await_previous();
   const int slabs = (a.d + 32 * V - 1) / (32 * V), lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const long long all = a.stretches * slabs;
+  const auto put = [&](long long h, float (&s)[V]) {
+    const int col = ((int)(h % slabs) * 32 + lane) * V;
+    if (col >= a.d) return;
+    mul_all(s, s, a.scale);
+    store_vec<T, V>(static_cast<T*>(a.gw) + (long long)a.keys[(h / slabs + 1) * a.per] * a.d + col, s);
+  };
   for (long long h0 = blockIdx.x; h0 < all; h0 += (long long)gridDim.x * kJoinThreads) {
     // what is cut among the next thousand of the block's, in order
     const long long mine = h0 + (long long)threadIdx.x * gridDim.x;
@@ -472,44 +507,33 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Reduce a) {
     for (int w = 0; w < kJoinWarps; w++) before += w < warp ? found[w] : 0, count += found[w];
     if (cut) heads[before + __popc(cuts & ((1u << lane) - 1))] = threadIdx.x;
     __syncthreads();
-    for (int k = 0; k < count; k++) {
-      const long long h = h0 + (long long)heads[k] * gridDim.x, stretch = h / slabs, i1 = (stretch + 1) * a.per;
-      const int col = ((int)(h % slabs) * 32 + lane) * V;
-      const unsigned cur = a.keys[i1];
-      long long low = i1, high = a.n;   // the first place that is not the row's, by 32 places at a time: low is the row's, high is not
-      while (high - low > 1) {
-        const long long step = (high - low + 32) / 33, at = low + (lane + 1) * step;
-        const int same = __popc(__ballot_sync(0xffffffffu, at < high && a.keys[min(at, a.n - 1)] == cur));
-        const long long past = low + (same + 1) * step;
-        low += same * step;
-        high = min(high, past);
-      }
-      const long long last = low / a.per;
+    for (int k = warp; k < count; k += kJoinWarps) {
+      const long long h = h0 + (long long)heads[k] * gridDim.x, stretch = h / slabs, end = last_stretch(a, stretch, lane);
+      const bool many = end - stretch >= kFewParts;
+      if (lane == 0) last[k] = many ? end : -1;
+      if (many) continue;
       float s[V];
-#pragma unroll
-      for (int k = 0; k < V; k++) s[k] = 0;
-      if (col < a.d)
-#pragma unroll 8
-        for (long long p = stretch + warp; p <= last; p += kJoinWarps) {
-          float g[V];
-          load_part<V>(a.part + (p * 2 + (p == stretch)) * a.d + col, g);
-          add_all(s, s, g);
-        }
+      add_parts(a, stretch, stretch, end, 1, ((int)(h % slabs) * 32 + lane) * V, s);
+      put(h, s);
+    }
+    __syncthreads();
+    for (int k = 0; k < count; k++) {
+      if (last[k] < 0) continue;
+      const long long h = h0 + (long long)heads[k] * gridDim.x, stretch = h / slabs;
+      float s[V];
+      add_parts(a, stretch, stretch + warp, last[k], kJoinWarps, ((int)(h % slabs) * 32 + lane) * V, s);
 #pragma unroll
       for (int half = kJoinWarps / 2; half; half /= 2) {
         if (warp >= half && warp < 2 * half)
 #pragma unroll
-          for (int k = 0; k < V; k++) of[warp - half][k * 32 + lane] = s[k];
+          for (int j = 0; j < V; j++) of[warp - half][j * 32 + lane] = s[j];
         __syncthreads();
         if (warp < half)
 #pragma unroll
-          for (int k = 0; k < V; k++) s[k] += of[warp][k * 32 + lane];
+          for (int j = 0; j < V; j++) s[j] += of[warp][j * 32 + lane];
         __syncthreads();
       }
-      if (warp == 0 && col < a.d) {
-        mul_all(s, s, a.scale);
-        store_vec<T, V>(static_cast<T*>(a.gw) + (long long)cur * a.d + col, s);
-      }
+      if (warp == 0) put(h, s);
     }
     __syncthreads();
   }
