@@ -79,6 +79,7 @@ struct TcArgs {
   int* status;
   int limit;                          // of the first waits: kWaitLimit, or 0 where a test makes them run out
   int bf16;
+  int leave;                          // slabs after which sums leave tensor memory
 };
 struct TcMaps {
   CUtensorMap a[kProblems], b[kProblems];
@@ -219,7 +220,8 @@ constexpr int kAcross = kChunk / 4, kRows = 32 / kAcross, kPasses = 32 / kRows;
 
 // E: what becomes of the sums.  For every item an E is made; `ahead` is told where the item lies (before the first sums are there, or with P = 3 after
 // the last), `take` gets the warp's chunks of 16 columns, a row per lane, `has` telling which there are, and `end` comes last.
-template <class E, int CG, int P>
+// kLeave: the sums leave tensor memory after every slab (P = 3) or args.leave of them, and are added in registers, with rounding; otherwise they stay to the end.
+template <class E, int CG, int P, bool kLeave>
 __global__ void __launch_bounds__(kThreads, 1) gemm_tc_kernel(const __grid_constant__ TcMaps maps, const __grid_constant__ TcArgs<typename E::Problem> args) {
   using S = Shape<CG, P>;
   extern __shared__ unsigned char raw[];
@@ -331,7 +333,14 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_tc_kernel(const __grid_const
       };
       if constexpr (P == 1) {
         if (!begin()) break;
+        int next = k0 + args.leave;
         for (int k = k0; k < k1; k++) {
+          if constexpr (kLeave)
+            if (k == next) {
+              end();
+              if (!begin()) break;
+              next += args.leave;
+            }
           if (!arrived(stage)) break;
           const int now = stage;
           if (++stage == S::kStages) stage = 0, phase ^= 1;
@@ -386,7 +395,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_tc_kernel(const __grid_const
       const uint32_t from = tmem + ((uint32_t)q << 21) + mine;
       auto has = [&](int c) { return c < kChunks && mine + c * 2 * kChunk < g.bn && n0 + c * 2 * kChunk < g.N; };
       E e;
-      if constexpr (P == 1) {
+      if constexpr (!kLeave) {
         e.template ahead<kChunks>(g, it, m0, n0, lane, mine != 0);
         if (!(ok = all_wait(&bars.sums_full[buf], buf_phase, args.limit))) break;
         tc::tc_fence_after();
@@ -399,12 +408,13 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_tc_kernel(const __grid_const
           }
         taken();
       } else {
+        if constexpr (P == 1) e.template ahead<kChunks>(g, it, m0, n0, lane, mine != 0);
         float sum[kChunks][kChunk];
 #pragma unroll
         for (int c = 0; c < kChunks; c++)
 #pragma unroll
           for (int j = 0; j < kChunk; j++) sum[c][j] = 0;
-        for (int k = it.k0; k < it.k1; k++) {
+        for (int k = it.k0; k < it.k1; k += P == 3 ? 1 : args.leave) {
           if (!(ok = all_wait(&bars.sums_full[buf], buf_phase, args.limit))) break;
           tc::tc_fence_after();
 #pragma unroll
@@ -418,7 +428,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_tc_kernel(const __grid_const
           taken();
         }
         if (!ok) break;
-        e.template ahead<kChunks>(g, it, m0, n0, lane, mine != 0);
+        if constexpr (P != 1) e.template ahead<kChunks>(g, it, m0, n0, lane, mine != 0);   // no registers for it before
 #pragma unroll
         for (int c = 0; c < kChunks; c++)
           if (has(c)) {
@@ -444,9 +454,9 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_tc_kernel(const __grid_const
 
 // ---- host -----------------------------------------------------------------------------------------------------------------------------
 
-template <class E, int CG, int P>
+template <class E, int CG, int P, bool kLeave>
 int launch_as(const char* fn, const TcMaps& maps, const TcArgs<typename E::Problem>& a, bool follows, cudaStream_t stream) {
-  auto kernel = gemm_tc_kernel<E, CG, P>;
+  auto kernel = gemm_tc_kernel<E, CG, P, kLeave>;
   constexpr int shared = Shape<CG, P>::kShared;
   static std::atomic<uint64_t> allowed{0};   // devices on which the kernel may have this much shared memory
   int device = 0;
@@ -472,9 +482,9 @@ int launch_as(const char* fn, const TcMaps& maps, const TcArgs<typename E::Probl
   return launched(fn);
 }
 
-template <class E, int P>
+template <class E, int P, bool kLeave = P == 3>
 int launch_config(const char* fn, int cg, const TcMaps& maps, const TcArgs<typename E::Problem>& a, bool follows, cudaStream_t stream) {
-  return cg == 2 ? launch_as<E, 2, P>(fn, maps, a, follows, stream) : launch_as<E, 1, P>(fn, maps, a, follows, stream);
+  return cg == 2 ? launch_as<E, 2, P, kLeave>(fn, maps, a, follows, stream) : launch_as<E, 1, P, kLeave>(fn, maps, a, follows, stream);
 }
 
 
