@@ -1,5 +1,4 @@
 // extern "C" entry points of embedding tables and losses: argument checks, then the kernels.  No exception passes them.
-#include <cmath>
 #include <exception>
 
 #include "heads.h"
@@ -36,7 +35,7 @@ int check_loss(const char* fn, const gelib_linear_loss_args* p, bool back) {
   if (p->reduction < GELIB_LOSS_NONE || p->reduction > GELIB_LOSS_MEAN) return fail(GELIB_INVALID, fn, "unknown reduction");
   if (p->top < 1 || p->top > GELIB_LOSS_MAX_TOP) return fail(GELIB_INVALID, fn, "a row has 1 to GELIB_LOSS_MAX_TOP of the teacher's logits");
   if (p->m && !p->teacher && p->top != 1) return fail(GELIB_INVALID, fn, "several classes per row without a teacher");
-  if (p->teacher && !(p->temperature > 0 && std::isfinite(p->temperature))) return fail(GELIB_INVALID, fn, "the temperature is not a positive number");
+  if (p->teacher && !(p->temperature >= 1e-15 && p->temperature <= 1e15)) return fail(GELIB_INVALID, fn, "the temperature is not between 1e-15 and 1e15");
   if (p->ldx < p->k || p->ldw < (p->w_transposed ? p->k : p->n)) return fail(GELIB_INVALID, fn, "rows overlap");
   const int width = type_bytes(p->type);
   for (const void* q : {p->x, p->w, p->bias, (const void*)p->gx, (const void*)p->gw, (const void*)p->gb})

@@ -631,9 +631,11 @@ struct LinearLossFunction : torch::autograd::Function<LinearLossFunction> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     variable_list out(8);
     if (!grads[0].defined()) return out;
+    const char* name;
     {
       const at::NoGradGuard off;
       const auto saved = ctx->get_saved_variables();
+      name = saved[4].defined() ? "linear_distillation" : "linear_cross_entropy";
       const at::Tensor &x = saved[0], gy = grads[0].resolve_neg().contiguous();
       c10::cuda::CUDAGuard guard(x.device());
       LossCall l;
@@ -650,9 +652,8 @@ struct LinearLossFunction : torch::autograd::Function<LinearLossFunction> {
       call([&] { return gelib_linear_loss_back(&l.a, ptr(space), s); });
       if (out[1].defined() && l.a.w_transposed) out[1] = out[1].t();
     }
-    return differentiable_once(std::move(out), saved_name(ctx));
+    return differentiable_once(std::move(out), name);
   }
-  static const char* saved_name(AutogradContext* ctx) { return ctx->get_saved_variables()[4].defined() ? "linear_distillation" : "linear_cross_entropy"; }
 };
 
 std::optional<at::Tensor> linear_loss(const at::Tensor& x, const at::Tensor& w, const OptTensor& bias, const at::Tensor& target, const OptTensor& teacher, int reduction,

@@ -154,6 +154,7 @@ int launch_prepare(const char* fn, const State& s, const Entries& e, const Teach
 __global__ void __launch_bounds__(1024) most_kernel(const float* gy, long long m, float* most) {
   __shared__ float of[32];
   float v = 0;
+#pragma unroll 8
   for (long long i = threadIdx.x; i < m; i += 1024) v = fmaxf(v, fabsf(gy[i]));
 #pragma unroll
   for (int d = 16; d; d /= 2) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));

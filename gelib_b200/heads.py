@@ -220,8 +220,8 @@ def linear_distillation(x, w, ids, logits, bias=None, temperature=1.0, reduction
     """
     fn = "linear_distillation"
     r, temperature = _reduction(fn, reduction), float(temperature)
-    if not 0 < temperature < float("inf"):
-        raise ValueError("%s: the temperature is a positive number; got %r" % (fn, temperature))
+    if not 1e-15 <= temperature <= 1e15:
+        raise ValueError("%s: the temperature is between 1e-15 and 1e15; got %r" % (fn, temperature))
     if isinstance(x, torch.Tensor) and isinstance(w, torch.Tensor) and isinstance(ids, torch.Tensor) and isinstance(logits, torch.Tensor):
         y = native().linear_loss(x, w, bias, ids, logits, r, 0, temperature)
         if y is not None:

@@ -303,7 +303,7 @@ int gelib_embedding_back(void* gw, const void* gy, const void* state, long long 
  *   teacher NULL (top 1): cross entropy, loss = log sum_j exp z_j - z_t, t = target[row]; rows with t = ignore_index have no loss.
  *   otherwise: divergence from a teacher's `top` logits per row, teacher (m, top) dense of teacher_type at the classes target (m, top): with q =
  *   softmax(teacher / T) over the entries whose class is not negative and p = softmax(z / T), loss = T^2 sum q (log q - log p); rows without entries
- *   have no loss.  At most GELIB_LOSS_MAX_TOP entries.
+ *   have no loss.  At most GELIB_LOSS_MAX_TOP entries; T is between 1e-15 and 1e15.
  * Rows without a loss count as 0, their gradients are zero, and no number of x there has any effect.  A class of n or more (for cross entropy any
  * other negative one too) makes its row's loss and gradients NaN.
  * reduction: GELIB_LOSS_NONE (loss (m)), GELIB_LOSS_SUM or GELIB_LOSS_MEAN over the rows that have a loss (loss (1); 0 when none has).  Losses are float.

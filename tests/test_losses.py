@@ -658,14 +658,19 @@ def test_cpu_tensors_are_refused(cabi):
         G.linear_distillation(torch.zeros(2, 8), torch.zeros(8, 4), torch.zeros(2, 3, dtype=torch.long), torch.zeros(2, 3))
 
 
-@pytest.mark.parametrize("name", ["reduction", "temperature"])
-def test_values_that_are_refused_before_tensors_are_looked_at(cabi, name):
+def test_values_that_are_refused_before_tensors_are_looked_at(cabi):
     import gelib_b200 as G
-    with pytest.raises(ValueError, match=name):
-        if name == "reduction":
-            G.linear_cross_entropy(None, None, None, reduction="max")
-        else:
-            G.linear_distillation(None, None, None, None, temperature=0)
+    with pytest.raises(ValueError, match="reduction"):
+        G.linear_cross_entropy(None, None, None, reduction="max")
+    for temperature in (0, -1, 1e-16, 1e16, float("inf"), float("nan")):
+        with pytest.raises(ValueError, match="temperature"):
+            G.linear_distillation(None, None, None, None, temperature=temperature)
+
+
+@pytest.mark.gpu
+def test_hot_and_cold_teachers():
+    for temperature in (1e-3, 0.1, 30.0, 1e4):
+        check(make(100, 48, 70, torch.float32, top=9), temperature=temperature)
 
 
 REFUSALS = {
