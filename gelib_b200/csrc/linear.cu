@@ -15,7 +15,7 @@
 // is left.  A backward call is three launches: what goes before the products (one pass over gy and z beside the operands'
 // copies), both products, and the joins of partial sums beside the bias's gradient.  With gradients, us a pass of the Python call: 777 x
 // 204 x 131 bfloat16 86 and 1000 x 1280 x 512 float32 87, of which autograd's own hand-over is about 50; 65536 x 112 x 112 float32 with
-// a residual 142: copies 14 and 28, whose bytes the operator could do without, products 40 and 52, where a tile's two slabs, sums and results follow one
+// a residual 131: copies 13 and 27, whose bytes the operator could do without, products 41 and 42, where a tile's two slabs, sums and results follow one
 // another (tensor cores 17 and 32 %, DRAM 25 %); 4096 x 7168 x 2048 bfloat16 326, the products 260 (tensor cores 80 and 91 %).
 #include <algorithm>
 
