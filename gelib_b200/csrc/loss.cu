@@ -187,27 +187,68 @@ struct Total {
   }
 };
 constexpr int kRows = 32, kRowThreads = 32 * kRows, kBatch = 4;
+constexpr int kFew = 8;   // tiles and entries of a row that a thread takes by itself
+
+struct Rows {
+  Entries e;
+  State s;
+  const float2* part;      // (parts, M)
+  const float* at_entry;   // (M, top)
+  int parts;
+  long long M;
+  float c, temperature;
+  Total total;
+  RowSum* sums;            // of the blocks, where there are several
+};
+
+// An entry's share of a row's loss; v: the row's largest z and its sum.
+__device__ __forceinline__ float entry_of(const Rows& a, long long row, int first, int k, float2 v) {
+  if (first == kInvalid || (k == 0 ? first : a.e.ids[row * a.e.top + k]) == kNone) return 0.f;
+  const float q = a.e.q ? a.e.q[row * a.e.top + k] : 1.f, to = (v.x - a.at_entry[row * a.e.top + k]) / a.temperature;
+  return q == 1.f ? to : q * (logf(q) + to);
+}
+// The row's loss, from the sum of its entries' shares.
+__device__ __forceinline__ float loss_of(const Rows& a, int first, float d, float2 v) {
+  return first == kNone ? 0.f : first == kInvalid ? NAN : a.temperature * a.temperature * (d + logf(v.y));
+}
+__device__ __forceinline__ void put_row(const Rows& a, long long row, int first, float loss, float2 v) {
+  // a row of -infinity alone has no softmax
+  a.s.lse[row] = {v.x, first == kNone ? INFINITY : first == kInvalid || v.x == -INFINITY ? NAN : log2f(v.y)};
+  if (a.total.reduction == GELIB_LOSS_NONE) a.total.loss[row] = loss;
+}
+
+// What the threads of a block have, added in a fixed order: a warp's by halves, then the warps' by one thread.
+__device__ __forceinline__ void put_sum(const Rows& a, RowSum mine) {
+  __shared__ RowSum of[kRows];
+  if (a.total.reduction == GELIB_LOSS_NONE) return;
+#pragma unroll
+  for (int d = 16; d; d /= 2) mine.loss += __shfl_xor_sync(0xffffffffu, mine.loss, d), mine.count += __shfl_xor_sync(0xffffffffu, mine.count, d);
+  if (threadIdx.x % 32 == 0) of[threadIdx.x / 32] = mine;
+  __syncthreads();
+  if (threadIdx.x) return;
+  for (int w = 1; w < (int)blockDim.x / 32; w++) mine.loss += of[w].loss, mine.count += of[w].count;
+  if (gridDim.x == 1) a.total.put(mine);
+  else a.sums[blockIdx.x] = mine;
+}
 
 // A block takes 32 rows at a time: 32 warps share the rows' tiles, a row a lane, then every warp joins one row and adds up its entries.  What there is
 // is a few numbers a row, so that a handful of blocks waits for memory and little else: kBatch tiles are asked for at a time.
-__global__ void __launch_bounds__(kRowThreads) rows_kernel(Entries e, State s, const float2* part, const float* at_entry, int parts, long long M, float c, float temperature,
-                                                           Total total, RowSum* sums) {
+__global__ void __launch_bounds__(kRowThreads) rows_kernel(const Rows a) {
   __shared__ float2 of[kRows][kRows + 1];
-  __shared__ RowSum rows[kRows];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   RowSum mine = {0, 0};
   let_next_begin();
   await_previous();
-  for (long long m0 = (long long)blockIdx.x * kRows; m0 < M; m0 += (long long)gridDim.x * kRows) {
+  for (long long m0 = (long long)blockIdx.x * kRows; m0 < a.M; m0 += (long long)gridDim.x * kRows) {
     const long long m = m0 + lane, row = m0 + warp;
     float2 v = {-INFINITY, 0.f};
-    if (m < M)
-      for (int i = warp; i < parts; i += 32 * kBatch) {
+    if (m < a.M)
+      for (int i = warp; i < a.parts; i += 32 * kBatch) {
         float2 w[kBatch];
 #pragma unroll
-        for (int j = 0; j < kBatch; j++) w[j] = i + 32 * j < parts ? part[(long long)(i + 32 * j) * M + m] : float2{-INFINITY, 0.f};
+        for (int j = 0; j < kBatch; j++) w[j] = i + 32 * j < a.parts ? a.part[(long long)(i + 32 * j) * a.M + m] : float2{-INFINITY, 0.f};
 #pragma unroll
-        for (int j = 0; j < kBatch; j++) v = joined(v, w[j], c);
+        for (int j = 0; j < kBatch; j++) v = joined(v, w[j], a.c);
       }
     of[warp][lane] = v;
     __syncthreads();
@@ -216,34 +257,39 @@ __global__ void __launch_bounds__(kRowThreads) rows_kernel(Entries e, State s, c
 #pragma unroll
     for (int d = 16; d; d /= 2) {
       const float2 w = {__shfl_xor_sync(0xffffffffu, v.x, d), __shfl_xor_sync(0xffffffffu, v.y, d)};
-      v = joined(v, w, c);
+      v = joined(v, w, a.c);
     }
-    if (row >= M) continue;
-    const int t = first_class(e, row);
+    if (row >= a.M) continue;
+    const int first = first_class(a.e, row);
     float d = 0;
-    for (int k = lane; k < e.top; k += 32) {
-      if (t == kInvalid || (k == 0 ? t : e.ids[row * e.top + k]) == kNone) continue;
-      const float q = e.q ? e.q[row * e.top + k] : 1.f, to = (v.x - at_entry[row * e.top + k]) / temperature;
-      d += q == 1.f ? to : q * (logf(q) + to);
-    }
+    for (int k = lane; k < a.e.top; k += 32) d += entry_of(a, row, first, k, v);
 #pragma unroll
     for (int i = 16; i; i /= 2) d += __shfl_xor_sync(0xffffffffu, d, i);
-    d = t == kNone ? 0.f : t == kInvalid ? NAN : temperature * temperature * (d + logf(v.y));
+    d = loss_of(a, first, d, v);
     if (lane == 0) {
-      // a row of -infinity alone has no softmax
-      s.lse[row] = {v.x, t == kNone ? INFINITY : t == kInvalid || v.x == -INFINITY ? NAN : log2f(v.y)};
-      if (total.reduction == GELIB_LOSS_NONE) total.loss[row] = d;
+      put_row(a, row, first, d, v);
+      mine.loss += d, mine.count += first != kNone;
     }
-    mine.loss += d, mine.count += t != kNone;
   }
-  if (total.reduction == GELIB_LOSS_NONE) return;
-  if (lane == 0) rows[warp] = mine;
-  __syncthreads();
-  if (threadIdx.x) return;
-  RowSum all = {0, 0};
-  for (int r = 0; r < kRows; r++) all.loss += rows[r].loss, all.count += rows[r].count;
-  if (gridDim.x == 1) total.put(all);
-  else sums[blockIdx.x] = all;
+  put_sum(a, mine);
+}
+
+// A thread per row, where a row has few tiles and entries: a training step of 262144 rows, 64 channels and 100 classes 410 to 285 us.
+__global__ void __launch_bounds__(kThreads) short_rows_kernel(const Rows a) {
+  RowSum mine = {0, 0};
+  let_next_begin();
+  await_previous();
+  for (long long row = (long long)blockIdx.x * kThreads + threadIdx.x; row < a.M; row += (long long)gridDim.x * kThreads) {
+    float2 v = {-INFINITY, 0.f};
+    for (int i = 0; i < a.parts; i++) v = joined(v, a.part[(long long)i * a.M + row], a.c);
+    const int first = first_class(a.e, row);
+    float d = 0;
+    for (int k = 0; k < a.e.top; k++) d += entry_of(a, row, first, k, v);
+    d = loss_of(a, first, d, v);
+    put_row(a, row, first, d, v);
+    mine.loss += d, mine.count += first != kNone;
+  }
+  put_sum(a, mine);
 }
 
 __global__ void __launch_bounds__(kThreads) total_kernel(const RowSum* sums, int parts, Total total) {
@@ -285,9 +331,6 @@ int piece_of(const gelib_linear_loss_args& p) {
 
 long long groups_of(long long m) { return (m + 31) / 32; }
 
-// Blocks of rows: one for a few rows, which then adds them all up without another launch.
-int row_blocks(long long m) { return m <= 4 * kRows ? 1 : (int)std::min<long long>((m + kRows - 1) / kRows, 148 * 2); }
-
 ForwardProduct forward_of(const gelib_linear_loss_args& p) {
   return {x_of(p), w_of(p), !p.w_transposed, p.bias, p.m, p.n, p.k, p.type, entries_of(p, state_of(p)), slope_of(p), nullptr, nullptr};
 }
@@ -295,6 +338,13 @@ ForwardProduct forward_of(const gelib_linear_loss_args& p) {
 int parts_of(const gelib_linear_loss_args& p) {
   const ForwardProduct f = forward_of(p);
   return takes_few(f) ? few_parts(f) : forward_parts(p.m, p.n, p.k, p.type);
+}
+
+// Whether a thread takes a row, and how many blocks: one for a few rows, which then adds them all up without another launch.
+bool short_rows(const gelib_linear_loss_args& p) { return parts_of(p) <= kFew && p.top <= kFew; }
+int row_blocks(const gelib_linear_loss_args& p) {
+  if (short_rows(p)) return p.m <= 2 * kThreads ? 1 : (int)std::min<long long>((p.m + kThreads - 1) / kThreads, 148 * 4);
+  return p.m <= 4 * kRows ? 1 : (int)std::min<long long>((p.m + kRows - 1) / kRows, 148 * 2);
 }
 
 int forward(const gelib_linear_loss_args& p, char* at, cudaStream_t stream) {
@@ -312,13 +362,14 @@ int forward(const gelib_linear_loss_args& p, char* at, cudaStream_t stream) {
   }
   if ((st = launch_prepare(fn, s, e, {p.teacher, p.teacher_type, p.m, c}, jobs, nullptr, p.type, stream)) != GELIB_OK) return st;
   const bool follows = p.teacher || jobs.count > 0;
-  const int parts = parts_of(p), blocks = row_blocks(p.m);
+  const int parts = parts_of(p), blocks = row_blocks(p);
   f.part = (float2*)at, at += up(8LL * parts * p.m);
   f.at_entry = (float*)at, at += up(4 * p.m * p.top);
   if ((st = few ? launch_few(fn, f, follows, stream) : launch_forward_product(fn, f, follows, stream)) != GELIB_OK) return st;
   const Total total = {p.reduction, (float*)p.loss, s.scale};
-  st = launch_after(fn, true, rows_kernel, dim3(blocks), kRowThreads, 0, stream, e, s, (const float2*)f.part, (const float*)f.at_entry, parts, (long long)p.m, c,
-                    temperature_of(p), total, (RowSum*)at);
+  const Rows rows = {e, s, f.part, f.at_entry, parts, p.m, c, temperature_of(p), total, (RowSum*)at};
+  const bool few_tiles = short_rows(p);
+  st = launch_after(fn, true, few_tiles ? short_rows_kernel : rows_kernel, dim3(blocks), few_tiles ? kThreads : kRowThreads, 0, stream, rows);
   if (st != GELIB_OK || p.reduction == GELIB_LOSS_NONE || blocks == 1) return st;
   return launch_after(fn, true, total_kernel, dim3(1), kThreads, 0, stream, (const RowSum*)at, blocks, total);
 }
@@ -423,7 +474,7 @@ long long linear_loss_workspace(const gelib_linear_loss_args& p, bool backward) 
   if (backward) return p.gx || p.gw || p.gb ? room_of(p, nullptr).bytes : 0;
   const long long copies = takes_few(forward_of(p)) ? 0 : copy_bytes(x_of(p), p.type) + copy_bytes(w_of(p), p.type);
   return copies + up(8LL * parts_of(p) * p.m) + up(4 * p.m * p.top) +
-         up(row_blocks(p.m) * (long long)sizeof(RowSum));
+         up(row_blocks(p) * (long long)sizeof(RowSum));
 }
 
 int launch_linear_loss(const gelib_linear_loss_args& p, void* workspace, cudaStream_t stream) {
