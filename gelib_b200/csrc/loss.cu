@@ -16,8 +16,8 @@
 // Rows without a loss have dz = 0, and their x is read as zero: what stands there, NaN say, must not reach gw.
 //
 // What bounds it: the tensor cores, 2 m k n for the loss and 6 m k n for the gradients, a third of them to have z again, which keeping it would save.
-// bfloat16, 4096 x 2048 x 65536: 667 us, and two pieces of 340 + 670 (1650 TFLOP/s), 3.3 ms among passes that follow one another, where the power limit
-// brings the clock down (the library's sustained rate makes it 3.25).  4096 x 1280 x 32768 with 64 entries a row: 244, 252, 422; 1140 us.  float32, 1000 x 1280 x
+// bfloat16, 4096 x 2048 x 65536: 670 us, and two pieces of 365 + 680 (1590 TFLOP/s), 3.3 ms among passes that follow one another, where the power limit
+// brings the clock down (the library's sustained rate makes it 3.25).  4096 x 1280 x 32768 with 64 entries a row: 214, 252, 425; 1100 us.  float32, 1000 x 1280 x
 // 8192: 97, 113, 191 beside 2 x 18 for the three planes of x and w; 498 us.  Small calls wait for the host: seven launches and autograd, 85 us.
 #include <algorithm>
 #include <cmath>
@@ -341,9 +341,9 @@ int parts_of(const gelib_linear_loss_args& p) {
 }
 
 // Whether a thread takes a row, and how many blocks: one for a few rows, which then adds them all up without another launch.
-bool short_rows(const gelib_linear_loss_args& p) { return parts_of(p) <= kFew && p.top <= kFew; }
-int row_blocks(const gelib_linear_loss_args& p) {
-  if (short_rows(p)) return p.m <= 2 * kThreads ? 1 : (int)std::min<long long>((p.m + kThreads - 1) / kThreads, 148 * 4);
+bool short_rows(const gelib_linear_loss_args& p, int parts) { return parts <= kFew && p.top <= kFew; }
+int row_blocks(const gelib_linear_loss_args& p, int parts) {
+  if (short_rows(p, parts)) return p.m <= 2 * kThreads ? 1 : (int)std::min<long long>((p.m + kThreads - 1) / kThreads, 148 * 4);
   return p.m <= 4 * kRows ? 1 : (int)std::min<long long>((p.m + kRows - 1) / kRows, 148 * 2);
 }
 
@@ -362,13 +362,13 @@ int forward(const gelib_linear_loss_args& p, char* at, cudaStream_t stream) {
   }
   if ((st = launch_prepare(fn, s, e, {p.teacher, p.teacher_type, p.m, c}, jobs, nullptr, p.type, stream)) != GELIB_OK) return st;
   const bool follows = p.teacher || jobs.count > 0;
-  const int parts = parts_of(p), blocks = row_blocks(p);
+  const int parts = parts_of(p), blocks = row_blocks(p, parts);
   f.part = (float2*)at, at += up(8LL * parts * p.m);
   f.at_entry = (float*)at, at += up(4 * p.m * p.top);
   if ((st = few ? launch_few(fn, f, follows, stream) : launch_forward_product(fn, f, follows, stream)) != GELIB_OK) return st;
   const Total total = {p.reduction, (float*)p.loss, s.scale};
   const Rows rows = {e, s, f.part, f.at_entry, parts, p.m, c, temperature_of(p), total, (RowSum*)at};
-  const bool few_tiles = short_rows(p);
+  const bool few_tiles = short_rows(p, parts);
   st = launch_after(fn, true, few_tiles ? short_rows_kernel : rows_kernel, dim3(blocks), few_tiles ? kThreads : kRowThreads, 0, stream, rows);
   if (st != GELIB_OK || p.reduction == GELIB_LOSS_NONE || blocks == 1) return st;
   return launch_after(fn, true, total_kernel, dim3(1), kThreads, 0, stream, (const RowSum*)at, blocks, total);
@@ -473,8 +473,9 @@ long long linear_loss_state_bytes(const gelib_linear_loss_args& p) {
 long long linear_loss_workspace(const gelib_linear_loss_args& p, bool backward) {
   if (backward) return p.gx || p.gw || p.gb ? room_of(p, nullptr).bytes : 0;
   const long long copies = takes_few(forward_of(p)) ? 0 : copy_bytes(x_of(p), p.type) + copy_bytes(w_of(p), p.type);
-  return copies + up(8LL * parts_of(p) * p.m) + up(4 * p.m * p.top) +
-         up(row_blocks(p) * (long long)sizeof(RowSum));
+  const int parts = parts_of(p);
+  return copies + up(8LL * parts * p.m) + up(4 * p.m * p.top) +
+         up(row_blocks(p, parts) * (long long)sizeof(RowSum));
 }
 
 int launch_linear_loss(const gelib_linear_loss_args& p, void* workspace, cudaStream_t stream) {

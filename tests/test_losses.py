@@ -301,6 +301,12 @@ def test_large_logits_and_sure_classes():
         sure[7] = 4000.0
         got = run(x, w, sure, torch.full_like(target, 7), None, torch.tensor(1.0, device="cuda"))
         assert all((t == 0).all() for t in got)
+        # both passes have the same z, however long its sums
+        for k in (1280, 1281, 2048, 5000):
+            x, w, bias, target, _ = make(150, k, 300, dtype)
+            got = run(x, w, sure, torch.full_like(target, 7), None, torch.tensor(1.0, device="cuda"))
+            assert all((t == 0).all() for t in got), k
+            check((x, w, bias, target, None))
 
 
 @pytest.mark.gpu
