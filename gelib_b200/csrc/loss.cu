@@ -146,8 +146,7 @@ int launch_prepare_as(const char* fn, const State& s, const Entries& e, const Te
   if (shared > 48 * 1024) {   // asked for anew each time: it is the device's, and the largest is the same for all
     GELIB_CUDA_TRY(fn, cudaFuncSetAttribute(prepare_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)teacher_shared(GELIB_LOSS_MAX_TOP)));
   }
-  prepare_kernel<T><<<(unsigned)blocks, kCopyThreads, shared, stream>>>(s, e, t, (int)teachers, jobs, rows_out);
-  return launched(fn);
+  return launch_after(fn, false, prepare_kernel<T>, dim3((unsigned)blocks), kCopyThreads, shared, stream, s, e, t, (int)teachers, jobs, rows_out);
 }
 int launch_prepare(const char* fn, const State& s, const Entries& e, const Teacher& t, const PlaneJobs& jobs, const float2* rows_out, int type, cudaStream_t stream) {
   if (jobs.count == 0 && !t.logits) return GELIB_OK;
