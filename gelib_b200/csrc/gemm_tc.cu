@@ -148,7 +148,7 @@ __device__ __forceinline__ void load_bias(const TcProblem& g, int n0, int lane, 
 template <class T, int P>
 struct DenseEnd {
   using Problem = TcProblem;
-  static constexpr bool kTwo = true;
+  static constexpr bool kTwo = true, kBefore = false;
   Rest<T> rest[2];                    // of a chunk, and of the next, asked for before the first is stored
   float bias[P == 1 ? 8 : 1][4];
   long long m0;

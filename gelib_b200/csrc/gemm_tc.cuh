@@ -219,7 +219,8 @@ struct Walk {
 constexpr int kAcross = kChunk / 4, kRows = 32 / kAcross, kPasses = 32 / kRows;
 
 // E: what becomes of the sums.  For every item an E is made; `ahead` is told where the item lies (before the first sums are there, or with P = 3 after
-// the last), `take` gets the warp's chunks of 16 columns, a row per lane, `has` telling which there are, and `end` comes last.
+// the last), `take` gets the warp's chunks of 16 columns, a row per lane, `has` telling which there are, and `end` comes last.  Before all items the
+// epilogue's threads of all blocks may do something else (kBefore).
 // kLeave: the sums leave tensor memory after every slab (P = 3) or args.leave of them, and are added in registers, with rounding; otherwise they stay to the end.
 template <class E, int CG, int P, bool kLeave>
 __global__ void __launch_bounds__(kThreads, 1) gemm_tc_kernel(const __grid_constant__ TcMaps maps, const __grid_constant__ TcArgs<typename E::Problem> args) {
@@ -378,6 +379,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_tc_kernel(const __grid_const
     const int mine = (warp - 3) / 4 * kChunk;        // its first chunk
     const uint32_t block = ring_at + S::kStages * S::kStage + (warp - 3) * 32 * kPitch * 4;
     constexpr int kChunks = S::kBnMost / (2 * kChunk);   // at most
+    if constexpr (E::kBefore) E::before(args.p[0], (blockIdx.x * kWarps + warp - 3) * 32 + lane, gridDim.x * kWarps * 32);
     int buf = 0;
     uint32_t buf_phase = 0;
     auto taken = [&] {   // tensor memory has been read

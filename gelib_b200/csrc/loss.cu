@@ -18,7 +18,7 @@
 // What bounds it: the tensor cores, 2 m k n for the loss and 6 m k n for the gradients, a third of them to have z again, which keeping it would save.
 // bfloat16, 4096 x 2048 x 65536: 670 us, and two pieces of 365 + 680 (1590 TFLOP/s), 3.3 ms among passes that follow one another, where the power limit
 // brings the clock down (the library's sustained rate makes it 3.25).  4096 x 1280 x 32768 with 64 entries a row: 214, 252, 425; 1100 us.  float32, 1000 x 1280 x
-// 8192: 97, 113, 191 beside 2 x 18 for the three planes of x and w; 498 us.  Small calls wait for the host: seven launches and autograd, 85 us.
+// 8192: 97, 113, 191 beside 2 x 18 for the three planes of x and w; 498 us.  Small calls wait for the host: six launches and autograd, 83 us.
 #include <algorithm>
 #include <cmath>
 

@@ -52,7 +52,7 @@ struct ForwardProblem : TcShape {
 template <class T>
 struct ForwardEnd {
   using Problem = ForwardProblem;
-  static constexpr bool kTwo = false;
+  static constexpr bool kTwo = false, kBefore = false;
   float2 sum;
   Next next;
   long long row;
@@ -122,7 +122,7 @@ __device__ __forceinline__ void take_from_shared(uint32_t at, float x) {
 template <class T>
 struct SlopeEnd {
   using Problem = SlopeProblem;
-  static constexpr bool kTwo = false;
+  static constexpr bool kTwo = false, kBefore = false;
   Next next;
   long long m0;
   float2 lse;
@@ -215,6 +215,9 @@ struct GradProblem : TcShape {
   int vec_f, vec_y;       // four columns at a time: in `part` and `sum`, in y
   const float *a0, *a1;
   float a2;
+  const float* sums;      // of the launch's first problem: sum_parts rows of sum_n numbers, added up into gb; gb null: not here
+  void* gb;
+  int sum_parts, sum_n;
 };
 
 __device__ __forceinline__ float scale_of(const float* a0, const float* a1, float a2) { return a2 * (a0 ? *a0 : 1.f) * (a1 ? *a1 : 1.f); }
@@ -238,10 +241,23 @@ __device__ __forceinline__ void finish_grad(T* y, float* sum, bool begun, float 
 template <class T>
 struct GradEnd {
   using Problem = GradProblem;
-  static constexpr bool kTwo = true;
+  static constexpr bool kTwo = true, kBefore = true;
   long long m0;
   int split;
   float scale;
+
+  // The bias's gradient, while the first tiles are summed: a column a thread.
+  static __device__ __forceinline__ void before(const Problem& g, int thread, int threads) {
+    if (!g.gb) return;
+    const float scale = scale_of(g.a0, g.a1, g.a2);
+    for (int c = thread; c < g.sum_n; c += threads) {
+      float s = 0;
+#pragma unroll 8
+      for (int i = 0; i < g.sum_parts; i++) s += g.sums[(long long)i * g.sum_n + c];
+      static_cast<T*>(g.gb)[c] = from_float<T>(s * scale);
+    }
+    __syncwarp();
+  }
 
   template <int kChunks>
   __device__ __forceinline__ void ahead(const Problem& g, const Item& it, long long m, int, int, bool) {
@@ -458,10 +474,14 @@ long long grads_workspace(const Grads& g) {
   return bytes;
 }
 
+// Rows of sums that a thread adds up before its first tile: 32 of them (1024 rows of x) take some 2 us, the launch saved 3.
+constexpr long long kShortSum = 32;
+
 int launch_grads(const char* fn, const Grads& q, bool follows, void* workspace, cudaStream_t stream) {
   GradJoins joins = {};
   joins.a0 = q.a0, joins.a1 = q.a1, joins.a2 = q.a2;
   int joined = 0;
+  bool bias_done = false;
   if (q.count) {
     Sizes z[kProblems];
     const Plan plan = plan_for(q, z);
@@ -492,13 +512,19 @@ int launch_grads(const char* fn, const Grads& q, bool follows, void* workspace, 
     }
     if (q.count == 1) maps.a[1] = maps.a[0], maps.b[1] = maps.b[0];
     finish_args(&a, plan, q.type);
+    // the bias's gradient goes along where no other launch is needed and a thread's sum is short
+    if (q.gb && !joined && q.sum_parts <= kShortSum) {
+      GradProblem& p = a.p[0];
+      p.sums = q.sums, p.gb = q.gb, p.sum_parts = (int)q.sum_parts, p.sum_n = q.sum_n;
+      bias_done = true;
+    }
     const int st = q.type == GELIB_F32    ? launch_config<GradEnd<float>, 3>(fn, plan.cg, maps, a, follows, stream)
                    : q.type == GELIB_BF16 ? launch_config<GradEnd<__nv_bfloat16>, 1>(fn, plan.cg, maps, a, follows, stream)
                                           : launch_config<GradEnd<__half>, 1>(fn, plan.cg, maps, a, follows, stream);
     if (st != GELIB_OK) return st;
   }
   long long blocks = joins.j[0].blocks + joins.j[1].blocks;
-  if (q.gb) {
+  if (q.gb && !bias_done) {
     joins.sums = q.sums, joins.gb = q.gb, joins.sum_parts = q.sum_parts, joins.sum_n = q.sum_n;
     blocks += (q.sum_n + 7) / 8;
   }
