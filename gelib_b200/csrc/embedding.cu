@@ -10,7 +10,7 @@
 //
 // 32768 rows of 2048 bfloat16 over 65536 entries: lookup 38 us, sort 24 beside it, sums 74 (402 MB, 5.4 TB/s), joins 8; a pass with its gradient 148 us for 643 MB,
 // 4.3 TB/s, the copy rate being 6.5: rows of 4 KB come from all over memory, and reads and writes take turns.  65536 rows of 112 float32 over 100 entries:
-// 9, 19, 13, 23, of a pass of 61, where autograd's hand-over takes 50.
+// 9, 19, 14, 20, of a pass of 61, where autograd's hand-over takes 50.
 // Steps: a warp per entry that looks through all numbers 15.5 ms and 7.9 ms for these two; sorted numbers 174 and 76; teams of lanes, any alignment and a
 // list of what is cut 165 and 64; a sort in one cluster that writes in runs 151 and 60; beside the lookup 148.
 #include <algorithm>
