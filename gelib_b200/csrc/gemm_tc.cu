@@ -344,7 +344,7 @@ int launch_tc_gemm(const Gemm* g, int count, bool follows, void* workspace, Join
   Sizes z[kProblems];
   const int type = g[0].type;
   const Plan plan = plan_for(g, count, z);
-  TcMaps maps;
+  TcMaps maps = {};
   TcArgs<TcProblem> a = {};
   char* at = (char*)workspace;
   const bool other = swapped(plan, z, count, type);

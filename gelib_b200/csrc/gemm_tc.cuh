@@ -80,9 +80,12 @@ struct TcArgs {
   int limit;                          // of the first waits: kWaitLimit, or 0 where a test makes them run out
   int bf16;
   int leave;                          // slabs after which sums leave tensor memory
+  const int* other;                   // null, or not zero where maps.other stands for the operand (B if other_b) of problem other_of
+  int other_of, other_b;
 };
 struct TcMaps {
   CUtensorMap a[kProblems], b[kProblems];
+  CUtensorMap other;                  // of an operand that there are two of, where args.other says to take it
 };
 
 // A tile has 128 CG rows and up to kBnMost columns, a multiple of 16 (32 in a pair).
@@ -263,11 +266,12 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_tc_kernel(const __grid_const
     int stage = 0;
     uint32_t phase = 0, ready = args.limit > 0 && over(&bars.empty[0], 1);
     long long issued = 0;
+    const int other_of = args.other && (args.other_b != 0) == of_b && *args.other ? args.other_of : -1;
     while (ok && walk.next(args, mine_of, blocks)) {
       const TcShape& g = args.p[walk.which];
       const Item it = item_of(g, walk.at);
       const bool across = of_b ? g.b_across : g.a_across;
-      const CUtensorMap* map = of_b ? &maps.b[walk.which] : &maps.a[walk.which];
+      const CUtensorMap* map = walk.which == other_of ? &maps.other : of_b ? &maps.b[walk.which] : &maps.a[walk.which];
       const int mine = of_b ? g.bn / CG : 128, boxes = across ? (mine + 63) / 64 : 1;   // rows or columns in this block
       const uint32_t bytes = CG * (across ? boxes * 8192 : mine * 128);
       const int at = of_b ? it.n * g.bn + (int)rank * mine : (it.m * CG + (int)rank) * 128;

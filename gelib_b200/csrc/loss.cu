@@ -13,7 +13,8 @@
 // dz is an operand of the tensor cores: in 16 bits it is rounded to them.  float16 has no room for the small shares of a large vocabulary, so there dz is
 // 2^14 (p - q), times a row's g over the largest g where rows have their own; the rest of the factors comes after the sums.
 //
-// Rows without a loss have dz = 0, and their x is read as zero: what stands there, NaN say, must not reach gw.
+// Rows without a loss have dz = 0, and their x is read as zero: what stands there, NaN say, must not reach gw.  The forward call looks at such rows of a
+// 16-bit x, and where one holds what is no finite number the product for gw takes a copy (65536 x 1280 x 100: 62 of 350 us when x was always copied).
 //
 // What bounds it: the tensor cores, 2 m k n for the loss and 6 m k n for the gradients, a third of them to have z again, which keeping it would save.
 // bfloat16, 4096 x 2048 x 65536: 670 us, and two pieces of 365 + 680 (1590 TFLOP/s), 3.3 ms among passes that follow one another, where the power limit
@@ -32,6 +33,8 @@ namespace {
 
 constexpr int kThreads = 256;
 
+constexpr int kRowBlocks = 148 * 4;   // of a launch over rows, at most
+
 // Buckets of a row's classes: 128 at the most.
 int bucket_of(int n) { return (int)((n + 32767LL) / 32768) * 256; }
 int buckets_of(int n) { return (n + bucket_of(n) - 1) / bucket_of(n); }
@@ -41,6 +44,7 @@ State state_of(const gelib_linear_loss_args& p, long long* bytes = nullptr) {
   char* at = (char*)p.state;
   State s = {};
   s.scale = (float*)at, at += 256;
+  s.odd = (int*)at, at += up(4 * (1 + kRowBlocks));
   s.lse = (float2*)at, at += up(p.m * 8);
   if (p.teacher) {
     s.ids = (int*)at, at += up(p.m * p.top * 4);
@@ -122,14 +126,24 @@ __device__ __forceinline__ void prepare_row(const State& s, const Entries& e, co
   }
 }
 
-// The teacher's rows in the first blocks, the operands' copies in the others.
+// The teacher's rows in the first blocks, the operands' copies in the others.  use_copy, where it is given: the first operand is only copied, and *use_copy
+// set, if the forward call found x of a row without a loss to hold what is no finite number (s.odd).
 template <class T>
 __global__ void __launch_bounds__(kCopyThreads) prepare_kernel(const State s, const Entries e, const Teacher t, int teachers, const __grid_constant__ PlaneJobs jobs,
-                                                               const float2* rows_out) {
+                                                               const float2* rows_out, int* use_copy) {
   extern __shared__ int shared[];
   let_next_begin();
   if ((int)blockIdx.x >= teachers) {
-    copy_planes<T, true>(jobs, blockIdx.x - teachers, gridDim.x - teachers, rows_out);
+    long long from = 0;
+    if (use_copy) {
+      bool odd = false;
+      const int found = *s.odd;
+      for (int i = threadIdx.x; i < found; i += kCopyThreads) odd |= s.odd[1 + i] != 0;
+      const int any = __syncthreads_or(odd);
+      if (blockIdx.x == 0 && threadIdx.x == 0) *use_copy = any;
+      if (!any) from = jobs.first[1];
+    }
+    copy_planes<T, true>(jobs, blockIdx.x - teachers, gridDim.x - teachers, rows_out, from);
     return;
   }
   const int warp = threadIdx.x / 32;
@@ -139,19 +153,21 @@ __global__ void __launch_bounds__(kCopyThreads) prepare_kernel(const State s, co
 }
 
 template <class T>
-int launch_prepare_as(const char* fn, const State& s, const Entries& e, const Teacher& t, const PlaneJobs& jobs, const float2* rows_out, cudaStream_t stream) {
+int launch_prepare_as(const char* fn, const State& s, const Entries& e, const Teacher& t, const PlaneJobs& jobs, const float2* rows_out, int* use_copy, cudaStream_t stream) {
   const long long teachers = t.logits ? (t.m + kTeacherRows - 1) / kTeacherRows : 0;
   const long long blocks = teachers + std::min((jobs.first[jobs.count] + kCopyThreads - 1) / kCopyThreads, 148LL * 8);
   const size_t shared = t.logits ? (size_t)teacher_shared(e.top) : 0;
   if (shared > 48 * 1024) {   // asked for anew each time: it is the device's, and the largest is the same for all
     GELIB_CUDA_TRY(fn, cudaFuncSetAttribute(prepare_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)teacher_shared(GELIB_LOSS_MAX_TOP)));
   }
-  return launch_after(fn, false, prepare_kernel<T>, dim3((unsigned)blocks), kCopyThreads, shared, stream, s, e, t, (int)teachers, jobs, rows_out);
+  return launch_after(fn, false, prepare_kernel<T>, dim3((unsigned)blocks), kCopyThreads, shared, stream, s, e, t, (int)teachers, jobs, rows_out, use_copy);
 }
-int launch_prepare(const char* fn, const State& s, const Entries& e, const Teacher& t, const PlaneJobs& jobs, const float2* rows_out, int type, cudaStream_t stream) {
+int launch_prepare(const char* fn, const State& s, const Entries& e, const Teacher& t, const PlaneJobs& jobs, const float2* rows_out, int* use_copy, int type,
+                   cudaStream_t stream) {
   if (jobs.count == 0 && !t.logits) return GELIB_OK;
-  return type == GELIB_F32    ? launch_prepare_as<float>(fn, s, e, t, jobs, rows_out, stream)
-         : type == GELIB_BF16 ? launch_prepare_as<__nv_bfloat16>(fn, s, e, t, jobs, rows_out, stream) : launch_prepare_as<__half>(fn, s, e, t, jobs, rows_out, stream);
+  return type == GELIB_F32    ? launch_prepare_as<float>(fn, s, e, t, jobs, rows_out, use_copy, stream)
+         : type == GELIB_BF16 ? launch_prepare_as<__nv_bfloat16>(fn, s, e, t, jobs, rows_out, use_copy, stream)
+                              : launch_prepare_as<__half>(fn, s, e, t, jobs, rows_out, use_copy, stream);
 }
 
 // The largest |gy|; 1 where that is zero or no finite number.
@@ -198,7 +214,25 @@ struct Rows {
   float c, temperature;
   Total total;
   RowSum* sums;            // of the blocks, where there are several
+  const unsigned short* x; // 16-bit x, or null
+  long long ldx;
+  int K;
+  unsigned exponent;       // all ones in an infinity or NaN of x's type
 };
+
+// Whether x of the row holds what is no finite number; asked by a whole warp.
+__device__ __forceinline__ bool is_odd(const Rows& a, long long row) {
+  bool odd = false;
+  for (int k = threadIdx.x % 32; k < a.K; k += 32) odd |= (a.x[row * a.ldx + k] & a.exponent) == a.exponent;
+  return __any_sync(0xffffffffu, odd);
+}
+// What the threads of a block found.
+__device__ __forceinline__ void put_odd(const Rows& a, bool odd) {
+  const int any = __syncthreads_or(odd);
+  if (threadIdx.x) return;
+  a.s.odd[1 + blockIdx.x] = any;
+  if (blockIdx.x == 0) a.s.odd[0] = gridDim.x;
+}
 
 // An entry's share of a row's loss; v: the row's largest z and its sum.
 __device__ __forceinline__ float entry_of(const Rows& a, long long row, int first, int k, float2 v) {
@@ -236,6 +270,7 @@ __global__ void __launch_bounds__(kRowThreads) rows_kernel(const Rows a) {
   __shared__ float2 of[kRows][kRows + 1];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   RowSum mine = {0, 0};
+  bool odd = false;
   let_next_begin();
   await_previous();
   for (long long m0 = (long long)blockIdx.x * kRows; m0 < a.M; m0 += (long long)gridDim.x * kRows) {
@@ -269,25 +304,40 @@ __global__ void __launch_bounds__(kRowThreads) rows_kernel(const Rows a) {
       put_row(a, row, first, d, v);
       mine.loss += d, mine.count += first != kNone;
     }
+    if (first == kNone && a.x) odd |= is_odd(a, row);
   }
+  put_odd(a, odd);
   put_sum(a, mine);
+}
+
+__device__ __forceinline__ RowSum take_row(const Rows& a, long long row, RowSum sum, int* first) {
+  float2 v = {-INFINITY, 0.f};
+  for (int i = 0; i < a.parts; i++) v = joined(v, a.part[(long long)i * a.M + row], a.c);
+  *first = first_class(a.e, row);
+  float d = 0;
+  for (int k = 0; k < a.e.top; k++) d += entry_of(a, row, *first, k, v);
+  d = loss_of(a, *first, d, v);
+  put_row(a, row, *first, d, v);
+  return {sum.loss + d, sum.count + (*first != kNone)};
 }
 
 // A thread per row, where a row has few tiles and entries: a training step of 262144 rows, 64 channels and 100 classes 410 to 285 us.
 __global__ void __launch_bounds__(kThreads) short_rows_kernel(const Rows a) {
   RowSum mine = {0, 0};
+  bool odd = false;
   let_next_begin();
   await_previous();
-  for (long long row = (long long)blockIdx.x * kThreads + threadIdx.x; row < a.M; row += (long long)gridDim.x * kThreads) {
-    float2 v = {-INFINITY, 0.f};
-    for (int i = 0; i < a.parts; i++) v = joined(v, a.part[(long long)i * a.M + row], a.c);
-    const int first = first_class(a.e, row);
-    float d = 0;
-    for (int k = 0; k < a.e.top; k++) d += entry_of(a, row, first, k, v);
-    d = loss_of(a, first, d, v);
-    put_row(a, row, first, d, v);
-    mine.loss += d, mine.count += first != kNone;
+  for (long long row0 = (long long)blockIdx.x * kThreads + threadIdx.x / 32 * 32; row0 < a.M; row0 += (long long)gridDim.x * kThreads) {
+    const long long row = row0 + threadIdx.x % 32;
+    int first = 0;
+    if (row < a.M) mine = take_row(a, row, mine, &first);
+    unsigned out = a.x ? __ballot_sync(0xffffffffu, row < a.M && first == kNone) : 0;
+    while (out) {
+      odd |= is_odd(a, row0 + __ffs(out) - 1);
+      out &= out - 1;
+    }
   }
+  put_odd(a, odd);
   put_sum(a, mine);
 }
 
@@ -342,7 +392,7 @@ int parts_of(const gelib_linear_loss_args& p) {
 // Whether a thread takes a row, and how many blocks: one for a few rows, which then adds them all up without another launch.
 bool short_rows(const gelib_linear_loss_args& p, int parts) { return parts <= kFew && p.top <= kFew; }
 int row_blocks(const gelib_linear_loss_args& p, int parts) {
-  if (short_rows(p, parts)) return p.m <= 2 * kThreads ? 1 : (int)std::min<long long>((p.m + kThreads - 1) / kThreads, 148 * 4);
+  if (short_rows(p, parts)) return p.m <= 2 * kThreads ? 1 : (int)std::min<long long>((p.m + kThreads - 1) / kThreads, kRowBlocks);
   return p.m <= 4 * kRows ? 1 : (int)std::min<long long>((p.m + kRows - 1) / kRows, 148 * 2);
 }
 
@@ -359,26 +409,43 @@ int forward(const gelib_linear_loss_args& p, char* at, cudaStream_t stream) {
     copy_if_needed(&f.x, p.type, at, &jobs);
     copy_if_needed(&f.w, p.type, at, &jobs);
   }
-  if ((st = launch_prepare(fn, s, e, {p.teacher, p.teacher_type, p.m, c}, jobs, nullptr, p.type, stream)) != GELIB_OK) return st;
+  if ((st = launch_prepare(fn, s, e, {p.teacher, p.teacher_type, p.m, c}, jobs, nullptr, nullptr, p.type, stream)) != GELIB_OK) return st;
   const bool follows = p.teacher || jobs.count > 0;
   const int parts = parts_of(p), blocks = row_blocks(p, parts);
   f.part = (float2*)at, at += up(8LL * parts * p.m);
   f.at_entry = (float*)at, at += up(4 * p.m * p.top);
   if ((st = few ? launch_few(fn, f, follows, stream) : launch_forward_product(fn, f, follows, stream)) != GELIB_OK) return st;
   const Total total = {p.reduction, (float*)p.loss, s.scale};
-  const Rows rows = {e, s, f.part, f.at_entry, parts, p.m, c, temperature_of(p), total, (RowSum*)at};
+  const bool wide = p.type == GELIB_F32;
+  const Rows rows = {e, s, f.part, f.at_entry, parts, p.m, c, temperature_of(p), total, (RowSum*)at, wide ? nullptr : (const unsigned short*)p.x, p.ldx, p.k,
+                     p.type == GELIB_BF16 ? 0x7f80u : 0x7c00u};
   const bool few_tiles = short_rows(p, parts);
   st = launch_after(fn, true, few_tiles ? short_rows_kernel : rows_kernel, dim3(blocks), few_tiles ? kThreads : kRowThreads, 0, stream, rows);
   if (st != GELIB_OK || p.reduction == GELIB_LOSS_NONE || blocks == 1) return st;
   return launch_after(fn, true, total_kernel, dim3(1), kThreads, 0, stream, (const RowSum*)at, blocks, total);
 }
 
+// Where things lie in a backward call's workspace.
+struct Room {
+  Stored x, w, dz;
+  Stored x_copy;   // base null, or what stands for x in gw's product where *use_copy is not zero
+  int* use_copy;
+  PlaneJobs jobs;
+  const float2* rows_out;
+  float *sums, *sum, *most;
+  char* parts;
+  long long bytes;
+  int piece;
+};
+
 // What a backward call does with a piece of `width` classes from `first` on; addresses in the workspace where `at` is one.
 struct Piece {
   SlopeProduct slope;
   Grads grads;
 };
-Piece piece_at(const gelib_linear_loss_args& p, const State& s, const Stored& x, const Stored& w, const Stored& dz, int first, int width, float* sum, float* most) {
+Piece piece_at(const gelib_linear_loss_args& p, const State& s, const Room& r, int first, int width) {
+  const Stored &x = r.x, &w = r.w, &dz = r.dz;
+  float *sum = r.sum, *most = r.most;
   Piece q = {};
   const bool none = p.reduction == GELIB_LOSS_NONE;
   const float up = p.type == GELIB_F16 ? 16384.f : 1.f;
@@ -397,30 +464,23 @@ Piece piece_at(const gelib_linear_loss_args& p, const State& s, const Stored& x,
   if (p.gw) {   // in w's own layout: x^T dz, or its transpose dz^T x
     const Operand a = {t ? f.dz : x, true}, b = {t ? x : f.dz, true};
     char* y = (char*)p.gw + (long long)first * (t ? p.k : 1) * type_bytes(p.type);
-    g.g[g.count++] = {a, b, t ? width : p.k, t ? p.k : width, p.m, y, t ? p.k : p.n, nullptr, true, true};
+    g.g[g.count++] = {a, b, t ? width : p.k, t ? p.k : width, p.m, y, t ? p.k : p.n, nullptr, true, true, r.x_copy, t};
+    g.use_other = r.use_copy;
   }
   return q;
 }
 
-// Where things lie in a backward call's workspace.
-struct Room {
-  Stored x, w, dz;
-  PlaneJobs jobs;
-  const float2* rows_out;
-  float *sums, *sum, *most;
-  char* parts;
-  long long bytes;
-  int piece;
-};
 Room room_of(const gelib_linear_loss_args& p, char* begin) {
   Room r = {};
   char* at = begin;
   r.piece = piece_of(p);
   r.x = x_of(p), r.w = w_of(p);
-  if (p.gw) {   // a copy in which rows without a loss are zero
+  if (p.gw) {   // a copy in which rows without a loss are zero; in 16 bits only where they have to be
     const Stored to = planes_at(r.x, p.type, at);
     r.jobs.add(r.x, to, p.type);
-    r.x = to, r.rows_out = state_of(p).lse;
+    if (tc_ready(r.x, p.type)) r.x_copy = to, r.use_copy = (int*)at, at += 256;
+    else r.x = to;
+    r.rows_out = state_of(p).lse;
   } else {
     copy_if_needed(&r.x, p.type, at, &r.jobs);
   }
@@ -432,7 +492,7 @@ Room room_of(const gelib_linear_loss_args& p, char* begin) {
   r.parts = at;
   long long most = 0;
   for (int first : {0, (p.n - 1) / r.piece * r.piece})
-    most = std::max(most, grads_workspace(piece_at(p, state_of(p), r.x, r.w, r.dz, first, std::min(r.piece, p.n - first), r.sum, r.most).grads));
+    most = std::max(most, grads_workspace(piece_at(p, state_of(p), r, first, std::min(r.piece, p.n - first)).grads));
   r.bytes = at - begin + most;
   return r;
 }
@@ -447,11 +507,11 @@ int backward(const gelib_linear_loss_args& p, char* workspace, cudaStream_t stre
     most_kernel<<<1, 1024, 0, stream>>>((const float*)p.gy, p.m, r.most);
     if ((st = launched(fn)) != GELIB_OK) return st;
   }
-  if ((st = launch_prepare(fn, s, entries_of(p, s), {}, r.jobs, r.rows_out, p.type, stream)) != GELIB_OK) return st;
+  if ((st = launch_prepare(fn, s, entries_of(p, s), {}, r.jobs, r.rows_out, r.use_copy, p.type, stream)) != GELIB_OK) return st;
   bool follows = r.jobs.count > 0;
   for (int first = 0; first < p.n; first += r.piece) {
     const int width = std::min(r.piece, p.n - first);
-    Piece q = piece_at(p, s, r.x, r.w, r.dz, first, width, r.sum, r.most);
+    Piece q = piece_at(p, s, r, first, width);
     q.slope.sums = r.sums;
     if (p.gb) q.grads.sums = r.sums, q.grads.gb = (char*)p.gb + (long long)first * type_bytes(p.type), q.grads.sum_parts = groups_of(p.m), q.grads.sum_n = width;
     if ((st = launch_slope_product(fn, q.slope, follows, stream)) != GELIB_OK) return st;

@@ -13,6 +13,7 @@ constexpr int kInvalid = -2;     // a row's first class: one of its classes does
 // What the forward call leaves for the backward call.
 struct State {
   float* scale;   // 1 over the rows that have a loss, or 1
+  int* odd;       // how many numbers follow, and whether x of a row without a loss holds what is no finite number, by blocks of rows (16-bit x)
   float2* lse;    // (m) the largest z and log2 sum exp2(c (z - largest)), c = log2(e) / T; their sum by itself would cost digits where z is in the thousands.
                   // The second is infinite where a row has no loss
   int* ids;       // (m, top) with a teacher: the classes of entries with q > 0 in ascending order, then kNone
@@ -76,6 +77,8 @@ struct GradProduct {
   long long ldy;
   float* sum;     // (M, N), or null: one piece
   bool first, last;
+  Stored other;          // base null, or what stands for b (other_b) or a
+  bool other_b;
 };
 struct Grads {
   GradProduct g[2];
@@ -86,6 +89,7 @@ struct Grads {
   void* gb = nullptr;
   long long sum_parts = 0;
   int sum_n = 0;
+  const int* use_other = nullptr;   // not zero: the products' `other` operands are taken
 };
 long long grads_workspace(const Grads& g);
 int launch_grads(const char* fn, const Grads& g, bool follows, void* workspace, cudaStream_t stream);

@@ -417,7 +417,7 @@ constexpr int kMostSlabs = 20;
 template <template <class> class E, class Problem>
 int launch_whole(const char* fn, const Sizes& z, const Operand& x, const Operand& w, int type, const Problem& more, bool follows, cudaStream_t stream) {
   const Plan plan = plan_of(&z, 1, type, true);
-  TcMaps maps;
+  TcMaps maps = {};
   TcArgs<Problem> a = {};
   a.p[0] = more;
   const int st = shape_of(fn, plan, plan.c[0], z, x, w, type, &a.p[0], &maps.a[0], &maps.b[0]);
@@ -486,7 +486,7 @@ int launch_grads(const char* fn, const Grads& q, bool follows, void* workspace, 
   if (q.count) {
     Sizes z[kProblems];
     const Plan plan = plan_for(q, z);
-    TcMaps maps;
+    TcMaps maps = {};
     TcArgs<GradProblem> a = {};
     char* at = (char*)workspace;
     const bool other = swapped(plan, z, q.count, q.type);
@@ -497,6 +497,12 @@ int launch_grads(const char* fn, const Grads& q, bool follows, void* workspace, 
       GradProblem& p = a.p[k];
       const int st = shape_of(fn, plan, c, z[i], g.a, g.b, q.type, &p, &maps.a[k], &maps.b[k]);
       if (st != GELIB_OK) return st;
+      if (g.other.base) {
+        const Operand& stands = g.other_b ? g.b : g.a;
+        const int rows = stands.by_sum ? 64 : g.other_b ? c.bn / plan.cg : 128;
+        if (!encode(&maps.other, g.other, q.type, 64, rows)) return fail(GELIB_CUDA_ERROR, fn, "a tensor map could not be made");
+        a.other = q.use_other, a.other_of = k, a.other_b = g.other_b;
+      }
       p.sum = g.sum, p.begun = !g.first, p.y = g.last ? g.y : nullptr, p.ldy = g.ldy;
       p.a0 = q.a0, p.a1 = q.a1, p.a2 = q.a2;
       p.vec_f = g.N % 4 == 0;

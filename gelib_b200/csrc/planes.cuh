@@ -28,10 +28,10 @@ struct PlaneJobs {
   }
 };
 
-// rows_out, where it is given: the rows r of the first operand with rows_out[r].y infinite become zero.
+// rows_out, where it is given: the rows r of the first operand with rows_out[r].y infinite become zero.  from: the first chunk that is copied.
 template <class T, bool kOut = false>
-__device__ __forceinline__ void copy_planes(const PlaneJobs& jobs, long long block, long long blocks, const float2* rows_out = nullptr) {
-  for (long long c = block * kCopyThreads + threadIdx.x; c < jobs.first[jobs.count]; c += blocks * kCopyThreads) {
+__device__ __forceinline__ void copy_planes(const PlaneJobs& jobs, long long block, long long blocks, const float2* rows_out = nullptr, long long from = 0) {
+  for (long long c = from + block * kCopyThreads + threadIdx.x; c < jobs.first[jobs.count]; c += blocks * kCopyThreads) {
     int job = 0;
     while (job + 1 < jobs.count && c >= jobs.first[job + 1]) job++;
     const Stored& f = jobs.from[job];

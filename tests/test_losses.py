@@ -205,10 +205,13 @@ def test_without_bias_only_some_gradients_and_repeats(dtype, top):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("top", [0, 6])
-def test_rows_without_a_loss(dtype, top):
+@pytest.mark.parametrize("top", [0, 6, 12])
+@pytest.mark.parametrize("m,k,n,wt", [(150, 64, 90, False), (150, 64, 90, True), (150, 63, 90, False), (600, 72, 3000, True), (2, 64, 90, False)])
+def test_rows_without_a_loss(m, k, n, wt, dtype, top):
     """Whatever stands in such rows, and in the teacher's missing entries, changes no bit of anything; all rows like that: zeros."""
-    x, w, bias, target, logits = make(150, 64, 90, dtype, top=top)
+    x, w, bias, target, logits = make(m, k, n, dtype, wt=wt, top=top)
+    if m == 2:
+        target[1] = -100
     gy = torch.tensor(1.0, device="cuda")
     for bad in (float("nan"), float("inf")):
         clean = run(x, w, bias, target, logits, gy)
@@ -222,7 +225,7 @@ def test_rows_without_a_loss(dtype, top):
         assert not torch.equal(x2, x)
         got = run(x2, w, bias, target, logits2, gy)
         assert all(torch.equal(a, b) for a, b in zip(got, clean))
-        none = run(x2, w, bias, target, logits2, torch.ones(150, device="cuda"), reduction="none")
+        none = run(x2, w, bias, target, logits2, torch.ones(m, device="cuda"), reduction="none")
         rows = (target < 0).all(1) if top else target < 0
         assert (none[0][rows] == 0).all() and (none[1][rows] == 0).all()
     nothing = torch.full_like(target, -100)
