@@ -11,7 +11,7 @@
 // row.  Backward: z again, piece by piece of the classes, whose epilogue makes dz of it, and two products with that.
 //
 // dz is an operand of the tensor cores: in 16 bits it is rounded to them.  float16 has no room for the small shares of a large vocabulary, so there dz is
-// 2^14 (p - q), times a row's g over the largest g where rows have their own; the rest of the factors comes after the sums.
+// 2^14 (p - q), times a row's g over the largest finite g of rows with a loss where rows have their own; the rest of the factors comes after the sums.
 //
 // Rows without a loss have dz = 0, and their x is read as zero: what stands there, NaN say, must not reach gw.  The forward call looks at such rows of a
 // 16-bit x, and where one holds what is no finite number the product for gw takes a copy (65536 x 1280 x 100: 62 of 350 us when x was always copied).
@@ -170,19 +170,23 @@ int launch_prepare(const char* fn, const State& s, const Entries& e, const Teach
                               : launch_prepare_as<__half>(fn, s, e, t, jobs, rows_out, use_copy, stream);
 }
 
-// The largest |gy|; 1 where that is zero or no finite number.
-__global__ void __launch_bounds__(1024) most_kernel(const float* gy, long long m, float* most) {
+// The largest finite |gy| of rows that have a loss (lse); 1 where that is zero or there is none.  Rows without a loss have no say in how the others are
+// scaled, and an infinity in one row leaves the others their scale.
+__global__ void __launch_bounds__(1024) most_kernel(const float* gy, const float2* lse, long long m, float* most) {
   __shared__ float of[32];
   float v = 0;
 #pragma unroll 8
-  for (long long i = threadIdx.x; i < m; i += 1024) v = fmaxf(v, fabsf(gy[i]));
+  for (long long i = threadIdx.x; i < m; i += 1024) {
+    const float g = fabsf(gy[i]);
+    v = fmaxf(v, g < INFINITY && lse[i].y != INFINITY ? g : 0.f);
+  }
 #pragma unroll
   for (int d = 16; d; d /= 2) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
   if (threadIdx.x % 32 == 0) of[threadIdx.x / 32] = v;
   __syncthreads();
   if (threadIdx.x) return;
   for (int i = 1; i < 32; i++) v = fmaxf(v, of[i]);
-  *most = v > 0.f && v < INFINITY ? v : 1.f;
+  *most = v > 0.f ? v : 1.f;
 }
 
 // ---- rows and their losses ----------------------------------------------------------------------------------------------------
@@ -504,7 +508,7 @@ int backward(const gelib_linear_loss_args& p, char* workspace, cudaStream_t stre
   const Room r = room_of(p, workspace);
   int st;
   if (r.most) {
-    most_kernel<<<1, 1024, 0, stream>>>((const float*)p.gy, p.m, r.most);
+    most_kernel<<<1, 1024, 0, stream>>>((const float*)p.gy, s.lse, p.m, r.most);
     if ((st = launched(fn)) != GELIB_OK) return st;
   }
   if ((st = launch_prepare(fn, s, entries_of(p, s), {}, r.jobs, r.rows_out, r.use_copy, p.type, stream)) != GELIB_OK) return st;
