@@ -400,6 +400,11 @@ int row_blocks(const gelib_linear_loss_args& p, int parts) {
   return p.m <= 4 * kRows ? 1 : (int)std::min<long long>((p.m + kRows - 1) / kRows, 148 * 2);
 }
 
+int launch_rows(const char* fn, const gelib_linear_loss_args& p, const Rows& rows, int blocks, cudaStream_t stream) {
+  const bool few_tiles = short_rows(p, rows.parts);
+  return launch_after(fn, true, few_tiles ? short_rows_kernel : rows_kernel, dim3(blocks), few_tiles ? kThreads : kRowThreads, 0, stream, rows);
+}
+
 int forward(const gelib_linear_loss_args& p, char* at, cudaStream_t stream) {
   static const char* fn = "linear_loss";
   const State s = state_of(p);
@@ -423,8 +428,7 @@ int forward(const gelib_linear_loss_args& p, char* at, cudaStream_t stream) {
   const bool wide = p.type == GELIB_F32;
   const Rows rows = {e, s, f.part, f.at_entry, parts, p.m, c, temperature_of(p), total, (RowSum*)at, wide ? nullptr : (const unsigned short*)p.x, p.ldx, p.k,
                      p.type == GELIB_BF16 ? 0x7f80u : 0x7c00u};
-  const bool few_tiles = short_rows(p, parts);
-  st = launch_after(fn, true, few_tiles ? short_rows_kernel : rows_kernel, dim3(blocks), few_tiles ? kThreads : kRowThreads, 0, stream, rows);
+  st = launch_rows(fn, p, rows, blocks, stream);
   if (st != GELIB_OK || p.reduction == GELIB_LOSS_NONE || blocks == 1) return st;
   return launch_after(fn, true, total_kernel, dim3(1), kThreads, 0, stream, (const RowSum*)at, blocks, total);
 }
@@ -437,10 +441,40 @@ struct Room {
   PlaneJobs jobs;
   const float2* rows_out;
   float *sums, *sum, *most;
+  char* again;     // of few rows, or null
   char* parts;
   long long bytes;
   int piece;
 };
+
+// The forward product of few rows adds in another order than the tensor cores (loss_rows.cu), which make z again.  A share is exp of a difference of z and
+// the row's log-sum: where z is in the thousands its last place is some 2^-12, and a class that is certain would have that for a gradient instead of
+// nothing.  So the largest z and the log-sum of few rows are made again too, of the z that the gradients have: one more product of a row of tiles, whose
+// weights are read once more (a step of 1 x 1280 x 32768: bfloat16 143 to 175 us, float32 362 to 464).
+struct Again {
+  State s;             // odd and lse are the backward call's own
+  ForwardProduct f;
+  float* loss;
+  long long bytes;
+};
+Again again_at(const gelib_linear_loss_args& p, const Stored& x, const Stored& w, char* begin) {
+  char* at = begin;
+  Again a = {state_of(p), forward_of(p)};
+  a.s.odd = (int*)at, at += 256;
+  a.s.lse = (float2*)at, at += up(8 * p.m);
+  a.loss = (float*)at, at += up(4 * p.m);
+  a.f.x = x, a.f.w = w;
+  a.f.part = (float2*)at, at += up(8LL * forward_parts(p.m, p.n, p.k, p.type) * p.m);
+  a.f.at_entry = (float*)at, at += up(4 * p.m * p.top);
+  a.bytes = at - begin;
+  return a;
+}
+int launch_again(const char* fn, const gelib_linear_loss_args& p, const Again& a, bool follows, cudaStream_t stream) {
+  const int parts = forward_parts(p.m, p.n, p.k, p.type), st = launch_forward_product(fn, a.f, follows, stream);
+  if (st != GELIB_OK) return st;
+  const Rows rows = {a.f.e, a.s, a.f.part, a.f.at_entry, parts, p.m, a.f.c, temperature_of(p), {GELIB_LOSS_NONE, a.loss, nullptr}, nullptr, nullptr, p.ldx, p.k, 0};
+  return launch_rows(fn, p, rows, 1, stream);
+}
 
 // What a backward call does with a piece of `width` classes from `first` on; addresses in the workspace where `at` is one.
 struct Piece {
@@ -493,6 +527,7 @@ Room room_of(const gelib_linear_loss_args& p, char* begin) {
   if (p.gb) r.sums = (float*)at, at += up(4 * groups_of(p.m) * r.piece);
   if (p.gx && r.piece < p.n) r.sum = (float*)at, at += up(4LL * p.m * p.k);
   if (p.reduction == GELIB_LOSS_NONE && p.type == GELIB_F16) r.most = (float*)at, at += 256;
+  if (takes_few(forward_of(p))) r.again = at, at += again_at(p, r.x, r.w, at).bytes;
   r.parts = at;
   long long most = 0;
   for (int first : {0, (p.n - 1) / r.piece * r.piece})
@@ -504,7 +539,7 @@ Room room_of(const gelib_linear_loss_args& p, char* begin) {
 int backward(const gelib_linear_loss_args& p, char* workspace, cudaStream_t stream) {
   static const char* fn = "linear_loss_back";
   if (!p.gx && !p.gw && !p.gb) return GELIB_OK;
-  const State s = state_of(p);
+  State s = state_of(p);
   const Room r = room_of(p, workspace);
   int st;
   if (r.most) {
@@ -513,6 +548,12 @@ int backward(const gelib_linear_loss_args& p, char* workspace, cudaStream_t stre
   }
   if ((st = launch_prepare(fn, s, entries_of(p, s), {}, r.jobs, r.rows_out, r.use_copy, p.type, stream)) != GELIB_OK) return st;
   bool follows = r.jobs.count > 0;
+  if (r.again) {
+    const Again a = again_at(p, r.x, r.w, r.again);
+    if ((st = launch_again(fn, p, a, follows, stream)) != GELIB_OK) return st;
+    s.lse = a.s.lse;
+    follows = true;
+  }
   for (int first = 0; first < p.n; first += r.piece) {
     const int width = std::min(r.piece, p.n - first);
     Piece q = piece_at(p, s, r, first, width);
