@@ -89,7 +89,7 @@ def embedding(ids, weight, scale=1.0, padding_idx=None):
         if not isinstance(weight, torch.Tensor) or weight.dim() != 2:
             raise RuntimeError("embedding: weight must have 2 dimensions (entries, channels)")
         if weight.dtype == torch.complex64:
-            y = embedding(ids, torch.view_as_real(weight.resolve_conj()).reshape(weight.size(0), -1), scale, padding_idx)
+            y = embedding(ids, torch.view_as_real(weight.resolve_conj()).reshape(weight.size(0), 2 * weight.size(1)), scale, padding_idx)
             return torch.view_as_complex(y.view(y.shape[:-1] + (weight.size(1), 2)))
         _checked("embedding", weight, ())
         _numbers("embedding", "ids", ids, weight, None)
