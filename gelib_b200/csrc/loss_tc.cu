@@ -408,10 +408,13 @@ __global__ void __launch_bounds__(kJoinThreads) grad_join_kernel(const __grid_co
 // ---- host ---------------------------------------------------------------------------------------------------------------------
 
 // The tensor cores cut every sum off at float's last bit, always to the same side, which over 3271 products of float16 put a loss 2.0e-6 of itself off (the
-// products summed in float: 1.5e-8).  A loss is float, so z leaves its accumulator after 1280 products (so far a loss
-// was at most 1e-6 off, and shorter runs cost the epilogue's time); in both passes, since a class that is certain has
-// a gradient of p - 1, which is nothing only where the log-sum comes of the same z (of few rows the backward call makes it again).  4096 x 2048 x 32768: forward 334 us either way, slope 340 and 365.
-constexpr int kMostSlabs = 20;
+// products summed in float: 1.5e-8).  A loss is float, so z leaves its accumulator often enough that losses are off by less than 2^-20 (9.5e-7) of themselves
+// on average.  That grows with the products that stay together: float16, over 12288 rows of 256 classes, 1024 5.1e-7, 1280 6.2e-7, 1792 8.6e-7, 1920
+// 9.3e-7, 1984 9.5e-7, 2048 9.9e-7 (bfloat16 8.1e-7 at 1920).  So up to 1920 stay, and longer sums leave in equal runs of at most that.  Leaving costs the epilogue's time,
+// which longer sums hide (a step of 4096 x 32768 classes, bfloat16: 1088 products staying 823 us, in two runs 922; 1280 908 and 984, 1536 1057 and 1111, 1920 1342 and 1372).
+// It is done in both passes, since a class that is certain has a gradient of p - 1, which is nothing only where the log-sum comes of the same z (of
+// few rows the backward call makes it again).
+constexpr int kMostSlabs = 30;
 
 // One product whose sums may not be split.
 template <template <class> class E, class Problem>
@@ -427,7 +430,8 @@ int launch_whole(const char* fn, const Sizes& z, const Operand& x, const Operand
   finish_args(&a, plan, type);
   if (type == GELIB_F32) return launch_config<E<float>, 3>(fn, plan.cg, maps, a, follows, stream);
   if (a.p[0].slabs > kMostSlabs) {
-    a.leave = kMostSlabs;
+    const int runs = (a.p[0].slabs + kMostSlabs - 1) / kMostSlabs;
+    a.leave = (a.p[0].slabs + runs - 1) / runs;
     return type == GELIB_BF16 ? launch_config<E<__nv_bfloat16>, 1, true>(fn, plan.cg, maps, a, follows, stream)
                               : launch_config<E<__half>, 1, true>(fn, plan.cg, maps, a, follows, stream);
   }
