@@ -118,3 +118,41 @@ def test_classes_that_a_bias_takes_out(m, dtype):
         got = run(odd, w, bias, target, None, gy, reduction="none")
         others = torch.arange(m, device="cuda") != 1
         assert not torch.isfinite(got[0][1]) and torch.equal(got[0][others], clean[0][others]) and torch.equal(got[1][others], clean[1][others])
+
+
+@pytest.mark.parametrize("top", [0, 5])
+@pytest.mark.parametrize("m,dtype", [(1, torch.bfloat16), (2, torch.float16), (8, torch.float32)])
+def test_a_captured_step_beside_eager_ones(m, dtype, top):
+    x, w, bias, target, logits = make(m, 200, 3000, dtype, top=top)
+    gy = torch.tensor(64.0, device="cuda")
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        run(x, w, bias, target, logits, gy)
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run(x, w, bias, target, logits, gy)
+    for turn in range(3):
+        x.mul_(1.5)
+        w.neg_()
+        gy.mul_(0.5)
+        graph.replay()
+        eager = run(x, w, bias, target, logits, gy)
+        assert all(torch.equal(a, b) for a, b in zip(out, eager))
+        for t, want in zip(out, reference(x, w, bias, target, logits, 2.0, gy, "mean")):
+            near(t, want, "replayed")
+
+
+@pytest.mark.parametrize("top", [0, 5])
+@pytest.mark.parametrize("m", [1, 8])
+def test_the_python_host_side_gives_the_same(m, top, monkeypatch):
+    import gelib_b200 as G
+    for wt in (False, True):
+        for dtype in DTYPES:
+            args = make(m, 90, 36, dtype, wt=wt, top=top)
+            gy = torch.ones(m, device="cuda")
+            want = run(*args, gy, reduction="none")
+            with monkeypatch.context() as patch:
+                patch.setattr(G._lib, "_native", G._lib._Declines())
+                assert all(torch.equal(a, b) for a, b in zip(run(*args, gy, reduction="none"), want))
