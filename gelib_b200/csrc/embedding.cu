@@ -6,13 +6,15 @@
 //
 // Numbers repeat, in a point cloud's species hundreds of times, so gw's sums are made by number: the numbers are sorted (stably, with their places), and
 // teams of lanes add up the rows of gy of a stretch of them in registers.  Every sum has its order, nothing is added by atomics, and a call repeats bit for
-// bit.  The sort has nothing to do with the rows and keeps eight SMs busy, so it runs beside the lookup; its result is kept for the gradient.
+// bit.  The sort has nothing to do with the rows and keeps eight SMs busy; the lookup is launched beside it, and its result is kept for the
+// gradient.  The lookup's blocks stay on their SMs until the sort has ended, and where there are more of them than the SMs hold at a time, the rest begin then:
+// 32768 rows of 2048 bfloat16 are 8192 blocks, a tenth of which runs beside the sort (a call alone 45 us without the sort, 64 with it).
 //
-// 32768 rows of 2048 bfloat16 over 65536 entries: lookup 38 us, sort 24 beside it, sums 74 (402 MB, 5.4 TB/s), joins 8; a pass with its gradient 148 us for 643 MB,
+// 32768 rows of 2048 bfloat16 over 65536 entries: sort 23 us, lookup 38, sums 74 (402 MB, 5.4 TB/s), joins 8; a pass with its gradient 148 us for 643 MB,
 // 4.3 TB/s, the copy rate being 6.5: rows of 4 KB come from all over memory, and reads and writes take turns.  65536 rows of 112 float32 over 100 entries:
 // 9, 19, 14, 20, of a pass of 61, where autograd's hand-over takes 50.
 // Steps: a warp per entry that looks through all numbers 15.5 ms and 7.9 ms for these two; sorted numbers 174 and 76; teams of lanes, any alignment and a
-// list of what is cut 165 and 64; a sort in one cluster that writes in runs 151 and 60; beside the lookup 148.
+// list of what is cut 165 and 64; a sort in one cluster that writes in runs 151 and 60; launched beside the lookup 148.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -71,7 +73,7 @@ __global__ void __launch_bounds__(kThreads) embedding_kernel(const EmbeddingCall
   const long long team = ((long long)blockIdx.x * kThreads + threadIdx.x) / t.lanes, group = team / t.slabs, i0 = group * kRows;
   const int col = ((int)(team - group * t.slabs) * t.lanes + threadIdx.x % t.lanes) * V;
   if (i0 < c.n && col < c.d) look_up<T, V>(c, i0, col);
-  await_previous();   // the sort that this kernel runs beside: what comes after the two follows this one
+  await_previous();   // the sort that this kernel is launched beside: what comes after the two follows this one
 }
 
 // ---- the numbers in order -----------------------------------------------------------------------------------------------------
@@ -690,7 +692,7 @@ long long embedding_workspace(long long n, int, int d, int type) {
   return bytes;
 }
 
-// The sort takes eight SMs and has nothing to do with the rows, so the two run side by side.
+// The sort is made wherever a gradient may be asked for: its numbers are those of this call, which the caller may change before the backward call.
 int launch_embedding(const EmbeddingCall& c, void* state, cudaStream_t stream) {
   if (state) {
     Sort s = sort_of(c.n, c.v, state, nullptr);

@@ -17,9 +17,11 @@
 // 16-bit x, and where one holds what is no finite number the product for gw takes a copy (65536 x 1280 x 100: 62 of 350 us when x was always copied).
 //
 // What bounds it: the tensor cores, 2 m k n for the loss and 6 m k n for the gradients, a third of them to have z again, which keeping it would save.
-// bfloat16, 4096 x 2048 x 65536: 670 us, and two pieces of 365 + 680 (1590 TFLOP/s), 3.3 ms among passes that follow one another, where the power limit
-// brings the clock down (the library's sustained rate makes it 3.25).  4096 x 1280 x 32768 with 64 entries a row: 214, 252, 425; 1100 us.  float32, 1000 x 1280 x
-// 8192: 97, 113, 191 beside 2 x 18 for the three planes of x and w; 498 us.  Small calls wait for the host: six launches and autograd, 83 us.
+// bfloat16, 4096 x 2048 x 65536: 670 us, and two pieces of 365 + 680 (1590 TFLOP/s), 3.3 to 3.4 ms among passes that follow one another, where the power
+// limit brings the clock down (the library's sustained rate makes it 3.25).  4096 x 1280 x 32768 with 64 entries a row: 214, 252, 425; 1100 us.  float32, 1000 x 1280 x
+// 8192: 97, 113, 191 beside 2 x 18 for the three planes of x and w; 498 us.  Small calls wait for the host: 64 x 192 x 100 float32 84 us, of which the forward
+// call takes the host 16, the backward call 55 (an elementwise product's 37: autograd's hand-over) and the rest what two calls in turn cost over each by itself;
+// the kernels take 42.
 #include <algorithm>
 #include <cmath>
 

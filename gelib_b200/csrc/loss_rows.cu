@@ -8,7 +8,8 @@
 //
 // One row of 1280 bfloat16 over 32768 classes, weights from memory: 21 us for 84 MB (4.0 TB/s; 65536 classes 4.5), 27 with the join of the rows; by the tensor cores,
 // whose tiles of 128 rows would be empty but for one, 29 and 35.  Which rows are few, in us a call, 1280 x 32768, here and there: bfloat16 two rows 26 and 30, four 43
-// and 33, eight 57 and 33; float32, whose planes need not be made, one 42 and 163, eight 68 and 163.
+// and 33, eight 57 and 33.  float32, whose planes need not be made, one 42 and 163, eight 68 and 163: eight rows are what these kernels hold in registers, and
+// the times would cross at more.
 #include <algorithm>
 
 #include "loss.h"
@@ -223,7 +224,7 @@ int launch_rows_type(const char* fn, const RowsArgs& a, bool along, int blocks, 
 
 }  // namespace
 
-// Rows that are few: by the times above.
+// Rows that are few: 16-bit ones by the times above, float32 ones as many as the kernels take.
 bool takes_few(const ForwardProduct& p) { return p.M <= (p.type == GELIB_F32 ? 8 : 2); }
 
 int few_parts(const ForwardProduct& p) {

@@ -7,8 +7,8 @@
 // A lane of the epilogue's warps has 16 columns of a row at a time, so that a row's maximum and sum stay in its registers over a tile.  Largest and sum
 // are kept apart for every tile: the sum's exponents are of differences, whatever the size of z.
 //
-// Tensor cores busy (4096 x 2048 x 16384 bfloat16): forward 89 %, slope 88 %, gradients 92 %; with 64 entries a row and sums of 1280 81, 67 and 87 %, where the
-// epilogue of a tile takes as long as its products.  float32 (1000 x 1280 x 8192): 75, 64 and 68 %.
+// Tensor cores busy (4096 x 2048 x 16384 bfloat16, z in two runs): forward 87 %, slope 80 %, gradients 91 %; with 64 entries a row and sums of 1280 79, 65 and
+// 86 %, where the epilogue of a tile takes as long as its products.  float32 (1000 x 1280 x 8192): 73, 63 and 65 %.
 #include "loss.h"
 
 #include "gemm_tc.cuh"

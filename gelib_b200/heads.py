@@ -78,7 +78,8 @@ def embedding(ids, weight, scale=1.0, padding_idx=None):
 
     weight is real or complex64, whose rows then are those of an l=0 part.  The gradient of weight is dense; what falls on a row is added in the
     order of ids, in float32, and rounded once, so that it repeats bit for bit.  Row padding_idx has no gradient.  An id outside [0, v)
-    gives a row of NaN, and no gradient.
+    gives a row of NaN, and no gradient.  Where weight requires a gradient the ids are sorted for it in this call (16 bytes an id are kept): a
+    validation pass that needs none runs under ``torch.no_grad()``.
     """
     scale = float(scale)
     if isinstance(ids, torch.Tensor) and isinstance(weight, torch.Tensor) and (padding_idx is None or type(padding_idx) is int):
