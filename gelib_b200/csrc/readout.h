@@ -30,8 +30,8 @@ int launch_sum_parts(void* gw, void* gb, const float* sums, int parts, int n, in
 #ifdef __CUDACC__
 
 // Kernels of one call that follow one another: the later one is launched while the earlier one ends, and its blocks wait where they begin to read (or
-// write) what that one wrote.  Every block that does so waits, and at least one block in any case: a kernel has ended when all its blocks have, so nothing that comes after can then begin
-// before the earlier kernel has ended.
+// write) what that one wrote.  Every block that does so waits, and at least one block in any case: a kernel has ended when all its blocks have, so nothing that
+// comes after can then begin before the earlier kernel has ended.
 __device__ __forceinline__ void let_next_begin() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void await_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 

@@ -101,7 +101,8 @@ def embedding(ids, weight, scale=1.0, padding_idx=None):
             if not -v <= padding < v:
                 raise RuntimeError("embedding: padding_idx %d is none of the %d rows" % (padding, v))
             padding %= v
-        return EmbeddingFn.apply(ids.reshape(-1), weight, scale, padding).view(ids.shape + (d,))
+        wanted = weight if torch.is_grad_enabled() else weight.detach()   # needs_input_grad does not tell: nothing is sorted where no gradient follows
+        return EmbeddingFn.apply(ids.reshape(-1), wanted, scale, padding).view(ids.shape + (d,))
 
 
 def _loss_args(x, w, bias, target, teacher, transposed, reduction, ignore_index, temperature):
